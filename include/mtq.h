@@ -335,6 +335,66 @@ MTQ_API int mtq_dequant_gather(int dtype, int bits, uint32_t group_size, const v
                                const void *biases, const uint32_t *indices, void *out, uint32_t n_tokens,
                                uint32_t hidden, uint32_t vocab);
 
+/* ---- 8-bit floating point in blocks of 128 ------------------------------- */
+
+/* A second weight format next to the packed codes (no counterpart in the reference's quantized path): codes are bytes,
+ * e4m3 as OCP defines it (four exponent and three mantissa bits, largest 448), row-major, and every block of 128 along a
+ * row has one f32 scale; value = code * scale. Activations have blocks of 1 x 128 (scales f32[rows, ceil(cols / 128)]),
+ * weights of 128 x 128 (scales f32[ceil(rows / 128), ceil(cols / 128)]); blocks at the right and lower edge may be cut.
+ * All four calls: cols (K) a multiple of 16; x, codes and w on 16 bytes, rows packed.
+ *
+ * fp8_quantize: block_rows 1 or 128. scale = max |x| / 448 over the block, not less than 2^-126 (1 where all are zero);
+ * code = the e4m3 value nearest to the f32 quotient x / scale, ties to even. A NaN's code is NaN and does not count for
+ * the maximum; a block with an infinity has scale inf, NaN for the infinity and zeros for the rest (its values are NaN). */
+MTQ_API int mtq_fp8_quantize(int dtype, const void *x, void *codes, float *scales, uint32_t rows, uint32_t cols,
+                             uint32_t block_rows);
+
+/* out[m, n] = sum_k x[m, k] w[n, k] over the values of both: w codes [N, K] with w_scales f32[ceil(N / 128), ceil(K / 128)],
+ * x codes [M, K] with x_scales f32[M, ceil(K / 128)], out T[M, N]. Products of codes are exact, their sums over a block of
+ * 128 and the scaled sums of the blocks f32, rounded to T once. Any M. */
+MTQ_API int mtq_fp8_qmm(int dtype, const void *w, const float *w_scales, const void *x, const float *x_scales, void *out,
+                        uint32_t M, uint32_t N, uint32_t K);
+
+/* The same from activations T[M, K], quantised as mtq_fp8_quantize does with block_rows 1: the decode step's call. Codes
+ * and scales go through a library-owned buffer (allocated on first use, grown on demand). Any M. */
+MTQ_API int mtq_fp8_qmv(int dtype, const void *w, const float *w_scales, const void *x, void *out, uint32_t M, uint32_t N,
+                        uint32_t K);
+
+/* ---- either side of a model's layers ------------------------------------- */
+
+/* The gated delta rule: the recurrence of a linear-attention layer, between its input projections and
+ * mtq_gated_rms_norm_qmv, which takes a token's y. For every sequence, its tokens t in order, and every value head h with
+ * state S f32[dv, dk]:
+ *   S = exp(g[t, h]) S,  u = beta[t, h] (v[t, h] - S k[t, h']),  S += u k[t, h']^T,  y[t, h] = scale S q[t, h'],
+ * h' = h / (hv / hk). norm_eps >= 0: q and k over sqrt(sum of their squares + norm_eps) first; < 0: as they are.
+ * q, k: T, a token's hk heads of dk side by side, tokens q_stride / k_stride elements apart; v: hv heads of dv, v_stride
+ * (so that the three may be parts of one row). g (logarithm of the decay) and beta f32[n_tokens, hv]; y f32[n_tokens, hv, dv]
+ * for every T. state_in / state_out f32[n_slots, hv, dv, dk]: the same array or two that do not overlap; state_in NULL:
+ * sequences begin with zeros. All sums and the state are f32.
+ * Sequence i has the tokens offsets[i] .. offsets[i + 1] - 1 (u32[n_seqs + 1] on the device, ascending; none: its state is
+ * passed on as it is), or with offsets NULL n_tokens / n_seqs each; its state is slot slots[i] (u32[n_seqs] on the device, no slot
+ * twice) or, with slots NULL, slot i. A slot >= n_slots names no state: nothing is written for that sequence. Tokens outside all
+ * sequences are left alone, and offsets behind n_tokens read as n_tokens. hk divides hv; dk <= 256. */
+MTQ_API int mtq_gated_delta_rule(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v,
+                                 size_t v_stride, const float *g, const float *beta, const uint32_t *offsets,
+                                 const uint32_t *slots, const float *state_in, float *state_out, float *y, uint32_t n_seqs,
+                                 uint32_t n_tokens, uint32_t n_slots, uint32_t hk, uint32_t hv, uint32_t dk, uint32_t dv,
+                                 float scale, float norm_eps);
+
+/* Log probabilities behind the output head: of given tokens, of the most likely ones, and the entropy. logits T[n_rows,
+ * vocab], rows row_stride elements apart (>= vocab; any alignment of T). With lse = log sum_i exp(x[i]) over a row:
+ *   token_logprobs f32[n_rows, n_given] = x[tokens] - lse (tokens u32[n_rows, n_given]; an id >= vocab names no token, its
+ *     entry keeps its bytes),
+ *   entropy f32[n_rows] = lse - sum_i exp(x[i] - lse) x[i] (NULL: not wanted),
+ *   top_ids u32[n_rows, n_top] / top_logprobs f32[n_rows, n_top]: the n_top (0..32, <= vocab) largest logits in order, of equal
+ *     ones the lower index first (either may be NULL).
+ * A logit of -inf has probability 0. A row of nothing but -inf: log probabilities -inf, entropy 0, the lowest indices. A row with a NaN or
+ * +inf: all of its log probabilities and its entropy NaN; a NaN is never among the top, and where those run out the id is 0xFFFFFFFF.
+ * Few rows are cut over workgroups and joined through a library-owned buffer (allocated on first use). vocab <= 2^30. */
+MTQ_API int mtq_token_logprobs(int dtype, const void *logits, size_t row_stride, const uint32_t *tokens, uint32_t n_given,
+                               float *token_logprobs, float *entropy, uint32_t *top_ids, float *top_logprobs, uint32_t n_top,
+                               uint32_t n_rows, uint32_t vocab);
+
 /* ---- name-keyed dispatch (the reference's binding convention) ----------- */
 
 /* Replaces Context::dispatch_with_grid (crates/metaltile-runtime/src/context.rs:269-283)
@@ -402,7 +462,12 @@ enum mtq_op {
     MTQ_OP_GATHER_CSR = 4,
     MTQ_OP_GATHER_INDICES = 5,
     MTQ_OP_GATHER_SINGLE = 6,
-    MTQ_OP_RMS_NORM_QMV = 7
+    MTQ_OP_RMS_NORM_QMV = 7,
+    MTQ_OP_FP8_QUANTIZE = 8,    /* M rows, K columns, group_size = block_rows */
+    MTQ_OP_FP8_QMM = 9,         /* M, N, K */
+    MTQ_OP_FP8_QMV = 10,
+    MTQ_OP_GATED_DELTA_RULE = 11, /* E sequences of T tokens in all (by offsets), M = hk, N = hv, K = dk, group_size = dv */
+    MTQ_OP_TOKEN_LOGPROBS = 12  /* M rows, N = vocab, K = n_top */
 };
 #define MTQ_PLAN_MAX_LAUNCHES 8
 typedef struct mtq_plan_launch {

@@ -90,6 +90,12 @@ SIGNATURES = {
                                             _vp, _vp, _vp, _u32, _u32, _u32]),
     "mtq_affine_quantize": (C.c_int, [C.c_int, C.c_int, _u32, _vp, _vp, _vp, _vp, C.c_size_t]),
     "mtq_affine_dequantize": (C.c_int, [C.c_int, C.c_int, _u32, _vp, _vp, _vp, _vp, C.c_size_t]),
+    "mtq_fp8_quantize": (C.c_int, [C.c_int, _vp, _vp, _vp, _u32, _u32, _u32]),
+    "mtq_fp8_qmm": (C.c_int, [C.c_int, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32]),
+    "mtq_fp8_qmv": (C.c_int, [C.c_int, _vp, _vp, _vp, _vp, _u32, _u32, _u32]),
+    "mtq_gated_delta_rule": (C.c_int, [C.c_int, _vp, C.c_size_t, _vp, C.c_size_t, _vp, C.c_size_t, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                       _u32, _u32, _u32, _u32, _u32, _u32, _u32, C.c_float, C.c_float]),
+    "mtq_token_logprobs": (C.c_int, [C.c_int, _vp, C.c_size_t, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _u32, _u32]),
     "mtq_dispatch": (C.c_int, [C.c_char_p, C.c_int, _bufp, C.c_int, _u32p, C.c_int, _u32p, _u32p, _dblp]),
     "mtq_measure": (C.c_int, [C.c_char_p, C.c_int, _bufp, C.c_int, _u32p, C.c_int, _u32p, _u32p, C.c_int, C.c_int, _dblp]),
     "mtq_dispatch_chain": (C.c_int, [C.POINTER(MtqDispatchSpec), C.c_int, C.c_int, _dblp, _dblp, _dblp]),

@@ -16,6 +16,7 @@
 
 #include "../../include/mtq.h"
 #include "../../include/mtq_measure.h"
+#include "fp8_common.h"
 #include "mtq_internal.h"
 #include "qmm_direct_plan.h"
 
@@ -1359,6 +1360,102 @@ static int dispatch_desc(const KernelDesc& d, int dtype, const mtq_buf* bufs, in
 using namespace mtq;
 
 // ---------------------------------------------------------------------------
+// 8-bit floating point in blocks of 128, and the steps either side of a model's layers
+// ---------------------------------------------------------------------------
+
+static int check_dtype(int dtype) {
+    if (dtype != DT_F32 && dtype != DT_F16 && dtype != DT_BF16) return fail(ERR_BAD_ARG, "dtype must be MTQ_F32, MTQ_F16 or MTQ_BF16");
+    return ERR_OK;
+}
+static bool on_16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+static constexpr uint32_t kFp8Longest = 1u << 30;   // (indexes of a row, a column or a block past the last fit 32 bits)
+
+static int op_fp8_quantize(int dtype, const void* x, void* codes, float* scales, uint32_t rows, uint32_t cols, uint32_t block_rows, const LaunchCtx& lc) {
+    int rc = check_dtype(dtype);
+    if (rc) return rc;
+    if (block_rows != 1 && block_rows != kFp8Block) return fail(ERR_BAD_ARG, "block_rows must be 1 or 128");
+    if (cols == 0 || cols % 16 || cols > kFp8Longest) return fail(ERR_SHAPE, "cols must be a non-zero multiple of 16 up to 2^30");
+    if (rows > kFp8Longest) return fail(ERR_SHAPE, "rows must be at most 2^30");
+    if (rows == 0) return ERR_OK;
+    if (!x || !codes || !scales) return fail(ERR_BAD_ARG, "null buffer");
+    if (!on_16(x) || !on_16(codes)) return fail(ERR_BAD_ARG, "x and codes must be on 16 bytes");
+    return launch_fp8_quantize(dtype, x, codes, scales, rows, cols, block_rows, lc);
+}
+
+static int check_fp8(int dtype, const void* w, const float* ws, const void* x, const void* out, uint32_t M, uint32_t N, uint32_t K) {
+    int rc = check_dtype(dtype);
+    if (rc) return rc;
+    if (M > kFp8Longest || N == 0 || N > kFp8Longest) return fail(ERR_SHAPE, "M and N must be at most 2^30, N not 0");
+    if (K == 0 || K % 16 || K > kFp8Longest) return fail(ERR_SHAPE, "K must be a non-zero multiple of 16 up to 2^30");
+    if (!w || !ws || !x || !out) return fail(ERR_BAD_ARG, "null buffer");
+    if (!on_16(w) || !on_16(x)) return fail(ERR_BAD_ARG, "w and x must be on 16 bytes");
+    return ERR_OK;
+}
+
+static int op_fp8_qmm(int dtype, const void* w, const float* ws, const void* x, const float* xs, void* out, uint32_t M, uint32_t N, uint32_t K, const LaunchCtx& lc) {
+    if (M == 0) return check_dtype(dtype);
+    int rc = check_fp8(dtype, w, ws, x, out, M, N, K);
+    if (rc) return rc;
+    if (!xs) return fail(ERR_BAD_ARG, "null buffer");
+    Fp8Args a{(const uint8_t*)w, ws, x, xs, out, M, N, K};
+    return launch_fp8_rows(dtype, a, lc);
+}
+
+static int op_fp8_qmv(int dtype, const void* w, const float* ws, const void* x, void* out, uint32_t M, uint32_t N, uint32_t K, const LaunchCtx& lc) {
+    if (M == 0) return check_dtype(dtype);
+    int rc = check_fp8(dtype, w, ws, x, out, M, N, K);
+    if (rc) return rc;
+    const size_t codes = ((size_t)M * K + 255) / 256 * 256, scales = (size_t)M * ((K + kFp8Block - 1) / kFp8Block) * 4;
+    rc = ensure_scratch(codes + scales);
+    if (rc) return rc;
+    float* xs = (float*)((char*)g.scratch_buf + codes);
+    LaunchCtx first = lc, last = lc;
+    first.stop = nullptr;
+    last.start = nullptr;
+    rc = launch_fp8_quantize(dtype, x, g.scratch_buf, xs, M, K, 1, first);
+    if (rc) return rc;
+    return op_fp8_qmm(dtype, w, ws, g.scratch_buf, xs, out, M, N, K, last);
+}
+
+static int op_gated_delta_rule(const DeltaArgs& a, const LaunchCtx& lc) {
+    int rc = check_dtype(a.dtype);
+    if (rc) return rc;
+    if (a.n_seqs == 0) return ERR_OK;
+    if (a.hk == 0 || a.hv == 0 || a.hv % a.hk) return fail(ERR_SHAPE, "hk must be non-zero and divide hv");
+    if (a.dk == 0 || a.dk > 256) return fail(ERR_SHAPE, "dk must be in 1..256");
+    if (a.dv == 0 || a.dv > 65536) return fail(ERR_SHAPE, "dv must be in 1..65536");
+    if (!a.offsets && a.n_tokens % a.n_seqs) return fail(ERR_SHAPE, "without offsets n_seqs must divide n_tokens");
+    if (!a.slots && a.n_slots < a.n_seqs) return fail(ERR_SHAPE, "without slots there must be a state for each sequence");
+    if (!a.state_out) return fail(ERR_BAD_ARG, "null buffer");
+    if (a.n_tokens) {
+        if (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.y) return fail(ERR_BAD_ARG, "null buffer");
+        if (a.q_stride < (uint64_t)a.hk * a.dk || a.k_stride < (uint64_t)a.hk * a.dk || a.v_stride < (uint64_t)a.hv * a.dv)
+            return fail(ERR_SHAPE, "a token's heads do not fit its stride");
+    }
+    if ((uint64_t)a.n_seqs * a.hv > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more sequences and heads than a launch can have workgroups");
+    return launch_delta_tokens(a, lc);
+}
+
+static int op_token_logprobs(int dtype, const void* logits, size_t stride, const uint32_t* tokens, uint32_t n_given, float* token_logprobs, float* entropy,
+                             uint32_t* top_ids, float* top_logprobs, uint32_t n_top, uint32_t rows, uint32_t vocab, const LaunchCtx& lc) {
+    int rc = check_dtype(dtype);
+    if (rc) return rc;
+    if (vocab == 0 || vocab > (1u << 30)) return fail(ERR_SHAPE, "vocab must be in 1..2^30");
+    if (stride < vocab) return fail(ERR_SHAPE, "row_stride must be at least vocab");
+    if (n_top > 32 || n_top > vocab) return fail(ERR_SHAPE, "n_top must be at most 32 and vocab");
+    if (rows == 0) return ERR_OK;
+    if (!logits || (n_given && (!tokens || !token_logprobs))) return fail(ERR_BAD_ARG, "null buffer");
+    if ((uintptr_t)logits % esize(dtype)) return fail(ERR_BAD_ARG, "logits must be aligned to their type");
+    if (!top_ids && !top_logprobs) n_top = 0;
+    if (!n_given && !entropy && !n_top) return ERR_OK;
+    const size_t need = logprobs_scratch_bytes(rows, vocab, n_top);
+    // (no memory for the slices' sums: a workgroup has each row to itself)
+    void* scratch = need && ensure_scratch(need) == ERR_OK ? g.scratch_buf : nullptr;
+    return launch_logprobs(dtype, logits, stride, tokens, n_given, token_logprobs, entropy, top_ids, top_logprobs, n_top, rows, vocab, scratch, lc);
+}
+
+// ---------------------------------------------------------------------------
 // extern "C"
 // ---------------------------------------------------------------------------
 
@@ -1671,6 +1768,44 @@ int mtq_affine_dequantize(int dtype, int bits, uint32_t group_size, const void* 
                          const_cast<void*>(biases), n_elem, make_ctx());
 }
 
+int mtq_fp8_quantize(int dtype, const void* x, void* codes, float* scales, uint32_t rows, uint32_t cols, uint32_t block_rows) {
+    int rc = need_ready();
+    if (rc) return rc;
+    return op_fp8_quantize(dtype, x, codes, scales, rows, cols, block_rows, make_ctx());
+}
+
+int mtq_fp8_qmm(int dtype, const void* w, const float* w_scales, const void* x, const float* x_scales, void* out, uint32_t M, uint32_t N, uint32_t K) {
+    int rc = need_ready();
+    if (rc) return rc;
+    return op_fp8_qmm(dtype, w, w_scales, x, x_scales, out, M, N, K, make_ctx());
+}
+
+int mtq_fp8_qmv(int dtype, const void* w, const float* w_scales, const void* x, void* out, uint32_t M, uint32_t N, uint32_t K) {
+    int rc = need_ready();
+    if (rc) return rc;
+    return op_fp8_qmv(dtype, w, w_scales, x, out, M, N, K, make_ctx());
+}
+
+int mtq_gated_delta_rule(int dtype, const void* q, size_t q_stride, const void* k, size_t k_stride, const void* v, size_t v_stride, const float* gate,
+                         const float* beta, const uint32_t* offsets, const uint32_t* slots, const float* state_in, float* state_out, float* y,
+                         uint32_t n_seqs, uint32_t n_tokens, uint32_t n_slots, uint32_t hk, uint32_t hv, uint32_t dk, uint32_t dv, float scale, float norm_eps) {
+    int rc = need_ready();
+    if (rc) return rc;
+    DeltaArgs a;
+    a.dtype = dtype;
+    a.q = q; a.k = k; a.v = v; a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+    a.g = gate; a.beta = beta; a.offsets = offsets; a.slots = slots; a.state_in = state_in; a.state_out = state_out; a.y = y;
+    a.n_seqs = n_seqs; a.n_tokens = n_tokens; a.n_slots = n_slots; a.hk = hk; a.hv = hv; a.dk = dk; a.dv = dv; a.scale = scale; a.norm_eps = norm_eps;
+    return op_gated_delta_rule(a, make_ctx());
+}
+
+int mtq_token_logprobs(int dtype, const void* logits, size_t row_stride, const uint32_t* tokens, uint32_t n_given, float* token_logprobs, float* entropy,
+                       uint32_t* top_ids, float* top_logprobs, uint32_t n_top, uint32_t n_rows, uint32_t vocab) {
+    int rc = need_ready();
+    if (rc) return rc;
+    return op_token_logprobs(dtype, logits, row_stride, tokens, n_given, token_logprobs, entropy, top_ids, top_logprobs, n_top, n_rows, vocab, make_ctx());
+}
+
 int mtq_kernel_supported(const char* kernel_name) { return find_kernel(kernel_name) ? 1 : 0; }
 int mtq_kernel_count(void) { return kTableLen; }
 const char* mtq_kernel_name(int i) { return i >= 0 && i < kTableLen ? kTable[i].name : nullptr; }
@@ -1879,10 +2014,10 @@ int mtq_plan(int op, int dtype, int bits, uint32_t group_size, uint32_t M, uint3
              mtq_plan_info* info) {
     if (!info) return fail(ERR_BAD_ARG, "plan: info must not be null");
     memset(info, 0, sizeof(*info));
-    if (op < MTQ_OP_QMV || op > MTQ_OP_RMS_NORM_QMV) return fail(ERR_BAD_ARG, "plan: unknown op");
+    if (op < MTQ_OP_QMV || op > MTQ_OP_TOKEN_LOGPROBS) return fail(ERR_BAD_ARG, "plan: unknown op");
     // Stand-in operand addresses: distinct, 256-byte aligned, never dereferenced (no launch happens).
     auto at = [](int i) { return (void*)(uintptr_t)(0x100000000ull + ((uint64_t)i << 36)); };
-    const void *w = at(1), *s = at(2), *b = at(3), *x = at(4), *aux = at(6), *aux2 = at(7);
+    void *w = at(1), *s = at(2), *b = at(3), *x = at(4), *aux = at(6), *aux2 = at(7);
     void* out = at(5);
     void* const real_scratch = g.scratch_buf;
     const size_t real_held = g.scratch_held;
@@ -1900,6 +2035,22 @@ int mtq_plan(int op, int dtype, int bits, uint32_t group_size, uint32_t M, uint3
         case MTQ_OP_GATHER_CSR: rc = op_gather(GATHER_CSR, dtype, bits, group_size, x, w, s, b, (const uint32_t*)aux, out, T, N, K, E, lc); break;
         case MTQ_OP_GATHER_INDICES: rc = op_gather(GATHER_INDICES, dtype, bits, group_size, x, w, s, b, (const uint32_t*)aux, out, T, N, K, E, lc); break;
         case MTQ_OP_GATHER_SINGLE: rc = op_gather(GATHER_SINGLE, dtype, bits, group_size, x, w, s, b, (const uint32_t*)aux, out, 1, N, K, E, lc); break;
+        case MTQ_OP_FP8_QUANTIZE: rc = op_fp8_quantize(dtype, x, out, (float*)aux, M, K, group_size, lc); break;
+        case MTQ_OP_FP8_QMM: rc = op_fp8_qmm(dtype, w, (const float*)s, x, (const float*)aux, out, M, N, K, lc); break;
+        case MTQ_OP_FP8_QMV: rc = op_fp8_qmv(dtype, w, (const float*)s, x, out, M, N, K, lc); break;
+        case MTQ_OP_GATED_DELTA_RULE: {
+            DeltaArgs d;
+            d.dtype = dtype;
+            d.q = x; d.k = w; d.v = b; d.g = (const float*)s; d.beta = (const float*)aux; d.offsets = (const uint32_t*)aux2;
+            d.state_in = (const float*)at(9); d.state_out = (float*)at(9); d.y = (float*)out;
+            d.hk = M; d.hv = N; d.dk = K; d.dv = group_size; d.n_seqs = d.n_slots = E; d.n_tokens = T;
+            d.q_stride = d.k_stride = (uint64_t)M * K; d.v_stride = (uint64_t)N * group_size;
+            rc = op_gated_delta_rule(d, lc);
+            break;
+        }
+        case MTQ_OP_TOKEN_LOGPROBS:
+            rc = op_token_logprobs(dtype, x, N, (const uint32_t*)aux, 1, (float*)out, (float*)s, (uint32_t*)b, (float*)w, K, M, N, lc);
+            break;
         default: rc = op_rms_norm_qmv(dtype, bits, group_size, x, aux, w, s, b, out, (const float*)aux2, N, K, lc); break;
     }
     info->n_launches = g_plan.n;

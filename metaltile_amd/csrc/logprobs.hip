@@ -1,0 +1,344 @@
+// Log probabilities of given tokens, entropy and top alternatives of rows of logits: what a server answers with, behind the
+// output head.
+//
+//   m = max x,  z = sum exp(x - m),  s = sum exp(x - m) (x - m)
+//   log p(t) = (x_t - m) - log z,    entropy = log z - s / z
+//
+// One read of the logits bounds it: everything else is a few numbers a row. Each lane runs through its part of a row with the
+// maximum so far and both sums relative to it (a larger maximum d above the old one turns z into z e^-d and s into (s - d z) e^-d),
+// so nothing is read twice and no exponent overflows. Sums, maxima and logarithms are f32 for every element type, and results are
+// not rounded to it.
+//
+// The top k come from the same pass. A wave keeps a list of candidates in LDS, a 64-bit key each: the logit's bits in an order of
+// unsigned integers, and below them the complement of the index, so that keys are distinct and equal logits go to the lower index.
+// An element joins the list if its key is above a bar that at least k of the wave's elements have reached; a lane's vectors are
+// asked for their maxima first, which the running maximum needs anyway, so that a wave pays for the list only where it grows
+// (k ln(n / k) times over n elements in no order). A wave whose list is long draws its top k out of it, and the k-th becomes the bar.
+#include "mtq_device.h"
+#include "mtq_internal.h"
+
+namespace mtq {
+
+namespace {
+
+constexpr uint32_t kTopMost = 32;        // alternatives a row
+constexpr uint32_t kListCap = 256;       // a wave's candidates: 4 keys a lane where they are selected from
+constexpr uint32_t kTileElems = 32;      // elements of a lane's tile: 64 bytes of 16-bit logits, 128 of f32
+constexpr int kWaves = 4;
+
+struct LogprobArgs {
+    const void* logits;
+    uint64_t stride;            // elements between rows
+    const uint32_t* tokens;     // [rows, n_given]
+    float* token_logprobs;      // [rows, n_given]
+    float* entropy;             // [rows]
+    uint32_t* top_ids;          // [rows, k]
+    float* top_logprobs;
+    float* part;                // [rows, slices, 4]: m, z, s
+    uint64_t* part_keys;        // [rows, slices, k]
+    uint32_t n_given, k, vocab, slices;
+};
+
+__device__ __forceinline__ uint32_t ordered(float v) {   // unsigned order; -0 as 0
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t u) {
+    return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+
+// Maximum over aligned segments of lanes (from .. to lanes, powers of two): every lane of a segment gets it.
+__device__ __forceinline__ uint32_t seg_max_u32(uint32_t v, int from, int to) {
+    for (int s = from; s < to; s <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, s, 64));
+    return v;
+}
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {   // (a lane without a source takes 0)
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
+// Maximum over the wave, in a scalar register: rows of 16 lanes by mirrors, then row to row, the whole in the last lane.
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = dpp_max<0xB1>(v);    // quad_perm [1,0,3,2]
+    v = dpp_max<0x4E>(v);    // quad_perm [2,3,0,1]
+    v = dpp_max<0x141>(v);   // row_half_mirror
+    v = dpp_max<0x140>(v);   // row_mirror
+    v = dpp_max<0x142>(v);   // row_bcast15
+    v = dpp_max<0x143>(v);   // row_bcast31
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// What a lane has seen of a row.
+struct Seen {
+    float m = -INFINITY, z = 0.f, s = 0.f;
+    __device__ __forceinline__ void raise(float to) {
+        if (to > m) {
+            if (z != 0.f) {   // (nothing summed yet: no difference to take)
+                const float d = m - to, f = __expf(d);
+                s = f > 0.f ? (s + d * z) * f : 0.f;
+                z *= f;
+            }
+            m = to;
+        }
+    }
+    __device__ __forceinline__ void join(float m2, float z2, float s2) {
+        Seen o;
+        o.m = m2; o.z = z2; o.s = s2;
+        const float top = fmaxf(m, o.m);
+        raise(top);
+        o.raise(top);
+        z += o.z;
+        s += o.s;
+    }
+};
+
+// The wave's top `k` of the `n` keys in list[0 .. n), in order, to out[0 .. k) (0: no more keys); returns the k-th. n <= kListCap,
+// and `out` may be `list`. k rounds of a wave maximum, the upper halves first and the lower ones among lanes that have it.
+__device__ __forceinline__ uint64_t draw_top(const uint64_t* list, uint32_t n, uint64_t* out, uint32_t k) {
+    const uint32_t lane = threadIdx.x & 63u;
+    constexpr int PER = kListCap / 64;
+    uint64_t mine[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) mine[i] = i * 64 + lane < n ? list[i * 64 + lane] : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) best = mine[i] > best ? mine[i] : best;
+    uint64_t last = 0;
+    for (uint32_t r = 0; r < k; r++) {
+        const uint32_t hi = wave_max_u32((uint32_t)(best >> 32));
+        const uint32_t lo = wave_max_u32((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+        last = ((uint64_t)hi << 32) | lo;
+        if (lane == 0) out[r] = last;
+        if (best == last) {   // its lane (every lane, once no keys are left) looks for its next
+            best = 0;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                if (mine[i] == last) mine[i] = 0;
+                best = mine[i] > best ? mine[i] : best;
+            }
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return last;
+}
+
+// A row's results, by one wave: z and s relative to m, keys in order.
+template <int DT> __device__ __forceinline__ void finish(const LogprobArgs& a, uint32_t row, const Seen& t, const uint64_t* keys) {
+    const uint32_t lane = threadIdx.x & 63u;
+    // No token has any probability where every logit is -inf (z = 0): log probabilities are -inf, the entropy 0. A NaN or +inf among
+    // the logits makes z NaN, and all of the row's results with it.
+    const bool none = t.z == 0.f;
+    const float log_z = none ? 0.f : logf(t.z);
+    auto lp = [&](float x) { return none ? -INFINITY : (x - t.m) - log_z; };
+    if (a.entropy && lane == 0) a.entropy[row] = none ? 0.f : log_z - t.s / t.z;
+    for (uint32_t j = lane; j < a.n_given; j += 64) {
+        const uint64_t at = (uint64_t)row * a.n_given + j;
+        const uint32_t id = a.tokens[at];
+        if (id < a.vocab) a.token_logprobs[at] = lp(load_elem<DT>(a.logits, (size_t)row * a.stride + id));
+    }
+    if (lane < a.k) {
+        const uint64_t key = keys[lane], at = (uint64_t)row * a.k + lane;
+        if (a.top_ids) a.top_ids[at] = ~(uint32_t)key;             // (0, no key: 0xFFFFFFFF)
+        if (a.top_logprobs) a.top_logprobs[at] = key ? lp(unordered((uint32_t)(key >> 32))) : NAN;
+    }
+}
+
+// A wave's candidates.
+struct Candidates {
+    uint64_t* list;
+    uint32_t n = 0, k;
+    uint64_t bar = 0;            // keys above it join
+    float bar_value = -INFINITY; // no smaller logit has such a key
+    __device__ __forceinline__ void draw() {
+        const uint64_t kth = draw_top(list, n, list, k);
+        n = n < k ? n : k;
+        if (kth) raise_bar(kth);
+    }
+    __device__ __forceinline__ void raise_bar(uint64_t key) {
+        bar = key;
+        bar_value = unordered((uint32_t)(key >> 32));
+    }
+    // One key a lane; 64 of them always fit.
+    __device__ __forceinline__ void offer(uint64_t key) {
+        uint64_t who = __ballot(key > bar);
+        if (!who) return;
+        if (n + 64 > kListCap) {
+            draw();
+            who = __ballot(key > bar);
+        }
+        if (key > bar) list[n + __popcll(who & ((1ull << (threadIdx.x & 63u)) - 1))] = key;
+        n += __popcll(who);
+    }
+};
+
+// What the workgroup's waves have seen and the top k of their lists, joined in its first wave (all of its lanes get it); keys to `comb`.
+__device__ __forceinline__ Seen join_waves(Seen t, const Candidates& c, float (*sums)[3], uint64_t* comb) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    for (int s = 1; s < 64; s <<= 1) t.join(__shfl_xor(t.m, s, 64), __shfl_xor(t.z, s, 64), __shfl_xor(t.s, s, 64));
+    if (c.k) draw_top(c.list, c.n, comb + wave * c.k, c.k);
+    if (lane == 0) { sums[wave][0] = t.m; sums[wave][1] = t.z; sums[wave][2] = t.s; }
+    __syncthreads();
+    if (wave == 0) {
+        for (int w = 1; w < kWaves; w++) t.join(sums[w][0], sums[w][1], sums[w][2]);
+        if (c.k) draw_top(comb, kWaves * c.k, comb, c.k);
+    }
+    return t;
+}
+
+// Workgroup (slice, row): its four waves take tiles of 64 lanes x 32 elements in turn. The row's vectors are the 16-byte blocks of
+// memory that hold any of it, so that rows of every alignment are read in whole vectors; elements before and behind the row count as nothing.
+template <int DT> __global__ __launch_bounds__(64 * kWaves) void logprobs_kernel(LogprobArgs a) {
+    constexpr int ES = DT == DT_F32 ? 4 : 2, PER = 16 / ES, NV = kTileElems / PER;
+    __shared__ uint64_t lists[kWaves][kListCap];
+    __shared__ uint64_t comb[kWaves * kTopMost];
+    __shared__ float sums[kWaves][3];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
+    const uint64_t at = (uint64_t)(uintptr_t)a.logits + (uint64_t)row * a.stride * ES;
+    const uint32_t skip = (uint32_t)(at & 15u) / ES;                          // elements of the first vector that are not the row's
+    const uint4* vecs = (const uint4*)(at & ~(uint64_t)15);
+    const uint32_t n_vecs = (skip + a.vocab + PER - 1) / PER;
+    constexpr uint32_t kTileVecs = 64 * NV;
+    const uint32_t n_tiles = (n_vecs + kTileVecs - 1) / kTileVecs;
+    Candidates c;
+    c.list = lists[wave];
+    c.k = a.k;
+    bool open = true;                // no bar yet
+    Seen t;
+    for (uint32_t tile = slice * kWaves + wave; tile < n_tiles; tile += a.slices * kWaves) {
+        uint4 raw[NV];
+        const uint32_t v0 = tile * kTileVecs + lane;
+#pragma unroll
+        for (int u = 0; u < NV; u++) raw[u] = v0 + u * 64 < n_vecs ? vecs[v0 + u * 64] : make_uint4(0, 0, 0, 0);
+        const bool edge = tile == 0 || tile == n_tiles - 1;
+        auto elem = [&](int u, int j) -> float {
+            const uint32_t w = ((const uint32_t*)&raw[u])[ES == 4 ? j : j >> 1];
+            if constexpr (DT == DT_F32) return __uint_as_float(w);
+            else if constexpr (DT == DT_BF16) return __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
+            else return f16_bits_to_f32(j & 1 ? w >> 16 : w & 0xFFFFu);
+        };
+        float vmax[NV], x[NV][PER];
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            vmax[u] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                x[u][j] = elem(u, j);
+                if (edge) {
+                    const uint32_t e = (v0 + u * 64) * PER + j - skip;        // (before the row: wraps past vocab)
+                    if (e >= a.vocab) x[u][j] = -INFINITY;
+                }
+                vmax[u] = fmaxf(vmax[u], x[u][j]);
+            }
+            top = fmaxf(top, vmax[u]);
+        }
+        t.raise(top);
+        const float base = t.m == -INFINITY ? 0.f : t.m;
+        float z = 0.f, s = 0.f;
+#pragma unroll
+        for (int u = 0; u < NV; u++)
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                const float d = x[u][j] - base, e = __expf(d);
+                z += e;
+                s += e * fmaxf(d, -200.f);                                    // (e^-200 is 0, and 0 * -200 no NaN)
+            }
+        t.z += z;
+        t.s += s;
+        if (!c.k) continue;
+        const bool first = open;
+        if (open) {
+            // A first bar: of 2^i groups of lanes, 2^i >= k, each has an element as large as the least of their maxima.
+            const int groups = c.k <= 1 ? 1 : 1 << (32 - __clz((int)c.k - 1));
+            uint32_t o = seg_max_u32(ordered(top), 1, 64 / groups);
+            o = ~seg_max_u32(~o, 64 / groups, 64);
+            c.raise_bar(((uint64_t)o << 32) - 1);
+            c.bar_value = unordered(o);
+            open = false;
+        }
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            if (!__ballot(!(vmax[u] < c.bar_value))) continue;
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                const float v = elem(u, j);
+                const uint32_t e = (v0 + u * 64) * PER + j - skip;
+                c.offer(v == v && e < a.vocab ? (uint64_t)ordered(v) << 32 | ~e : 0);
+            }
+        }
+        if (first || c.n >= 3 * kListCap / 4) c.draw();
+    }
+    t = join_waves(t, c, sums, comb);
+    if (wave) return;
+    if (a.slices == 1) {
+        finish<DT>(a, row, t, comb);
+    } else {
+        const size_t i = (size_t)row * a.slices + slice;
+        if (lane == 0) { a.part[4 * i] = t.m; a.part[4 * i + 1] = t.z; a.part[4 * i + 2] = t.s; }
+        if (lane < a.k) a.part_keys[i * a.k + lane] = comb[lane];
+    }
+}
+
+// A row's slices joined by one workgroup: at most kSlicesMost, so that their keys fit the waves' lists.
+constexpr uint32_t kSlicesMost = kWaves * kListCap / kTopMost;
+template <int DT> __global__ __launch_bounds__(64 * kWaves) void logprobs_join_kernel(LogprobArgs a) {
+    __shared__ uint64_t lists[kWaves][kListCap];
+    __shared__ uint64_t comb[kWaves * kTopMost];
+    __shared__ float sums[kWaves][3];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x;
+    const uint32_t mine = (a.slices + kWaves - 1) / kWaves, from = wave * mine < a.slices ? wave * mine : a.slices;
+    const uint32_t to = from + mine < a.slices ? from + mine : a.slices;
+    Candidates c;
+    c.list = lists[wave];
+    c.k = a.k;
+    c.n = (to - from) * a.k;
+    const uint64_t* keys = a.part_keys + ((size_t)row * a.slices + from) * a.k;
+    for (uint32_t i = lane; i < c.n; i += 64) c.list[i] = keys[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    Seen t;
+    if (from + lane < to) {
+        const float* p = a.part + 4 * ((size_t)row * a.slices + from + lane);
+        t.m = p[0]; t.z = p[1]; t.s = p[2];
+    }
+    t = join_waves(t, c, sums, comb);
+    if (wave == 0) finish<DT>(a, row, t, comb);
+}
+
+constexpr uint32_t kGridMost = 0x7FFFFFFF;
+
+}  // namespace
+
+static uint32_t logprob_slices(uint32_t rows, uint32_t vocab) {
+    const uint32_t tiles = vocab / (64 * kTileElems) + 1, most = (tiles + kWaves - 1) / kWaves;
+    uint32_t s = rows >= 1024 ? 1 : 1024 / rows;
+    if (s > most) s = most;
+    return s > kSlicesMost ? kSlicesMost : s;
+}
+
+size_t logprobs_scratch_bytes(uint32_t rows, uint32_t vocab, uint32_t k) {
+    const uint32_t s = logprob_slices(rows, vocab);
+    return s == 1 ? 0 : (size_t)rows * s * (16 + 8 * k);
+}
+
+int launch_logprobs(int dtype, const void* logits, size_t stride, const uint32_t* tokens, uint32_t n_given, float* token_logprobs, float* entropy,
+                    uint32_t* top_ids, float* top_logprobs, uint32_t k, uint32_t rows, uint32_t vocab, void* scratch, const LaunchCtx& lc) {
+    LogprobArgs a;
+    a.logits = logits; a.stride = stride; a.tokens = tokens; a.token_logprobs = token_logprobs; a.entropy = entropy; a.top_ids = top_ids;
+    a.top_logprobs = top_logprobs; a.n_given = n_given; a.k = k; a.vocab = vocab;
+    a.slices = scratch ? logprob_slices(rows, vocab) : 1;
+    a.part = (float*)scratch;
+    a.part_keys = scratch ? (uint64_t*)((char*)scratch + (size_t)rows * a.slices * 16) : nullptr;
+    if ((uint64_t)rows * a.slices > kGridMost) return fail(ERR_SHAPE, "more rows than a launch can have workgroups");
+    const void* fn = dtype == DT_F32 ? (const void*)logprobs_kernel<DT_F32> : dtype == DT_F16 ? (const void*)logprobs_kernel<DT_F16> : (const void*)logprobs_kernel<DT_BF16>;
+    void* args[] = {&a};
+    LaunchCtx first = lc;
+    if (a.slices > 1) first.stop = nullptr;
+    MTQ_HIP(launch_kernel(fn, dim3(rows * a.slices), dim3(64 * kWaves), args, 0, first));
+    if (a.slices == 1) return ERR_OK;
+    fn = dtype == DT_F32 ? (const void*)logprobs_join_kernel<DT_F32> : dtype == DT_F16 ? (const void*)logprobs_join_kernel<DT_F16> : (const void*)logprobs_join_kernel<DT_BF16>;
+    LaunchCtx last = lc;
+    last.start = nullptr;
+    MTQ_HIP(launch_kernel(fn, dim3(rows), dim3(64 * kWaves), args, 0, last));
+    return ERR_OK;
+}
+
+}  // namespace mtq

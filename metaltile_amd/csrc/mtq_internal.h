@@ -290,4 +290,30 @@ int launch_affine(bool quantize, int dtype, int bits, uint32_t group_size, const
 int launch_dequant_gather(int dtype, int bits, uint32_t group_size, const void* weight, const void* scales, const void* biases,
                           const uint32_t* ids, void* out, uint32_t n_tokens, uint32_t hidden, uint32_t vocab, const LaunchCtx& lc);
 
+// Log probabilities, entropy and top alternatives of rows of logits (logprobs.hip). scratch: logprobs_scratch_bytes() bytes, or null: a
+// workgroup has a row to itself.
+size_t logprobs_scratch_bytes(uint32_t rows, uint32_t vocab, uint32_t k);
+int launch_logprobs(int dtype, const void* logits, size_t stride, const uint32_t* tokens, uint32_t n_given, float* token_logprobs, float* entropy,
+                    uint32_t* top_ids, float* top_logprobs, uint32_t k, uint32_t rows, uint32_t vocab, void* scratch, const LaunchCtx& lc);
+
+// 8-bit floating point with a scale for each block of 128 (fp8_common.h): the quantiser, and products of its codes.
+struct Fp8Args;
+int launch_fp8_quantize(int dtype, const void* x, void* codes, float* scales, uint32_t rows, uint32_t cols, uint32_t block_rows, const LaunchCtx& lc);
+int launch_fp8_rows(int dtype, const Fp8Args& p, const LaunchCtx& lc);
+
+// The gated delta rule (gated_delta.h).
+struct DeltaArgs {
+    const void *q = nullptr, *k = nullptr, *v = nullptr;     // T, a token's heads side by side, tokens q_stride / k_stride / v_stride elements apart
+    uint64_t q_stride = 0, k_stride = 0, v_stride = 0;
+    const float *g = nullptr, *beta = nullptr;               // [n_tokens, hv]
+    const uint32_t *offsets = nullptr, *slots = nullptr;     // [n_seqs + 1], [n_seqs]; null: equal lengths, slot i
+    const float* state_in = nullptr;                         // [n_slots, hv, dv, dk]; null: zeros
+    float* state_out = nullptr;
+    float* y = nullptr;                                      // [n_tokens, hv, dv]
+    uint32_t n_seqs = 0, n_tokens = 0, n_slots = 0, hk = 0, hv = 0, dk = 0, dv = 0;
+    float scale = 1.f, norm_eps = -1.f;
+    int dtype = 0;
+};
+int launch_delta_tokens(const DeltaArgs& p, const LaunchCtx& lc);
+
 }  // namespace mtq

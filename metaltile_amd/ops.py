@@ -142,6 +142,47 @@ def dequant_gather(dtype, bits, group_size, weight, scales, biases, indices, out
                                       n_tokens, hidden, vocab))
 
 
+def fp8_quantize(dtype, x, codes, scales, rows, cols, block_rows=1):
+    """x T[rows, cols] -> e4m3 codes u8[rows, cols] and a f32 scale for each block of block_rows (1: activations, 128: weights) x 128."""
+    lib = _ensure_init()
+    _lib.check(lib.mtq_fp8_quantize(int(dtype), _p(x), _p(codes), _p(scales), rows, cols, block_rows))
+
+
+def fp8_qmm(dtype, w, w_scales, x, x_scales, out, M, N, K):
+    """out T[M, N] = x[M, K] @ w[N, K]^T, both e4m3 codes with a scale for each block of 128 (x: 1 x 128, w: 128 x 128)."""
+    lib = _ensure_init()
+    _lib.check(lib.mtq_fp8_qmm(int(dtype), _p(w), _p(w_scales), _p(x), _p(x_scales), _p(out), M, N, K))
+
+
+def fp8_qmv(dtype, w, w_scales, x, out, M, N, K):
+    """fp8_qmm of activations T[M, K], quantised on the way as fp8_quantize does."""
+    lib = _ensure_init()
+    _lib.check(lib.mtq_fp8_qmv(int(dtype), _p(w), _p(w_scales), _p(x), _p(out), M, N, K))
+
+
+def gated_delta_rule(dtype, q, k, v, g, beta, state_in, state_out, y, n_seqs, n_tokens, hk, hv, dk, dv, *, row_stride=None, offsets=None, slots=None,
+                     n_slots=None, scale=1.0, norm_eps=-1.0):
+    """The recurrence of a linear-attention layer over n_seqs sequences of n_tokens tokens in all: y f32[n_tokens, hv, dv] and the states
+    f32[n_slots, hv, dv, dk] behind it. q, k: T[n_tokens, hk, dk], v: T[n_tokens, hv, dv], tokens row_stride elements apart (one number, or
+    three for q, k and v; None: packed); g, beta f32[n_tokens, hv]. offsets u32[n_seqs + 1] (None: equal lengths), slots u32[n_seqs] (None:
+    0, 1, ..). state_in None: zeros. norm_eps >= 0: q and k over their 2-norms."""
+    lib = _ensure_init()
+    strides = (hk * dk, hk * dk, hv * dv) if row_stride is None else (row_stride,) * 3 if isinstance(row_stride, int) else tuple(row_stride)
+    at = lambda b: None if b is None else _p(b)
+    _lib.check(lib.mtq_gated_delta_rule(int(dtype), _p(q), strides[0], _p(k), strides[1], _p(v), strides[2], _p(g), _p(beta), at(offsets), at(slots),
+                                        at(state_in), _p(state_out), _p(y), n_seqs, n_tokens, n_seqs if n_slots is None else n_slots, hk, hv, dk, dv,
+                                        scale, norm_eps))
+
+
+def token_logprobs(dtype, logits, row_stride, tokens, n_given, token_logprobs, entropy, top_ids, top_logprobs, n_top, n_rows, vocab):
+    """Of logits T[n_rows, vocab]: log probabilities f32[n_rows, n_given] of tokens u32[n_rows, n_given], entropy f32[n_rows], and the
+    n_top most likely tokens with theirs (u32, f32 [n_rows, n_top]). Outputs that are None are not wanted."""
+    lib = _ensure_init()
+    at = lambda b: None if b is None else _p(b)
+    _lib.check(lib.mtq_token_logprobs(int(dtype), _p(logits), row_stride, at(tokens), n_given, at(token_logprobs), at(entropy), at(top_ids),
+                                      at(top_logprobs), n_top, n_rows, vocab))
+
+
 def timed(fn, *args, **kw) -> float:
     """Run one op with GPU timestamps attached to its kernel; returns microseconds."""
     lib = _ensure_init()
@@ -156,7 +197,8 @@ def sync():
     _lib.check(_ensure_init().mtq_sync())
 
 
-PLAN_OPS = {"qmv": 0, "qmm": 1, "qmm_mma": 2, "qvm": 3, "gather_csr": 4, "gather_indices": 5, "gather_single": 6, "rms_norm_qmv": 7}
+PLAN_OPS = {"qmv": 0, "qmm": 1, "qmm_mma": 2, "qvm": 3, "gather_csr": 4, "gather_indices": 5, "gather_single": 6, "rms_norm_qmv": 7,
+            "fp8_quantize": 8, "fp8_qmm": 9, "fp8_qmv": 10, "gated_delta_rule": 11, "token_logprobs": 12}
 
 
 def plan(op: str, dtype, bits: int, group_size: int, M: int = 1, N: int = 0, K: int = 0, E: int = 1, T: int = 0):
