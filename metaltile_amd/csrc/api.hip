@@ -1399,7 +1399,7 @@ static int op_fp8_qmm(int dtype, const void* w, const float* ws, const void* x, 
     if (rc) return rc;
     if (!xs) return fail(ERR_BAD_ARG, "null buffer");
     Fp8Args a{(const uint8_t*)w, ws, x, xs, out, M, N, K};
-    return launch_fp8_rows(dtype, a, lc);
+    return fp8_tiles_takes(dtype, a) ? launch_fp8_tiles(dtype, a, lc) : launch_fp8_rows(dtype, a, lc);
 }
 
 static int op_fp8_qmv(int dtype, const void* w, const float* ws, const void* x, void* out, uint32_t M, uint32_t N, uint32_t K, const LaunchCtx& lc) {

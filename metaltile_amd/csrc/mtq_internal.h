@@ -300,6 +300,8 @@ int launch_logprobs(int dtype, const void* logits, size_t stride, const uint32_t
 struct Fp8Args;
 int launch_fp8_quantize(int dtype, const void* x, void* codes, float* scales, uint32_t rows, uint32_t cols, uint32_t block_rows, const LaunchCtx& lc);
 int launch_fp8_rows(int dtype, const Fp8Args& p, const LaunchCtx& lc);
+bool fp8_tiles_takes(int dtype, const Fp8Args& p);
+int launch_fp8_tiles(int dtype, const Fp8Args& p, const LaunchCtx& lc);
 
 // The gated delta rule (gated_delta.h).
 struct DeltaArgs {
