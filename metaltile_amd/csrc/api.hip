@@ -1434,6 +1434,10 @@ static int op_gated_delta_rule(const DeltaArgs& a, const LaunchCtx& lc) {
             return fail(ERR_SHAPE, "a token's heads do not fit its stride");
     }
     if ((uint64_t)a.n_seqs * a.hv > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more sequences and heads than a launch can have workgroups");
+    if (delta_chunks_serve(a)) {
+        const size_t need = delta_chunks_scratch_bytes(a, options().scratch_most_kb ? (size_t)options().scratch_most_kb * 1024 : SIZE_MAX);
+        if (need && ensure_scratch(need) == ERR_OK) return launch_delta_chunks(a, g.scratch_buf, need, lc);   // (no memory: token by token)
+    }
     return launch_delta_tokens(a, lc);
 }
 

@@ -1,125 +1,15 @@
 // The gated delta rule token by token (gated_delta.h): single tokens, and sequences too short for chunks.
-//
-// A wave has 4 NC columns of the state (rows of S: dv) in registers, 16 lanes to a column, each with dk / 16 neighbouring values, so that
-// the state is read and written in whole lines. Both products with the state use what it was before the token,
-//   S k = exp(g) (S0 k),   S q = exp(g) (S0 q) + (k . q) u,
-// so that neither waits for the update. A single token is bound by reading and writing the state; many tokens by the seven operations
-// on each of its values, of which the vector units do one a lane and cycle. The next token's rows are loaded while one is computed.
 #include "gated_delta.h"
 
 namespace mtq {
 
 namespace {
 
-__device__ __forceinline__ float sum16(float v) { return seg_allreduce(v, 16); }
-
-template <int DT, int DKL, bool WHOLE> __device__ __forceinline__ void load_part(const void* p, size_t i, uint32_t d0, uint32_t dk, float (&v)[DKL]) {
-    if constexpr (WHOLE && DKL * (DT == DT_F32 ? 4 : 2) % 16 == 0) {
-        constexpr int ES = DT == DT_F32 ? 4 : 2, PER = 16 / ES;
-        const uint4* q = (const uint4*)((const char*)p + (i + d0) * ES);
-#pragma unroll
-        for (int c = 0; c < DKL / PER; c++) {
-            const uint4 r = q[c];
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int j = 0; j < PER; j++) {
-                if constexpr (DT == DT_F32) v[c * PER + j] = __uint_as_float(w[j]);
-                else {
-                    const uint32_t h = j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu;
-                    v[c * PER + j] = DT == DT_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < DKL; j++) v[j] = d0 + j < dk ? load_elem<DT>(p, i + d0 + j) : 0.f;
-    }
-}
-
 // DKL: values of k a lane; WHOLE: dk = 16 DKL and every row on 16 bytes; NC: columns a lane.
 template <int DT, int DKL, bool WHOLE, int NC> __global__ __launch_bounds__(256) void delta_tokens_kernel(DeltaArgs a) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t seq = blockIdx.x / a.hv, h = blockIdx.x % a.hv;
     const DeltaSeq s = delta_seq(a, seq);
-    if (!s.any) return;
-    const uint32_t d0 = (lane & 15u) * DKL, c0 = (blockIdx.y * 4 + wave) * (4 * NC) + (lane >> 4);
-    if (c0 - (lane >> 4) >= a.dv) return;
-    const uint32_t hk = h / (a.hv / a.hk);
-    const size_t state = ((size_t)s.slot * a.hv + h) * a.dv;
-    float S[NC][DKL];
-#pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const uint32_t col = c0 + 4 * c;
-        if (a.state_in && col < a.dv) load_part<DT_F32, DKL, WHOLE>(a.state_in, (state + col) * a.dk, d0, a.dk, S[c]);
-        else
-#pragma unroll
-            for (int j = 0; j < DKL; j++) S[c][j] = 0.f;
-    }
-    struct Token {
-        float q[DKL], k[DKL], v[NC], g, beta;
-    };
-    auto load = [&](uint32_t t, Token& x) {
-        load_part<DT, DKL, WHOLE>(a.q, (size_t)t * a.q_stride + (size_t)hk * a.dk, d0, a.dk, x.q);
-        load_part<DT, DKL, WHOLE>(a.k, (size_t)t * a.k_stride + (size_t)hk * a.dk, d0, a.dk, x.k);
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const uint32_t col = c0 + 4 * c;
-            x.v[c] = load_elem<DT>(a.v, (size_t)t * a.v_stride + (size_t)h * a.dv + (col < a.dv ? col : a.dv - 1));
-        }
-        x.g = a.g[(size_t)t * a.hv + h];
-        x.beta = a.beta[(size_t)t * a.hv + h];
-    };
-    Token x;
-    if (s.from < s.to) load(s.from, x);
-    for (uint32_t t = s.from; t < s.to; t++) {
-        Token next = x;
-        if (t + 1 < s.to) load(t + 1, next);
-        float qq = 0.f, kk = 0.f, qk = 0.f, Sk[NC], Sq[NC];
-#pragma unroll
-        for (int c = 0; c < NC; c++) Sk[c] = Sq[c] = 0.f;
-#pragma unroll
-        for (int j = 0; j < DKL; j++) {
-            qq += x.q[j] * x.q[j];
-            kk += x.k[j] * x.k[j];
-            qk += x.q[j] * x.k[j];
-#pragma unroll
-            for (int c = 0; c < NC; c++) {
-                Sk[c] += S[c][j] * x.k[j];
-                Sq[c] += S[c][j] * x.q[j];
-            }
-        }
-        qk = sum16(qk);
-        float rq = a.scale, rk = 1.f;
-        if (a.norm_eps >= 0.f) {
-            rq = a.scale / sqrtf(sum16(qq) + a.norm_eps);
-            rk = 1.f / sqrtf(sum16(kk) + a.norm_eps);
-        }
-        const float keep = expf(x.g);
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const uint32_t col = c0 + 4 * c;
-            const float u = x.beta * (x.v[c] - keep * rk * sum16(Sk[c])), uk = u * rk;
-            const float y = rq * (keep * sum16(Sq[c]) + qk * uk);
-            if ((lane & 15u) == 0 && col < a.dv) a.y[((size_t)t * a.hv + h) * a.dv + col] = y;
-#pragma unroll
-            for (int j = 0; j < DKL; j++) S[c][j] = keep * S[c][j] + x.k[j] * uk;
-        }
-        x = next;
-    }
-#pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const uint32_t col = c0 + 4 * c;
-        if (col >= a.dv) continue;
-        float* o = a.state_out + (state + col) * a.dk + d0;
-        if constexpr (WHOLE && DKL % 4 == 0) {
-#pragma unroll
-            for (int j = 0; j < DKL; j += 4) *(float4*)(o + j) = make_float4(S[c][j], S[c][j + 1], S[c][j + 2], S[c][j + 3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < DKL; j++)
-                if (d0 + j < a.dk) o[j] = S[c][j];
-        }
-    }
+    if (s.any) delta_tokens<DT, DKL, WHOLE, NC>(a, s, h, (blockIdx.y * 4 + (threadIdx.x >> 6)) * (4 * NC));
 }
 
 template <int DT, int NC> const void* tokens_fn(uint32_t dk, bool whole) {
@@ -135,9 +25,7 @@ template <int DT, int NC> const void* tokens_fn(uint32_t dk, bool whole) {
 int launch_delta_tokens(const DeltaArgs& p, const LaunchCtx& lc) {
     DeltaArgs a = p;
     constexpr int NC = 1;
-    const size_t es = a.dtype == DT_F32 ? 4 : 2;
-    auto on16 = [&](const void* b, size_t stride) { return (uintptr_t)b % 16 == 0 && stride * es % 16 == 0; };
-    const bool whole = on16(a.q, a.q_stride) && on16(a.k, a.k_stride) && (uintptr_t)a.state_in % 16 == 0 && (uintptr_t)a.state_out % 16 == 0;
+    const bool whole = delta_rows_whole(a);
     const void* fn = a.dtype == DT_F32 ? tokens_fn<DT_F32, NC>(a.dk, whole) : a.dtype == DT_F16 ? tokens_fn<DT_F16, NC>(a.dk, whole) : tokens_fn<DT_BF16, NC>(a.dk, whole);
     void* args[] = {&a};
     MTQ_HIP(launch_kernel(fn, dim3(a.n_seqs * a.hv, (a.dv + 16 * NC - 1) / (16 * NC)), dim3(256), args, 0, lc));

@@ -1,0 +1,557 @@
+// The gated delta rule (gated_delta.h) in chunks of 64 tokens, on the matrix cores.
+//
+// With G_t the sum of g over a chunk's tokens up to t, r_t and q_t's factor p_t = scale r'_t the norms' reciprocals (1 without them), and S0
+// the state before the chunk, the recurrence of the chunk's 64 updates u_t is one triangular system:
+//
+//   (1 + A) U = diag(beta) (V - diag(e^G r) K S0),    A_ts = beta_t r_t r_s e^(G_t - G_s) (k_t . k_s), s < t
+//   Y = diag(e^G p) Q S0 + P U,                       P_ts = p_t r_s e^(G_t - G_s) (q_t . k_s), s <= t
+//   S1 = e^(G_63) S0 + K^T diag(r e^(G_63 - G)) U
+//
+// Two launches. The first, a workgroup to a chunk and key head, works out what does not depend on the state: P and T = (1 + A)^-1 diag(beta)
+// (16 x 16 blocks on the diagonal by substitution, the rest from pairs of blocks: [A 0; C B]^-1 = [A' 0; -B' C A' B']). The second walks a
+// sequence's chunks in order, a workgroup to a head and 16 columns of the state: U = T (V - ..), Y and S1. Half of its waves carry what the
+// next chunk waits for (K S0, U), the others Q S0 and P U beside them; all update the state.
+//
+// Everything is held in f32 and multiplied as bf16 on the matrix cores without losing it: an f32 value is the sum of three bf16 terms (8
+// bits each, by rounding and taking the rest), a bf16 q or k is one, an f16 one two. Of the products of terms those of 2^-24 and less of the
+// whole are left out: 3 products for bf16 q and k against f32, 5 for f16, 6 for f32 against f32. That is f32 arithmetic at the rate of the
+// matrix cores over 3 to 6, two to five times what their own f32 instructions do. Sums of decays are f64 (differences of far ones would
+// lose an f32's last digits).
+//
+// What the first launch leaves for the second lies in the order in which lanes hand it to the matrix cores, 16 bytes a lane, so that the
+// walk reads whole lines into registers and waits for no transposition.
+#include "gated_delta.h"
+
+namespace mtq {
+
+namespace {
+
+constexpr uint32_t kChunk = 64;
+constexpr uint32_t kFewTokens = 16;       // sequences up to this length go token by token
+constexpr uint32_t kTriBytes = 6 * 3 * 1024;   // T or P: 6 steps of 16 x 32 that hold any of the triangle, three terms
+constexpr uint32_t kHeadBytes = 2 * kTriBytes + 1024;   // a value head's T, P, and four rows of 64 f32: e^G r, e^G p, r e^(G_63 - G), e^(G_63)
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct ChunkArgs {
+    DeltaArgs d;
+    uint8_t* scratch;
+    uint32_t lo, hi;        // this launch's slots for chunks: sequence i's chunk c has slot from_i / 64 + i + c
+    uint32_t whole;         // rows of q and k on 16 bytes
+};
+
+template <int DKP, int NT> struct Layout {
+    static constexpr uint32_t kOp = NT * kChunk * DKP * 2;      // K, Q or K^T of a key head
+    static constexpr uint32_t kKeyBytes = 3 * kOp;
+    static __device__ __host__ size_t slot_bytes(uint32_t hk, uint32_t hv) { return (size_t)hk * kKeyBytes + (size_t)hv * kHeadBytes; }
+};
+
+__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
+    typedef __attribute__((ext_vector_type(8))) __bf16 v8;
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+// The sum of products of terms i and j with i + j < MOST: small ones first.
+template <int NA, int NB> __device__ __forceinline__ f32x4 mfma_terms(const u32x4 (&a)[NA], const u32x4 (&b)[NB], f32x4 c) {
+    constexpr int MOST = 3;
+#pragma unroll
+    for (int s = MOST - 1; s >= 0; s--)
+#pragma unroll
+        for (int i = 0; i < NA; i++)
+            if (s - i >= 0 && s - i < NB) c = mfma_bf16(a[i], b[s - i], c);
+    return c;
+}
+
+// v as N bf16 terms, two values to a word: term k of (v0, v1) in w[k].
+template <int N> __device__ __forceinline__ void terms(float v0, float v1, uint32_t (&w)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const uint32_t a = f32_to_elem_bits<DT_BF16>(v0), b = f32_to_elem_bits<DT_BF16>(v1);
+        w[k] = a | b << 16;
+        v0 -= bf16_bits_to_f32(a);
+        v1 -= bf16_bits_to_f32(b);
+    }
+}
+template <int N> __device__ __forceinline__ void terms8(const float (&v)[8], u32x4 (&w)[N]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        uint32_t t[N];
+        terms<N>(v[2 * j], v[2 * j + 1], t);
+#pragma unroll
+        for (int k = 0; k < N; k++) w[k][j] = t[k];
+    }
+}
+
+template <int DT> __device__ __forceinline__ void load8(const void* p, size_t i, uint32_t d, uint32_t dk, bool whole, float (&v)[8]) {
+    if (whole && d + 8 <= dk) {
+        load_part<DT, 8, true>(p, i, d, dk, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = d + j < dk ? load_elem<DT>(p, i + d + j) : 0.f;
+    }
+}
+
+// The sequence that a slot belongs to: the last whose first slot is not behind it.
+__device__ __forceinline__ uint32_t first_slot(const DeltaSeq& s, uint32_t seq) { return s.from / kChunk + seq; }
+__device__ __forceinline__ uint32_t seq_of(const DeltaArgs& a, uint32_t slot) {
+    uint32_t lo = 0, hi = a.n_seqs;
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (first_slot(delta_seq(a, mid), mid) <= slot) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+constexpr int kPitch = 68;   // f32 of a row of a 64 x 64 matrix in LDS (rows on 16 bytes, in different banks)
+
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+// c += A B of 16 x 16 blocks in LDS, f32.
+__device__ __forceinline__ f32x4 block_product(const float* A, const float* B, f32x4 c) {
+    const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < 4; k++) c = mfma_f32(A[r * kPitch + 4 * k + g], B[(4 * k + g) * kPitch + r], c);
+    return c;
+}
+__device__ __forceinline__ void block_store(float* D, f32x4 v, float sign) {
+    const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; i++) D[(4 * g + i) * kPitch + r] = sign * v[i];
+}
+
+// ---- what does not depend on the state
+
+template <int DT, int DKP, int NT> __global__ __launch_bounds__(256) void delta_chunk_kernel(ChunkArgs a) {
+    using L = Layout<DKP, NT>;
+    constexpr int KS = DKP / 32;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    u32x4* kop = (u32x4*)lds;                                   // [NT][4][KS][64]
+    float* Am = (float*)(lds + L::kOp);                          // [64][kPitch]
+    float* Tm = Am + kChunk * kPitch;
+    float* Mm = Tm + kChunk * kPitch;                            // P, then products on the way to T
+    double* sums = (double*)(Mm + kChunk * kPitch);              // [64]
+    float* rk = (float*)(sums + kChunk);                         // [64]
+    float* rq = rk + kChunk;
+    float* bt = rq + kChunk;
+    const DeltaArgs& d = a.d;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
+    const uint32_t slot = a.lo + blockIdx.x / d.hk, kh = blockIdx.x % d.hk;
+    const uint32_t seq = seq_of(d, slot);
+    const DeltaSeq s = delta_seq(d, seq);
+    const uint32_t first = first_slot(s, seq);
+    if (!s.any || slot < first || s.to - s.from <= kFewTokens || (uint64_t)(slot - first) * kChunk >= s.to - s.from) return;
+    const uint32_t t0 = s.from + (slot - first) * kChunk, n = s.to - t0 < kChunk ? s.to - t0 : kChunk;
+    uint8_t* out = a.scratch + (size_t)(slot - a.lo) * L::slot_bytes(d.hk, d.hv);
+    uint8_t* key_out = out + (size_t)kh * L::kKeyBytes;
+    const uint32_t t = 16 * wave + r;                            // this lane's row of K and Q
+    u32x4 kf[KS][NT], qf[KS][NT];
+    float kk = 0.f, qq = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        float v[8] = {};
+        const uint32_t c = 32 * ks + 8 * g;
+        if (t < n) load8<DT>(d.k, (size_t)(t0 + t) * d.k_stride + (size_t)kh * d.dk, c, d.dk, a.whole, v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) kk += v[j] * v[j];
+        terms8<NT>(v, kf[ks]);
+        float w[8] = {};
+        if (t < n) load8<DT>(d.q, (size_t)(t0 + t) * d.q_stride + (size_t)kh * d.dk, c, d.dk, a.whole, w);
+#pragma unroll
+        for (int j = 0; j < 8; j++) qq += w[j] * w[j];
+        terms8<NT>(w, qf[ks]);
+    }
+    kk += __shfl_xor(kk, 16, 64);
+    kk += __shfl_xor(kk, 32, 64);
+    qq += __shfl_xor(qq, 16, 64);
+    qq += __shfl_xor(qq, 32, 64);
+    if (g == 0) {
+        const bool norm = d.norm_eps >= 0.f;
+        rk[t] = t >= n ? 0.f : norm ? 1.f / sqrtf(kk + d.norm_eps) : 1.f;
+        rq[t] = t >= n ? 0.f : norm ? d.scale / sqrtf(qq + d.norm_eps) : d.scale;
+    }
+#pragma unroll
+    for (int p = 0; p < NT; p++)
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const uint32_t at = ((p * 4 + wave) * KS + ks) * 64 + lane;
+            kop[at] = kf[ks][p];
+            ((u32x4*)key_out)[at] = kf[ks][p];
+            ((u32x4*)(key_out + L::kOp))[at] = qf[ks][p];
+        }
+    __syncthreads();
+    // K^T: row d of 16 dt + r, tokens 32 ts + 8 g + e
+    for (uint32_t u = wave; u < NT * (DKP / 16) * 2; u += 4) {
+        const uint32_t p = u / ((DKP / 16) * 2), dt = u / 2 % (DKP / 16), ts = u & 1u, dd = 16 * dt + r;
+        const uint16_t* from = (const uint16_t*)kop + (size_t)p * kChunk * DKP + ((dd >> 5) * 64 + ((dd >> 3) & 3u) * 16) * 8 + (dd & 7u);
+        u32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            uint32_t h[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const uint32_t tt = 32 * ts + 8 * g + 2 * j + e;
+                h[e] = from[((tt >> 4) * KS * 64 + (tt & 15u)) * 8];
+            }
+            v[j] = h[0] | h[1] << 16;
+        }
+        ((u32x4*)(key_out + 2 * L::kOp))[u * 64 + lane] = v;
+    }
+    // k_t . k_s and q_t . k_s of rows 16 wave .. and the blocks of columns up to the diagonal
+    f32x4 G[4] = {}, H[4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (j > (int)wave) break;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            u32x4 b[NT];
+#pragma unroll
+            for (int p = 0; p < NT; p++) b[p] = kop[((p * 4 + j) * KS + ks) * 64 + lane];
+            G[j] = mfma_terms(kf[ks], b, G[j]);
+            H[j] = mfma_terms(qf[ks], b, H[j]);
+        }
+    }
+    const uint32_t group = d.hv / d.hk;
+    for (uint32_t x = 0; x < group; x++) {
+        const uint32_t h = kh * group + x;
+        uint8_t* head_out = out + (size_t)d.hk * L::kKeyBytes + (size_t)h * kHeadBytes;
+        if (wave == 0) {
+            float gt = 0.f, beta = 0.f;
+            if (lane < n) {
+                gt = d.g[(size_t)(t0 + lane) * d.hv + h];
+                beta = d.beta[(size_t)(t0 + lane) * d.hv + h];
+            }
+            // (e^-100000 is 0, and a sum with -inf would have no differences)
+            double sum = gt < -1e5f ? -1e5 : (double)gt;
+            for (int o = 1; o < 64; o <<= 1) {
+                const double up = __shfl_up(sum, o, 64);
+                if ((int)lane >= o) sum += up;
+            }
+            sums[lane] = sum;
+            bt[lane] = beta;
+            const double last = __shfl(sum, 63, 64);
+            float* sc = (float*)(head_out + 2 * kTriBytes);
+            const float e = expf((float)sum);
+            sc[lane] = e * rk[lane];
+            sc[64 + lane] = e * rq[lane];
+            sc[128 + lane] = rk[lane] * expf((float)(last - sum));
+            sc[192 + lane] = expf((float)last);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t col = 16 * j + r;
+            const double cs = sums[col];
+            const float rs = rk[col];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t row = 16 * wave + 4 * g + i;
+                float av = 0.f, pv = 0.f;
+                if (j <= (int)wave && col <= row) {
+                    const float f = rs * expf((float)(sums[row] - cs));
+                    pv = rq[row] * f * H[j][i];
+                    if (col < row) av = bt[row] * rk[row] * f * G[j][i];
+                }
+                Am[row * kPitch + col] = av;
+                Mm[row * kPitch + col] = pv;
+                Tm[row * kPitch + col] = 0.f;
+            }
+        }
+        __syncthreads();
+        auto put = [&](const float* M, uint8_t* to, bool by_beta) {   // rows 16 wave .. of M in terms, the steps of the triangle
+            const uint32_t steps = wave < 2 ? 1 : 2, at = wave < 2 ? wave : 2 * wave - 2;
+            for (uint32_t ks = 0; ks < steps; ks++) {
+                const uint32_t c = 32 * ks + 8 * g;
+                float v[8];
+                const float4 lo = *(const float4*)(M + t * kPitch + c), hi = *(const float4*)(M + t * kPitch + c + 4);
+                v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+                if (by_beta)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] *= bt[c + e];
+                u32x4 w[3];
+                terms8<3>(v, w);
+#pragma unroll
+                for (int p = 0; p < 3; p++) ((u32x4*)to)[((at + ks) * 3 + p) * 64 + lane] = w[p];
+            }
+        };
+        put(Mm, head_out + kTriBytes, false);
+        {   // the block on the diagonal: each lane a column of its inverse (four lanes the same one), row by row
+            const float* D = Am + 16 * wave * (kPitch + 1);
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float sum = i == (int)r ? 1.f : 0.f;
+#pragma unroll
+                for (int k = 0; k < i; k++) sum -= D[i * kPitch + k] * v[k];
+                v[i] = sum;
+            }
+            float* to = Tm + 16 * wave * (kPitch + 1);
+            if (g == 0)
+#pragma unroll
+                for (int i = 0; i < 16; i++) to[i * kPitch + r] = v[i];
+        }
+        __syncthreads();
+        auto at = [&](float* M, int i, int j) { return M + 16 * (i * kPitch + j); };
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        // pairs of blocks: (1, 0) by wave 0, (3, 2) by wave 2
+        const int b = (int)wave;
+        if ((b & 1) == 0) block_store(at(Mm, b + 1, b), block_product(at(Am, b + 1, b), at(Tm, b, b), zero), 1.f);
+        __syncthreads();
+        if ((b & 1) == 0) block_store(at(Tm, b + 1, b), block_product(at(Tm, b + 1, b + 1), at(Mm, b + 1, b), zero), -1.f);
+        __syncthreads();
+        // the lower left quarter: wave 2 i + j its block (2 + i, j)
+        const int i = b >> 1, j = b & 1;
+        f32x4 m = block_product(at(Am, 2 + i, 1), at(Tm, 1, j), zero);   // (T's block (0, 1) is zero)
+        m = block_product(at(Am, 2 + i, 0), at(Tm, 0, j), m);
+        block_store(at(Mm, 2 + i, j), m, 1.f);
+        __syncthreads();
+        m = block_product(at(Tm, 2 + i, 2), at(Mm, 2, j), zero);
+        if (i) m = block_product(at(Tm, 3, 3), at(Mm, 3, j), m);
+        block_store(at(Tm, 2 + i, j), m, -1.f);
+        __syncthreads();
+        put(Tm, head_out, true);
+        __syncthreads();
+    }
+}
+
+// ---- the walk
+
+// Waves 0..3 ("ahead"): rows 16 w .. of K S0 and U; waves 4..7: the same rows of Q S0 and P U.
+template <int DT, int DKP, int NT> __global__ __launch_bounds__(512) void delta_walk_kernel(ChunkArgs a, uint32_t pairs, uint32_t columns) {
+    using L = Layout<DKP, NT>;
+    constexpr int KS = DKP / 32, PITCH = DKP + 8, NS = DKP / 16 > 8 ? DKP / 16 / 8 : 1;   // NS: 16-row tiles of the state a wave has
+    constexpr int TP = kChunk + 8;
+    __shared__ __attribute__((aligned(16))) uint16_t Sb[3][16][PITCH];     // terms of the state, column by column
+    __shared__ __attribute__((aligned(16))) uint16_t Xb[3][16][TP], Ub[3][16][TP], Wb[3][16][TP];
+    const DeltaArgs& d = a.d;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
+    // Workgroups go to the eight XCDs in turn: the column blocks of a head, and heads side by side, to one, whose L2 then has what they share.
+    const uint32_t per = (pairs + 7) / 8, pair = blockIdx.x % 8 * per + blockIdx.x / 8 / columns, c0 = blockIdx.x / 8 % columns * 16;
+    if (blockIdx.x / 8 / columns >= per || pair >= pairs) return;
+    const uint32_t seq = pair / d.hv, h = pair % d.hv, kh = h / (d.hv / d.hk);
+    const DeltaSeq s = delta_seq(d, seq);
+    if (!s.any) return;
+    const uint32_t len = s.to - s.from, first = first_slot(s, seq);
+    if (len <= kFewTokens) {
+        if (first < a.lo || first >= a.hi || wave >= 4) return;
+        if (a.whole && d.dk == DKP) delta_tokens<DT, DKP / 16, true, 1>(d, s, h, c0 + 4 * wave);
+        else delta_tokens<DT, DKP / 16, false, 1>(d, s, h, c0 + 4 * wave);
+        return;
+    }
+    const uint32_t chunks = (len + kChunk - 1) / kChunk;
+    const uint32_t begin = a.lo > first ? a.lo - first : 0, end = a.hi <= first ? 0 : a.hi - first < chunks ? a.hi - first : chunks;
+    if (begin >= end) return;
+    const uint32_t col = c0 + r;
+    const bool col_in = col < d.dv;
+    const bool ahead = wave < 4;
+    const uint32_t rb = wave & 3u, steps = rb < 2 ? 1 : 2, step0 = rb < 2 ? rb : 2 * rb - 2;
+    const size_t slot_bytes = L::slot_bytes(d.hk, d.hv);
+    const uint8_t* base = a.scratch + (size_t)(first + begin - a.lo) * slot_bytes;
+    // state: rows 16 tile + 4 g + i, column r
+    f32x4 S[NS] = {};
+    const float* from = begin ? d.state_out : d.state_in;
+    const size_t state = (((size_t)s.slot * d.hv + h) * d.dv + (col_in ? col : 0)) * d.dk;
+    if (from && col_in)
+#pragma unroll
+        for (int x = 0; x < NS; x++) {
+            const uint32_t row = 16 * (wave * NS + x) + 4 * g;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (row + i < d.dk) S[x][i] = from[state + row + i];
+        }
+    u32x4 mf[KS][NT], tf[2][3], kt[NS][2][NT];
+    float v[4];
+    auto load_rows = [&](const uint8_t* p) {        // K's or Q's rows
+        const u32x4* q = (const u32x4*)(p + (size_t)kh * L::kKeyBytes + (ahead ? 0 : L::kOp));
+#pragma unroll
+        for (int k = 0; k < NT; k++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) mf[ks][k] = q[((k * 4 + rb) * KS + ks) * 64 + lane];
+    };
+    auto head = [&](const uint8_t* p) { return p + (size_t)d.hk * L::kKeyBytes + (size_t)h * kHeadBytes; };
+    auto load_tri = [&](const uint8_t* p) {         // T's or P's
+        const u32x4* q = (const u32x4*)(head(p) + (ahead ? 0 : kTriBytes));
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+            for (int k = 0; k < 3; k++) tf[ks][k] = q[((step0 + (ks < (int)steps ? ks : 0)) * 3 + k) * 64 + lane];
+    };
+    auto load_kt = [&](const uint8_t* p) {
+        const u32x4* q = (const u32x4*)(p + (size_t)kh * L::kKeyBytes + 2 * L::kOp);
+#pragma unroll
+        for (int x = 0; x < NS; x++)
+#pragma unroll
+            for (int ts = 0; ts < 2; ts++)
+#pragma unroll
+                for (int k = 0; k < NT; k++)
+                    if (wave * NS + x < DKP / 16) kt[x][ts][k] = q[((k * (DKP / 16) + wave * NS + x) * 2 + ts) * 64 + lane];
+    };
+    auto load_v = [&](uint32_t t0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t t = t0 + 16 * rb + 4 * g + i;
+            v[i] = t < s.to && col_in ? load_elem<DT>(d.v, (size_t)t * d.v_stride + (size_t)h * d.dv + col) : 0.f;
+        }
+    };
+    auto put = [&](uint16_t* to, uint32_t plane, const f32x4& x) {   // four rows of a column, in terms
+        uint32_t w0[3], w1[3];
+        terms<3>(x[0], x[1], w0);
+        terms<3>(x[2], x[3], w1);
+#pragma unroll
+        for (int k = 0; k < 3; k++) *(uint2*)(to + k * plane) = make_uint2(w0[k], w1[k]);
+    };
+    auto put_state = [&]() {
+#pragma unroll
+        for (int x = 0; x < NS; x++)
+            if (wave * NS + x < DKP / 16) put(&Sb[0][r][16 * (wave * NS + x) + 4 * g], 16 * PITCH, S[x]);
+    };
+    auto times_state = [&]() {
+        f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            u32x4 b[3];
+#pragma unroll
+            for (int k = 0; k < 3; k++) b[k] = *(const u32x4*)&Sb[k][r][32 * ks + 8 * g];
+            c = mfma_terms(mf[ks], b, c);
+        }
+        return c;
+    };
+    auto triangle = [&](const uint16_t (*B)[16][TP], f32x4 c) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            if (ks >= (int)steps) break;
+            u32x4 b[3];
+#pragma unroll
+            for (int k = 0; k < 3; k++) b[k] = *(const u32x4*)&B[k][r][32 * ks + 8 * g];
+            c = mfma_terms(tf[ks], b, c);
+        }
+        return c;
+    };
+    load_rows(base);
+    if (ahead) { load_tri(base); load_v(s.from + begin * kChunk); }
+    load_kt(base);
+    put_state();
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t c = begin; c < end; c++) {
+        const uint8_t* p = base + (size_t)(c - begin) * slot_bytes;
+        const uint8_t* next = c + 1 < end ? p + slot_bytes : p;
+        const float* sc = (const float*)(head(p) + 2 * kTriBytes);
+        auto give_y = [&](uint32_t chunk) {       // P U of a chunk onto its Q S0
+            y = triangle(Ub, y);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t t = s.from + chunk * kChunk + 16 * rb + 4 * g + i;
+                if (t < s.to && col_in) d.y[((size_t)t * d.hv + h) * d.dv + col] = y[i];
+            }
+        };
+        __syncthreads();
+        if (ahead) {
+            const f32x4 e = *(const f32x4*)(sc + 16 * rb + 4 * g), ks0 = times_state();
+            f32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = v[i] - e[i] * ks0[i];
+            put(&Xb[0][r][16 * rb + 4 * g], 16 * TP, x);
+            load_rows(next);
+            load_v(s.from + (c + 1) * kChunk);
+        } else {
+            if (c > begin) give_y(c - 1);
+            load_tri(p);
+        }
+        __syncthreads();
+        if (ahead) {
+            const f32x4 w = *(const f32x4*)(sc + 128 + 16 * rb + 4 * g);
+            const f32x4 u = triangle(Xb, f32x4{0.f, 0.f, 0.f, 0.f});
+            put(&Ub[0][r][16 * rb + 4 * g], 16 * TP, u);
+            put(&Wb[0][r][16 * rb + 4 * g], 16 * TP, u * w);
+            load_tri(next);
+        } else {
+            const f32x4 e = *(const f32x4*)(sc + 64 + 16 * rb + 4 * g);
+            y = times_state() * e;
+            load_rows(next);
+        }
+        __syncthreads();
+        const float keep = sc[192];
+#pragma unroll
+        for (int x = 0; x < NS; x++) {
+            if (wave * NS + x >= DKP / 16) break;
+            S[x] *= keep;
+#pragma unroll
+            for (int ts = 0; ts < 2; ts++) {
+                u32x4 b[3];
+#pragma unroll
+                for (int k = 0; k < 3; k++) b[k] = *(const u32x4*)&Wb[k][r][32 * ts + 8 * g];
+                S[x] = mfma_terms(kt[x][ts], b, S[x]);
+            }
+        }
+        load_kt(next);
+        put_state();
+        if (c + 1 == end && !ahead) give_y(c);
+    }
+    if (col_in)
+#pragma unroll
+        for (int x = 0; x < NS; x++) {
+            const uint32_t row = 16 * (wave * NS + x) + 4 * g;
+            if (wave * NS + x < DKP / 16)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (row + i < d.dk) d.state_out[state + row + i] = S[x][i];
+        }
+}
+
+template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* scratch, size_t bytes, const LaunchCtx& lc) {
+    using L = Layout<DKP, NT>;
+    ChunkArgs a;
+    a.d = d;
+    a.scratch = (uint8_t*)scratch;
+    a.whole = delta_rows_whole(d);
+    const uint32_t total = d.n_tokens / kChunk + d.n_seqs, at_once = (uint32_t)(bytes / L::slot_bytes(d.hk, d.hv));
+    uint32_t pairs = d.n_seqs * d.hv, columns = (d.dv + 15) / 16;
+    const uint64_t grid = (uint64_t)((pairs + 7) / 8) * 8 * columns;
+    if (grid > 0x7FFFFFFFull || (uint64_t)total * d.hk > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more chunks or columns than a launch can have workgroups");
+    constexpr size_t lds = L::kOp + 3 * kChunk * kPitch * 4 + kChunk * 8 + 3 * kChunk * 4;
+    const void* chunk = (const void*)delta_chunk_kernel<DT, DKP, NT>;
+    MTQ_HIP(set_max_dynamic_lds(chunk, lds));
+    for (uint32_t lo = 0; lo < total; lo += at_once) {
+        a.lo = lo;
+        a.hi = total - lo < at_once ? total : lo + at_once;
+        LaunchCtx first = lc, second = lc;
+        first.stop = nullptr;
+        if (lo) first.start = nullptr;
+        second.start = nullptr;
+        if (a.hi < total) second.stop = nullptr;
+        void* args[] = {&a, &pairs, &columns};
+        MTQ_HIP(launch_kernel(chunk, dim3((a.hi - lo) * d.hk), dim3(256), args, lds, first));
+        MTQ_HIP(launch_kernel((const void*)delta_walk_kernel<DT, DKP, NT>, dim3((uint32_t)grid), dim3(512), args, 0, second));
+    }
+    return ERR_OK;
+}
+
+template <int DT, int NT> int pick(const DeltaArgs& d, void* scratch, size_t bytes, const LaunchCtx& lc) {
+    return d.dk <= 64 ? launch_chunks<DT, 64, NT>(d, scratch, bytes, lc) : d.dk <= 128 ? launch_chunks<DT, 128, NT>(d, scratch, bytes, lc)
+                                                                                        : launch_chunks<DT, 256, NT>(d, scratch, bytes, lc);
+}
+size_t slot_bytes_of(const DeltaArgs& d) {
+    const size_t terms = d.dtype == DT_BF16 ? 1 : d.dtype == DT_F16 ? 2 : 3, dkp = d.dk <= 64 ? 64 : d.dk <= 128 ? 128 : 256;
+    return d.hk * 3 * terms * kChunk * dkp * 2 + (size_t)d.hv * kHeadBytes;
+}
+
+}  // namespace
+
+// Chunks pay where a sequence may be long: with as many tokens beyond one for each sequence as this. (Sequences of up to kFewTokens go token
+// by token here too.)
+bool delta_chunks_serve(const DeltaArgs& d) {
+    return d.offsets ? d.n_tokens > d.n_seqs && d.n_tokens - d.n_seqs >= 2 * kFewTokens : d.n_tokens / d.n_seqs >= 2 * kFewTokens;
+}
+
+// All of the call's chunks at once up to a gigabyte (and what the caller allows); more go in windows, each sequence from the state that the
+// window before left. 0: not even one chunk fits.
+size_t delta_chunks_scratch_bytes(const DeltaArgs& d, size_t most) {
+    if (most > ((size_t)1 << 30)) most = (size_t)1 << 30;
+    const size_t one = slot_bytes_of(d), all = one * ((size_t)d.n_tokens / kChunk + d.n_seqs);
+    return all <= most ? all : most / one * one;
+}
+
+int launch_delta_chunks(const DeltaArgs& d, void* scratch, size_t bytes, const LaunchCtx& lc) {
+    return d.dtype == DT_F32 ? pick<DT_F32, 3>(d, scratch, bytes, lc) : d.dtype == DT_F16 ? pick<DT_F16, 2>(d, scratch, bytes, lc) : pick<DT_BF16, 1>(d, scratch, bytes, lc);
+}
+
+}  // namespace mtq

@@ -317,5 +317,9 @@ struct DeltaArgs {
     int dtype = 0;
 };
 int launch_delta_tokens(const DeltaArgs& p, const LaunchCtx& lc);
+// In chunks of 64 tokens (gated_delta_chunks.hip). scratch: delta_chunks_scratch_bytes() bytes, at most `most` (0: too little).
+bool delta_chunks_serve(const DeltaArgs& d);
+size_t delta_chunks_scratch_bytes(const DeltaArgs& d, size_t most);
+int launch_delta_chunks(const DeltaArgs& d, void* scratch, size_t bytes, const LaunchCtx& lc);
 
 }  // namespace mtq

@@ -8,7 +8,8 @@ min(tokens, 1 / (1 - max exp(g))) tokens add up: (dk / 16 + 16) 2^-24 x that man
 import numpy as np
 import pytest
 
-from metaltile_amd import DType, GpuBuffer, MtqError, ops, pack_f32, unpack_f32
+from metaltile_amd import DType, GpuBuffer, MtqError, _lib, ops, pack_f32, unpack_f32
+from metaltile_amd.runtime import _ensure_init
 from tests.hip_graph import Graph
 
 pytestmark = pytest.mark.gpu
@@ -171,6 +172,21 @@ def test_a_sequence_in_two_calls(cut):
     S2 = np.frombuffer(state.read_bytes(), "<f4").reshape(S.shape)
     rel = 2 * (8 + 16) * 2.0 ** -24 / (1 - np.exp(c.g.max()))
     assert np.abs(y - y2).max() <= rel * np.abs(y).max() and np.abs(S - S2).max() <= rel * np.abs(S).max()
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
+@pytest.mark.parametrize("most_kb", [1, 200, 400, 1000])
+def test_little_scratch(dt, most_kb):
+    """Chunks in windows of as many as fit the scratch that the caller allows, token by token where none does."""
+    lib = _ensure_init()
+    _lib.check(lib.mtq_set_option(b"scratch.most_kb", most_kb))
+    try:
+        for lens in ([300], [70, 5, 0, 130, 64], [3, 200, 0]):
+            c = Case(dt, lens, 1, 2, 64, 48)
+            c.call()
+            c.hold()
+    finally:
+        _lib.check(lib.mtq_set_option(b"scratch.most_kb", 0))
 
 
 def test_refusals():

@@ -63,7 +63,7 @@ def test_gated_delta_rule(dt):
         seqs = int(2 ** rng.uniform(0, 9))
         tokens = seqs * int(2 ** rng.uniform(0, 12))
         rc, launches, _, count = ops.plan("gated_delta_rule", dt, 0, dv, hk, hv, dk, seqs, tokens)
-        assert rc == OK and count == len(launches)
+        assert rc == OK and min(count, 8) == len(launches)   # (two launches for each window of chunks)
         _check(launches)
 
 
