@@ -21,6 +21,7 @@
 // What the first launch leaves for the second lies in the order in which lanes hand it to the matrix cores, 16 bytes a lane, so that the
 // walk reads whole lines into registers and waits for no transposition.
 #include "gated_delta.h"
+#include "mfma16.h"
 
 namespace mtq {
 
@@ -62,14 +63,27 @@ template <int NA, int NB> __device__ __forceinline__ f32x4 mfma_terms(const u32x
     return c;
 }
 
+// Two such sums over the same b, side by side.
+template <int NA, int NB> __device__ __forceinline__ void mfma_terms2(const u32x4 (&a0)[NA], const u32x4 (&a1)[NA], const u32x4 (&b)[NB], f32x4& c0, f32x4& c1) {
+    constexpr int MOST = 3;
+#pragma unroll
+    for (int s = MOST - 1; s >= 0; s--)
+#pragma unroll
+        for (int i = 0; i < NA; i++)
+            if (s - i >= 0 && s - i < NB) {
+                c0 = mfma_bf16(a0[i], b[s - i], c0);
+                c1 = mfma_bf16(a1[i], b[s - i], c1);
+            }
+}
+
 // v as N bf16 terms, two values to a word: term k of (v0, v1) in w[k].
 template <int N> __device__ __forceinline__ void terms(float v0, float v1, uint32_t (&w)[N]) {
+    typedef __attribute__((ext_vector_type(2))) float f32x2;
 #pragma unroll
     for (int k = 0; k < N; k++) {
-        const uint32_t a = f32_to_elem_bits<DT_BF16>(v0), b = f32_to_elem_bits<DT_BF16>(v1);
-        w[k] = a | b << 16;
-        v0 -= bf16_bits_to_f32(a);
-        v1 -= bf16_bits_to_f32(b);
+        w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v0, v1}), bf16x2_t));
+        v0 -= __uint_as_float(w[k] << 16);
+        v1 -= __uint_as_float(w[k] & 0xFFFF0000u);
     }
 }
 template <int N> __device__ __forceinline__ void terms8(const float (&v)[8], u32x4 (&w)[N]) {
@@ -315,19 +329,311 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256) void delta_
 
 // ---- the walk
 
-// Waves 0..3 ("ahead"): rows 16 w .. of K S0 and U; waves 4..7: the same rows of Q S0 and P U.
-template <int DT, int DKP, int NT> __global__ __launch_bounds__(512) void delta_walk_kernel(ChunkArgs a, uint32_t pairs, uint32_t columns) {
+// LDS is all that a workgroup's waves exchange: loads on their way to registers are not waited for.
+__device__ __forceinline__ void walk_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// Rows of N 16-bit values, one for each of 16 columns, read 16 bytes a lane at the same place of all columns, and written 8 bytes a lane: the
+// 16-byte pieces of column r lie in an order turned by r, so that the sixteen columns' are in different banks.
+template <int N> struct Columns {
+    uint16_t v[16][N];
+    static constexpr int PLANE = 16 * N;
+    __device__ __forceinline__ uint16_t* at(uint32_t r, uint32_t i) {
+        constexpr uint32_t PIECES = N / 8;
+        const uint32_t turn = PIECES >= 16 ? r : r >> 1;   // (rows of 128 bytes lie two and two in the banks' 256)
+        return &v[0][0] + r * N + (((i >> 3) ^ turn) & (PIECES - 1)) * 8 + (i & 7u);
+    }
+};
+
+template <int DKP> struct WalkLds {
+    Columns<DKP> S[3];                             // terms of the state
+    Columns<kChunk> X[3], U[3], W[3];
+    uint32_t touched[64];                          // where the words that bring lines into the L2 end up
+};
+
+struct WalkPlace {
+    const uint8_t* base;     // the first chunk's slot
+    size_t slot_bytes;
+    uint32_t begin, end;     // chunks
+    uint32_t from, to;       // tokens
+    uint32_t h, kh, c0;
+    size_t state;            // element of the states where this head's are
+    const float* state_from;
+};
+
+// Half of the waves (AHEAD) have K S0 and U, the others Q S0 and P U, each of NB blocks of 16 rows; all have a share of the state's rows. With
+// two blocks a wave uses what it reads from LDS twice (blocks 0 and 3, or 1 and 2: three steps of a triangle either way). Each role has a loop of
+// its own, so that each wave waits for just what it loaded: what a chunk needs is asked for in the step after the one that has used the same
+// registers, behind that step's reads of LDS. Between the barriers of a chunk (a, b, c):
+//   a..b: X = V - e^G r (K S0)         | Y = Q S0 + P U of the chunk before, to memory
+//   b..c: U = T X                      | Q S0
+//   c..a: S1 = e^G S0 + K^T (r e^.. U), its terms to LDS
+template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline__ void walk(const DeltaArgs& d, const WalkPlace& w, WalkLds<DKP>& lds, uint32_t wave) {
     using L = Layout<DKP, NT>;
-    constexpr int KS = DKP / 32, PITCH = DKP + 8, NS = DKP / 16 > 8 ? DKP / 16 / 8 : 1;   // NS: 16-row tiles of the state a wave has
-    constexpr int TP = kChunk + 8;
-    __shared__ __attribute__((aligned(16))) uint16_t Sb[3][16][PITCH];     // terms of the state, column by column
-    __shared__ __attribute__((aligned(16))) uint16_t Xb[3][16][TP], Ub[3][16][TP], Wb[3][16][TP];
+    constexpr int ES = DT == DT_F32 ? 4 : 2;
+    constexpr int KS = DKP / 32, TILES = DKP / 16, NS = TILES * NB > 8 ? TILES * NB / 8 : 1;   // NS: 16-row tiles of the state a wave has
+    const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+    const uint32_t mine = wave & (4 / NB - 1), rb[2] = {mine, 3 - mine};
+    const bool long_row = NB == 2 || mine >= 2;                            // the last block has two steps of a triangle
+    const bool has_state = wave * NS < TILES;
+    const uint32_t tile0 = has_state ? wave * NS : 0;
+    const uint32_t col = w.c0 + r;
+    const bool col_in = col < d.dv;
+    f32x4 S[NS] = {};
+    const size_t state = w.state + (size_t)(col_in ? col : 0) * d.dk;
+    if (w.state_from && col_in && has_state)
+#pragma unroll
+        for (int x = 0; x < NS; x++) {
+            const uint32_t row = 16 * (tile0 + x) + 4 * g;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (row + i < d.dk) S[x][i] = w.state_from[state + row + i];
+        }
+    u32x4 mf[NB][KS][NT], tf[NB + 1][3], kt[NS][2][NT];
+    f32x4 e[NB], wk[NB] = {};
+    float keep;
+    uint32_t v[NB][4] = {};
+    // Operands of a slot lie 16 bytes a lane; what differs between loads is the same for all lanes and goes into the scalar offset.
+    const uint32_t head_at = d.hk * L::kKeyBytes + w.h * kHeadBytes, rows_at = w.kh * L::kKeyBytes + (AHEAD ? 0 : L::kOp);
+    const uint32_t tri_at = head_at + (AHEAD ? 0 : kTriBytes), kt_at = w.kh * L::kKeyBytes + 2 * L::kOp + tile0 * 2048, scal_at = head_at + 2 * kTriBytes;
+    auto get = [&](__amdgpu_buffer_rsrc_t slot, uint32_t at) { return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(slot, lane * 16, at, 0)); };
+    auto slot = [&](uint32_t chunk) { return kr_rsrc((uint64_t)(uintptr_t)(w.base + (size_t)(chunk - w.begin) * w.slot_bytes), (uint32_t)w.slot_bytes); };
+    auto four = [&](__amdgpu_buffer_rsrc_t s, uint32_t at) { return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(s, g * 16, at, 0)); };
+    auto load_rows = [&](__amdgpu_buffer_rsrc_t s) {        // K's or Q's rows, and the factors of their products with the state
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int k = 0; k < NT; k++) mf[b][ks][k] = get(s, rows_at + ((k * 4 + rb[b]) * KS + ks) * 1024);
+#pragma unroll
+        for (int b = 0; b < NB; b++) e[b] = four(s, scal_at + (AHEAD ? 0 : 256) + 64 * rb[b]);
+    };
+    auto load_tri = [&](__amdgpu_buffer_rsrc_t s) {         // T's or P's: with two blocks the one step of the first and both of the second
+#pragma unroll
+        for (int j = 0; j < NB + 1; j++) {
+            const uint32_t block = j < NB ? rb[j] : rb[NB - 1], step = (block < 2 ? block : 2 * block - 2) + (j == NB && long_row ? 1 : 0);
+#pragma unroll
+            for (int k = 0; k < 3; k++) tf[j][k] = get(s, tri_at + (step * 3 + k) * 1024);
+        }
+        if (AHEAD)
+#pragma unroll
+            for (int b = 0; b < NB; b++) wk[b] = four(s, scal_at + 512 + 64 * rb[b]);
+    };
+    auto load_kt = [&](__amdgpu_buffer_rsrc_t s) {
+#pragma unroll
+        for (int x = 0; x < NS; x++)
+#pragma unroll
+            for (int ts = 0; ts < 2; ts++)
+#pragma unroll
+                for (int k = 0; k < NT; k++) kt[x][ts][k] = get(s, kt_at + ((k * TILES + x) * 2 + ts) * 1024);
+        keep = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(s, 0, scal_at + 768, 0));
+    };
+    uint32_t v_at[NB][4];                                   // a chunk's rows of v; rows behind the sequence are behind its buffer, and read as zeros
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v_at[b][i] = col_in ? ((16 * rb[b] + 4 * g + i) * (uint32_t)d.v_stride + w.h * d.dv + col) * ES : KR_OOB;
+    auto load_v = [&](uint32_t chunk) {
+        const uint32_t t0 = w.from + chunk * kChunk, n = t0 >= w.to ? 0 : w.to - t0 < kChunk ? w.to - t0 : kChunk;
+        const uint32_t bytes = n ? ((n - 1) * (uint32_t)d.v_stride + d.hv * d.dv) * ES : 0;
+        const __amdgpu_buffer_rsrc_t s = kr_rsrc((uint64_t)(uintptr_t)d.v + (uint64_t)(n ? t0 : w.from) * d.v_stride * ES, bytes);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (DT == DT_F32) v[b][i] = __builtin_amdgcn_raw_buffer_load_b32(s, v_at[b][i], 0, 0);
+                else v[b][i] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(s, v_at[b][i], 0, 0);
+            }
+    };
+    auto value = [&](uint32_t x) { return DT == DT_F32 ? __uint_as_float(x) : DT == DT_BF16 ? bf16_bits_to_f32(x) : f16_bits_to_f32(x); };
+    auto put = [&](uint16_t* to, uint32_t plane, const f32x4& x) {   // four rows of a column, in terms
+        uint32_t w0[3], w1[3];
+        terms<3>(x[0], x[1], w0);
+        terms<3>(x[2], x[3], w1);
+#pragma unroll
+        for (int k = 0; k < 3; k++) *(uint2*)(to + k * plane) = make_uint2(w0[k], w1[k]);
+    };
+    auto put_state = [&]() {
+        if (has_state)
+#pragma unroll
+            for (int x = 0; x < NS; x++) put(lds.S[0].at(r, 16 * (tile0 + x) + 4 * g), Columns<DKP>::PLANE, S[x]);
+    };
+    // `load` is what is asked for once the LDS reads are on their way.
+    auto times_state = [&](f32x4 (&c)[NB], auto&& load) {
+        constexpr int AT_ONCE = KS < 4 ? KS : 4;
+        f32x4 odd[NB] = {};
+#pragma unroll
+        for (int b = 0; b < NB; b++) c[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k0 = 0; k0 < KS; k0 += AT_ONCE) {
+            u32x4 b[AT_ONCE][3];
+#pragma unroll
+            for (int ks = 0; ks < AT_ONCE; ks++)
+#pragma unroll
+                for (int k = 0; k < 3; k++) b[ks][k] = *(const u32x4*)lds.S[k].at(r, 32 * (k0 + ks) + 8 * g);
+            __builtin_amdgcn_sched_barrier(0);
+            if (k0 == 0) load();
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < AT_ONCE; ks++) {
+                if constexpr (NB == 2) mfma_terms2(mf[0][k0 + ks], mf[1][k0 + ks], b[ks], c[0], c[1]);
+                else if (ks & 1) odd[0] = mfma_terms(mf[0][k0 + ks], b[ks], odd[0]);
+                else c[0] = mfma_terms(mf[0][k0 + ks], b[ks], c[0]);
+            }
+        }
+        if constexpr (NB == 1) c[0] += odd[0];
+    };
+    auto triangle = [&](Columns<kChunk>* B, f32x4 (&c)[NB], auto&& load) {
+        u32x4 b[2][3];
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+            for (int k = 0; k < 3; k++) b[ks][k] = *(const u32x4*)B[k].at(r, 32 * ks + 8 * g);
+        __builtin_amdgcn_sched_barrier(0);
+        load();
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (NB == 2) mfma_terms2(tf[0], tf[1], b[0], c[0], c[1]);
+        else c[0] = mfma_terms(tf[0], b[0], c[0]);
+        if (long_row) c[NB - 1] = mfma_terms(tf[NB], b[1], c[NB - 1]);
+    };
+    f32x4 y[NB] = {};
+    auto give_y = [&](uint32_t chunk, auto&& load) {  // P U of a chunk onto its Q S0
+        triangle(lds.U, y, load);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t t = w.from + chunk * kChunk + 16 * rb[b] + 4 * g + i;
+                if (t < w.to && col_in) d.y[((size_t)t * d.hv + w.h) * d.dv + col] = y[b][i];
+            }
+    };
+    auto nothing = [] {};
+    {
+        const auto s = slot(w.begin);
+        load_rows(s);
+        if (AHEAD) { load_tri(s); load_v(w.begin); }
+    }
+    put_state();
+    for (uint32_t c = w.begin; c < w.end; c++) {
+        const auto here = slot(c), next = slot(c + 1 < w.end ? c + 1 : c);
+        walk_barrier();
+        if constexpr (AHEAD) {
+            f32x4 x[NB];
+            times_state(x, [&] { load_kt(here); });
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[b][i] = value(v[b][i]) - e[b][i] * x[b][i];
+                asm volatile("" : "+v"(x[b]));   // (here, not behind the next loads into e's and v's registers)
+                put(lds.X[0].at(r, 16 * rb[b] + 4 * g), Columns<kChunk>::PLANE, x[b]);
+            }
+        } else if (c > w.begin) {
+            give_y(c - 1, [&] { load_kt(here); });
+        } else {
+            load_kt(here);
+        }
+        walk_barrier();
+        if constexpr (AHEAD) {
+            f32x4 u[NB] = {}, uw[NB];
+            triangle(lds.X, u, [&] { load_rows(next); load_v(c + 1); });
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                uw[b] = u[b] * wk[b];
+                asm volatile("" : "+v"(uw[b]));
+                put(lds.W[0].at(r, 16 * rb[b] + 4 * g), Columns<kChunk>::PLANE, uw[b]);
+                put(lds.U[0].at(r, 16 * rb[b] + 4 * g), Columns<kChunk>::PLANE, u[b]);
+            }
+        } else {
+            times_state(y, [&] { load_tri(here); });
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                y[b] *= e[b];
+                asm volatile("" : "+v"(y[b]));
+            }
+        }
+        walk_barrier();
+        u32x4 b[2][3];
+#pragma unroll
+        for (int ts = 0; ts < 2; ts++)
+#pragma unroll
+            for (int k = 0; k < 3; k++) b[ts][k] = *(const u32x4*)lds.W[k].at(r, 32 * ts + 8 * g);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (AHEAD) load_tri(next);
+        else load_rows(next);
+        __builtin_amdgcn_sched_barrier(0);
+        if (has_state) {
+#pragma unroll
+            for (int x = 0; x < NS; x++) S[x] *= keep;
+#pragma unroll
+            for (int ts = 0; ts < 2; ts++)
+#pragma unroll
+                for (int x = 0; x < NS; x += 2) {
+                    if constexpr (NS == 1) S[x] = mfma_terms(kt[x][ts], b[ts], S[x]);
+                    else mfma_terms2(kt[x][ts], kt[x + 1 < NS ? x + 1 : x][ts], b[ts], S[x], S[x + 1 < NS ? x + 1 : x]);
+                }
+        }
+        put_state();
+    }
+    if constexpr (!AHEAD) give_y(w.end - 1, nothing);
+    if (col_in && has_state)
+#pragma unroll
+        for (int x = 0; x < NS; x++) {
+            const uint32_t row = 16 * (tile0 + x) + 4 * g;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (row + i < d.dk) d.state_out[state + row + i] = S[x][i];
+        }
+}
+
+// The walk's last wave: brings what the others read kAheadChunks chunks later from memory into the XCD's L2, a word of every 128-byte line (a
+// chunk takes less time than a line's way from memory, and registers hold one chunk ahead). The words go to LDS, so that nothing waits for
+// them. The workgroups of a head's columns share its lines.
+constexpr uint32_t kAheadChunks = 4;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // M0 is a reserved register: naming it as clobbered is the point
+__device__ __forceinline__ void touch(const void* line, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(line) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+template <int DT, int DKP, int NT> __device__ __forceinline__ void walk_touch(const DeltaArgs& d, const WalkPlace& w, WalkLds<DKP>& lds, uint32_t columns) {
+    using L = Layout<DKP, NT>;
+    constexpr int ES = DT == DT_F32 ? 4 : 2;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint32_t*)lds.touched);
+    const uint32_t key_at = w.kh * L::kKeyBytes, head_at = d.hk * L::kKeyBytes + w.h * kHeadBytes;
+    constexpr uint32_t KEY_LINES = L::kKeyBytes / 128, LINES = KEY_LINES + kHeadBytes / 128;
+    auto chunk = [&](uint32_t c) {
+        const uint8_t* p = w.base + (size_t)(c - w.begin) * w.slot_bytes;
+        for (uint32_t i0 = w.c0 / 16 * 64; i0 < LINES; i0 += 64 * columns) {
+            const uint32_t i = i0 + lane < LINES ? i0 + lane : LINES - 1;
+            touch(p + (i < KEY_LINES ? key_at + i * 128 : head_at + (i - KEY_LINES) * 128), to);
+        }
+        const uint32_t t = w.from + c * kChunk + lane;
+        touch((const uint8_t*)d.v + ((size_t)(t < w.to ? t : w.to - 1) * d.v_stride + (size_t)w.h * d.dv + w.c0) * ES, to);
+    };
+    for (uint32_t c = w.begin; c < w.end && c < w.begin + kAheadChunks; c++) chunk(c);
+    for (uint32_t c = w.begin; c < w.end; c++) {
+        if (c + kAheadChunks < w.end) chunk(c + kAheadChunks);
+        walk_barrier();
+        walk_barrier();
+        walk_barrier();
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+template <int DT, int DKP, int NT, int NB> __global__ __launch_bounds__(64 * (8 / NB + 1)) void delta_walk_kernel(ChunkArgs a, uint32_t pairs, uint32_t columns) {
+    using L = Layout<DKP, NT>;
+    __shared__ __attribute__((aligned(16))) WalkLds<DKP> lds;
     const DeltaArgs& d = a.d;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Workgroups go to the eight XCDs in turn: the column blocks of a head, and heads side by side, to one, whose L2 then has what they share.
     const uint32_t per = (pairs + 7) / 8, pair = blockIdx.x % 8 * per + blockIdx.x / 8 / columns, c0 = blockIdx.x / 8 % columns * 16;
     if (blockIdx.x / 8 / columns >= per || pair >= pairs) return;
-    const uint32_t seq = pair / d.hv, h = pair % d.hv, kh = h / (d.hv / d.hk);
+    const uint32_t seq = pair / d.hv, h = pair % d.hv;
     const DeltaSeq s = delta_seq(d, seq);
     if (!s.any) return;
     const uint32_t len = s.to - s.from, first = first_slot(s, seq);
@@ -338,163 +644,22 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(512) void delta_
         return;
     }
     const uint32_t chunks = (len + kChunk - 1) / kChunk;
-    const uint32_t begin = a.lo > first ? a.lo - first : 0, end = a.hi <= first ? 0 : a.hi - first < chunks ? a.hi - first : chunks;
-    if (begin >= end) return;
-    const uint32_t col = c0 + r;
-    const bool col_in = col < d.dv;
-    const bool ahead = wave < 4;
-    const uint32_t rb = wave & 3u, steps = rb < 2 ? 1 : 2, step0 = rb < 2 ? rb : 2 * rb - 2;
-    const size_t slot_bytes = L::slot_bytes(d.hk, d.hv);
-    const uint8_t* base = a.scratch + (size_t)(first + begin - a.lo) * slot_bytes;
-    // state: rows 16 tile + 4 g + i, column r
-    f32x4 S[NS] = {};
-    const float* from = begin ? d.state_out : d.state_in;
-    const size_t state = (((size_t)s.slot * d.hv + h) * d.dv + (col_in ? col : 0)) * d.dk;
-    if (from && col_in)
-#pragma unroll
-        for (int x = 0; x < NS; x++) {
-            const uint32_t row = 16 * (wave * NS + x) + 4 * g;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (row + i < d.dk) S[x][i] = from[state + row + i];
-        }
-    u32x4 mf[KS][NT], tf[2][3], kt[NS][2][NT];
-    float v[4];
-    auto load_rows = [&](const uint8_t* p) {        // K's or Q's rows
-        const u32x4* q = (const u32x4*)(p + (size_t)kh * L::kKeyBytes + (ahead ? 0 : L::kOp));
-#pragma unroll
-        for (int k = 0; k < NT; k++)
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) mf[ks][k] = q[((k * 4 + rb) * KS + ks) * 64 + lane];
-    };
-    auto head = [&](const uint8_t* p) { return p + (size_t)d.hk * L::kKeyBytes + (size_t)h * kHeadBytes; };
-    auto load_tri = [&](const uint8_t* p) {         // T's or P's
-        const u32x4* q = (const u32x4*)(head(p) + (ahead ? 0 : kTriBytes));
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++)
-#pragma unroll
-            for (int k = 0; k < 3; k++) tf[ks][k] = q[((step0 + (ks < (int)steps ? ks : 0)) * 3 + k) * 64 + lane];
-    };
-    auto load_kt = [&](const uint8_t* p) {
-        const u32x4* q = (const u32x4*)(p + (size_t)kh * L::kKeyBytes + 2 * L::kOp);
-#pragma unroll
-        for (int x = 0; x < NS; x++)
-#pragma unroll
-            for (int ts = 0; ts < 2; ts++)
-#pragma unroll
-                for (int k = 0; k < NT; k++)
-                    if (wave * NS + x < DKP / 16) kt[x][ts][k] = q[((k * (DKP / 16) + wave * NS + x) * 2 + ts) * 64 + lane];
-    };
-    auto load_v = [&](uint32_t t0) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t t = t0 + 16 * rb + 4 * g + i;
-            v[i] = t < s.to && col_in ? load_elem<DT>(d.v, (size_t)t * d.v_stride + (size_t)h * d.dv + col) : 0.f;
-        }
-    };
-    auto put = [&](uint16_t* to, uint32_t plane, const f32x4& x) {   // four rows of a column, in terms
-        uint32_t w0[3], w1[3];
-        terms<3>(x[0], x[1], w0);
-        terms<3>(x[2], x[3], w1);
-#pragma unroll
-        for (int k = 0; k < 3; k++) *(uint2*)(to + k * plane) = make_uint2(w0[k], w1[k]);
-    };
-    auto put_state = [&]() {
-#pragma unroll
-        for (int x = 0; x < NS; x++)
-            if (wave * NS + x < DKP / 16) put(&Sb[0][r][16 * (wave * NS + x) + 4 * g], 16 * PITCH, S[x]);
-    };
-    auto times_state = [&]() {
-        f32x4 c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            u32x4 b[3];
-#pragma unroll
-            for (int k = 0; k < 3; k++) b[k] = *(const u32x4*)&Sb[k][r][32 * ks + 8 * g];
-            c = mfma_terms(mf[ks], b, c);
-        }
-        return c;
-    };
-    auto triangle = [&](const uint16_t (*B)[16][TP], f32x4 c) {
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++) {
-            if (ks >= (int)steps) break;
-            u32x4 b[3];
-#pragma unroll
-            for (int k = 0; k < 3; k++) b[k] = *(const u32x4*)&B[k][r][32 * ks + 8 * g];
-            c = mfma_terms(tf[ks], b, c);
-        }
-        return c;
-    };
-    load_rows(base);
-    if (ahead) { load_tri(base); load_v(s.from + begin * kChunk); }
-    load_kt(base);
-    put_state();
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t c = begin; c < end; c++) {
-        const uint8_t* p = base + (size_t)(c - begin) * slot_bytes;
-        const uint8_t* next = c + 1 < end ? p + slot_bytes : p;
-        const float* sc = (const float*)(head(p) + 2 * kTriBytes);
-        auto give_y = [&](uint32_t chunk) {       // P U of a chunk onto its Q S0
-            y = triangle(Ub, y);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t t = s.from + chunk * kChunk + 16 * rb + 4 * g + i;
-                if (t < s.to && col_in) d.y[((size_t)t * d.hv + h) * d.dv + col] = y[i];
-            }
-        };
-        __syncthreads();
-        if (ahead) {
-            const f32x4 e = *(const f32x4*)(sc + 16 * rb + 4 * g), ks0 = times_state();
-            f32x4 x;
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = v[i] - e[i] * ks0[i];
-            put(&Xb[0][r][16 * rb + 4 * g], 16 * TP, x);
-            load_rows(next);
-            load_v(s.from + (c + 1) * kChunk);
-        } else {
-            if (c > begin) give_y(c - 1);
-            load_tri(p);
-        }
-        __syncthreads();
-        if (ahead) {
-            const f32x4 w = *(const f32x4*)(sc + 128 + 16 * rb + 4 * g);
-            const f32x4 u = triangle(Xb, f32x4{0.f, 0.f, 0.f, 0.f});
-            put(&Ub[0][r][16 * rb + 4 * g], 16 * TP, u);
-            put(&Wb[0][r][16 * rb + 4 * g], 16 * TP, u * w);
-            load_tri(next);
-        } else {
-            const f32x4 e = *(const f32x4*)(sc + 64 + 16 * rb + 4 * g);
-            y = times_state() * e;
-            load_rows(next);
-        }
-        __syncthreads();
-        const float keep = sc[192];
-#pragma unroll
-        for (int x = 0; x < NS; x++) {
-            if (wave * NS + x >= DKP / 16) break;
-            S[x] *= keep;
-#pragma unroll
-            for (int ts = 0; ts < 2; ts++) {
-                u32x4 b[3];
-#pragma unroll
-                for (int k = 0; k < 3; k++) b[k] = *(const u32x4*)&Wb[k][r][32 * ts + 8 * g];
-                S[x] = mfma_terms(kt[x][ts], b, S[x]);
-            }
-        }
-        load_kt(next);
-        put_state();
-        if (c + 1 == end && !ahead) give_y(c);
-    }
-    if (col_in)
-#pragma unroll
-        for (int x = 0; x < NS; x++) {
-            const uint32_t row = 16 * (wave * NS + x) + 4 * g;
-            if (wave * NS + x < DKP / 16)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (row + i < d.dk) d.state_out[state + row + i] = S[x][i];
-        }
+    WalkPlace w;
+    w.begin = a.lo > first ? a.lo - first : 0;
+    w.end = a.hi <= first ? 0 : a.hi - first < chunks ? a.hi - first : chunks;
+    if (w.begin >= w.end) return;
+    w.slot_bytes = L::slot_bytes(d.hk, d.hv);
+    w.base = a.scratch + (size_t)(first + w.begin - a.lo) * w.slot_bytes;
+    w.from = s.from;
+    w.to = s.to;
+    w.h = h;
+    w.kh = h / (d.hv / d.hk);
+    w.c0 = c0;
+    w.state = ((size_t)s.slot * d.hv + h) * d.dv * d.dk;
+    w.state_from = w.begin ? d.state_out : d.state_in;
+    if (wave < 4 / NB) walk<DT, DKP, NT, NB, true>(d, w, lds, wave);
+    else if (wave < 8 / NB) walk<DT, DKP, NT, NB, false>(d, w, lds, wave);
+    else walk_touch<DT, DKP, NT>(d, w, lds, columns);
 }
 
 template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* scratch, size_t bytes, const LaunchCtx& lc) {
@@ -507,6 +672,7 @@ template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* s
     uint32_t pairs = d.n_seqs * d.hv, columns = (d.dv + 15) / 16;
     const uint64_t grid = (uint64_t)((pairs + 7) / 8) * 8 * columns;
     if (grid > 0x7FFFFFFFull || (uint64_t)total * d.hk > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more chunks or columns than a launch can have workgroups");
+    constexpr int NB = 1;
     constexpr size_t lds = L::kOp + 3 * kChunk * kPitch * 4 + kChunk * 8 + 3 * kChunk * 4;
     const void* chunk = (const void*)delta_chunk_kernel<DT, DKP, NT>;
     MTQ_HIP(set_max_dynamic_lds(chunk, lds));
@@ -520,7 +686,7 @@ template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* s
         if (a.hi < total) second.stop = nullptr;
         void* args[] = {&a, &pairs, &columns};
         MTQ_HIP(launch_kernel(chunk, dim3((a.hi - lo) * d.hk), dim3(256), args, lds, first));
-        MTQ_HIP(launch_kernel((const void*)delta_walk_kernel<DT, DKP, NT>, dim3((uint32_t)grid), dim3(512), args, 0, second));
+        MTQ_HIP(launch_kernel((const void*)delta_walk_kernel<DT, DKP, NT, NB>, dim3((uint32_t)grid), dim3(64 * (8 / NB + 1)), args, 0, second));
     }
     return ERR_OK;
 }
@@ -538,7 +704,9 @@ size_t slot_bytes_of(const DeltaArgs& d) {
 
 // Chunks pay where a sequence may be long: with as many tokens beyond one for each sequence as this. (Sequences of up to kFewTokens go token
 // by token here too.)
+// The walk reads a chunk's rows of v and a slot by 31-bit offsets.
 bool delta_chunks_serve(const DeltaArgs& d) {
+    if (d.v_stride > (1u << 22) || slot_bytes_of(d) >= ((size_t)1 << 31)) return false;
     return d.offsets ? d.n_tokens > d.n_seqs && d.n_tokens - d.n_seqs >= 2 * kFewTokens : d.n_tokens / d.n_seqs >= 2 * kFewTokens;
 }
 
