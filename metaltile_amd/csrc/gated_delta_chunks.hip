@@ -63,16 +63,16 @@ template <int NA, int NB> __device__ __forceinline__ f32x4 mfma_terms(const u32x
     return c;
 }
 
-// Two such sums over the same b, side by side.
-template <int NA, int NB> __device__ __forceinline__ void mfma_terms2(const u32x4 (&a0)[NA], const u32x4 (&a1)[NA], const u32x4 (&b)[NB], f32x4& c0, f32x4& c1) {
+// The same onto several sums in turn, so that an instruction does not wait for the one before: sum number `at`, at + 1, .. of N.
+template <int NA, int NB, int N> __device__ __forceinline__ void mfma_terms_on(const u32x4 (&a)[NA], const u32x4 (&b)[NB], f32x4 (&c)[N], int at) {
     constexpr int MOST = 3;
 #pragma unroll
     for (int s = MOST - 1; s >= 0; s--)
 #pragma unroll
         for (int i = 0; i < NA; i++)
             if (s - i >= 0 && s - i < NB) {
-                c0 = mfma_bf16(a0[i], b[s - i], c0);
-                c1 = mfma_bf16(a1[i], b[s - i], c1);
+                c[at % N] = mfma_bf16(a[i], b[s - i], c[at % N]);
+                at++;
             }
 }
 
@@ -465,9 +465,7 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
     // `load` is what is asked for once the LDS reads are on their way.
     auto times_state = [&](f32x4 (&c)[NB], auto&& load) {
         constexpr int AT_ONCE = KS < 4 ? KS : 4;
-        f32x4 odd[NB] = {};
-#pragma unroll
-        for (int b = 0; b < NB; b++) c[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 part[NB][4 / NB] = {};
 #pragma unroll
         for (int k0 = 0; k0 < KS; k0 += AT_ONCE) {
             u32x4 b[AT_ONCE][3];
@@ -479,13 +477,12 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
             if (k0 == 0) load();
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int ks = 0; ks < AT_ONCE; ks++) {
-                if constexpr (NB == 2) mfma_terms2(mf[0][k0 + ks], mf[1][k0 + ks], b[ks], c[0], c[1]);
-                else if (ks & 1) odd[0] = mfma_terms(mf[0][k0 + ks], b[ks], odd[0]);
-                else c[0] = mfma_terms(mf[0][k0 + ks], b[ks], c[0]);
-            }
+            for (int ks = 0; ks < AT_ONCE; ks++)
+#pragma unroll
+                for (int x = 0; x < NB; x++) mfma_terms_on(mf[x][k0 + ks], b[ks], part[x], 0);
         }
-        if constexpr (NB == 1) c[0] += odd[0];
+#pragma unroll
+        for (int x = 0; x < NB; x++) c[x] = NB == 2 ? part[x][0] + part[x][1] : (part[x][0] + part[x][1]) + (part[x][2 / NB] + part[x][3 / NB]);
     };
     auto triangle = [&](Columns<kChunk>* B, f32x4 (&c)[NB], auto&& load) {
         u32x4 b[2][3];
@@ -496,20 +493,27 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
         __builtin_amdgcn_sched_barrier(0);
         load();
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (NB == 2) mfma_terms2(tf[0], tf[1], b[0], c[0], c[1]);
-        else c[0] = mfma_terms(tf[0], b[0], c[0]);
-        if (long_row) c[NB - 1] = mfma_terms(tf[NB], b[1], c[NB - 1]);
+        f32x4 part[NB][3] = {};
+#pragma unroll
+        for (int x = 0; x < NB; x++) {
+            part[x][0] = c[x];
+            mfma_terms_on(tf[x], b[0], part[x], 0);
+        }
+        if (long_row) mfma_terms_on(tf[NB], b[1], part[NB - 1], 0);
+#pragma unroll
+        for (int x = 0; x < NB; x++) c[x] = part[x][0] + part[x][1] + part[x][2];
     };
     f32x4 y[NB] = {};
+    const uint32_t y_at = (4 * g * d.hv * d.dv + w.h * d.dv + col) * 4;
     auto give_y = [&](uint32_t chunk, auto&& load) {  // P U of a chunk onto its Q S0
         triangle(lds.U, y, load);
+        const uint32_t t0 = w.from + chunk * kChunk, n = w.to - t0 < kChunk ? w.to - t0 : kChunk, row = d.hv * d.dv * 4;
+        const __amdgpu_buffer_rsrc_t s = kr_rsrc((uint64_t)(uintptr_t)d.y + (uint64_t)t0 * row, n * row);   // (rows behind the sequence are not written)
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t t = w.from + chunk * kChunk + 16 * rb[b] + 4 * g + i;
-                if (t < w.to && col_in) d.y[((size_t)t * d.hv + w.h) * d.dv + col] = y[b][i];
-            }
+            for (int i = 0; i < 4; i++)
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[b][i]), s, col_in ? y_at + (16 * rb[b] + i) * row : KR_OOB, 0, 0);
     };
     auto nothing = [] {};
     {
@@ -518,6 +522,7 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
         if (AHEAD) { load_tri(s); load_v(w.begin); }
     }
     put_state();
+    if (AHEAD) __builtin_amdgcn_s_setprio(3);
     for (uint32_t c = w.begin; c < w.end; c++) {
         const auto here = slot(c), next = slot(c + 1 < w.end ? c + 1 : c);
         walk_barrier();
@@ -537,6 +542,7 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
             load_kt(here);
         }
         walk_barrier();
+        f32x4 late[NB];
         if constexpr (AHEAD) {
             f32x4 u[NB] = {}, uw[NB];
             triangle(lds.X, u, [&] { load_rows(next); load_v(c + 1); });
@@ -545,7 +551,7 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
                 uw[b] = u[b] * wk[b];
                 asm volatile("" : "+v"(uw[b]));
                 put(lds.W[0].at(r, 16 * rb[b] + 4 * g), Columns<kChunk>::PLANE, uw[b]);
-                put(lds.U[0].at(r, 16 * rb[b] + 4 * g), Columns<kChunk>::PLANE, u[b]);
+                late[b] = u[b];   // (U itself is asked for from the next chunk on: it is put beside the state's update)
             }
         } else {
             times_state(y, [&] { load_tri(here); });
@@ -562,22 +568,26 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
 #pragma unroll
             for (int k = 0; k < 3; k++) b[ts][k] = *(const u32x4*)lds.W[k].at(r, 32 * ts + 8 * g);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (AHEAD) load_tri(next);
-        else load_rows(next);
+        if constexpr (AHEAD) {
+            load_tri(next);
+#pragma unroll
+            for (int x = 0; x < NB; x++) put(lds.U[0].at(r, 16 * rb[x] + 4 * g), Columns<kChunk>::PLANE, late[x]);
+        } else {
+            load_rows(next);
+        }
         __builtin_amdgcn_sched_barrier(0);
         if (has_state) {
 #pragma unroll
-            for (int x = 0; x < NS; x++) S[x] *= keep;
+            for (int x = 0; x < NS; x++) {
+                f32x4 part[2] = {S[x] * keep, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-            for (int ts = 0; ts < 2; ts++)
-#pragma unroll
-                for (int x = 0; x < NS; x += 2) {
-                    if constexpr (NS == 1) S[x] = mfma_terms(kt[x][ts], b[ts], S[x]);
-                    else mfma_terms2(kt[x][ts], kt[x + 1 < NS ? x + 1 : x][ts], b[ts], S[x], S[x + 1 < NS ? x + 1 : x]);
-                }
+                for (int ts = 0; ts < 2; ts++) mfma_terms_on(kt[x][ts], b[ts], part, ts);
+                S[x] = part[0] + part[1];
+            }
         }
         put_state();
     }
+    walk_barrier();   // (the last chunk's U)
     if constexpr (!AHEAD) give_y(w.end - 1, nothing);
     if (col_in && has_state)
 #pragma unroll
@@ -622,6 +632,7 @@ template <int DT, int DKP, int NT> __device__ __forceinline__ void walk_touch(co
         walk_barrier();
         walk_barrier();
     }
+    walk_barrier();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
