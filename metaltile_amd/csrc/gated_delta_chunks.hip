@@ -135,18 +135,24 @@ __device__ __forceinline__ void block_store(float* D, f32x4 v, float sign) {
 
 // ---- what does not depend on the state
 
-template <int DT, int DKP, int NT> __global__ __launch_bounds__(256) void delta_chunk_kernel(ChunkArgs a) {
+// LDS: K's terms while products of q and k are made, then two 64 x 64 matrices in their place; what belongs to rows behind them.
+template <int DKP, int NT> struct ChunkLds {
+    static constexpr uint32_t kMatrix = kChunk * kPitch * 4, kRows = Layout<DKP, NT>::kOp > 2 * kMatrix ? Layout<DKP, NT>::kOp : 2 * kMatrix;
+    static constexpr uint32_t kBytes = kRows + 4 * kChunk * 12 + 2 * kChunk * 4;
+};
+
+template <int DT, int DKP, int NT> __global__ __launch_bounds__(256, DKP * NT <= 256 ? 4 : 2) void delta_chunk_kernel(ChunkArgs a) {
     using L = Layout<DKP, NT>;
+    using C = ChunkLds<DKP, NT>;
     constexpr int KS = DKP / 32;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     u32x4* kop = (u32x4*)lds;                                   // [NT][4][KS][64]
-    float* Am = (float*)(lds + L::kOp);                          // [64][kPitch]
-    float* Tm = Am + kChunk * kPitch;
-    float* Mm = Tm + kChunk * kPitch;                            // P, then products on the way to T
-    double* sums = (double*)(Mm + kChunk * kPitch);              // [64]
-    float* rk = (float*)(sums + kChunk);                         // [64]
+    float* Am = (float*)lds;                                     // [64][kPitch]: A, and block by block T in its place
+    float* Mm = Am + kChunk * kPitch;                            // P, then products on the way to T
+    double* sums = (double*)(lds + C::kRows);                    // [4][64]: of four heads
+    float* bt = (float*)(sums + 4 * kChunk);                     // [4][64]
+    float* rk = bt + 4 * kChunk;                                 // [64]
     float* rq = rk + kChunk;
-    float* bt = rq + kChunk;
     const DeltaArgs& d = a.d;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
     const uint32_t slot = a.lo + blockIdx.x / d.hk, kh = blockIdx.x % d.hk;
@@ -228,11 +234,13 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256) void delta_
     for (uint32_t x = 0; x < group; x++) {
         const uint32_t h = kh * group + x;
         uint8_t* head_out = out + (size_t)d.hk * L::kKeyBytes + (size_t)h * kHeadBytes;
-        if (wave == 0) {
+        __syncthreads();   // (K's terms, and the head before: no longer read)
+        if (x % 4 == 0 && x + wave < group) {   // four heads' decays and betas, one to a wave
+            const uint32_t hx = h + wave;
             float gt = 0.f, beta = 0.f;
             if (lane < n) {
-                gt = d.g[(size_t)(t0 + lane) * d.hv + h];
-                beta = d.beta[(size_t)(t0 + lane) * d.hv + h];
+                gt = d.g[(size_t)(t0 + lane) * d.hv + hx];
+                beta = d.beta[(size_t)(t0 + lane) * d.hv + hx];
             }
             // (e^-100000 is 0, and a sum with -inf would have no differences)
             double sum = gt < -1e5f ? -1e5 : (double)gt;
@@ -240,34 +248,35 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256) void delta_
                 const double up = __shfl_up(sum, o, 64);
                 if ((int)lane >= o) sum += up;
             }
-            sums[lane] = sum;
-            bt[lane] = beta;
+            sums[wave * 64 + lane] = sum;
+            bt[wave * 64 + lane] = beta;
             const double last = __shfl(sum, 63, 64);
-            float* sc = (float*)(head_out + 2 * kTriBytes);
+            float* sc = (float*)(head_out + (size_t)wave * kHeadBytes + 2 * kTriBytes);
             const float e = expf((float)sum);
             sc[lane] = e * rk[lane];
             sc[64 + lane] = e * rq[lane];
             sc[128 + lane] = rk[lane] * expf((float)(last - sum));
             sc[192 + lane] = expf((float)last);
         }
-        __syncthreads();
+        if (x % 4 == 0) __syncthreads();
+        const double* sm = sums + x % 4 * 64;
+        const float* bx = bt + x % 4 * 64;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const uint32_t col = 16 * j + r;
-            const double cs = sums[col];
+            const double cs = sm[col];
             const float rs = rk[col];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const uint32_t row = 16 * wave + 4 * g + i;
                 float av = 0.f, pv = 0.f;
                 if (j <= (int)wave && col <= row) {
-                    const float f = rs * expf((float)(sums[row] - cs));
+                    const float f = rs * expf((float)(sm[row] - cs));
                     pv = rq[row] * f * H[j][i];
-                    if (col < row) av = bt[row] * rk[row] * f * G[j][i];
+                    if (col < row) av = bx[row] * rk[row] * f * G[j][i];
                 }
                 Am[row * kPitch + col] = av;
                 Mm[row * kPitch + col] = pv;
-                Tm[row * kPitch + col] = 0.f;
             }
         }
         __syncthreads();
@@ -280,7 +289,7 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256) void delta_
                 v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
                 if (by_beta)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] *= bt[c + e];
+                    for (int e = 0; e < 8; e++) v[e] *= bx[c + e];
                 u32x4 w[3];
                 terms8<3>(v, w);
 #pragma unroll
@@ -289,7 +298,7 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256) void delta_
         };
         put(Mm, head_out + kTriBytes, false);
         {   // the block on the diagonal: each lane a column of its inverse (four lanes the same one), row by row
-            const float* D = Am + 16 * wave * (kPitch + 1);
+            float* D = Am + 16 * wave * (kPitch + 1);
             float v[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
@@ -298,32 +307,32 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256) void delta_
                 for (int k = 0; k < i; k++) sum -= D[i * kPitch + k] * v[k];
                 v[i] = sum;
             }
-            float* to = Tm + 16 * wave * (kPitch + 1);
             if (g == 0)
 #pragma unroll
-                for (int i = 0; i < 16; i++) to[i * kPitch + r] = v[i];
+                for (int i = 0; i < 16; i++) D[i * kPitch + r] = v[i];
         }
         __syncthreads();
         auto at = [&](float* M, int i, int j) { return M + 16 * (i * kPitch + j); };
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
         // pairs of blocks: (1, 0) by wave 0, (3, 2) by wave 2
         const int b = (int)wave;
-        if ((b & 1) == 0) block_store(at(Mm, b + 1, b), block_product(at(Am, b + 1, b), at(Tm, b, b), zero), 1.f);
-        __syncthreads();
-        if ((b & 1) == 0) block_store(at(Tm, b + 1, b), block_product(at(Tm, b + 1, b + 1), at(Mm, b + 1, b), zero), -1.f);
+        if ((b & 1) == 0) {
+            block_store(at(Mm, b + 1, b), block_product(at(Am, b + 1, b), at(Am, b, b), zero), 1.f);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            block_store(at(Am, b + 1, b), block_product(at(Am, b + 1, b + 1), at(Mm, b + 1, b), zero), -1.f);
+        }
         __syncthreads();
         // the lower left quarter: wave 2 i + j its block (2 + i, j)
         const int i = b >> 1, j = b & 1;
-        f32x4 m = block_product(at(Am, 2 + i, 1), at(Tm, 1, j), zero);   // (T's block (0, 1) is zero)
-        m = block_product(at(Am, 2 + i, 0), at(Tm, 0, j), m);
+        f32x4 m = block_product(at(Am, 2 + i, 1), at(Am, 1, j), zero);   // (block (0, 1) is zero)
+        m = block_product(at(Am, 2 + i, 0), at(Am, 0, j), m);
         block_store(at(Mm, 2 + i, j), m, 1.f);
         __syncthreads();
-        m = block_product(at(Tm, 2 + i, 2), at(Mm, 2, j), zero);
-        if (i) m = block_product(at(Tm, 3, 3), at(Mm, 3, j), m);
-        block_store(at(Tm, 2 + i, j), m, -1.f);
+        m = block_product(at(Am, 2 + i, 2), at(Mm, 2, j), zero);
+        if (i) m = block_product(at(Am, 3, 3), at(Mm, 3, j), m);
+        block_store(at(Am, 2 + i, j), m, -1.f);
         __syncthreads();
-        put(Tm, head_out, true);
-        __syncthreads();
+        put(Am, head_out, true);
     }
 }
 
@@ -636,7 +645,7 @@ template <int DT, int DKP, int NT> __device__ __forceinline__ void walk_touch(co
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <int DT, int DKP, int NT, int NB> __global__ __launch_bounds__(64 * (8 / NB + 1)) void delta_walk_kernel(ChunkArgs a, uint32_t pairs, uint32_t columns) {
+template <int DT, int DKP, int NT, int NB, bool TOUCH, int PER_SIMD> __global__ __launch_bounds__(64 * (8 / NB + TOUCH), PER_SIMD) void delta_walk_kernel(ChunkArgs a, uint32_t pairs, uint32_t columns) {
     using L = Layout<DKP, NT>;
     __shared__ __attribute__((aligned(16))) WalkLds<DKP> lds;
     const DeltaArgs& d = a.d;
@@ -670,7 +679,7 @@ template <int DT, int DKP, int NT, int NB> __global__ __launch_bounds__(64 * (8 
     w.state_from = w.begin ? d.state_out : d.state_in;
     if (wave < 4 / NB) walk<DT, DKP, NT, NB, true>(d, w, lds, wave);
     else if (wave < 8 / NB) walk<DT, DKP, NT, NB, false>(d, w, lds, wave);
-    else walk_touch<DT, DKP, NT>(d, w, lds, columns);
+    else if constexpr (TOUCH) walk_touch<DT, DKP, NT>(d, w, lds, columns);
 }
 
 template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* scratch, size_t bytes, const LaunchCtx& lc) {
@@ -683,8 +692,17 @@ template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* s
     uint32_t pairs = d.n_seqs * d.hv, columns = (d.dv + 15) / 16;
     const uint64_t grid = (uint64_t)((pairs + 7) / 8) * 8 * columns;
     if (grid > 0x7FFFFFFFull || (uint64_t)total * d.hk > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more chunks or columns than a launch can have workgroups");
-    constexpr int NB = 1;
-    constexpr size_t lds = L::kOp + 3 * kChunk * kPitch * 4 + kChunk * 8 + 3 * kChunk * 4;
+    // A wave more makes three on one of the four SIMDs, 168 registers each: rows of 384 terms and more need up to 256, and go without. Two
+    // workgroups to a compute unit need 128: rows of 64 bf16 or f16 values do with them, and where there are more workgroups than compute units
+    // that gives more than the lines brought early (nine prompts of 1 to 1024 tokens, f16: 72 -> 59 us). Four prompts of 2048 tokens, dk 128: bf16
+    // 317 us with the wave, 361 without; f16 447, 532; f32 978 (its registers do not fit), 625.
+    constexpr bool wide = DKP * NT >= 384, narrow = DKP == 64 && NT <= 2;
+    const bool touch = !wide && !(narrow && grid > 256);
+    const void* fn;
+    if constexpr (wide) fn = (const void*)delta_walk_kernel<DT, DKP, NT, 1, false, 2>;
+    else if constexpr (narrow) fn = touch ? (const void*)delta_walk_kernel<DT, DKP, NT, 1, true, 1> : (const void*)delta_walk_kernel<DT, DKP, NT, 1, false, 4>;
+    else fn = (const void*)delta_walk_kernel<DT, DKP, NT, 1, true, 1>;
+    constexpr size_t lds = ChunkLds<DKP, NT>::kBytes;
     const void* chunk = (const void*)delta_chunk_kernel<DT, DKP, NT>;
     MTQ_HIP(set_max_dynamic_lds(chunk, lds));
     for (uint32_t lo = 0; lo < total; lo += at_once) {
@@ -697,7 +715,7 @@ template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* s
         if (a.hi < total) second.stop = nullptr;
         void* args[] = {&a, &pairs, &columns};
         MTQ_HIP(launch_kernel(chunk, dim3((a.hi - lo) * d.hk), dim3(256), args, lds, first));
-        MTQ_HIP(launch_kernel((const void*)delta_walk_kernel<DT, DKP, NT, NB>, dim3((uint32_t)grid), dim3(64 * (8 / NB + 1)), args, 0, second));
+        MTQ_HIP(launch_kernel(fn, dim3((uint32_t)grid), dim3(64 * (8 + touch)), args, 0, second));
     }
     return ERR_OK;
 }
