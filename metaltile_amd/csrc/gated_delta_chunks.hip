@@ -40,6 +40,7 @@ struct ChunkArgs {
     uint8_t* scratch;
     uint32_t lo, hi;        // this launch's slots for chunks: sequence i's chunk c has slot from_i / 64 + i + c
     uint32_t whole;         // rows of q and k on 16 bytes
+    uint32_t parts;         // workgroups of the first launch for a chunk and key head
 };
 
 template <int DKP, int NT> struct Layout {
@@ -108,13 +109,26 @@ template <int DT> __device__ __forceinline__ void load8(const void* p, size_t i,
 // The sequence that a slot belongs to: the last whose first slot is not behind it.
 __device__ __forceinline__ uint32_t first_slot(const DeltaSeq& s, uint32_t seq) { return s.from / kChunk + seq; }
 __device__ __forceinline__ uint32_t seq_of(const DeltaArgs& a, uint32_t slot) {
-    uint32_t lo = 0, hi = a.n_seqs;
-    while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (first_slot(delta_seq(a, mid), mid) <= slot) lo = mid;
-        else hi = mid;
+    if (!a.offsets) {   // (equal lengths: no memory to be read)
+        uint32_t lo = 0, hi = a.n_seqs;
+        const uint32_t each = a.n_tokens / a.n_seqs;
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (mid * each / kChunk + mid <= slot) lo = mid;
+            else hi = mid;
+        }
+        return lo;
     }
-    return lo;
+    // 64 sequences at a time, so that a few reads of memory after one another find it: those whose first slot is not behind it come first
+    uint32_t lo = 0, step = 1;
+    while (step * 64 < a.n_seqs) step *= 64;
+    for (;; step /= 64) {
+        const uint32_t i = lo + (threadIdx.x & 63u) * step;
+        const bool before = i < a.n_seqs && min(a.offsets[i < a.n_seqs ? i : 0], a.n_tokens) / kChunk + i <= slot;
+        const uint32_t n = (uint32_t)__popcll(__ballot(before));
+        if (n) lo += (n - 1) * step;
+        if (step == 1) return lo;
+    }
 }
 
 constexpr int kPitch = 68;   // f32 of a row of a 64 x 64 matrix in LDS (rows on 16 bytes, in different banks)
@@ -154,8 +168,8 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256, DKP * NT <=
     float* rk = bt + 4 * kChunk;                                 // [64]
     float* rq = rk + kChunk;
     const DeltaArgs& d = a.d;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = lane & 15u, g = lane >> 4;
-    const uint32_t slot = a.lo + blockIdx.x / d.hk, kh = blockIdx.x % d.hk;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15u, g = lane >> 4;
+    const uint32_t units = d.hk * a.parts, slot = a.lo + blockIdx.x / units, kh = blockIdx.x % units / a.parts, part = blockIdx.x % a.parts;
     const uint32_t seq = seq_of(d, slot);
     const DeltaSeq s = delta_seq(d, seq);
     const uint32_t first = first_slot(s, seq);
@@ -164,6 +178,17 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256, DKP * NT <=
     uint8_t* out = a.scratch + (size_t)(slot - a.lo) * L::slot_bytes(d.hk, d.hv);
     uint8_t* key_out = out + (size_t)kh * L::kKeyBytes;
     const uint32_t t = 16 * wave + r;                            // this lane's row of K and Q
+    // its value heads: all that share the key head, or one of them
+    const uint32_t all = d.hv / d.hk, group = a.parts > 1 ? part + 1 : all, x0 = a.parts > 1 ? part : 0;
+    float gt = 0.f, beta = 0.f;                                  // of a token of one of the first four heads
+    auto load_decay = [&](uint32_t x) {
+        gt = beta = 0.f;
+        if (lane < n && x + wave < group) {
+            gt = d.g[(size_t)(t0 + lane) * d.hv + kh * all + x + wave];
+            beta = d.beta[(size_t)(t0 + lane) * d.hv + kh * all + x + wave];
+        }
+    };
+    load_decay(x0);
     u32x4 kf[KS][NT], qf[KS][NT];
     float kk = 0.f, qq = 0.f;
 #pragma unroll
@@ -195,12 +220,14 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256, DKP * NT <=
         for (int ks = 0; ks < KS; ks++) {
             const uint32_t at = ((p * 4 + wave) * KS + ks) * 64 + lane;
             kop[at] = kf[ks][p];
-            ((u32x4*)key_out)[at] = kf[ks][p];
-            ((u32x4*)(key_out + L::kOp))[at] = qf[ks][p];
+            if (part == 0) {
+                ((u32x4*)key_out)[at] = kf[ks][p];
+                ((u32x4*)(key_out + L::kOp))[at] = qf[ks][p];
+            }
         }
     __syncthreads();
     // K^T: row d of 16 dt + r, tokens 32 ts + 8 g + e
-    for (uint32_t u = wave; u < NT * (DKP / 16) * 2; u += 4) {
+    for (uint32_t u = part ? NT * (DKP / 16) * 2 : wave; u < NT * (DKP / 16) * 2; u += 4) {
         const uint32_t p = u / ((DKP / 16) * 2), dt = u / 2 % (DKP / 16), ts = u & 1u, dd = 16 * dt + r;
         const uint16_t* from = (const uint16_t*)kop + (size_t)p * kChunk * DKP + ((dd >> 5) * 64 + ((dd >> 3) & 3u) * 16) * 8 + (dd & 7u);
         u32x4 v;
@@ -220,7 +247,7 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256, DKP * NT <=
     f32x4 G[4] = {}, H[4] = {};
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        if (j > (int)wave) break;
+        if (j <= (int)wave)
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
             u32x4 b[NT];
@@ -230,18 +257,12 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256, DKP * NT <=
             H[j] = mfma_terms(qf[ks], b, H[j]);
         }
     }
-    const uint32_t group = d.hv / d.hk;
-    for (uint32_t x = 0; x < group; x++) {
-        const uint32_t h = kh * group + x;
+    for (uint32_t x = x0; x < group; x++) {
+        const uint32_t h = kh * all + x, of = (x - x0) % 4;
         uint8_t* head_out = out + (size_t)d.hk * L::kKeyBytes + (size_t)h * kHeadBytes;
         __syncthreads();   // (K's terms, and the head before: no longer read)
-        if (x % 4 == 0 && x + wave < group) {   // four heads' decays and betas, one to a wave
-            const uint32_t hx = h + wave;
-            float gt = 0.f, beta = 0.f;
-            if (lane < n) {
-                gt = d.g[(size_t)(t0 + lane) * d.hv + hx];
-                beta = d.beta[(size_t)(t0 + lane) * d.hv + hx];
-            }
+        if (of == 0 && x + wave < group) {   // four heads' decays and betas, one to a wave
+            if (x != x0) load_decay(x);
             // (e^-100000 is 0, and a sum with -inf would have no differences)
             double sum = gt < -1e5f ? -1e5 : (double)gt;
             for (int o = 1; o < 64; o <<= 1) {
@@ -252,28 +273,43 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256, DKP * NT <=
             bt[wave * 64 + lane] = beta;
             const double last = __shfl(sum, 63, 64);
             float* sc = (float*)(head_out + (size_t)wave * kHeadBytes + 2 * kTriBytes);
-            const float e = expf((float)sum);
+            const float e = __expf((float)sum);
             sc[lane] = e * rk[lane];
             sc[64 + lane] = e * rq[lane];
-            sc[128 + lane] = rk[lane] * expf((float)(last - sum));
-            sc[192 + lane] = expf((float)last);
+            sc[128 + lane] = rk[lane] * __expf((float)(last - sum));
+            sc[192 + lane] = __expf((float)last);
         }
-        if (x % 4 == 0) __syncthreads();
-        const double* sm = sums + x % 4 * 64;
-        const float* bx = bt + x % 4 * 64;
+        if (of == 0) __syncthreads();
+        const double* sm = sums + of * 64;
+        const float* bx = bt + of * 64;
+        double rs64[4];
+        float rbeta[4], rqs[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t row = 16 * wave + 4 * g + i;
+            rs64[i] = sm[row];
+            rbeta[i] = bx[row] * rk[row];
+            rqs[i] = rq[row];
+        }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const uint32_t col = 16 * j + r;
+            if (j > (int)wave) {   // (of the blocks above the diagonal (0, 1) and (2, 3) are read)
+                if (j == (int)(wave ^ 1u))
+#pragma unroll
+                    for (int i = 0; i < 4; i++) Am[(16 * wave + 4 * g + i) * kPitch + col] = Mm[(16 * wave + 4 * g + i) * kPitch + col] = 0.f;
+                continue;
+            }
             const double cs = sm[col];
             const float rs = rk[col];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const uint32_t row = 16 * wave + 4 * g + i;
-                float av = 0.f, pv = 0.f;
-                if (j <= (int)wave && col <= row) {
-                    const float f = rs * expf((float)(sm[row] - cs));
-                    pv = rq[row] * f * H[j][i];
-                    if (col < row) av = bx[row] * rk[row] * f * G[j][i];
+                const float f = rs * __expf((float)(rs64[i] - cs));   // (off by 2^-24 times its exponent: at most 2^-25 of 1)
+                float pv = rqs[i] * f * H[j][i], av = rbeta[i] * f * G[j][i];
+                if (j == (int)wave) {
+                    if (col > row) pv = 0.f;
+                    if (col >= row) av = 0.f;
                 }
                 Am[row * kPitch + col] = av;
                 Mm[row * kPitch + col] = pv;
@@ -691,7 +727,7 @@ template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* s
     const uint32_t total = d.n_tokens / kChunk + d.n_seqs, at_once = (uint32_t)(bytes / L::slot_bytes(d.hk, d.hv));
     uint32_t pairs = d.n_seqs * d.hv, columns = (d.dv + 15) / 16;
     const uint64_t grid = (uint64_t)((pairs + 7) / 8) * 8 * columns;
-    if (grid > 0x7FFFFFFFull || (uint64_t)total * d.hk > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more chunks or columns than a launch can have workgroups");
+    if (grid > 0x7FFFFFFFull || (uint64_t)total * d.hv > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more chunks or columns than a launch can have workgroups");
     // A wave more makes three on one of the four SIMDs, 168 registers each: rows of 384 terms and more need up to 256, and go without. Two
     // workgroups to a compute unit need 128: rows of 64 bf16 or f16 values do with them, and where there are more workgroups than compute units
     // that gives more than the lines brought early (nine prompts of 1 to 1024 tokens, f16: 72 -> 59 us). Four prompts of 2048 tokens, dk 128: bf16
@@ -714,7 +750,9 @@ template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* s
         second.start = nullptr;
         if (a.hi < total) second.stop = nullptr;
         void* args[] = {&a, &pairs, &columns};
-        MTQ_HIP(launch_kernel(chunk, dim3((a.hi - lo) * d.hk), dim3(256), args, lds, first));
+        // Few chunks: a workgroup for each value head, which all work out the products of q and k that they share.
+        a.parts = (uint64_t)(a.hi - lo) * d.hk < 512 ? d.hv / d.hk : 1;
+        MTQ_HIP(launch_kernel(chunk, dim3((a.hi - lo) * d.hk * a.parts), dim3(256), args, lds, first));
         MTQ_HIP(launch_kernel(fn, dim3((uint32_t)grid), dim3(64 * (8 + touch)), args, 0, second));
     }
     return ERR_OK;
