@@ -22,7 +22,7 @@ namespace mtq {
 namespace {
 
 constexpr uint32_t kTopMost = 32;        // alternatives a row
-constexpr uint32_t kListCap = 256;       // a wave's candidates: 4 keys a lane where they are selected from
+constexpr uint32_t kListCap = 576;       // a wave's candidates: 32 kept, and a vector of 8 elements of 64 lanes
 constexpr uint32_t kTileElems = 32;      // elements of a lane's tile: 64 bytes of 16-bit logits, 128 of f32
 constexpr int kWaves = 4;
 
@@ -47,28 +47,10 @@ __device__ __forceinline__ float unordered(uint32_t u) {
     return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
 }
 
-// Maximum over aligned segments of lanes (from .. to lanes, powers of two): every lane of a segment gets it.
-__device__ __forceinline__ uint32_t seg_max_u32(uint32_t v, int from, int to) {
-    for (int s = from; s < to; s <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, s, 64));
-    return v;
-}
-template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {   // (a lane without a source takes 0)
-    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
-}
-// Maximum over the wave, in a scalar register: rows of 16 lanes by mirrors, then row to row, the whole in the last lane.
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-    v = dpp_max<0xB1>(v);    // quad_perm [1,0,3,2]
-    v = dpp_max<0x4E>(v);    // quad_perm [2,3,0,1]
-    v = dpp_max<0x141>(v);   // row_half_mirror
-    v = dpp_max<0x140>(v);   // row_mirror
-    v = dpp_max<0x142>(v);   // row_bcast15
-    v = dpp_max<0x143>(v);   // row_bcast31
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-}
-
-// What a lane has seen of a row.
+// What a lane, and then a wave, has seen of a row.
 struct Seen {
     float m = -INFINITY, z = 0.f, s = 0.f;
+    // The sums relative to a maximum that is not below m.
     __device__ __forceinline__ void raise(float to) {
         if (to > m) {
             if (z != 0.f) {   // (nothing summed yet: no difference to take)
@@ -88,41 +70,71 @@ struct Seen {
         z += o.z;
         s += o.s;
     }
+    __device__ __forceinline__ void join_lanes() {
+        float top = m;
+        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        raise(top);
+        z = seg_allreduce(z, 64);
+        s = seg_allreduce(s, 64);
+    }
 };
 
-// The wave's top `k` of the `n` keys in list[0 .. n), in order, to out[0 .. k) (0: no more keys); returns the k-th. n <= kListCap,
-// and `out` may be `list`. k rounds of a wave maximum, the upper halves first and the lower ones among lanes that have it.
-__device__ __forceinline__ uint64_t draw_top(const uint64_t* list, uint32_t n, uint64_t* out, uint32_t k) {
+// The top `k` of the wave's `n` keys in list[0 .. n), in order, to out[0 .. k) (0: no more keys); returns the k-th. `spare` has room for k;
+// out may be `list`. Keys other than 0 are distinct: a lane counts for each of its keys how many of all are larger (reads of LDS that all
+// lanes share), and the count is the key's place.
+template <int P> __device__ __forceinline__ void place_top(const uint64_t* list, uint32_t from, uint32_t n, uint64_t* out, uint32_t k) {
     const uint32_t lane = threadIdx.x & 63u;
-    constexpr int PER = kListCap / 64;
-    uint64_t mine[PER];
+    uint64_t mine[P];
+    uint32_t above[P] = {};
 #pragma unroll
-    for (int i = 0; i < PER; i++) mine[i] = i * 64 + lane < n ? list[i * 64 + lane] : 0;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    uint64_t best = 0;
+    for (int i = 0; i < P; i++) mine[i] = from + i * 64 + lane < n ? list[from + i * 64 + lane] : 0;
+    uint32_t j = 0;
+    for (; j + 4 <= n; j += 4) {
+        uint64_t o[4];
 #pragma unroll
-    for (int i = 0; i < PER; i++) best = mine[i] > best ? mine[i] : best;
-    uint64_t last = 0;
-    for (uint32_t r = 0; r < k; r++) {
-        const uint32_t hi = wave_max_u32((uint32_t)(best >> 32));
-        const uint32_t lo = wave_max_u32((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
-        last = ((uint64_t)hi << 32) | lo;
-        if (lane == 0) out[r] = last;
-        if (best == last) {   // its lane (every lane, once no keys are left) looks for its next
-            best = 0;
+        for (int u = 0; u < 4; u++) o[u] = list[j + u];
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
-                if (mine[i] == last) mine[i] = 0;
-                best = mine[i] > best ? mine[i] : best;
-            }
-        }
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int i = 0; i < P; i++) above[i] += o[u] > mine[i];
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    return last;
+    for (; j < n; j++) {
+        const uint64_t o = list[j];
+#pragma unroll
+        for (int i = 0; i < P; i++) above[i] += o > mine[i];
+    }
+#pragma unroll
+    for (int i = 0; i < P; i++)
+        if (mine[i] && above[i] < k) out[above[i]] = mine[i];
+}
+__device__ __forceinline__ uint64_t draw_top(const uint64_t* list, uint32_t n, uint64_t* spare, uint64_t* out, uint32_t k) {
+    const uint32_t lane = threadIdx.x & 63u;
+    auto turned = [] { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); };   // (LDS operations of a wave complete in order)
+    turned();
+    if (lane < k) spare[lane] = 0;
+    turned();
+    if (n <= 64) place_top<1>(list, 0, n, spare, k);
+    else
+        for (uint32_t from = 0; from < n; from += 128) place_top<2>(list, from, n, spare, k);
+    turned();
+    const uint64_t mine = lane < k ? spare[lane] : 0, last = spare[k - 1];
+    if (lane < k) out[lane] = mine;
+    turned();
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(last >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)last);
 }
 
+// A row's given tokens' logits, the first 64 of them: asked for before anything else of the row.
+template <int DT> struct Given {
+    uint32_t id = 0xFFFFFFFFu;
+    float x = 0.f;
+    __device__ __forceinline__ void load(const LogprobArgs& a, uint32_t row, uint32_t j) {
+        id = j < a.n_given ? a.tokens[(uint64_t)row * a.n_given + j] : 0xFFFFFFFFu;
+        if (id < a.vocab) x = load_elem<DT>(a.logits, (size_t)row * a.stride + id);
+    }
+};
+
 // A row's results, by one wave: z and s relative to m, keys in order.
-template <int DT> __device__ __forceinline__ void finish(const LogprobArgs& a, uint32_t row, const Seen& t, const uint64_t* keys) {
+template <int DT> __device__ __forceinline__ void finish(const LogprobArgs& a, uint32_t row, const Seen& t, const uint64_t* keys, Given<DT> given) {
     const uint32_t lane = threadIdx.x & 63u;
     // No token has any probability where every logit is -inf (z = 0): log probabilities are -inf, the entropy 0. A NaN or +inf among
     // the logits makes z NaN, and all of the row's results with it.
@@ -131,9 +143,8 @@ template <int DT> __device__ __forceinline__ void finish(const LogprobArgs& a, u
     auto lp = [&](float x) { return none ? -INFINITY : (x - t.m) - log_z; };
     if (a.entropy && lane == 0) a.entropy[row] = none ? 0.f : log_z - t.s / t.z;
     for (uint32_t j = lane; j < a.n_given; j += 64) {
-        const uint64_t at = (uint64_t)row * a.n_given + j;
-        const uint32_t id = a.tokens[at];
-        if (id < a.vocab) a.token_logprobs[at] = lp(load_elem<DT>(a.logits, (size_t)row * a.stride + id));
+        if (j >= 64) given.load(a, row, j);
+        if (given.id < a.vocab) a.token_logprobs[(uint64_t)row * a.n_given + j] = lp(given.x);
     }
     if (lane < a.k) {
         const uint64_t key = keys[lane], at = (uint64_t)row * a.k + lane;
@@ -142,14 +153,19 @@ template <int DT> __device__ __forceinline__ void finish(const LogprobArgs& a, u
     }
 }
 
+struct WaveLists {
+    uint64_t list[kWaves][kListCap], spare[kWaves][kTopMost], comb[kWaves * kTopMost];
+    float sums[kWaves][3];
+};
+
 // A wave's candidates.
 struct Candidates {
-    uint64_t* list;
+    uint64_t *list, *spare;
     uint32_t n = 0, k;
     uint64_t bar = 0;            // keys above it join
     float bar_value = -INFINITY; // no smaller logit has such a key
     __device__ __forceinline__ void draw() {
-        const uint64_t kth = draw_top(list, n, list, k);
+        const uint64_t kth = draw_top(list, n, spare, list, k);
         n = n < k ? n : k;
         if (kth) raise_bar(kth);
     }
@@ -157,41 +173,32 @@ struct Candidates {
         bar = key;
         bar_value = unordered((uint32_t)(key >> 32));
     }
-    // One key a lane; 64 of them always fit.
-    __device__ __forceinline__ void offer(uint64_t key) {
-        uint64_t who = __ballot(key > bar);
-        if (!who) return;
-        if (n + 64 > kListCap) {
-            draw();
-            who = __ballot(key > bar);
-        }
-        if (key > bar) list[n + __popcll(who & ((1ull << (threadIdx.x & 63u)) - 1))] = key;
-        n += __popcll(who);
-    }
 };
 
 // What the workgroup's waves have seen and the top k of their lists, joined in its first wave (all of its lanes get it); keys to `comb`.
-__device__ __forceinline__ Seen join_waves(Seen t, const Candidates& c, float (*sums)[3], uint64_t* comb) {
+__device__ __forceinline__ Seen join_waves(Seen t, const Candidates& c, WaveLists& w) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    for (int s = 1; s < 64; s <<= 1) t.join(__shfl_xor(t.m, s, 64), __shfl_xor(t.z, s, 64), __shfl_xor(t.s, s, 64));
-    if (c.k) draw_top(c.list, c.n, comb + wave * c.k, c.k);
-    if (lane == 0) { sums[wave][0] = t.m; sums[wave][1] = t.z; sums[wave][2] = t.s; }
+    t.join_lanes();
+    if (c.k) draw_top(c.list, c.n, c.spare, w.comb + wave * c.k, c.k);
+    if (lane == 0) { w.sums[wave][0] = t.m; w.sums[wave][1] = t.z; w.sums[wave][2] = t.s; }
     __syncthreads();
     if (wave == 0) {
-        for (int w = 1; w < kWaves; w++) t.join(sums[w][0], sums[w][1], sums[w][2]);
-        if (c.k) draw_top(comb, kWaves * c.k, comb, c.k);
+        Seen all;
+        if (lane < kWaves) { all.m = w.sums[lane][0]; all.z = w.sums[lane][1]; all.s = w.sums[lane][2]; }
+        all.join_lanes();
+        t = all;
+        if (c.k) draw_top(w.comb, kWaves * c.k, c.spare, w.comb, c.k);
     }
     return t;
 }
 
-// Workgroup (slice, row): its four waves take tiles of 64 lanes x 32 elements in turn. The row's vectors are the 16-byte blocks of
-// memory that hold any of it, so that rows of every alignment are read in whole vectors; elements before and behind the row count as nothing.
-template <int DT> __global__ __launch_bounds__(64 * kWaves) void logprobs_kernel(LogprobArgs a) {
+// Workgroup (slice, row): its four waves take tiles of 64 lanes x 32 elements in turn, the next tile's on its way while one is worked on. The
+// row's vectors are the 16-byte blocks of memory that hold any of it, so that rows of every alignment are read in whole vectors; elements
+// before and behind the row count as nothing.
+template <int DT> __global__ __launch_bounds__(64 * kWaves, 4) void logprobs_kernel(LogprobArgs a) {
     constexpr int ES = DT == DT_F32 ? 4 : 2, PER = 16 / ES, NV = kTileElems / PER;
-    __shared__ uint64_t lists[kWaves][kListCap];
-    __shared__ uint64_t comb[kWaves * kTopMost];
-    __shared__ float sums[kWaves][3];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
+    __shared__ WaveLists lds;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
     const uint64_t at = (uint64_t)(uintptr_t)a.logits + (uint64_t)row * a.stride * ES;
     const uint32_t skip = (uint32_t)(at & 15u) / ES;                          // elements of the first vector that are not the row's
     const uint4* vecs = (const uint4*)(at & ~(uint64_t)15);
@@ -199,22 +206,34 @@ template <int DT> __global__ __launch_bounds__(64 * kWaves) void logprobs_kernel
     constexpr uint32_t kTileVecs = 64 * NV;
     const uint32_t n_tiles = (n_vecs + kTileVecs - 1) / kTileVecs;
     Candidates c;
-    c.list = lists[wave];
+    c.list = lds.list[wave];
+    c.spare = lds.spare[wave];
     c.k = a.k;
     bool open = true;                // no bar yet
     Seen t;
-    for (uint32_t tile = slice * kWaves + wave; tile < n_tiles; tile += a.slices * kWaves) {
-        uint4 raw[NV];
-        const uint32_t v0 = tile * kTileVecs + lane;
+    uint4 raw[NV], next[NV];
+    auto load = [&](uint32_t tile) {
 #pragma unroll
-        for (int u = 0; u < NV; u++) raw[u] = v0 + u * 64 < n_vecs ? vecs[v0 + u * 64] : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < NV; u++) {
+            const uint32_t v = tile * kTileVecs + lane + u * 64;
+            next[u] = v < n_vecs ? vecs[v] : make_uint4(0, 0, 0, 0);
+        }
+    };
+    auto value = [](const uint4& r, int j) -> float {
+        const uint32_t w = ((const uint32_t*)&r)[ES == 4 ? j : j >> 1];
+        if constexpr (DT == DT_F32) return __uint_as_float(w);
+        else if constexpr (DT == DT_BF16) return __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
+        else return f16_bits_to_f32(j & 1 ? w >> 16 : w & 0xFFFFu);
+    };
+    load(slice * kWaves + wave);
+    Given<DT> given;
+    if (a.slices == 1 && wave == 0) given.load(a, row, lane);
+    for (uint32_t tile = slice * kWaves + wave; tile < n_tiles; tile += a.slices * kWaves) {
+#pragma unroll
+        for (int u = 0; u < NV; u++) raw[u] = next[u];
+        load(tile + a.slices * kWaves);
+        const uint32_t v0 = tile * kTileVecs + lane;
         const bool edge = tile == 0 || tile == n_tiles - 1;
-        auto elem = [&](int u, int j) -> float {
-            const uint32_t w = ((const uint32_t*)&raw[u])[ES == 4 ? j : j >> 1];
-            if constexpr (DT == DT_F32) return __uint_as_float(w);
-            else if constexpr (DT == DT_BF16) return __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
-            else return f16_bits_to_f32(j & 1 ? w >> 16 : w & 0xFFFFu);
-        };
         float vmax[NV], x[NV][PER];
         float top = -INFINITY;
 #pragma unroll
@@ -222,7 +241,7 @@ template <int DT> __global__ __launch_bounds__(64 * kWaves) void logprobs_kernel
             vmax[u] = -INFINITY;
 #pragma unroll
             for (int j = 0; j < PER; j++) {
-                x[u][j] = elem(u, j);
+                x[u][j] = value(raw[u], j);
                 if (edge) {
                     const uint32_t e = (v0 + u * 64) * PER + j - skip;        // (before the row: wraps past vocab)
                     if (e >= a.vocab) x[u][j] = -INFINITY;
@@ -245,62 +264,85 @@ template <int DT> __global__ __launch_bounds__(64 * kWaves) void logprobs_kernel
         t.z += z;
         t.s += s;
         if (!c.k) continue;
-        const bool first = open;
         if (open) {
-            // A first bar: of 2^i groups of lanes, 2^i >= k, each has an element as large as the least of their maxima.
-            const int groups = c.k <= 1 ? 1 : 1 << (32 - __clz((int)c.k - 1));
-            uint32_t o = seg_max_u32(ordered(top), 1, 64 / groups);
-            o = ~seg_max_u32(~o, 64 / groups, 64);
-            c.raise_bar(((uint64_t)o << 32) - 1);
-            c.bar_value = unordered(o);
-            open = false;
-        }
+            // A first bar: the k-th largest of the lanes' maxima (of equal ones the lower lane's first) is reached by k elements, and by few more.
+            const uint32_t o = ordered(top);
+            uint32_t above = 0;
 #pragma unroll
-        for (int u = 0; u < NV; u++) {
-            if (!__ballot(!(vmax[u] < c.bar_value))) continue;
-#pragma unroll
-            for (int j = 0; j < PER; j++) {
-                const float v = elem(u, j);
-                const uint32_t e = (v0 + u * 64) * PER + j - skip;
-                c.offer(v == v && e < a.vocab ? (uint64_t)ordered(v) << 32 | ~e : 0);
+            for (int i = 0; i < 64; i++) {
+                const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)o, i);
+                above += other > o || (other == o && i < (int)lane);
             }
+            const uint32_t kth = (uint32_t)__builtin_amdgcn_readlane((int)o, __builtin_ctzll(__ballot(above == c.k - 1)));
+            c.raise_bar(((uint64_t)kth << 32) - 1);
+            c.bar_value = unordered(kth);
         }
-        if (first || c.n >= 3 * kListCap / 4) c.draw();
+        const bool more = tile + a.slices * kWaves < n_tiles;
+        if (__ballot(!(top < c.bar_value))) {
+            uint32_t hot = 0;
+#pragma unroll
+            for (int u = 0; u < NV; u++) hot |= __ballot(!(vmax[u] < c.bar_value)) ? 1u << u : 0u;
+            while (hot) {
+                const uint32_t u = __builtin_ctz(hot);
+                hot &= hot - 1;
+                uint4 r = raw[0];
+#pragma unroll
+                for (int i = 1; i < NV; i++)
+                    if (u == i) r = raw[i];
+                uint32_t most = 0;
+#pragma unroll
+                for (int j = 0; j < PER; j++) most += __popcll(__ballot(!(value(r, j) < c.bar_value)));
+                if (c.n + most > kListCap) c.draw();                          // (then they fit: at most 32 and 512)
+#pragma unroll
+                for (int j = 0; j < PER; j++) {
+                    const float v = value(r, j);
+                    if (!__ballot(!(v < c.bar_value))) continue;
+                    const uint32_t e = (v0 + u * 64) * PER + j - skip;
+                    const uint64_t key = v == v && e < a.vocab ? (uint64_t)ordered(v) << 32 | (uint32_t)~e : 0;
+                    const uint64_t who = __ballot(key > c.bar);
+                    if (key > c.bar) c.list[c.n + __popcll(who & ((1ull << lane) - 1))] = key;
+                    c.n += __popcll(who);
+                }
+            }
+            if (more && (open || c.n > c.k + 8)) c.draw();
+        }
+        open = false;
     }
-    t = join_waves(t, c, sums, comb);
+    t = join_waves(t, c, lds);
     if (wave) return;
     if (a.slices == 1) {
-        finish<DT>(a, row, t, comb);
+        finish<DT>(a, row, t, lds.comb, given);
     } else {
         const size_t i = (size_t)row * a.slices + slice;
         if (lane == 0) { a.part[4 * i] = t.m; a.part[4 * i + 1] = t.z; a.part[4 * i + 2] = t.s; }
-        if (lane < a.k) a.part_keys[i * a.k + lane] = comb[lane];
+        if (lane < a.k) a.part_keys[i * a.k + lane] = lds.comb[lane];
     }
 }
 
 // A row's slices joined by one workgroup: at most kSlicesMost, so that their keys fit the waves' lists.
-constexpr uint32_t kSlicesMost = kWaves * kListCap / kTopMost;
+constexpr uint32_t kSlicesMost = 32;
+static_assert(kSlicesMost / kWaves * kTopMost <= kListCap && kSlicesMost <= 64, "a wave's share of the slices fits its list and its lanes");
 template <int DT> __global__ __launch_bounds__(64 * kWaves) void logprobs_join_kernel(LogprobArgs a) {
-    __shared__ uint64_t lists[kWaves][kListCap];
-    __shared__ uint64_t comb[kWaves * kTopMost];
-    __shared__ float sums[kWaves][3];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x;
+    __shared__ WaveLists lds;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.x;
+    Given<DT> given;
+    if (wave == 0) given.load(a, row, lane);
     const uint32_t mine = (a.slices + kWaves - 1) / kWaves, from = wave * mine < a.slices ? wave * mine : a.slices;
     const uint32_t to = from + mine < a.slices ? from + mine : a.slices;
     Candidates c;
-    c.list = lists[wave];
+    c.list = lds.list[wave];
+    c.spare = lds.spare[wave];
     c.k = a.k;
     c.n = (to - from) * a.k;
     const uint64_t* keys = a.part_keys + ((size_t)row * a.slices + from) * a.k;
     for (uint32_t i = lane; i < c.n; i += 64) c.list[i] = keys[i];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     Seen t;
     if (from + lane < to) {
         const float* p = a.part + 4 * ((size_t)row * a.slices + from + lane);
         t.m = p[0]; t.z = p[1]; t.s = p[2];
     }
-    t = join_waves(t, c, sums, comb);
-    if (wave == 0) finish<DT>(a, row, t, comb);
+    t = join_waves(t, c, lds);
+    if (wave == 0) finish<DT>(a, row, t, lds.comb, given);
 }
 
 constexpr uint32_t kGridMost = 0x7FFFFFFF;
