@@ -1399,14 +1399,17 @@ static int op_fp8_qmm(int dtype, const void* w, const float* ws, const void* x, 
     if (rc) return rc;
     if (!xs) return fail(ERR_BAD_ARG, "null buffer");
     Fp8Args a{(const uint8_t*)w, ws, x, xs, out, M, N, K};
-    return fp8_tiles_takes(dtype, a) ? launch_fp8_tiles(dtype, a, lc) : launch_fp8_rows(dtype, a, lc);
+    const int mt = fp8_rows_tiles(dtype, a);
+    return mt ? launch_fp8_rows(dtype, a, mt, lc) : launch_fp8_tiles(dtype, a, lc);
 }
 
 static int op_fp8_qmv(int dtype, const void* w, const float* ws, const void* x, void* out, uint32_t M, uint32_t N, uint32_t K, const LaunchCtx& lc) {
     if (M == 0) return check_dtype(dtype);
     int rc = check_fp8(dtype, w, ws, x, out, M, N, K);
     if (rc) return rc;
-    const size_t codes = ((size_t)M * K + 255) / 256 * 256, scales = (size_t)M * ((K + kFp8Block - 1) / kFp8Block) * 4;
+    const Fp8Args direct{(const uint8_t*)w, ws, x, nullptr, out, M, N, K};
+    if (fp8_fused_takes(direct)) return launch_fp8_fused(dtype, direct, lc);
+    const size_t codes = ((size_t)M * K + 255) / 256 * 256, scales = (size_t)M * fp8_blocks(K) * 4;
     rc = ensure_scratch(codes + scales);
     if (rc) return rc;
     float* xs = (float*)((char*)g.scratch_buf + codes);

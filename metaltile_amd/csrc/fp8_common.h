@@ -83,6 +83,26 @@ template <int DT> __device__ __forceinline__ fp8_f32x4 fp8_mfma(uint4 a0, uint4 
     }
 }
 
+__device__ __host__ __forceinline__ uint32_t fp8_blocks(uint32_t k) { return (k >> 7) + ((k & 127u) != 0); }
+
+// Four neighbouring results of row m, n a multiple of 4.
+template <int DT> __device__ __forceinline__ void fp8_store4(void* out, uint32_t m, uint32_t n, uint32_t N, fp8_f32x4 v) {
+    constexpr int ES = DT == DT_F32 ? 4 : 2;
+    const size_t i0 = (size_t)m * N + n;
+    if (N % 4 == 0 && (uintptr_t)out % (4 * ES) == 0 && n < N) {
+        if constexpr (DT == DT_F32) {
+            *(fp8_f32x4*)((float*)out + i0) = v;
+        } else {
+            *(uint2*)((uint16_t*)out + i0) = make_uint2(f32_to_elem_bits<DT>(v[0]) | (uint32_t)f32_to_elem_bits<DT>(v[1]) << 16,
+                                                        f32_to_elem_bits<DT>(v[2]) | (uint32_t)f32_to_elem_bits<DT>(v[3]) << 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (n + i < N) store_elem<DT>(out, i0 + i, v[i]);
+    }
+}
+
 struct Fp8Args {
     const uint8_t* w;      // codes [N, K]
     const float* ws;       // [ceil(N / 128), ceil(K / 128)]
@@ -91,5 +111,14 @@ struct Fp8Args {
     void* out;             // T [M, N]
     uint32_t M, N, K;
 };
+
+inline int fp8_num_cus() {
+    static int n = 0;
+    if (n == 0) {
+        int dev = 0, v = 0;
+        n = (hipGetDevice(&dev) == hipSuccess && hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0) ? v : 256;
+    }
+    return n;
+}
 
 }  // namespace mtq

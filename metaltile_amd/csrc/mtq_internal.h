@@ -299,8 +299,12 @@ int launch_logprobs(int dtype, const void* logits, size_t stride, const uint32_t
 // 8-bit floating point with a scale for each block of 128 (fp8_common.h): the quantiser, and products of its codes.
 struct Fp8Args;
 int launch_fp8_quantize(int dtype, const void* x, void* codes, float* scales, uint32_t rows, uint32_t cols, uint32_t block_rows, const LaunchCtx& lc);
-int launch_fp8_rows(int dtype, const Fp8Args& p, const LaunchCtx& lc);
-bool fp8_tiles_takes(int dtype, const Fp8Args& p);
+// (mt: sixteens of activation rows that a workgroup has; fp8_rows_tiles: how many it should have, or 0 where launch_fp8_tiles is the faster)
+int fp8_rows_tiles(int dtype, const Fp8Args& p);
+int launch_fp8_rows(int dtype, const Fp8Args& p, int mt, const LaunchCtx& lc);
+// (x: T, quantised on the way)
+bool fp8_fused_takes(const Fp8Args& p);
+int launch_fp8_fused(int dtype, const Fp8Args& p, const LaunchCtx& lc);
 int launch_fp8_tiles(int dtype, const Fp8Args& p, const LaunchCtx& lc);
 
 // The gated delta rule (gated_delta.h).

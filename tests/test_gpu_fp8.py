@@ -118,6 +118,35 @@ def test_products(dt, m, n, k):
     assert m > 16 or np.allclose(unpack_f32(results[0][:size], dt), unpack_f32(results[1][:size], dt), rtol=2 * HALF_STEP[dt], atol=float(tol.max()))
 
 
+# More tiles than the CUs take as groups of rows: 128 x 128, 256 x 256, those cut in two (with a lower half behind the last row), f32 as well.
+TILED = [(40, 16500, 272), (129, 4112, 400), (300, 4200, 656), (65, 8200, 1168), (400, 8300, 144), (2600, 4700, 272), (4100, 4360, 400)]
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
+@pytest.mark.parametrize("m,n,k", TILED)
+def test_products_in_tiles(dt, m, n, k):
+    test_products(dt, m, n, k)
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
+@pytest.mark.parametrize("m,n,k", [(129, 4112, 400), (300, 4200, 656), (400, 8300, 144), (2600, 4700, 272), (4100, 4360, 144)])
+def test_exact_in_tiles(dt, m, n, k):
+    """Codes of -1, 0 and 1 and scales of 1: every sum is a whole number, which bf16 holds up to 256."""
+    rng = np.random.default_rng(m)
+    wi, xi = rng.integers(-1, 2, (n, k)), rng.integers(-1, 2, (m, k)) * (rng.random((m, k)) < 0.1)
+    w, x = ref.e4m3_codes(wi), ref.e4m3_codes(xi)
+    ws, xs = np.ones((ref.blocks(n), ref.blocks(k)), np.float32), np.ones((m, ref.blocks(k)), np.float32)
+    want = xi.astype(np.float32) @ wi.astype(np.float32).T
+    assert np.abs(want).max() <= 256
+    wb, wsb, xb, xsb = (GpuBuffer.from_bytes(v.tobytes()) for v in (w, ws, x, xs))
+    size = m * n * dt.size_bytes
+    out = GpuBuffer.from_bytes(b"\xff" * (size + 64))
+    ops.fp8_qmm(dt, wb, wsb, xb, xsb, out, m, n, k)
+    raw = out.read_bytes()
+    assert raw[size:] == b"\xff" * 64
+    assert np.array_equal(unpack_f32(raw[:size], dt).reshape(m, n), want)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 200, 400), (40, 300, 272), (300, 300, 400)])
 def test_exact_where_sums_are_small_whole_numbers(m, n, k):
     """Codes of small whole numbers and scales of powers of two: every sum is exact, so is the result."""
