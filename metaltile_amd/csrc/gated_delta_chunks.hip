@@ -409,20 +409,19 @@ struct WalkPlace {
     const float* state_from;
 };
 
-// Half of the waves (AHEAD) have K S0 and U, the others Q S0 and P U, each of NB blocks of 16 rows; all have a share of the state's rows. With
-// two blocks a wave uses what it reads from LDS twice (blocks 0 and 3, or 1 and 2: three steps of a triangle either way). Each role has a loop of
-// its own, so that each wave waits for just what it loaded: what a chunk needs is asked for in the step after the one that has used the same
+// Half of the waves (AHEAD) have K S0 and U, the others Q S0 and P U, each of 16 rows; all have a share of the state's rows. Each role has a loop
+// of its own, so that each wave waits for just what it loaded: what a chunk needs is asked for in the step after the one that has used the same
 // registers, behind that step's reads of LDS. Between the barriers of a chunk (a, b, c):
 //   a..b: X = V - e^G r (K S0)         | Y = Q S0 + P U of the chunk before, to memory
 //   b..c: U = T X                      | Q S0
 //   c..a: S1 = e^G S0 + K^T (r e^.. U), its terms to LDS
-template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline__ void walk(const DeltaArgs& d, const WalkPlace& w, WalkLds<DKP>& lds, uint32_t wave) {
+template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ void walk(const DeltaArgs& d, const WalkPlace& w, WalkLds<DKP>& lds, uint32_t wave) {
     using L = Layout<DKP, NT>;
     constexpr int ES = DT == DT_F32 ? 4 : 2;
-    constexpr int KS = DKP / 32, TILES = DKP / 16, NS = TILES * NB > 8 ? TILES * NB / 8 : 1;   // NS: 16-row tiles of the state a wave has
+    constexpr int KS = DKP / 32, TILES = DKP / 16, NS = TILES > 8 ? TILES / 8 : 1;   // NS: 16-row tiles of the state a wave has
     const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
-    const uint32_t mine = wave & (4 / NB - 1), rb[2] = {mine, 3 - mine};
-    const bool long_row = NB == 2 || mine >= 2;                            // the last block has two steps of a triangle
+    const uint32_t mine = wave & 3u;
+    const bool long_row = mine >= 2;                                       // two steps of a triangle
     const bool has_state = wave * NS < TILES;
     const uint32_t tile0 = has_state ? wave * NS : 0;
     const uint32_t col = w.c0 + r;
@@ -437,10 +436,10 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
             for (int i = 0; i < 4; i++)
                 if (row + i < d.dk) S[x][i] = w.state_from[state + row + i];
         }
-    u32x4 mf[NB][KS][NT], tf[NB + 1][3], kt[NS][2][NT];
-    f32x4 e[NB], wk[NB] = {};
+    u32x4 mf[KS][NT], tf[2][3], kt[NS][2][NT];
+    f32x4 e, wk = {};
     float keep;
-    uint32_t v[NB][4] = {};
+    uint32_t v[4] = {};
     // Operands of a slot lie 16 bytes a lane; what differs between loads is the same for all lanes and goes into the scalar offset.
     const uint32_t head_at = d.hk * L::kKeyBytes + w.h * kHeadBytes, rows_at = w.kh * L::kKeyBytes + (AHEAD ? 0 : L::kOp);
     const uint32_t tri_at = head_at + (AHEAD ? 0 : kTriBytes), kt_at = w.kh * L::kKeyBytes + 2 * L::kOp + tile0 * 2048, scal_at = head_at + 2 * kTriBytes;
@@ -449,24 +448,19 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
     auto four = [&](__amdgpu_buffer_rsrc_t s, uint32_t at) { return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(s, g * 16, at, 0)); };
     auto load_rows = [&](__amdgpu_buffer_rsrc_t s) {        // K's or Q's rows, and the factors of their products with the state
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+        for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int k = 0; k < NT; k++) mf[b][ks][k] = get(s, rows_at + ((k * 4 + rb[b]) * KS + ks) * 1024);
-#pragma unroll
-        for (int b = 0; b < NB; b++) e[b] = four(s, scal_at + (AHEAD ? 0 : 256) + 64 * rb[b]);
+            for (int k = 0; k < NT; k++) mf[ks][k] = get(s, rows_at + ((k * 4 + mine) * KS + ks) * 1024);
+        e = four(s, scal_at + (AHEAD ? 0 : 256) + 64 * mine);
     };
-    auto load_tri = [&](__amdgpu_buffer_rsrc_t s) {         // T's or P's: with two blocks the one step of the first and both of the second
+    auto load_tri = [&](__amdgpu_buffer_rsrc_t s) {         // T's or P's
 #pragma unroll
-        for (int j = 0; j < NB + 1; j++) {
-            const uint32_t block = j < NB ? rb[j] : rb[NB - 1], step = (block < 2 ? block : 2 * block - 2) + (j == NB && long_row ? 1 : 0);
+        for (int j = 0; j < 2; j++) {
+            const uint32_t step = (mine < 2 ? mine : 2 * mine - 2) + (j && long_row ? 1 : 0);
 #pragma unroll
             for (int k = 0; k < 3; k++) tf[j][k] = get(s, tri_at + (step * 3 + k) * 1024);
         }
-        if (AHEAD)
-#pragma unroll
-            for (int b = 0; b < NB; b++) wk[b] = four(s, scal_at + 512 + 64 * rb[b]);
+        if (AHEAD) wk = four(s, scal_at + 512 + 64 * mine);
     };
     auto load_kt = [&](__amdgpu_buffer_rsrc_t s) {
 #pragma unroll
@@ -477,22 +471,18 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
                 for (int k = 0; k < NT; k++) kt[x][ts][k] = get(s, kt_at + ((k * TILES + x) * 2 + ts) * 1024);
         keep = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(s, 0, scal_at + 768, 0));
     };
-    uint32_t v_at[NB][4];                                   // a chunk's rows of v; rows behind the sequence are behind its buffer, and read as zeros
+    uint32_t v_at[4];                                       // a chunk's rows of v; rows behind the sequence are behind its buffer, and read as zeros
 #pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) v_at[b][i] = col_in ? ((16 * rb[b] + 4 * g + i) * (uint32_t)d.v_stride + w.h * d.dv + col) * ES : KR_OOB;
+    for (int i = 0; i < 4; i++) v_at[i] = col_in ? ((16 * mine + 4 * g + i) * (uint32_t)d.v_stride + w.h * d.dv + col) * ES : KR_OOB;
     auto load_v = [&](uint32_t chunk) {
         const uint32_t t0 = w.from + chunk * kChunk, n = t0 >= w.to ? 0 : w.to - t0 < kChunk ? w.to - t0 : kChunk;
         const uint32_t bytes = n ? ((n - 1) * (uint32_t)d.v_stride + d.hv * d.dv) * ES : 0;
         const __amdgpu_buffer_rsrc_t s = kr_rsrc((uint64_t)(uintptr_t)d.v + (uint64_t)(n ? t0 : w.from) * d.v_stride * ES, bytes);
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if constexpr (DT == DT_F32) v[b][i] = __builtin_amdgcn_raw_buffer_load_b32(s, v_at[b][i], 0, 0);
-                else v[b][i] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(s, v_at[b][i], 0, 0);
-            }
+        for (int i = 0; i < 4; i++) {
+            if constexpr (DT == DT_F32) v[i] = __builtin_amdgcn_raw_buffer_load_b32(s, v_at[i], 0, 0);
+            else v[i] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(s, v_at[i], 0, 0);
+        }
     };
     auto value = [&](uint32_t x) { return DT == DT_F32 ? __uint_as_float(x) : DT == DT_BF16 ? bf16_bits_to_f32(x) : f16_bits_to_f32(x); };
     auto put = [&](uint16_t* to, uint32_t plane, const f32x4& x) {   // four rows of a column, in terms
@@ -508,9 +498,9 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
             for (int x = 0; x < NS; x++) put(lds.S[0].at(r, 16 * (tile0 + x) + 4 * g), Columns<DKP>::PLANE, S[x]);
     };
     // `load` is what is asked for once the LDS reads are on their way.
-    auto times_state = [&](f32x4 (&c)[NB], auto&& load) {
+    auto times_state = [&](f32x4& c, auto&& load) {
         constexpr int AT_ONCE = KS < 4 ? KS : 4;
-        f32x4 part[NB][4 / NB] = {};
+        f32x4 part[4] = {};
 #pragma unroll
         for (int k0 = 0; k0 < KS; k0 += AT_ONCE) {
             u32x4 b[AT_ONCE][3];
@@ -522,14 +512,11 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
             if (k0 == 0) load();
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int ks = 0; ks < AT_ONCE; ks++)
-#pragma unroll
-                for (int x = 0; x < NB; x++) mfma_terms_on(mf[x][k0 + ks], b[ks], part[x], 0);
+            for (int ks = 0; ks < AT_ONCE; ks++) mfma_terms_on(mf[k0 + ks], b[ks], part, 0);
         }
-#pragma unroll
-        for (int x = 0; x < NB; x++) c[x] = NB == 2 ? part[x][0] + part[x][1] : (part[x][0] + part[x][1]) + (part[x][2 / NB] + part[x][3 / NB]);
+        c = (part[0] + part[1]) + (part[2] + part[3]);
     };
-    auto triangle = [&](Columns<kChunk>* B, f32x4 (&c)[NB], auto&& load) {
+    auto triangle = [&](Columns<kChunk>* B, f32x4& c, auto&& load) {
         u32x4 b[2][3];
 #pragma unroll
         for (int ks = 0; ks < 2; ks++)
@@ -538,27 +525,19 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
         __builtin_amdgcn_sched_barrier(0);
         load();
         __builtin_amdgcn_sched_barrier(0);
-        f32x4 part[NB][3] = {};
-#pragma unroll
-        for (int x = 0; x < NB; x++) {
-            part[x][0] = c[x];
-            mfma_terms_on(tf[x], b[0], part[x], 0);
-        }
-        if (long_row) mfma_terms_on(tf[NB], b[1], part[NB - 1], 0);
-#pragma unroll
-        for (int x = 0; x < NB; x++) c[x] = part[x][0] + part[x][1] + part[x][2];
+        f32x4 part[3] = {c};
+        mfma_terms_on(tf[0], b[0], part, 0);
+        if (long_row) mfma_terms_on(tf[1], b[1], part, 0);
+        c = part[0] + part[1] + part[2];
     };
-    f32x4 y[NB] = {};
+    f32x4 y = {};
     const uint32_t y_at = (4 * g * d.hv * d.dv + w.h * d.dv + col) * 4;
     auto give_y = [&](uint32_t chunk, auto&& load) {  // P U of a chunk onto its Q S0
         triangle(lds.U, y, load);
         const uint32_t t0 = w.from + chunk * kChunk, n = w.to - t0 < kChunk ? w.to - t0 : kChunk, row = d.hv * d.dv * 4;
         const __amdgpu_buffer_rsrc_t s = kr_rsrc((uint64_t)(uintptr_t)d.y + (uint64_t)t0 * row, n * row);   // (rows behind the sequence are not written)
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[b][i]), s, col_in ? y_at + (16 * rb[b] + i) * row : KR_OOB, 0, 0);
+        for (int i = 0; i < 4; i++) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[i]), s, col_in ? y_at + (16 * mine + i) * row : KR_OOB, 0, 0);
     };
     auto nothing = [] {};
     {
@@ -572,39 +551,30 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
         const auto here = slot(c), next = slot(c + 1 < w.end ? c + 1 : c);
         walk_barrier();
         if constexpr (AHEAD) {
-            f32x4 x[NB];
+            f32x4 x;
             times_state(x, [&] { load_kt(here); });
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[b][i] = value(v[b][i]) - e[b][i] * x[b][i];
-                asm volatile("" : "+v"(x[b]));   // (here, not behind the next loads into e's and v's registers)
-                put(lds.X[0].at(r, 16 * rb[b] + 4 * g), Columns<kChunk>::PLANE, x[b]);
-            }
+            for (int i = 0; i < 4; i++) x[i] = value(v[i]) - e[i] * x[i];
+            asm volatile("" : "+v"(x));   // (here, not behind the next loads into e's and v's registers)
+            put(lds.X[0].at(r, 16 * mine + 4 * g), Columns<kChunk>::PLANE, x);
         } else if (c > w.begin) {
             give_y(c - 1, [&] { load_kt(here); });
         } else {
             load_kt(here);
         }
         walk_barrier();
-        f32x4 late[NB];
+        f32x4 late;
         if constexpr (AHEAD) {
-            f32x4 u[NB] = {}, uw[NB];
+            f32x4 u = {};
             triangle(lds.X, u, [&] { load_rows(next); load_v(c + 1); });
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                uw[b] = u[b] * wk[b];
-                asm volatile("" : "+v"(uw[b]));
-                put(lds.W[0].at(r, 16 * rb[b] + 4 * g), Columns<kChunk>::PLANE, uw[b]);
-                late[b] = u[b];   // (U itself is asked for from the next chunk on: it is put beside the state's update)
-            }
+            f32x4 uw = u * wk;
+            asm volatile("" : "+v"(uw));
+            put(lds.W[0].at(r, 16 * mine + 4 * g), Columns<kChunk>::PLANE, uw);
+            late = u;   // (U itself is asked for from the next chunk on: it is put beside the state's update)
         } else {
             times_state(y, [&] { load_tri(here); });
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                y[b] *= e[b];
-                asm volatile("" : "+v"(y[b]));
-            }
+            y *= e;
+            asm volatile("" : "+v"(y));
         }
         walk_barrier();
         u32x4 b[2][3];
@@ -615,8 +585,7 @@ template <int DT, int DKP, int NT, int NB, bool AHEAD> __device__ __forceinline_
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (AHEAD) {
             load_tri(next);
-#pragma unroll
-            for (int x = 0; x < NB; x++) put(lds.U[0].at(r, 16 * rb[x] + 4 * g), Columns<kChunk>::PLANE, late[x]);
+            put(lds.U[0].at(r, 16 * mine + 4 * g), Columns<kChunk>::PLANE, late);
         } else {
             load_rows(next);
         }
@@ -681,7 +650,7 @@ template <int DT, int DKP, int NT> __device__ __forceinline__ void walk_touch(co
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <int DT, int DKP, int NT, int NB, bool TOUCH, int PER_SIMD> __global__ __launch_bounds__(64 * (8 / NB + TOUCH), PER_SIMD) void delta_walk_kernel(ChunkArgs a, uint32_t pairs, uint32_t columns) {
+template <int DT, int DKP, int NT, bool TOUCH, int PER_SIMD> __global__ __launch_bounds__(64 * (8 + TOUCH), PER_SIMD) void delta_walk_kernel(ChunkArgs a, uint32_t pairs, uint32_t columns) {
     using L = Layout<DKP, NT>;
     __shared__ __attribute__((aligned(16))) WalkLds<DKP> lds;
     const DeltaArgs& d = a.d;
@@ -713,8 +682,8 @@ template <int DT, int DKP, int NT, int NB, bool TOUCH, int PER_SIMD> __global__ 
     w.c0 = c0;
     w.state = ((size_t)s.slot * d.hv + h) * d.dv * d.dk;
     w.state_from = w.begin ? d.state_out : d.state_in;
-    if (wave < 4 / NB) walk<DT, DKP, NT, NB, true>(d, w, lds, wave);
-    else if (wave < 8 / NB) walk<DT, DKP, NT, NB, false>(d, w, lds, wave);
+    if (wave < 4) walk<DT, DKP, NT, true>(d, w, lds, wave);
+    else if (wave < 8) walk<DT, DKP, NT, false>(d, w, lds, wave);
     else if constexpr (TOUCH) walk_touch<DT, DKP, NT>(d, w, lds, columns);
 }
 
@@ -735,9 +704,9 @@ template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* s
     constexpr bool wide = DKP * NT >= 384, narrow = DKP == 64 && NT <= 2;
     const bool touch = !wide && !(narrow && grid > 256);
     const void* fn;
-    if constexpr (wide) fn = (const void*)delta_walk_kernel<DT, DKP, NT, 1, false, 2>;
-    else if constexpr (narrow) fn = touch ? (const void*)delta_walk_kernel<DT, DKP, NT, 1, true, 1> : (const void*)delta_walk_kernel<DT, DKP, NT, 1, false, 4>;
-    else fn = (const void*)delta_walk_kernel<DT, DKP, NT, 1, true, 1>;
+    if constexpr (wide) fn = (const void*)delta_walk_kernel<DT, DKP, NT, false, 2>;
+    else if constexpr (narrow) fn = touch ? (const void*)delta_walk_kernel<DT, DKP, NT, true, 1> : (const void*)delta_walk_kernel<DT, DKP, NT, false, 4>;
+    else fn = (const void*)delta_walk_kernel<DT, DKP, NT, true, 1>;
     constexpr size_t lds = ChunkLds<DKP, NT>::kBytes;
     const void* chunk = (const void*)delta_chunk_kernel<DT, DKP, NT>;
     MTQ_HIP(set_max_dynamic_lds(chunk, lds));
