@@ -1,0 +1,239 @@
+"""The served operators where sizes, sharing and order are at their edges: offsets past 32 bits, scratch that grows behind a captured graph, calls one
+behind the other, many sequences, streams of the caller's.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from metaltile_amd import DType, GpuBuffer, _lib, ops, pack_f32, unpack_f32
+from metaltile_amd.runtime import _ensure_init
+from tests import fp8_reference as ref
+from tests.hip_graph import Graph
+from tests.test_gpu_fp8 import _tolerance, _weights
+from tests.test_gpu_gated_delta import Case
+from tests.test_gpu_token_logprobs import _close, _reference
+
+pytestmark = pytest.mark.gpu
+DTYPES = [DType.F32, DType.F16, DType.BF16]
+
+
+def _put(buf, at, data):
+    arr = np.frombuffer(data, np.uint8)
+    assert at + arr.nbytes <= buf.nbytes
+    _lib.check(_ensure_init().mtq_upload(buf.ptr + at, arr.ctypes.data_as(C.c_void_p), arr.nbytes))
+
+
+def _get(buf, at, dtype, count):
+    out = np.empty(count, dtype)
+    assert at + out.nbytes <= buf.nbytes
+    _lib.check(_ensure_init().mtq_download(out.ctypes.data_as(C.c_void_p), buf.ptr + at, out.nbytes))
+    return out
+
+
+# ---- many chunks, sequences and heads
+
+MANY = [  # lens, hk, hv, dk, dv: one workgroup for a key head's value heads, more than four of these, more sequences than a wave has lanes, more walks than CUs
+    ([4480], 8, 16, 64, 16), ([260] * 64, 2, 12, 32, 16), ([(7 * i) % 5 * 40 + i % 3 for i in range(150)], 2, 4, 64, 32), ([0] * 70 + [100, 0, 33] + [1] * 70 + [65], 1, 2, 128, 16),
+    ([90, 70, 33, 1, 17] * 8, 1, 4, 64, 80), ([130] * 20, 4, 8, 128, 64)]
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
+@pytest.mark.parametrize("lens,hk,hv,dk,dv", MANY, ids=lambda v: str(v).replace(" ", "")[:40])
+def test_delta_many(dt, lens, hk, hv, dk, dv):
+    print(f"[case] gated_delta_rule {dt.name} {len(lens)} sequences of {sum(lens)} tokens hk{hk} hv{hv} dk{dk} dv{dv}", flush=True)
+    c = Case(dt, lens, hk, hv, dk, dv)
+    c.call()
+    c.hold()
+
+
+def test_delta_slots_of_a_large_pool():
+    """States past 2^32 elements: only the named slots are written."""
+    hk, hv, dk, dv, n_slots = 2, 32, 128, 128, 8300
+    one = hv * dv * dk
+    assert (n_slots - 1) * one > 1 << 32
+    for lens in ([1, 1], [40, 70]):
+        c = Case(DType.BF16, lens, hk, hv, dk, dv, slots=[8299, 3], n_slots=1)   # (its own states are not used)
+        pool = GpuBuffer(n_slots * one * 4)
+        rng = np.random.default_rng(5)
+        states = (0.3 * rng.standard_normal((2, hv, dv, dk))).astype(np.float32)
+        for slot, s in zip(c.slots, states):
+            _put(pool, slot * one * 4, s.tobytes())
+        _put(pool, 8298 * one * 4, np.full(one, 5.5, "<f4").tobytes())
+        ops.gated_delta_rule(c.dt, *c.at, c.gb, c.bb, pool, pool, c.y, 2, c.tokens, hk, hv, dk, dv, row_stride=c.strides, offsets=c.ob, slots=c.sb, n_slots=n_slots, scale=c.scale, norm_eps=c.eps)
+        far = [_get(pool, slot * one * 4, "<f4", one) for slot in c.slots]
+        y = c.y.read_bytes()
+        assert np.all(_get(pool, 8298 * one * 4, "<f4", one) == 5.5)
+        pool.free()
+        near = Case(DType.BF16, lens, hk, hv, dk, dv)
+        near.state = states
+        near.state_in.upload(states.tobytes())
+        near.call()
+        near.hold()
+        assert y == near.y.read_bytes()
+        assert np.array_equal(np.stack(far).reshape(states.shape), near.results()[1])
+
+
+# ---- offsets past 32 bits
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_logprobs_far_rows(rows):
+    vocab, k = 1000, 4
+    stride = ((1 << 32) // (rows - 1) // 8 + 1) * 8
+    rng = np.random.default_rng(rows)
+    x = rng.standard_normal((1, vocab)).astype(np.float32)
+    logits = GpuBuffer(((rows - 1) * stride + vocab) * 2)
+    _put(logits, (rows - 1) * stride * 2, pack_f32(x, DType.BF16))
+    given = GpuBuffer.from_bytes(np.full(rows, 17, "<u4").tobytes())
+    lp, ent, ids, top = (GpuBuffer(4 * n) for n in (rows, rows, rows * k, rows * k))
+    ops.token_logprobs(DType.BF16, logits, stride, given, 1, lp, ent, ids, top, k, rows, vocab)
+    xv = unpack_f32(pack_f32(x, DType.BF16), DType.BF16).reshape(1, vocab).astype(np.float64)
+    wlp, went, wids, wtop, size, d, z = _reference(xv, np.array([[17]]), k)
+    tol = 1e-5 + 2.0 ** -22 * 10
+    assert _close(_get(lp, 4 * (rows - 1), "<f4", 1), wlp[0], tol) and _close(_get(ent, 4 * (rows - 1), "<f4", 1), went, 1e-5 * size)
+    assert np.array_equal(_get(ids, 4 * (rows - 1) * k, "<u4", k), wids[0]) and _close(_get(top, 4 * (rows - 1) * k, "<f4", k), wtop[0], tol)
+
+
+@pytest.mark.parametrize("block", [1, 128])
+def test_quantize_far_rows(block):
+    rows, cols = 65540, 65552
+    x = GpuBuffer(rows * cols * 2)
+    rng = np.random.default_rng(block)
+    last = unpack_f32(pack_f32(rng.standard_normal((4, cols)).astype(np.float32), DType.BF16), DType.BF16).reshape(4, cols)   # the last block's only rows
+    _put(x, (rows - 4) * cols * 2, pack_f32(last, DType.BF16))
+    codes, scales = GpuBuffer(rows * cols), GpuBuffer(4 * -(-rows // block) * ref.blocks(cols))
+    ops.fp8_quantize(DType.BF16, x, codes, scales, rows, cols, block)
+    wc, ws = ref.quantize(last, block)
+    assert np.array_equal(_get(codes, (rows - 4) * cols, np.uint8, 4 * cols).reshape(4, cols), wc)
+    n = ws.size
+    assert np.array_equal(_get(scales, scales.nbytes - 4 * n, "<f4", n).reshape(ws.shape), ws)
+
+
+@pytest.mark.parametrize("m", [1, 5, 40, 300])
+def test_product_far_weights(m):
+    """Rows of w past 4 GiB; before them is whatever the memory held."""
+    n, k, dt, tail = 66000, 65552, DType.F32, 80          # (the last rows are a block of 128 rows of their own: 66000 = 515 x 128 + 80)
+    rng = np.random.default_rng(m)
+    wt, wst = _weights(rng, tail, k)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    codes, scales = ref.quantize(x, 1)
+    w, ws = GpuBuffer(n * k), GpuBuffer(4 * ref.blocks(n) * ref.blocks(k))
+    _put(w, (n - tail) * k, wt.tobytes())
+    _put(ws, ws.nbytes - wst.nbytes, wst.tobytes())
+    xb, out = GpuBuffer.from_bytes(x.tobytes()), GpuBuffer(4 * m * n)
+    ops.fp8_qmv(dt, w, ws, xb, out, m, n, k)
+    got = np.frombuffer(out.read_bytes(), "<f4").reshape(m, n)[:, n - tail:].astype(np.float64)
+    xv, wv = ref.values(codes, scales, 1), ref.values(wt, wst, 128)
+    want = xv @ wv.T
+    assert np.all(np.abs(got - want) <= _tolerance(xv, wv, want, dt, k))
+
+
+def test_product_far_rows_and_results():
+    """Results past 2^32 bytes and rows of x past 2^32 bytes, in tiles."""
+    m, n, k, dt, tail = 600000, 4096, 16384, DType.BF16, 40
+    rng = np.random.default_rng(1)
+    w, ws = _weights(rng, n, k)
+    xt, xst = ref.quantize(rng.standard_normal((tail, k)).astype(np.float32), 1)
+    wb, wsb = GpuBuffer.from_bytes(w.tobytes()), GpuBuffer.from_bytes(ws.tobytes())
+    x, xs, out = GpuBuffer(m * k), GpuBuffer(4 * m * ref.blocks(k)), GpuBuffer(2 * m * n)
+    _put(x, (m - tail) * k, xt.tobytes())
+    _put(xs, 4 * (m - tail) * ref.blocks(k), xst.tobytes())
+    ops.fp8_qmm(dt, wb, wsb, x, xs, out, m, n, k)
+    got = unpack_f32(_get(out, 2 * (m - tail) * n, np.uint8, 2 * tail * n).tobytes(), dt).reshape(tail, n).astype(np.float64)
+    xv, wv = ref.values(xt, xst, 1), ref.values(w, ws, 128)
+    want = xv @ wv.T
+    assert np.all(np.abs(got - want) <= _tolerance(xv, wv, want, dt, k))
+
+
+# ---- scratch and streams
+
+class _Product:
+    def __init__(self, m, n, k, seed):
+        rng = np.random.default_rng(seed)
+        self.shape = m, n, k
+        w, ws = _weights(rng, n, k)
+        self.w, self.ws = GpuBuffer.from_bytes(w.tobytes()), GpuBuffer.from_bytes(ws.tobytes())
+        self.x = GpuBuffer.from_bytes(pack_f32(rng.standard_normal((m, k)).astype(np.float32), DType.BF16))
+        self.out = GpuBuffer(2 * m * n)
+
+    def call(self):
+        ops.fp8_qmv(DType.BF16, self.w, self.ws, self.x, self.out, *self.shape)
+
+
+def test_calls_one_behind_the_other_share_scratch():
+    """No wait between them: each uses the scratch that the one before may still have."""
+    delta, small, large = Case(DType.F16, [300, 1, 90], 2, 4, 64, 64), _Product(8, 300, 512, 1), _Product(500, 700, 1024, 2)
+    rng = np.random.default_rng(3)
+    x = GpuBuffer.from_bytes(rng.standard_normal((3, 70000)).astype(np.float32).tobytes())
+    ids, top = GpuBuffer(4 * 3 * 8), GpuBuffer(4 * 3 * 8)
+    logprobs = lambda: ops.token_logprobs(DType.F32, x, 70000, None, 0, None, None, ids, top, 8, 3, 70000)
+    calls, outs = [delta.call, small.call, large.call, logprobs], [delta.y, delta.state_out, small.out, large.out, ids, top]
+    for c in calls:
+        c()
+        ops.sync()
+    want = [b.read_bytes() for b in outs]
+    for order in ([0, 1, 2, 3], [3, 2, 1, 0], [1, 0, 3, 2], [2, 3, 0, 1]):
+        for b in outs:
+            b.zero()
+        for i in order * 2:
+            calls[i]()
+        assert [b.read_bytes() for b in outs] == want, order
+
+
+def test_scratch_that_grows_behind_a_graph():
+    """Two graphs captured around a call that needs more scratch, replayed among eager calls that use it."""
+    a, b, large, huge = _Product(8, 300, 512, 1), Case(DType.BF16, [200, 90], 2, 4, 128, 64), _Product(700, 500, 2048, 2), Case(DType.BF16, [3000, 2000], 2, 4, 128, 64)
+    for c in (a, b):
+        c.call()
+    want = a.out.read_bytes(), b.y.read_bytes(), b.state_out.read_bytes()
+    first, second = Graph(), None
+    try:
+        with first:
+            a.call()
+            b.call()
+        large.call()
+        second = Graph()   # (waits for the stream that is left)
+        with second:
+            b.call()
+            a.call()
+        huge.call()
+        ops.sync()
+        for turn in range(3):
+            for g in (first, second):
+                for buf in (a.out, b.y, b.state_out):
+                    buf.zero()
+                ops.sync()   # (the graphs have streams of their own)
+                g.replay()
+                assert (a.out.read_bytes(), b.y.read_bytes(), b.state_out.read_bytes()) == want
+                (large, huge)[turn % 2].call()
+                ops.sync()
+    finally:
+        if second is not None:
+            second.close()
+        first.close()
+
+
+def test_streams_of_the_callers():
+    """From the library's own stream to two of the caller's."""
+    lib, hip = _ensure_init(), C.CDLL("libamdhip64.so")
+    hip.hipStreamCreate.argtypes, hip.hipStreamDestroy.argtypes = [C.POINTER(C.c_void_p)], [C.c_void_p]
+    delta, product = Case(DType.F32, [150, 40], 1, 2, 64, 64), _Product(40, 300, 512, 1)
+    streams = [C.c_void_p(), C.c_void_p()]
+    for s in streams:
+        assert hip.hipStreamCreate(C.byref(s)) == 0
+    try:
+        got = []
+        for s in (None, *streams):
+            _lib.check(lib.mtq_set_stream(s))
+            for b in (delta.y, delta.state_out, product.out):
+                b.zero()
+            delta.call()
+            product.call()
+            ops.sync()
+            got.append([b.read_bytes() for b in (delta.y, delta.state_out, product.out)])
+        assert got[0] == got[1] == got[2]
+    finally:
+        _lib.check(lib.mtq_sync())
+        _lib.check(lib.mtq_set_stream(None))
+        for s in streams:
+            assert hip.hipStreamDestroy(s) == 0
