@@ -350,13 +350,14 @@ MTQ_API int mtq_fp8_quantize(int dtype, const void *x, void *codes, float *scale
                              uint32_t block_rows);
 
 /* out[m, n] = sum_k x[m, k] w[n, k] over the values of both: w codes [N, K] with w_scales f32[ceil(N / 128), ceil(K / 128)],
- * x codes [M, K] with x_scales f32[M, ceil(K / 128)], out T[M, N]. Products of codes are exact, their sums over a block of
- * 128 and the scaled sums of the blocks f32, rounded to T once. Any M. */
+ * x codes [M, K] with x_scales f32[M, ceil(K / 128)], out T[M, N]. Sums over a block of 128 and the scaled sums of the blocks
+ * are f32, rounded to T once. With T = f32 products of codes are exact; with f16 and bf16 the matrix cores drop of eight
+ * neighbouring products what lies below 2^-13 of the largest one's power of two. Any M. */
 MTQ_API int mtq_fp8_qmm(int dtype, const void *w, const float *w_scales, const void *x, const float *x_scales, void *out,
                         uint32_t M, uint32_t N, uint32_t K);
 
 /* The same from activations T[M, K], quantised as mtq_fp8_quantize does with block_rows 1: the decode step's call. Codes
- * and scales go through a library-owned buffer (allocated on first use, grown on demand). Any M. */
+ * and scales of more than a row go through a library-owned buffer (allocated on first use, grown on demand). Any M. */
 MTQ_API int mtq_fp8_qmv(int dtype, const void *w, const float *w_scales, const void *x, void *out, uint32_t M, uint32_t N,
                         uint32_t K);
 
@@ -374,7 +375,9 @@ MTQ_API int mtq_fp8_qmv(int dtype, const void *w, const float *w_scales, const v
  * Sequence i has the tokens offsets[i] .. offsets[i + 1] - 1 (u32[n_seqs + 1] on the device, ascending; none: its state is
  * passed on as it is), or with offsets NULL n_tokens / n_seqs each; its state is slot slots[i] (u32[n_seqs] on the device, no slot
  * twice) or, with slots NULL, slot i. A slot >= n_slots names no state: nothing is written for that sequence. Tokens outside all
- * sequences are left alone, and offsets behind n_tokens read as n_tokens. hk divides hv; dk <= 256. */
+ * sequences are left alone, and offsets behind n_tokens read as n_tokens. hk divides hv; dk <= 256, dv <= 65536.
+ * Sequences that may be long go in chunks of 64 tokens through a library-owned buffer (allocated on first use, grown on demand up
+ * to a gigabyte, or what the option scratch.most_kb allows; more chunks than fit go in turns). */
 MTQ_API int mtq_gated_delta_rule(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v,
                                  size_t v_stride, const float *g, const float *beta, const uint32_t *offsets,
                                  const uint32_t *slots, const float *state_in, float *state_out, float *y, uint32_t n_seqs,

@@ -45,10 +45,25 @@ __device__ __forceinline__ float seg16_max(float v) {   // over rows of 16 lanes
 __device__ __forceinline__ float fp8_scale(float most) { return most > 0.f ? fmaxf(most / kFp8Most, 1.17549435e-38f) : 1.f; }
 
 // Codes of eight elements: the quotient by the scale in f32 (correctly rounded), then the nearest e4m3 value, ties to even.
+// A division is a dozen instructions, which is more than memory leaves time for (4096 x 4096 bf16 by rows: 13.2 us, 10.6 without). With r the
+// correctly rounded 1 / scale, v r is within 1.5 ulp of the quotient; a step q + r (v - q scale) makes it one of the two nearest, and a
+// second the nearest (Markstein's theorem: the difference is exact, and no quotient is closer to the middle of two f32 than the error that is
+// left). That holds while nothing underflows: a quotient that rounds to more than zero is 2^-10 or more, and the difference a multiple of 2^-47
+// of v = 2^-10 scale: scales of 2^-80 and more leave it in range, others are divided by (a scale that is infinite, too).
 __device__ __forceinline__ uint2 fp8_codes(const float (&v)[8], float scale) {
     float q[8];
+    if (scale >= 8.27180613e-25f && scale < INFINITY) {
+        const float r = 1.f / scale;
 #pragma unroll
-    for (int j = 0; j < 8; j++) q[j] = v[j] / scale;
+        for (int j = 0; j < 8; j++) {
+            q[j] = v[j] * r;
+            q[j] = fmaf(fmaf(-q[j], scale, v[j]), r, q[j]);
+            q[j] = copysignf(fmaf(fmaf(-q[j], scale, v[j]), r, q[j]), v[j]);   // (of zeros the sums lose the sign)
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) q[j] = v[j] / scale;
+    }
     int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false), hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
     hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);

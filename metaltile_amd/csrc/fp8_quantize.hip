@@ -15,9 +15,11 @@ struct Fp8QuantArgs {
 
 // 1 x 128 blocks, one to 16 lanes of eight elements each.
 template <int DT> __global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(Fp8QuantArgs a) {
-    const uint64_t at = (uint64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    // The workgroup's first block by one division for all lanes, a lane's from there (blocks are less than 2^23).
+    const uint64_t at0 = (uint64_t)blockIdx.x * 16, at = at0 + (threadIdx.x >> 4);
     if (at >= (uint64_t)a.rows * a.blocks) return;   // (all 16 lanes of a block or none)
-    const uint32_t row = (uint32_t)(at / a.blocks), block = (uint32_t)(at % a.blocks), col = block * kFp8Block + (threadIdx.x & 15u) * 8;
+    const uint32_t row0 = at0 <= UINT32_MAX ? (uint32_t)at0 / a.blocks : (uint32_t)(at0 / a.blocks), from = (uint32_t)(at0 - (uint64_t)row0 * a.blocks) + (threadIdx.x >> 4);
+    const uint32_t on = from / a.blocks, row = row0 + on, block = from - on * a.blocks, col = block * kFp8Block + (threadIdx.x & 15u) * 8;
     const bool in = col < a.cols;
     const size_t i = (size_t)row * a.cols + col;
     float v[8] = {};

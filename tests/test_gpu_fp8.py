@@ -72,6 +72,30 @@ def test_quantize_values_of_their_own(block):
     assert _same_codes(np.frombuffer(cb.read_bytes(), np.uint8).reshape(codes.shape), codes)
 
 
+@pytest.mark.parametrize("lo,hi", [(-20, 20), (-149, -60), (60, 118)])
+def test_quotients_beside_ties(lo, hi):
+    """Elements whose quotients lie on the middle between two codes, or up to two f32 steps beside it, under scales of any mantissa: the f32
+    quotient is the correctly rounded one, and so is the code. Blocks of the smallest scales, which are divided by in another way, too."""
+    rng = np.random.default_rng(hi + 200)
+    finite = np.sort(ref.e4m3_values()[np.isfinite(ref.e4m3_values())])
+    ties = (finite[1:] + finite[:-1]) / 2
+    x = np.zeros((4096, 128), np.float32)
+    most = (448 * (1 + rng.random(4096)) * 2.0 ** rng.integers(lo, hi, 4096)).astype(np.float32)
+    with np.errstate(all="ignore"):
+        scale = np.maximum(most / np.float32(448), np.float32(2.0 ** -126)).astype(np.float64)
+        v = (rng.choice(ties, x.shape) * scale[:, None]).astype(np.float32)
+        for _ in range(2):
+            v = np.where(rng.random(x.shape) < 0.4, np.nextafter(v, np.where(rng.random(x.shape) < 0.5, np.float32(np.inf), np.float32(-np.inf))), v)
+    x[:] = np.clip(v, -most[:, None], most[:, None])
+    x[:, 7] = most
+    x[:, 9], x[:, 11] = -0.0, 0.0
+    codes, scales = ref.quantize(x, 1)
+    xb, cb, sb = GpuBuffer.from_bytes(x.tobytes()), GpuBuffer(x.size), GpuBuffer(4 * scales.size)
+    ops.fp8_quantize(DType.F32, xb, cb, sb, *x.shape, 1)
+    assert np.array_equal(np.frombuffer(sb.read_bytes(), "<f4").reshape(scales.shape), scales)
+    assert np.array_equal(np.frombuffer(cb.read_bytes(), np.uint8).reshape(codes.shape), codes)
+
+
 def _weights(rng, n, k):
     codes = ref.e4m3_codes(np.clip(64 * rng.standard_normal((n, k)), -448, 448))
     return codes, (1e-3 * (0.5 + rng.random((ref.blocks(n), ref.blocks(k))))).astype(np.float32)
