@@ -453,12 +453,13 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ void w
             for (int k = 0; k < NT; k++) mf[ks][k] = get(s, rows_at + ((k * 4 + mine) * KS + ks) * 1024);
         e = four(s, scal_at + (AHEAD ? 0 : 256) + 64 * mine);
     };
+    const uint32_t second = long_row ? lane * 16 : KR_OOB;   // (a row without a second step: nothing is read)
     auto load_tri = [&](__amdgpu_buffer_rsrc_t s) {         // T's or P's
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const uint32_t step = (mine < 2 ? mine : 2 * mine - 2) + (j && long_row ? 1 : 0);
 #pragma unroll
-            for (int k = 0; k < 3; k++) tf[j][k] = get(s, tri_at + (step * 3 + k) * 1024);
+            for (int k = 0; k < 3; k++) tf[j][k] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(s, j ? second : lane * 16, tri_at + (step * 3 + k) * 1024, 0));
         }
         if (AHEAD) wk = four(s, scal_at + 512 + 64 * mine);
     };

@@ -319,7 +319,8 @@ template <int DT> __global__ __launch_bounds__(64 * kWaves, 4) void logprobs_ker
     }
 }
 
-// A row's slices joined by one workgroup: at most kSlicesMost, so that their keys fit the waves' lists.
+// A row's slices joined by one workgroup: at most kSlicesMost, so that their keys fit the waves' lists. (A launch of its own: the last slice's
+// workgroup joining them behind a fence took longer, 33 x 50257 f32 with 20 alternatives 24.5 us against 17.9.)
 constexpr uint32_t kSlicesMost = 32;
 static_assert(kSlicesMost / kWaves * kTopMost <= kListCap && kSlicesMost <= 64, "a wave's share of the slices fits its list and its lanes");
 template <int DT> __global__ __launch_bounds__(64 * kWaves) void logprobs_join_kernel(LogprobArgs a) {
