@@ -265,15 +265,16 @@ template <int DT> __global__ __launch_bounds__(64 * kWaves, 4) void logprobs_ker
         t.s += s;
         if (!c.k) continue;
         if (open) {
-            // A first bar: the k-th largest of the lanes' maxima (of equal ones the lower lane's first) is reached by k elements, and by few more.
+            // A first bar: the k-th largest of the lanes' maxima, bit by bit, is reached by k elements, and by few more. (What 16-bit types leave
+            // below their bits is the same for all values of a sign.)
+            constexpr int LOW = DT == DT_F32 ? 0 : DT == DT_F16 ? 13 : 16;
             const uint32_t o = ordered(top);
-            uint32_t above = 0;
+            uint32_t kth = 0;
 #pragma unroll
-            for (int i = 0; i < 64; i++) {
-                const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)o, i);
-                above += other > o || (other == o && i < (int)lane);
+            for (int b = 31; b >= LOW; b--) {
+                const uint32_t to = kth | 1u << b;
+                kth = (uint32_t)__popcll(__ballot(o >= to)) >= c.k ? to : kth;
             }
-            const uint32_t kth = (uint32_t)__builtin_amdgcn_readlane((int)o, __builtin_ctzll(__ballot(above == c.k - 1)));
             c.raise_bar(((uint64_t)kth << 32) - 1);
             c.bar_value = unordered(kth);
         }
