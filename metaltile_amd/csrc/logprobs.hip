@@ -290,10 +290,12 @@ template <int DT> __global__ __launch_bounds__(64 * kWaves, 4) void logprobs_ker
 #pragma unroll
                 for (int i = 1; i < NV; i++)
                     if (u == i) r = raw[i];
-                uint32_t most = 0;
+                if (c.n + 64 * PER > kListCap) {                              // (a vector of candidates might not fit)
+                    uint32_t most = 0;
 #pragma unroll
-                for (int j = 0; j < PER; j++) most += __popcll(__ballot(!(value(r, j) < c.bar_value)));
-                if (c.n + most > kListCap) c.draw();                          // (then they fit: at most 32 and 512)
+                    for (int j = 0; j < PER; j++) most += __popcll(__ballot(!(value(r, j) < c.bar_value)));
+                    if (c.n + most > kListCap) c.draw();                      // (then they fit: at most 32 and 512)
+                }
 #pragma unroll
                 for (int j = 0; j < PER; j++) {
                     const float v = value(r, j);
@@ -305,7 +307,7 @@ template <int DT> __global__ __launch_bounds__(64 * kWaves, 4) void logprobs_ker
                     c.n += __popcll(who);
                 }
             }
-            if (more && (open || c.n > c.k + 8)) c.draw();
+            if (more && c.n > c.k + 12) c.draw();
         }
         open = false;
     }
