@@ -81,6 +81,21 @@ template <int DT, int BM, int BN, int WM, int WN, int STAGES> __device__ __force
     for (int b = 0; b < STAGES; b++) load(b, 0, QX + QW);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+    auto meet = [&] {   // the next block is whole when no more of a wave's loads are on their way than those for the stages behind it, and all waves say so
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * (QX + QW)) : "memory");
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    };
+    if (wm * (BM / WM) >= rows_m) {   // all of this wave's rows are behind the last: it has loads only, and leaves the LDS to the others
+        static_assert(BM / 64 <= WN, "the scales are brought by waves of the first rows");
+        for (uint32_t b = 0; b < blocks; b++) {
+            meet();
+            load(b + STAGES, 0, QX + QW);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        return;
+    }
     const uint32_t o0 = r * 128 + ((g ^ (r & 7u)) << 4), o1 = o0 ^ 64u;   // pieces g and 4 + g of row r
     uint4 wv[TN][2], xv[2][2];
     float scale[2] = {};
@@ -119,12 +134,7 @@ template <int DT, int BM, int BN, int WM, int WN, int STAGES> __device__ __force
             if (t + 1 < TM) {
                 read_x(b, t + 1, w);
             } else {
-                // All of this block is read. The next one is whole when no more of this wave's loads are on their way than those for the
-                // stages behind it; what other waves brought is there, and this block's stage is free, behind the barrier.
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * (QX + QW)) : "memory");
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-                __builtin_amdgcn_s_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+                meet();   // (all of this block is read: its stage is free behind this)
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
