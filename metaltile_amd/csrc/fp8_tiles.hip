@@ -16,7 +16,8 @@
 //
 // 256 x 256 tiles do twice the products of 128 x 128 ones for each byte that they read, but come in few: 224 of them (1024 x 14336) take as
 // long as 256, and what is left over after whole rounds costs a round. Their time by the round, with K = 4096: 58 us, as tiles cut in two 38,
-// of 128 x 128 ones 25 (16 waves, four stages); f32 results, whose codes are unpacked to bf16 for the products (fp8_common.h), have two
+// of 128 x 128 ones 25 (16 waves, four stages). Where 128 x 64 ones (8 waves) are no more than the CUs they end sooner: 128 x 14336 23.4 us with
+// the quantising against 26.8, 512 x 4096 23.6 against 26.5. f32 results, whose codes are unpacked to bf16 for the products (fp8_common.h), have two
 // workgroups of 128 x 128 a CU (4096^3: 143 us against 231 with one and four stages).
 #include "fp8_common.h"
 
@@ -27,8 +28,8 @@ namespace {
 // 16 bytes a lane from rsrc + voff (past the end: zeros) to LDS: lane l's at lds + 16 l. No register is written; counts in vmcnt.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"   // M0 is a reserved register: naming it as clobbered is the point
-__device__ __forceinline__ void lds_load16(uint32_t lds, uint32_t voff, uint32_t soff, __attribute__((ext_vector_type(4))) uint32_t rsrc) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
+__device__ __forceinline__ void lds_load16(uint32_t lds, uint32_t voff, __attribute__((ext_vector_type(4))) uint32_t rsrc) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 __device__ __forceinline__ __attribute__((ext_vector_type(4))) uint32_t tile_rsrc(const uint8_t* base, uint32_t bytes) {
@@ -61,16 +62,17 @@ template <int DT, int BM, int BN, int WM, int WN, int STAGES> __device__ __force
     auto load = [&](uint32_t b, int from, int end) {   // a part of block b's codes into its stage; behind the last block: zeros
         const bool in = b * kFp8Block < k_left && 16 * chunk < a.K;
         const uint32_t to = lds0 + (b & (STAGES - 1)) * STAGE;
-        const uint32_t v = in ? v0 + b * kFp8Block : kOutOfRange;
+        uint32_t v = in ? v0 + b * kFp8Block : kOutOfRange;   // (rows are added here and not as a scalar offset: some are behind the tile's last)
+        asm volatile("" : "+v"(v));                           // (the pieces' offsets are not kept from block to block: the registers are the results')
 #pragma unroll
-        for (int q = 0; q < QX; q++) if (q >= from && q < end) lds_load16(__builtin_amdgcn_readfirstlane(to + (wave * QX + q) * 1024), v, 8 * (wave * QX + q) * a.K, rx);
+        for (int q = 0; q < QX; q++) if (q >= from && q < end) lds_load16(__builtin_amdgcn_readfirstlane(to + (wave * QX + q) * 1024), v + 8 * (wave * QX + q) * a.K, rx);
 #pragma unroll
-        for (int q = 0; q < QW; q++) if (QX + q >= from && QX + q < end) lds_load16(__builtin_amdgcn_readfirstlane(to + BM * 128 + (wave * QW + q) * 1024), v, 8 * (wave * QW + q) * a.K, rw);
+        for (int q = 0; q < QW; q++) if (QX + q >= from && QX + q < end) lds_load16(__builtin_amdgcn_readfirstlane(to + BM * 128 + (wave * QW + q) * 1024), v + 8 * (wave * QW + q) * a.K, rw);
     };
     auto load_scales = [&](uint32_t w) {   // window w's, of row 64 wave + lane (what is behind a row's last block is not used)
         if (wave >= BM / 64) return;
         const uint32_t row = 64 * wave + lane;
-        lds_load16(__builtin_amdgcn_readfirstlane(lds0 + SCALES + (w & 1u) * (BM * kWindow * 4) + wave * 1024), row < rows_m ? (row * blocks + w * kWindow) * 4 : kOutOfRange, 0, rs);
+        lds_load16(__builtin_amdgcn_readfirstlane(lds0 + SCALES + (w & 1u) * (BM * kWindow * 4) + wave * 1024), row < rows_m ? (row * blocks + w * kWindow) * 4 : kOutOfRange, rs);
     };
     // (a wave's n lie in one block of 128: BN / WN divides it)
     const uint32_t nb = (n0 + wn * (BN / WN)) / kFp8Block, nbs = fp8_blocks(a.N);
@@ -184,16 +186,16 @@ template <int DT, int BM, int BN, int WM, int WN, int STAGES, bool HALVES> __glo
     fp8_tile<DT, BM, BN, WM, WN, STAGES>(a, m0, n0, lds);
 }
 
-uint64_t tiles_of(const Fp8Args& a, uint32_t side) { return (uint64_t)((a.M + side - 1) / side) * ((a.N + side - 1) / side); }
+uint64_t tiles_of(const Fp8Args& a, uint32_t bm, uint32_t bn) { return (uint64_t)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); }
 
-template <int SIDE, int WM, int WN, int STAGES, bool HALVES, int... DTS> int launch(int dtype, const Fp8Args& p, uint32_t halved, const LaunchCtx& lc) {
+template <int BM, int BN, int WM, int WN, int STAGES, bool HALVES, int... DTS> int launch(int dtype, const Fp8Args& p, uint32_t halved, const LaunchCtx& lc) {
     Fp8Args a = p;
-    const uint64_t total = tiles_of(a, SIDE);
+    const uint64_t total = tiles_of(a, BM, BN);
     if (total + halved > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more tiles than a launch can have workgroups");
-    uint32_t tm = (a.M + SIDE - 1) / SIDE, tn = (a.N + SIDE - 1) / SIDE, whole = (uint32_t)total - halved;
+    uint32_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN, whole = (uint32_t)total - halved;
     const void* fn = nullptr;
-    ((dtype == DTS ? (void)(fn = (const void*)fp8_tiles_kernel<DTS, SIDE, SIDE, WM, WN, STAGES, HALVES>) : (void)0), ...);
-    constexpr size_t lds = STAGES * 2 * SIDE * 128 + 2 * SIDE * kWindow * sizeof(float);
+    ((dtype == DTS ? (void)(fn = (const void*)fp8_tiles_kernel<DTS, BM, BN, WM, WN, STAGES, HALVES>) : (void)0), ...);
+    constexpr size_t lds = STAGES * (BM + BN) * 128 + 2 * BM * kWindow * sizeof(float);
     static_assert(lds <= 160 * 1024, "");
     MTQ_HIP(set_max_dynamic_lds(fn, lds));
     void* args[] = {&a, &tm, &tn, &whole};
@@ -204,14 +206,16 @@ template <int SIDE, int WM, int WN, int STAGES, bool HALVES, int... DTS> int lau
 }  // namespace
 
 int launch_fp8_tiles(int dtype, const Fp8Args& p, const LaunchCtx& lc) {
-    if (dtype == DT_F32) return launch<128, 2, 2, 2, false, DT_F32>(dtype, p, 0, lc);
-    const uint64_t cus = (uint64_t)fp8_num_cus(), large = tiles_of(p, 256), small = tiles_of(p, 128), over = large % cus;
+    if (dtype == DT_F32) return launch<128, 128, 2, 2, 2, false, DT_F32>(dtype, p, 0, lc);
+    const uint64_t cus = (uint64_t)fp8_num_cus();
+    if (tiles_of(p, 128, 64) <= cus) return launch<128, 64, 4, 2, 4, false, DT_F16, DT_BF16>(dtype, p, 0, lc);
+    const uint64_t large = tiles_of(p, 256, 256), small = tiles_of(p, 128, 128), over = large % cus;
     // What is over after whole rounds of the CUs is cut in two where that gives each CU one half at most.
     const uint32_t halved = over && 2 * over <= cus ? (uint32_t)over : 0;
     // (the rounds' times as measured, in units of a tenth of a round of small tiles)
     const uint64_t large_time = large / cus * 24 + (halved ? 15 : over ? 24 : 0), small_time = (small + cus - 1) / cus * 10;
-    if (large_time < small_time) return launch<256, 2, 4, 2, true, DT_F16, DT_BF16>(dtype, p, halved, lc);
-    return launch<128, 4, 4, 4, false, DT_F16, DT_BF16>(dtype, p, 0, lc);
+    if (large_time < small_time) return launch<256, 256, 2, 4, 2, true, DT_F16, DT_BF16>(dtype, p, halved, lc);
+    return launch<128, 128, 4, 4, 4, false, DT_F16, DT_BF16>(dtype, p, 0, lc);
 }
 
 }  // namespace mtq

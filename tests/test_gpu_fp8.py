@@ -142,8 +142,8 @@ def test_products(dt, m, n, k):
     assert m > 16 or np.allclose(unpack_f32(results[0][:size], dt), unpack_f32(results[1][:size], dt), rtol=2 * HALF_STEP[dt], atol=float(tol.max()))
 
 
-# More tiles than the CUs take as groups of rows: 128 x 128, 256 x 256, those cut in two (with a lower half behind the last row), f32 as well.
-TILED = [(40, 16500, 272), (129, 4112, 400), (300, 4200, 656), (65, 8200, 1168), (400, 8300, 144), (2600, 4700, 272), (4100, 4360, 400)]
+# More tiles than the CUs take as groups of rows: 128 x 128, 128 x 64, 256 x 256, those cut in two (with a lower half behind the last row), f32 as well.
+TILED = [(40, 16500, 272), (129, 4112, 400), (300, 4200, 656), (65, 8200, 1168), (400, 8300, 144), (2600, 4700, 272), (4100, 4360, 400), (130, 8300, 784)]
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
@@ -153,7 +153,7 @@ def test_products_in_tiles(dt, m, n, k):
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
-@pytest.mark.parametrize("m,n,k", [(129, 4112, 400), (300, 4200, 656), (400, 8300, 144), (2600, 4700, 272), (4100, 4360, 144)])
+@pytest.mark.parametrize("m,n,k", [(129, 4112, 400), (300, 4200, 656), (400, 8300, 144), (2600, 4700, 272), (4100, 4360, 144), (130, 8300, 400)])
 def test_exact_in_tiles(dt, m, n, k):
     """Codes of -1, 0 and 1 and scales of 1: every sum is a whole number, which bf16 holds up to 256."""
     rng = np.random.default_rng(m)
