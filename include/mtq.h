@@ -376,6 +376,7 @@ MTQ_API int mtq_fp8_qmv(int dtype, const void *w, const float *w_scales, const v
  * passed on as it is), or with offsets NULL n_tokens / n_seqs each; its state is slot slots[i] (u32[n_seqs] on the device, no slot
  * twice) or, with slots NULL, slot i. A slot >= n_slots names no state: nothing is written for that sequence. Tokens outside all
  * sequences are left alone, and offsets behind n_tokens read as n_tokens. hk divides hv; dk <= 256, dv <= 65536.
+ * A NaN or an infinity among the inputs reaches what comes behind it in its sequence and head (from v and the state: in its column).
  * Sequences that may be long go in chunks of 64 tokens through a library-owned buffer (allocated on first use, grown on demand up
  * to a gigabyte, or what the option scratch.most_kb allows; more chunks than fit go in turns). */
 MTQ_API int mtq_gated_delta_rule(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v,

@@ -274,9 +274,10 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256, DKP * NT <=
             const double last = __shfl(sum, 63, 64);
             float* sc = (float*)(head_out + (size_t)wave * kHeadBytes + 2 * kTriBytes);
             const float e = __expf((float)sum);
-            sc[lane] = e * rk[lane];
+            const float later = __expf((float)(last - sum));
+            sc[lane] = beta * later * 0.f == 0.f ? e * rk[lane] : NAN;   // (what is no number would meet zeros in T and W, too: the walk is told here)
             sc[64 + lane] = e * rq[lane];
-            sc[128 + lane] = rk[lane] * __expf((float)(last - sum));
+            sc[128 + lane] = rk[lane] * later;
             sc[192 + lane] = __expf((float)last);
         }
         if (of == 0) __syncthreads();
@@ -397,6 +398,7 @@ template <int DKP> struct WalkLds {
     Columns<DKP> S[3];                             // terms of the state
     Columns<kChunk> X[3], U[3], W[3];
     uint32_t touched[64];                          // where the words that bring lines into the L2 end up
+    uint32_t bad;                                  // a chunk's X has an infinity or a NaN
 };
 
 struct WalkPlace {
@@ -415,7 +417,10 @@ struct WalkPlace {
 //   a..b: X = V - e^G r (K S0)         | Y = Q S0 + P U of the chunk before, to memory
 //   b..c: U = T X                      | Q S0
 //   c..a: S1 = e^G S0 + K^T (r e^.. U), its terms to LDS
-template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ void walk(const DeltaArgs& d, const WalkPlace& w, WalkLds<DKP>& lds, uint32_t wave) {
+//
+// A product with a triangle multiplies what is behind a token by zero, which an infinity or a NaN there survives: a chunk with one in X is left,
+// with the tokens behind it, to the token by token form, and the state before it to state_out. Returns that chunk, or w.end.
+template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ uint32_t walk(const DeltaArgs& d, const WalkPlace& w, WalkLds<DKP>& lds, uint32_t wave) {
     using L = Layout<DKP, NT>;
     constexpr int ES = DT == DT_F32 ? 4 : 2;
     constexpr int KS = DKP / 32, TILES = DKP / 16, NS = TILES > 8 ? TILES / 8 : 1;   // NS: 16-row tiles of the state a wave has
@@ -453,8 +458,10 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ void w
             for (int k = 0; k < NT; k++) mf[ks][k] = get(s, rows_at + ((k * 4 + mine) * KS + ks) * 1024);
         e = four(s, scal_at + (AHEAD ? 0 : 256) + 64 * mine);
     };
-    const uint32_t second = long_row ? lane * 16 : KR_OOB;   // (a row without a second step: nothing is read)
-    auto load_tri = [&](__amdgpu_buffer_rsrc_t s) {         // T's or P's
+    auto load_tri = [&](__amdgpu_buffer_rsrc_t s) {         // T's or P's (a row without a second step: nothing is read there)
+        uint32_t none = long_row ? 0 : KR_OOB;
+        asm volatile("" : "+s"(none));                      // (added anew: a register less)
+        const uint32_t second = lane * 16 + none;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const uint32_t step = (mine < 2 ? mine : 2 * mine - 2) + (j && long_row ? 1 : 0);
@@ -548,7 +555,8 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ void w
     }
     put_state();
     if (AHEAD) __builtin_amdgcn_s_setprio(3);
-    for (uint32_t c = w.begin; c < w.end; c++) {
+    uint32_t c = w.begin;
+    for (; c < w.end; c++) {
         const auto here = slot(c), next = slot(c + 1 < w.end ? c + 1 : c);
         walk_barrier();
         if constexpr (AHEAD) {
@@ -557,6 +565,7 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ void w
 #pragma unroll
             for (int i = 0; i < 4; i++) x[i] = value(v[i]) - e[i] * x[i];
             asm volatile("" : "+v"(x));   // (here, not behind the next loads into e's and v's registers)
+            if (__ballot(!(x[0] * 0.f + x[1] * 0.f + x[2] * 0.f + x[3] * 0.f == 0.f))) lds.bad = 1;
             put(lds.X[0].at(r, 16 * mine + 4 * g), Columns<kChunk>::PLANE, x);
         } else if (c > w.begin) {
             give_y(c - 1, [&] { load_kt(here); });
@@ -564,6 +573,7 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ void w
             load_kt(here);
         }
         walk_barrier();
+        const uint32_t bad = lds.bad;
         f32x4 late;
         if constexpr (AHEAD) {
             f32x4 u = {};
@@ -578,6 +588,7 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ void w
             asm volatile("" : "+v"(y));
         }
         walk_barrier();
+        if (__builtin_amdgcn_readfirstlane(bad)) break;
         u32x4 b[2][3];
 #pragma unroll
         for (int ts = 0; ts < 2; ts++)
@@ -602,8 +613,11 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ void w
         }
         put_state();
     }
-    walk_barrier();   // (the last chunk's U)
-    if constexpr (!AHEAD) give_y(w.end - 1, nothing);
+    if (AHEAD) __builtin_amdgcn_s_setprio(0);
+    if (c == w.end) {
+        walk_barrier();   // (the last chunk's U)
+        if constexpr (!AHEAD) give_y(w.end - 1, nothing);
+    }
     if (col_in && has_state)
 #pragma unroll
         for (int x = 0; x < NS; x++) {
@@ -612,6 +626,7 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ void w
             for (int i = 0; i < 4; i++)
                 if (row + i < d.dk) d.state_out[state + row + i] = S[x][i];
         }
+    return c;
 }
 
 // The walk's last wave: brings what the others read kAheadChunks chunks later from memory into the XCD's L2, a word of every 128-byte line (a
@@ -646,6 +661,10 @@ template <int DT, int DKP, int NT> __device__ __forceinline__ void walk_touch(co
         walk_barrier();
         walk_barrier();
         walk_barrier();
+        if (__builtin_amdgcn_readfirstlane(lds.bad)) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            return;
+        }
     }
     walk_barrier();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -664,29 +683,46 @@ template <int DT, int DKP, int NT, bool TOUCH, int PER_SIMD> __global__ __launch
     const DeltaSeq s = delta_seq(d, seq);
     if (!s.any) return;
     const uint32_t len = s.to - s.from, first = first_slot(s, seq);
+    DeltaSeq one = s;                      // what goes token by token, and from which states
+    const float* from = d.state_in;
     if (len <= kFewTokens) {
-        if (first < a.lo || first >= a.hi || wave >= 4) return;
-        if (a.whole && d.dk == DKP) delta_tokens<DT, DKP / 16, true, 1>(d, s, h, c0 + 4 * wave);
-        else delta_tokens<DT, DKP / 16, false, 1>(d, s, h, c0 + 4 * wave);
-        return;
+        if (first < a.lo || first >= a.hi) return;
+    } else {
+        const uint32_t chunks = (len + kChunk - 1) / kChunk;
+        WalkPlace w;
+        w.begin = a.lo > first ? a.lo - first : 0;
+        w.end = a.hi <= first ? 0 : a.hi - first < chunks ? a.hi - first : chunks;
+        if (w.begin >= w.end) return;
+        w.slot_bytes = L::slot_bytes(d.hk, d.hv);
+        w.base = a.scratch + (size_t)(first + w.begin - a.lo) * w.slot_bytes;
+        w.from = s.from;
+        w.to = s.to;
+        w.h = h;
+        w.kh = h / (d.hv / d.hk);
+        w.c0 = c0;
+        w.state = ((size_t)s.slot * d.hv + h) * d.dv * d.dk;
+        w.state_from = w.begin ? d.state_out : d.state_in;
+        if (threadIdx.x == 0) lds.bad = 0;
+        uint32_t done;
+        if (wave < 4) {
+            done = walk<DT, DKP, NT, true>(d, w, lds, wave);
+        } else if (wave < 8) {
+            done = walk<DT, DKP, NT, false>(d, w, lds, wave);
+        } else {
+            if constexpr (TOUCH) walk_touch<DT, DKP, NT>(d, w, lds, columns);
+            return;
+        }
+        if (done == w.end) return;
+        __syncthreads();                   // (the states are in memory)
+        one.from = s.from + done * kChunk;
+        if (w.end < chunks) one.to = s.from + w.end * kChunk;
+        from = d.state_out;
     }
-    const uint32_t chunks = (len + kChunk - 1) / kChunk;
-    WalkPlace w;
-    w.begin = a.lo > first ? a.lo - first : 0;
-    w.end = a.hi <= first ? 0 : a.hi - first < chunks ? a.hi - first : chunks;
-    if (w.begin >= w.end) return;
-    w.slot_bytes = L::slot_bytes(d.hk, d.hv);
-    w.base = a.scratch + (size_t)(first + w.begin - a.lo) * w.slot_bytes;
-    w.from = s.from;
-    w.to = s.to;
-    w.h = h;
-    w.kh = h / (d.hv / d.hk);
-    w.c0 = c0;
-    w.state = ((size_t)s.slot * d.hv + h) * d.dv * d.dk;
-    w.state_from = w.begin ? d.state_out : d.state_in;
-    if (wave < 4) walk<DT, DKP, NT, true>(d, w, lds, wave);
-    else if (wave < 8) walk<DT, DKP, NT, false>(d, w, lds, wave);
-    else if constexpr (TOUCH) walk_touch<DT, DKP, NT>(d, w, lds, columns);
+    if (wave >= 4) return;
+    DeltaArgs tokens = d;
+    tokens.state_in = from;
+    if (a.whole && d.dk == DKP) delta_tokens<DT, DKP / 16, true, 1>(tokens, one, h, c0 + 4 * wave);
+    else delta_tokens<DT, DKP / 16, false, 1>(tokens, one, h, c0 + 4 * wave);
 }
 
 template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* scratch, size_t bytes, const LaunchCtx& lc) {

@@ -11,7 +11,7 @@ from metaltile_amd.runtime import _ensure_init
 from tests import fp8_reference as ref
 from tests.hip_graph import Graph
 from tests.test_gpu_fp8 import _tolerance, _weights
-from tests.test_gpu_gated_delta import Case
+from tests.test_gpu_gated_delta import Case, rule
 from tests.test_gpu_token_logprobs import _close, _reference
 
 pytestmark = pytest.mark.gpu
@@ -72,6 +72,40 @@ def test_delta_slots_of_a_large_pool():
         near.hold()
         assert y == near.y.read_bytes()
         assert np.array_equal(np.stack(far).reshape(states.shape), near.results()[1])
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
+@pytest.mark.parametrize("what", ["q", "k", "v", "g", "beta", "state"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf], ids=str)
+@pytest.mark.parametrize("most_kb", [0, 400])
+def test_delta_no_numbers(dt, what, bad, most_kb):
+    """A NaN or an infinity reaches what comes behind it in its sequence, its head and, from v and the state, its column, and nothing else: not the tokens
+    before it, of the same chunk or others, in prompts, short sequences and single tokens, with all chunks at once or in windows."""
+    lens, hk, hv, dk, dv = [150, 5, 200, 1, 70, 64], 2, 4, 64, 48
+    c = Case(dt, lens, hk, hv, dk, dv)
+    at = {"q": (c.q, [(70, 1, 3), (352, 0, 0), (375, 0, 5)]), "k": (c.k, [(70, 1, 3), (152, 0, 0), (300, 0, 9)]), "v": (c.v, [(70, 1, 3), (153, 2, 5), (300, 0, 40), (420, 3, 47), (489, 0, 0)]),
+          "g": (c.g, [(70, 1), (152, 0), (300, 3)]), "beta": (c.beta, [(70, 1), (152, 0), (300, 3), (355, 2)]), "state": (c.state, [(0, 1, 3, 5), (2, 0, 0, 0), (3, 2, 40, 63)])}[what]
+    for i in at[1]:
+        at[0][i] = bad
+    c.bufs[0].upload(pack_f32(np.concatenate([x.reshape(c.tokens, -1) for x in (c.q, c.k, c.v)], 1).astype(np.float32), dt))
+    c.gb.upload(c.g.tobytes())
+    c.bb.upload(c.beta.tobytes())
+    c.state_in.upload(c.state.tobytes())
+    lib = _ensure_init()
+    try:
+        _lib.check(lib.mtq_set_option(b"scratch.most_kb", most_kb))
+        c.call()
+        y, S = c.results()
+    finally:
+        _lib.check(lib.mtq_set_option(b"scratch.most_kb", 0))
+    with np.errstate(all="ignore"):
+        wy, wS = rule(*(x.astype(np.float64) for x in (c.q, c.k, c.v, c.g, c.beta, c.state)), list(zip(c.offsets[:-1], c.offsets[1:])), range(len(lens)), c.scale, c.eps)
+        assert np.array_equal(np.isfinite(y), np.isfinite(wy)) and np.array_equal(np.isfinite(S), np.isfinite(wS))
+        assert not np.isfinite(y).all() and np.isfinite(y).mean() > 0.5
+        rel = (dk / 16 + 16) * 2.0 ** -24 * 200
+        for got, want in ((y, wy), (S, wS)):
+            fine = np.isfinite(want)
+            assert np.all(np.abs(got[fine] - want[fine]) <= rel * np.abs(want[fine]).max())
 
 
 # ---- offsets past 32 bits
