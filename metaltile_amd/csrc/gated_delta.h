@@ -56,41 +56,35 @@ template <int DT, int DKL, bool WHOLE> __device__ __forceinline__ void load_part
     }
 }
 
-// A wave's columns `first` .. first + 4 NC - 1 of head h, over a sequence's tokens one by one.
+// A wave's columns `first` .. first + 3 of head h, over a sequence's tokens one by one.
 //
-// A wave has 4 NC columns of the state (rows of S: dv) in registers, 16 lanes to a column, each with dk / 16 neighbouring values, so that
+// A wave has four columns of the state (rows of S: dv) in registers, 16 lanes to a column, each with dk / 16 neighbouring values, so that
 // the state is read and written in whole lines. Both products with the state use what it was before the token,
 //   S k = exp(g) (S0 k),   S q = exp(g) (S0 q) + (k . q) u,
-// so that neither waits for the update. A single token is bound by reading and writing the state; many tokens by the seven operations
-// on each of its values, of which the vector units do one a lane and cycle. The next token's rows are loaded while one is computed.
+// so that neither waits for the update. A single token is bound by reading and writing the state (64 sequences of 32 heads, dk = dv = 128: 57.7 us
+// for 270 MB); many tokens by the seven operations on each of its values, of which the vector units do one a lane and cycle. The next token's
+// rows are loaded while one is computed.
 //
-// DKL: values of k a lane; WHOLE: dk = 16 DKL and every row on 16 bytes; NC: columns a lane.
-template <int DT, int DKL, bool WHOLE, int NC> __device__ __forceinline__ void delta_tokens(const DeltaArgs& a, const DeltaSeq& s, uint32_t h, uint32_t first) {
+// DKL: values of k a lane; WHOLE: dk = 16 DKL and every row on 16 bytes.
+template <int DT, int DKL, bool WHOLE> __device__ __forceinline__ void delta_tokens(const DeltaArgs& a, const DeltaSeq& s, uint32_t h, uint32_t first) {
     const uint32_t lane = threadIdx.x & 63u;
     if (first >= a.dv) return;
-    const uint32_t d0 = (lane & 15u) * DKL, c0 = first + (lane >> 4);
+    const uint32_t d0 = (lane & 15u) * DKL, col = first + (lane >> 4);
+    const bool in = col < a.dv;
     const uint32_t hk = h / (a.hv / a.hk);
-    const size_t state = ((size_t)s.slot * a.hv + h) * a.dv;
-    float S[NC][DKL];
+    const size_t state = (((size_t)s.slot * a.hv + h) * a.dv + col) * a.dk;
+    float S[DKL];
+    if (a.state_in && in) load_part<DT_F32, DKL, WHOLE>(a.state_in, state, d0, a.dk, S);
+    else
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const uint32_t col = c0 + 4 * c;
-        if (a.state_in && col < a.dv) load_part<DT_F32, DKL, WHOLE>(a.state_in, (state + col) * a.dk, d0, a.dk, S[c]);
-        else
-#pragma unroll
-            for (int j = 0; j < DKL; j++) S[c][j] = 0.f;
-    }
+        for (int j = 0; j < DKL; j++) S[j] = 0.f;
     struct Token {
-        float q[DKL], k[DKL], v[NC], g, beta;
+        float q[DKL], k[DKL], v, g, beta;
     };
     auto load = [&](uint32_t t, Token& x) {
         load_part<DT, DKL, WHOLE>(a.q, (size_t)t * a.q_stride + (size_t)hk * a.dk, d0, a.dk, x.q);
         load_part<DT, DKL, WHOLE>(a.k, (size_t)t * a.k_stride + (size_t)hk * a.dk, d0, a.dk, x.k);
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const uint32_t col = c0 + 4 * c;
-            x.v[c] = load_elem<DT>(a.v, (size_t)t * a.v_stride + (size_t)h * a.dv + (col < a.dv ? col : a.dv - 1));
-        }
+        x.v = load_elem<DT>(a.v, (size_t)t * a.v_stride + (size_t)h * a.dv + (in ? col : a.dv - 1));
         x.g = a.g[(size_t)t * a.hv + h];
         x.beta = a.beta[(size_t)t * a.hv + h];
     };
@@ -99,19 +93,14 @@ template <int DT, int DKL, bool WHOLE, int NC> __device__ __forceinline__ void d
     for (uint32_t t = s.from; t < s.to; t++) {
         Token next = x;
         if (t + 1 < s.to) load(t + 1, next);
-        float qq = 0.f, kk = 0.f, qk = 0.f, Sk[NC], Sq[NC];
-#pragma unroll
-        for (int c = 0; c < NC; c++) Sk[c] = Sq[c] = 0.f;
+        float qq = 0.f, kk = 0.f, qk = 0.f, Sk = 0.f, Sq = 0.f;
 #pragma unroll
         for (int j = 0; j < DKL; j++) {
             qq += x.q[j] * x.q[j];
             kk += x.k[j] * x.k[j];
             qk += x.q[j] * x.k[j];
-#pragma unroll
-            for (int c = 0; c < NC; c++) {
-                Sk[c] += S[c][j] * x.k[j];
-                Sq[c] += S[c][j] * x.q[j];
-            }
+            Sk += S[j] * x.k[j];
+            Sq += S[j] * x.q[j];
         }
         qk = sum16(qk);
         float rq = a.scale, rk = 1.f;
@@ -120,30 +109,22 @@ template <int DT, int DKL, bool WHOLE, int NC> __device__ __forceinline__ void d
             rk = 1.f / sqrtf(sum16(kk) + a.norm_eps);
         }
         const float keep = expf(x.g);
+        const float u = x.beta * (x.v - keep * rk * sum16(Sk)), uk = u * rk;
+        const float y = rq * (keep * sum16(Sq) + qk * uk);
+        if ((lane & 15u) == 0 && in) a.y[((size_t)t * a.hv + h) * a.dv + col] = y;
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const uint32_t col = c0 + 4 * c;
-            const float u = x.beta * (x.v[c] - keep * rk * sum16(Sk[c])), uk = u * rk;
-            const float y = rq * (keep * sum16(Sq[c]) + qk * uk);
-            if ((lane & 15u) == 0 && col < a.dv) a.y[((size_t)t * a.hv + h) * a.dv + col] = y;
-#pragma unroll
-            for (int j = 0; j < DKL; j++) S[c][j] = keep * S[c][j] + x.k[j] * uk;
-        }
+        for (int j = 0; j < DKL; j++) S[j] = keep * S[j] + x.k[j] * uk;
         x = next;
     }
+    if (!in) return;
+    float* o = a.state_out + state + d0;
+    if constexpr (WHOLE && DKL % 4 == 0) {
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const uint32_t col = c0 + 4 * c;
-        if (col >= a.dv) continue;
-        float* o = a.state_out + (state + col) * a.dk + d0;
-        if constexpr (WHOLE && DKL % 4 == 0) {
+        for (int j = 0; j < DKL; j += 4) *(float4*)(o + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+    } else {
 #pragma unroll
-            for (int j = 0; j < DKL; j += 4) *(float4*)(o + j) = make_float4(S[c][j], S[c][j + 1], S[c][j + 2], S[c][j + 3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < DKL; j++)
-                if (d0 + j < a.dk) o[j] = S[c][j];
-        }
+        for (int j = 0; j < DKL; j++)
+            if (d0 + j < a.dk) o[j] = S[j];
     }
 }
 

@@ -721,8 +721,8 @@ template <int DT, int DKP, int NT, bool TOUCH, int PER_SIMD> __global__ __launch
     if (wave >= 4) return;
     DeltaArgs tokens = d;
     tokens.state_in = from;
-    if (a.whole && d.dk == DKP) delta_tokens<DT, DKP / 16, true, 1>(tokens, one, h, c0 + 4 * wave);
-    else delta_tokens<DT, DKP / 16, false, 1>(tokens, one, h, c0 + 4 * wave);
+    if (a.whole && d.dk == DKP) delta_tokens<DT, DKP / 16, true>(tokens, one, h, c0 + 4 * wave);
+    else delta_tokens<DT, DKP / 16, false>(tokens, one, h, c0 + 4 * wave);
 }
 
 template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* scratch, size_t bytes, const LaunchCtx& lc) {
