@@ -1368,6 +1368,8 @@ static int check_dtype(int dtype) {
     return ERR_OK;
 }
 static bool on_16(const void* p) { return (uintptr_t)p % 16 == 0; }
+// Whether all of these begin on a multiple of `bytes` (a null pointer does).
+template <class... P> static bool on(size_t bytes, P... p) { return ((uintptr_t)p | ...) % bytes == 0; }
 
 static constexpr uint32_t kFp8Longest = 1u << 30;   // (indexes of a row, a column or a block past the last fit 32 bits)
 
@@ -1380,6 +1382,7 @@ static int op_fp8_quantize(int dtype, const void* x, void* codes, float* scales,
     if (rows == 0) return ERR_OK;
     if (!x || !codes || !scales) return fail(ERR_BAD_ARG, "null buffer");
     if (!on_16(x) || !on_16(codes)) return fail(ERR_BAD_ARG, "x and codes must be on 16 bytes");
+    if (!on(4, scales)) return fail(ERR_BAD_ARG, "scales must be on 4 bytes");
     return launch_fp8_quantize(dtype, x, codes, scales, rows, cols, block_rows, lc);
 }
 
@@ -1390,6 +1393,7 @@ static int check_fp8(int dtype, const void* w, const float* ws, const void* x, c
     if (K == 0 || K % 16 || K > kFp8Longest) return fail(ERR_SHAPE, "K must be a non-zero multiple of 16 up to 2^30");
     if (!w || !ws || !x || !out) return fail(ERR_BAD_ARG, "null buffer");
     if (!on_16(w) || !on_16(x)) return fail(ERR_BAD_ARG, "w and x must be on 16 bytes");
+    if (!on(4, ws) || !on(esize(dtype), out)) return fail(ERR_BAD_ARG, "scales and results must be aligned to their types");
     return ERR_OK;
 }
 
@@ -1398,6 +1402,7 @@ static int op_fp8_qmm(int dtype, const void* w, const float* ws, const void* x, 
     int rc = check_fp8(dtype, w, ws, x, out, M, N, K);
     if (rc) return rc;
     if (!xs) return fail(ERR_BAD_ARG, "null buffer");
+    if (!on(4, xs)) return fail(ERR_BAD_ARG, "scales must be on 4 bytes");
     Fp8Args a{(const uint8_t*)w, ws, x, xs, out, M, N, K};
     const int mt = fp8_rows_tiles(dtype, a);
     return mt ? launch_fp8_rows(dtype, a, mt, lc) : launch_fp8_tiles(dtype, a, lc);
@@ -1436,6 +1441,8 @@ static int op_gated_delta_rule(const DeltaArgs& a, const LaunchCtx& lc) {
         if (a.q_stride < (uint64_t)a.hk * a.dk || a.k_stride < (uint64_t)a.hk * a.dk || a.v_stride < (uint64_t)a.hv * a.dv)
             return fail(ERR_SHAPE, "a token's heads do not fit its stride");
     }
+    if (!on(esize(a.dtype), a.q, a.k, a.v) || !on(4, a.g, a.beta, a.offsets, a.slots, a.state_in, a.state_out, a.y))
+        return fail(ERR_BAD_ARG, "buffers must be aligned to their types");
     if ((uint64_t)a.n_seqs * a.hv > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more sequences and heads than a launch can have workgroups");
     if (delta_chunks_serve(a)) {
         const size_t need = delta_chunks_scratch_bytes(a, options().scratch_most_kb ? (size_t)options().scratch_most_kb * 1024 : SIZE_MAX);
@@ -1453,7 +1460,7 @@ static int op_token_logprobs(int dtype, const void* logits, size_t stride, const
     if (n_top > 32 || n_top > vocab) return fail(ERR_SHAPE, "n_top must be at most 32 and vocab");
     if (rows == 0) return ERR_OK;
     if (!logits || (n_given && (!tokens || !token_logprobs))) return fail(ERR_BAD_ARG, "null buffer");
-    if ((uintptr_t)logits % esize(dtype)) return fail(ERR_BAD_ARG, "logits must be aligned to their type");
+    if (!on(esize(dtype), logits) || !on(4, tokens, token_logprobs, entropy, top_ids, top_logprobs)) return fail(ERR_BAD_ARG, "buffers must be aligned to their types");
     if (!top_ids && !top_logprobs) n_top = 0;
     if (!n_given && !entropy && !n_top) return ERR_OK;
     const size_t need = logprobs_scratch_bytes(rows, vocab, n_top);

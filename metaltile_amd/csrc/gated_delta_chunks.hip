@@ -653,7 +653,8 @@ template <int DT, int DKP, int NT> __device__ __forceinline__ void walk_touch(co
             touch(p + (i < KEY_LINES ? key_at + i * 128 : head_at + (i - KEY_LINES) * 128), to);
         }
         const uint32_t t = w.from + c * kChunk + lane;
-        touch((const uint8_t*)d.v + ((size_t)(t < w.to ? t : w.to - 1) * d.v_stride + (size_t)w.h * d.dv + w.c0) * ES, to);
+        // (the whole word that holds the row's first element: nothing past the last page of v)
+        touch((const uint8_t*)(((uintptr_t)d.v + ((size_t)(t < w.to ? t : w.to - 1) * d.v_stride + (size_t)w.h * d.dv + w.c0) * ES) & ~(uintptr_t)3), to);
     };
     for (uint32_t c = w.begin; c < w.end && c < w.begin + kAheadChunks; c++) chunk(c);
     for (uint32_t c = w.begin; c < w.end; c++) {

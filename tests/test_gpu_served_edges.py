@@ -6,7 +6,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from metaltile_amd import DType, GpuBuffer, _lib, ops, pack_f32, unpack_f32
+from metaltile_amd import DType, GpuBuffer, MtqError, _lib, ops, pack_f32, unpack_f32
 from metaltile_amd.runtime import _ensure_init
 from tests import fp8_reference as ref
 from tests.hip_graph import Graph
@@ -271,3 +271,26 @@ def test_streams_of_the_callers():
         _lib.check(lib.mtq_set_stream(None))
         for s in streams:
             assert hip.hipStreamDestroy(s) == 0
+
+
+def test_misaligned_buffers_are_refused():
+    """Every pointer in turn off its type's alignment: an error before any launch."""
+    b = GpuBuffer(1 << 16)
+    p = b.ptr
+    def refused(call, args, off):
+        call(*args)   # (as they are: fine)
+        for i, by in off:
+            bad = list(args)
+            bad[i] += by
+            with pytest.raises(MtqError):
+                call(*bad)
+    # (one zero-filled buffer stands for all arguments: results land where nothing reads them, ids are 0)
+    o = p + (1 << 15)
+    refused(lambda x, c, s: ops.fp8_quantize(DType.BF16, x, c, s, 2, 64, 1), (p, o, o + 4096), ((0, 2), (0, 8), (1, 4), (2, 2)))
+    refused(lambda w, ws, x, xs, out: ops.fp8_qmm(DType.BF16, w, ws, x, xs, out, 2, 16, 64), (p, p + 4096, p, p + 4096, o), ((0, 8), (1, 2), (2, 8), (3, 2), (4, 1)))
+    refused(lambda w, ws, x, out: ops.fp8_qmv(DType.F32, w, ws, x, out, 1, 16, 64), (p, p + 4096, p, o), ((0, 8), (1, 2), (2, 8), (3, 2)))
+    refused(lambda q, k, v, g, beta, si, so, y: ops.gated_delta_rule(DType.F16, q, k, v, g, beta, si, so, y, 1, 2, 1, 1, 16, 16), (p, p, p, p, p, p + 4096, o, o + 8192),
+            ((0, 1), (1, 1), (2, 1), (3, 2), (4, 2), (5, 2), (6, 2), (7, 2)))
+    refused(lambda x, t, lp, e, ids, top: ops.token_logprobs(DType.BF16, x, 64, t, 1, lp, e, ids, top, 2, 1, 64), (p, p, o, o + 64, o + 128, o + 256),
+            ((0, 1), (1, 2), (2, 2), (3, 2), (4, 2), (5, 2)))
+    ops.sync()
