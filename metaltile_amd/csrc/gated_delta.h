@@ -73,11 +73,10 @@ template <int DT, int DKL, bool WHOLE> __device__ __forceinline__ void delta_tok
     const bool in = col < a.dv;
     const uint32_t hk = h / (a.hv / a.hk);
     const size_t state = (((size_t)s.slot * a.hv + h) * a.dv + col) * a.dk;
+    // Read before anything else and without a branch, which would wait for it: a column that there is not reads the last one, and a sequence that
+    // begins with zeros what state_out holds.
     float S[DKL];
-    if (a.state_in && in) load_part<DT_F32, DKL, WHOLE>(a.state_in, state, d0, a.dk, S);
-    else
-#pragma unroll
-        for (int j = 0; j < DKL; j++) S[j] = 0.f;
+    load_part<DT_F32, DKL, WHOLE>(a.state_in ? a.state_in : a.state_out, in ? state : state - (size_t)(col - a.dv + 1) * a.dk, d0, a.dk, S);
     struct Token {
         float q[DKL], k[DKL], v, g, beta;
     };
@@ -90,6 +89,9 @@ template <int DT, int DKL, bool WHOLE> __device__ __forceinline__ void delta_tok
     };
     Token x;
     if (s.from < s.to) load(s.from, x);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < DKL; j++) S[j] = a.state_in && in ? S[j] : 0.f;
     for (uint32_t t = s.from; t < s.to; t++) {
         Token next = x;
         if (t + 1 < s.to) load(t + 1, next);
