@@ -733,15 +733,15 @@ template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* s
     a.scratch = (uint8_t*)scratch;
     a.whole = delta_rows_whole(d);
     const uint32_t total = d.n_tokens / kChunk + d.n_seqs, at_once = (uint32_t)(bytes / L::slot_bytes(d.hk, d.hv));
-    // Heads that share a key head go to one XCD where that leaves none without (nine prompts of 1 to 1024 tokens, f16: 75 -> 53 us in all
+    // Heads that share a key head go to one XCD where that leaves none without (nine prompts of 1 to 1024 tokens, f16: 75 -> 53 us in both launches
     // against runs of heads, the long prompt's all on one).
     uint32_t pairs = d.n_seqs * d.hv, columns = (d.dv + 15) / 16, beside = (uint64_t)d.n_seqs * d.hk >= 8 ? d.hv / d.hk : 1;
     const uint64_t grid = ((uint64_t)pairs / beside + 7) / 8 * 8 * beside * columns;
     if (grid > 0x7FFFFFFFull || (uint64_t)total * d.hv > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more chunks or columns than a launch can have workgroups");
     // A wave more makes three on one of the four SIMDs, 168 registers each: rows of 384 terms and more need up to 256, and go without. Two
     // workgroups to a compute unit need 128: rows of 64 bf16 or f16 values do with them, and where there are more workgroups than compute units
-    // that gives more than the lines brought early (nine prompts of 1 to 1024 tokens, f16: 72 -> 59 us). Four prompts of 2048 tokens, dk 128: bf16
-    // 317 us with the wave, 361 without; f16 447, 532; f32 978 (its registers do not fit), 625.
+    // that gives more than the lines brought early (nine prompts of 1 to 1024 tokens, f16: 54 us against 64 with the wave and 60 without either).
+    // Four prompts of 2048 tokens, dk 128: bf16 298 us with the wave, 346 without; f16 376, 459; f32 878 (its registers do not fit), 563.
     constexpr bool wide = DKP * NT >= 384, narrow = DKP == 64 && NT <= 2;
     const bool touch = !wide && !(narrow && grid > 256);
     const void* fn;
