@@ -118,6 +118,12 @@ template <int DT> __device__ __forceinline__ void fp8_store4(void* out, uint32_t
     }
 }
 
+// Tile i of the n in a launch: workgroups go to the eight XCDs in turn, and each XCD gets a run of neighbours.
+__device__ __forceinline__ uint32_t xcd_run(uint32_t i, uint32_t n) {
+    const uint32_t per = n / 8, extra = n % 8, xcd = i % 8;
+    return xcd * per + (xcd < extra ? xcd : extra) + i / 8;
+}
+
 struct Fp8Args {
     const uint8_t* w;      // codes [N, K]
     const float* ws;       // [ceil(N / 128), ceil(K / 128)]

@@ -165,12 +165,6 @@ template <int DT, int BM, int BN, int WM, int WN, int STAGES> __device__ __force
     }
 }
 
-// Tile i of the n in a launch: workgroups go to the eight XCDs in turn, and each XCD gets a run of neighbours.
-__device__ __forceinline__ uint32_t xcd_run(uint32_t i, uint32_t n) {
-    const uint32_t per = n / 8, extra = n % 8, xcd = i % 8;
-    return xcd * per + (xcd < extra ? xcd : extra) + i / 8;
-}
-
 // One workgroup a tile for the first `whole` tiles; HALVES: two for each of the others, the upper half of its rows and the lower.
 template <int DT, int BM, int BN, int WM, int WN, int STAGES, bool HALVES> __global__ __launch_bounds__(64 * WM * WN) void fp8_tiles_kernel(Fp8Args a, uint32_t tiles_m, uint32_t tiles_n, uint32_t whole) {
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];

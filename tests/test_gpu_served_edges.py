@@ -247,6 +247,33 @@ def test_scratch_that_grows_behind_a_graph():
         first.close()
 
 
+def test_without_scratch():
+    """No room for the slices of few rows: a workgroup has each row. Activations that go through scratch are an error; a single row does not."""
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((2, 50000)).astype(np.float32)
+    logits, given = GpuBuffer.from_bytes(x.tobytes()), GpuBuffer.from_bytes(np.array([5, 49999], "<u4").tobytes())
+    lp, ent, ids, top = (GpuBuffer(4 * n) for n in (2, 2, 10, 10))
+    several, single = _Product(40, 300, 512, 1), _Product(1, 300, 512, 1)
+    single.call()
+    want = single.out.read_bytes()
+    lib = _ensure_init()
+    try:
+        _lib.check(lib.mtq_set_option(b"scratch.most_kb", 1))
+        ops.token_logprobs(DType.F32, logits, 50000, given, 1, lp, ent, ids, top, 5, 2, 50000)
+        with pytest.raises(MtqError):
+            several.call()
+        single.out.zero()
+        single.call()
+        assert single.out.read_bytes() == want
+    finally:
+        _lib.check(lib.mtq_set_option(b"scratch.most_kb", 0))
+    wlp, went, wids, wtop, size, d, z = _reference(x.astype(np.float64), np.array([[5], [49999]]), 5)
+    read = lambda b, *shape: np.frombuffer(b.read_bytes(), "<f4").reshape(shape)
+    tol = 1e-5 + 2.0 ** -22 * 20
+    assert _close(read(lp, 2, 1), wlp, tol) and _close(read(ent, 2), went, 1e-5 * size) and _close(read(top, 2, 5), wtop, tol)
+    assert np.array_equal(np.frombuffer(ids.read_bytes(), "<u4").reshape(2, 5), wids)
+
+
 def test_streams_of_the_callers():
     """From the library's own stream to two of the caller's."""
     lib, hip = _ensure_init(), C.CDLL("libamdhip64.so")
