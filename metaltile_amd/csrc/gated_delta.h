@@ -112,7 +112,8 @@ template <int DT, int DKL, bool WHOLE> __device__ __forceinline__ void delta_tok
         }
         const float keep = expf(x.g);
         const float u = x.beta * (x.v - keep * rk * sum16(Sk)), uk = u * rk;
-        const float y = rq * (keep * sum16(Sq) + qk * uk);
+        // (a k whose squares pass f32's range counts as zeros, rk = 0, also where q . k is infinite)
+        const float y = rq * (keep * sum16(Sq) + (uk != 0.f ? qk * uk : 0.f));
         if ((lane & 15u) == 0 && in) a.y[((size_t)t * a.hv + h) * a.dv + col] = y;
 #pragma unroll
         for (int j = 0; j < DKL; j++) S[j] = keep * S[j] + x.k[j] * uk;

@@ -211,7 +211,8 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256, DKP * NT <=
     qq += __shfl_xor(qq, 32, 64);
     if (g == 0) {
         const bool norm = d.norm_eps >= 0.f;
-        rk[t] = t >= n ? 0.f : norm ? 1.f / sqrtf(kk + d.norm_eps) : 1.f;
+        // (sums of squares past f32's range: 0 * inf would be in A and P where token by token there are zeros, so the walk is told)
+        rk[t] = t >= n ? 0.f : !(kk + qq < INFINITY) ? NAN : norm ? 1.f / sqrtf(kk + d.norm_eps) : 1.f;
         rq[t] = t >= n ? 0.f : norm ? d.scale / sqrtf(qq + d.norm_eps) : d.scale;
     }
 #pragma unroll
@@ -398,7 +399,7 @@ template <int DKP> struct WalkLds {
     Columns<DKP> S[3];                             // terms of the state
     Columns<kChunk> X[3], U[3], W[3];
     uint32_t touched[64];                          // where the words that bring lines into the L2 end up
-    uint32_t bad;                                  // a chunk's X has an infinity or a NaN
+    uint32_t bad;                                  // a chunk's U has an infinity or a NaN, or is next to one
 };
 
 struct WalkPlace {
@@ -418,8 +419,9 @@ struct WalkPlace {
 //   b..c: U = T X                      | Q S0
 //   c..a: S1 = e^G S0 + K^T (r e^.. U), its terms to LDS
 //
-// A product with a triangle multiplies what is behind a token by zero, which an infinity or a NaN there survives: a chunk with one in X is left,
-// with the tokens behind it, to the token by token form, and the state before it to state_out. Returns that chunk, or w.end.
+// A product with a triangle multiplies what is behind a token by zero, which an infinity or a NaN there survives, and so does the inverse of one
+// whose updates leave f32's range: a chunk with such a number in U (all of X and T that is no number comes out there) is left, with the tokens
+// behind it, to the token by token form, and the state before it to state_out. Returns that chunk, or w.end.
 template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ uint32_t walk(const DeltaArgs& d, const WalkPlace& w, WalkLds<DKP>& lds, uint32_t wave) {
     using L = Layout<DKP, NT>;
     constexpr int ES = DT == DT_F32 ? 4 : 2;
@@ -565,7 +567,6 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ uint32
 #pragma unroll
             for (int i = 0; i < 4; i++) x[i] = value(v[i]) - e[i] * x[i];
             asm volatile("" : "+v"(x));   // (here, not behind the next loads into e's and v's registers)
-            if (__ballot(!(x[0] * 0.f + x[1] * 0.f + x[2] * 0.f + x[3] * 0.f == 0.f))) lds.bad = 1;
             put(lds.X[0].at(r, 16 * mine + 4 * g), Columns<kChunk>::PLANE, x);
         } else if (c > w.begin) {
             give_y(c - 1, [&] { load_kt(here); });
@@ -573,7 +574,6 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ uint32
             load_kt(here);
         }
         walk_barrier();
-        const uint32_t bad = lds.bad;
         f32x4 late;
         if constexpr (AHEAD) {
             f32x4 u = {};
@@ -581,6 +581,11 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ uint32
             f32x4 uw = u * wk;
             asm volatile("" : "+v"(uw));
             put(lds.W[0].at(r, 16 * mine + 4 * g), Columns<kChunk>::PLANE, uw);
+            // (magnitudes whose terms could round to infinities count, too: a term of 3.39e38 and more would)
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) most += fabsf(u[i]) + fabsf(uw[i]);
+            if (__ballot(!(most < 3.3e38f))) lds.bad = 1;
             late = u;   // (U itself is asked for from the next chunk on: it is put beside the state's update)
         } else {
             times_state(y, [&] { load_tri(here); });
@@ -588,7 +593,7 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ uint32
             asm volatile("" : "+v"(y));
         }
         walk_barrier();
-        if (__builtin_amdgcn_readfirstlane(bad)) break;
+        const uint32_t bad = lds.bad;
         u32x4 b[2][3];
 #pragma unroll
         for (int ts = 0; ts < 2; ts++)
@@ -602,6 +607,7 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ uint32
             load_rows(next);
         }
         __builtin_amdgcn_sched_barrier(0);
+        if (__builtin_amdgcn_readfirstlane(bad)) break;
         if (has_state) {
 #pragma unroll
             for (int x = 0; x < NS; x++) {
