@@ -375,7 +375,7 @@ MTQ_API int mtq_fp8_qmv(int dtype, const void *w, const float *w_scales, const v
  * Sequence i has the tokens offsets[i] .. offsets[i + 1] - 1 (u32[n_seqs + 1] on the device, ascending; none: its state is
  * passed on as it is), or with offsets NULL n_tokens / n_seqs each; its state is slot slots[i] (u32[n_seqs] on the device, no slot
  * twice) or, with slots NULL, slot i. A slot >= n_slots names no state: nothing is written for that sequence. Tokens outside all
- * sequences are left alone, and offsets behind n_tokens read as n_tokens. hk divides hv; dk <= 256, dv <= 65536.
+ * sequences are left alone, and offsets behind n_tokens read as n_tokens. hk divides hv; dk <= 256, dv <= 65536, n_seqs hv < 2^24.
  * A NaN or an infinity among the inputs reaches what comes behind it in its sequence and head (from v and the state: in its column).
  * So does one that the recurrence itself comes to (keys too long for their beta). Sums of squares are f32 as well: a q or k whose sum passes
  * its range counts as zeros where it is normalised.

@@ -1443,7 +1443,7 @@ static int op_gated_delta_rule(const DeltaArgs& a, const LaunchCtx& lc) {
     }
     if (!on(esize(a.dtype), a.q, a.k, a.v) || !on(4, a.g, a.beta, a.offsets, a.slots, a.state_in, a.state_out, a.y))
         return fail(ERR_BAD_ARG, "buffers must be aligned to their types");
-    if ((uint64_t)a.n_seqs * a.hv > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more sequences and heads than a launch can have workgroups");
+    if ((uint64_t)a.n_seqs * a.hv > max_workgroups(256)) return fail(ERR_SHAPE, "more sequences and heads than a launch can have workgroups");
     if (delta_chunks_serve(a)) {
         const size_t need = delta_chunks_scratch_bytes(a, options().scratch_most_kb ? (size_t)options().scratch_most_kb * 1024 : SIZE_MAX);
         if (need && ensure_scratch(need) == ERR_OK) return launch_delta_chunks(a, g.scratch_buf, need, lc);   // (no memory: token by token)

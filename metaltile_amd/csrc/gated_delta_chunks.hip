@@ -121,7 +121,7 @@ __device__ __forceinline__ uint32_t seq_of(const DeltaArgs& a, uint32_t slot) {
     }
     // 64 sequences at a time, so that a few reads of memory after one another find it: those whose first slot is not behind it come first
     uint32_t lo = 0, step = 1;
-    while (step * 64 < a.n_seqs) step *= 64;
+    while (step * 64 < a.n_seqs) step *= 64;   // (sequences are less than 2^24)
     for (;; step /= 64) {
         const uint32_t i = lo + (threadIdx.x & 63u) * step;
         const bool before = i < a.n_seqs && min(a.offsets[i < a.n_seqs ? i : 0], a.n_tokens) / kChunk + i <= slot;
@@ -732,6 +732,14 @@ template <int DT, int DKP, int NT, bool TOUCH, int PER_SIMD> __global__ __launch
     else delta_tokens<DT, DKP / 16, false>(tokens, one, h, c0 + 4 * wave);
 }
 
+// Heads that share a key head go to one XCD where that leaves none without (nine prompts of 1 to 1024 tokens, f16: 75 -> 53 us in both launches
+// against runs of heads, the long prompt's all on one).
+uint32_t heads_beside(const DeltaArgs& d) { return (uint64_t)d.n_seqs * d.hk >= 8 ? d.hv / d.hk : 1; }
+uint64_t walk_grid(const DeltaArgs& d) {
+    const uint32_t beside = heads_beside(d);
+    return ((uint64_t)d.n_seqs * d.hv / beside + 7) / 8 * 8 * beside * ((d.dv + 15) / 16);
+}
+
 template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* scratch, size_t bytes, const LaunchCtx& lc) {
     using L = Layout<DKP, NT>;
     ChunkArgs a;
@@ -739,11 +747,8 @@ template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* s
     a.scratch = (uint8_t*)scratch;
     a.whole = delta_rows_whole(d);
     const uint32_t total = d.n_tokens / kChunk + d.n_seqs, at_once = (uint32_t)(bytes / L::slot_bytes(d.hk, d.hv));
-    // Heads that share a key head go to one XCD where that leaves none without (nine prompts of 1 to 1024 tokens, f16: 75 -> 53 us in both launches
-    // against runs of heads, the long prompt's all on one).
-    uint32_t pairs = d.n_seqs * d.hv, columns = (d.dv + 15) / 16, beside = (uint64_t)d.n_seqs * d.hk >= 8 ? d.hv / d.hk : 1;
-    const uint64_t grid = ((uint64_t)pairs / beside + 7) / 8 * 8 * beside * columns;
-    if (grid > 0x7FFFFFFFull || (uint64_t)total * d.hv > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more chunks or columns than a launch can have workgroups");
+    uint32_t pairs = d.n_seqs * d.hv, columns = (d.dv + 15) / 16, beside = heads_beside(d);
+    const uint64_t grid = walk_grid(d);   // (the first launch has less than 2^16 workgroups, as a slot of the scratch has more than 16 KB a head)
     // A wave more makes three on one of the four SIMDs, 168 registers each: rows of 384 terms and more need up to 256, and go without. Two
     // workgroups to a compute unit need 128: rows of 64 bf16 or f16 values do with them, and where there are more workgroups than compute units
     // that gives more than the lines brought early (nine prompts of 1 to 1024 tokens, f16: 54 us against 64 with the wave and 60 without either).
@@ -787,9 +792,10 @@ size_t slot_bytes_of(const DeltaArgs& d) {
 
 // Chunks pay where a sequence may be long: with as many tokens beyond one for each sequence as this. (Sequences of up to kFewTokens go token
 // by token here too.)
-// The walk reads a chunk's rows of v and a slot by 31-bit offsets.
+// The walk reads a chunk's rows of v and a slot by 31-bit offsets, and has a workgroup for 16 columns of every head of every sequence: where these
+// are more than a launch can have, sequences go token by token, all of them at once.
 bool delta_chunks_serve(const DeltaArgs& d) {
-    if (d.v_stride > (1u << 22) || slot_bytes_of(d) >= ((size_t)1 << 31)) return false;
+    if (d.v_stride > (1u << 22) || slot_bytes_of(d) >= ((size_t)1 << 31) || walk_grid(d) > max_workgroups(64 * 9)) return false;
     return d.offsets ? d.n_tokens > d.n_seqs && d.n_tokens - d.n_seqs >= 2 * kFewTokens : d.n_tokens / d.n_seqs >= 2 * kFewTokens;
 }
 

@@ -43,6 +43,8 @@ struct LaunchCtx {
 
 hipError_t launch_kernel(const void* fn, dim3 grid, dim3 block, void** args, size_t shmem,
                          const LaunchCtx& lc);
+// Workgroups of so many threads that a launch can have along x: HIP launches fewer than 2^32 threads a dimension.
+constexpr uint64_t max_workgroups(uint32_t threads) { return 0xFFFFFFFFull / threads; }
 // Raises a kernel's dynamic LDS limit (needed above 48 KB).
 hipError_t set_max_dynamic_lds(const void* fn, size_t bytes);
 // Planning (mtq_plan): the routing and geometry code runs as for a real call, but launch_kernel and
