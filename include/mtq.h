@@ -341,7 +341,9 @@ MTQ_API int mtq_dequant_gather(int dtype, int bits, uint32_t group_size, const v
  * e4m3 as OCP defines it (four exponent and three mantissa bits, largest 448), row-major, and every block of 128 along a
  * row has one f32 scale; value = code * scale. Activations have blocks of 1 x 128 (scales f32[rows, ceil(cols / 128)]),
  * weights of 128 x 128 (scales f32[ceil(rows / 128), ceil(cols / 128)]); blocks at the right and lower edge may be cut.
- * All four calls: cols (K) a multiple of 16; x, codes and w on 16 bytes, rows packed.
+ * All three calls: cols (K) a multiple of 16; x, codes and w on 16 bytes, rows packed. What is more than a launch
+ * can have is MTQ_ERR_SHAPE: 2^28 blocks of 1 x 128 (2^24 of 128 x 128) and more in quantising, more than 2^28 rows of x,
+ * 2^28 - 16 of w or 2^37 results in a product.
  *
  * fp8_quantize: block_rows 1 or 128. scale = max |x| / 448 over the block, not less than 2^-126 (1 where all are zero);
  * code = the e4m3 value nearest to the f32 quotient x / scale, ties to even. A NaN's code is NaN and does not count for
@@ -352,12 +354,12 @@ MTQ_API int mtq_fp8_quantize(int dtype, const void *x, void *codes, float *scale
 /* out[m, n] = sum_k x[m, k] w[n, k] over the values of both: w codes [N, K] with w_scales f32[ceil(N / 128), ceil(K / 128)],
  * x codes [M, K] with x_scales f32[M, ceil(K / 128)], out T[M, N]. Sums over a block of 128 and the scaled sums of the blocks
  * are f32, rounded to T once. With T = f32 products of codes are exact; with f16 and bf16 the matrix cores drop of eight
- * neighbouring products what lies below 2^-13 of the largest one's power of two. Any M. */
+ * neighbouring products what lies below 2^-13 of the largest one's power of two. */
 MTQ_API int mtq_fp8_qmm(int dtype, const void *w, const float *w_scales, const void *x, const float *x_scales, void *out,
                         uint32_t M, uint32_t N, uint32_t K);
 
 /* The same from activations T[M, K], quantised as mtq_fp8_quantize does with block_rows 1: the decode step's call. Codes
- * and scales of more than a row go through a library-owned buffer (allocated on first use, grown on demand). Any M. */
+ * and scales of more than a row go through a library-owned buffer (allocated on first use, grown on demand). */
 MTQ_API int mtq_fp8_qmv(int dtype, const void *w, const float *w_scales, const void *x, void *out, uint32_t M, uint32_t N,
                         uint32_t K);
 
@@ -396,7 +398,7 @@ MTQ_API int mtq_gated_delta_rule(int dtype, const void *q, size_t q_stride, cons
  *     ones the lower index first (either may be NULL).
  * A logit of -inf has probability 0. A row of nothing but -inf: log probabilities -inf, entropy 0, the lowest indices. A row with a NaN or
  * +inf: all of its log probabilities and its entropy NaN; a NaN is never among the top, and where those run out the id is 0xFFFFFFFF.
- * Few rows are cut over workgroups and joined through a library-owned buffer (allocated on first use). vocab <= 2^30. */
+ * Few rows are cut over workgroups and joined through a library-owned buffer (allocated on first use). vocab <= 2^30, n_rows < 2^24. */
 MTQ_API int mtq_token_logprobs(int dtype, const void *logits, size_t row_stride, const uint32_t *tokens, uint32_t n_given,
                                float *token_logprobs, float *entropy, uint32_t *top_ids, float *top_logprobs, uint32_t n_top,
                                uint32_t n_rows, uint32_t vocab);

@@ -1389,7 +1389,10 @@ static int op_fp8_quantize(int dtype, const void* x, void* codes, float* scales,
 static int check_fp8(int dtype, const void* w, const float* ws, const void* x, const void* out, uint32_t M, uint32_t N, uint32_t K) {
     int rc = check_dtype(dtype);
     if (rc) return rc;
-    if (M > kFp8Longest || N == 0 || N > kFp8Longest) return fail(ERR_SHAPE, "M and N must be at most 2^30, N not 0");
+    // What a launch can have (max_workgroups), whichever kernel takes the call: 16 weight rows to 256 threads; tiles of 128 x 128 results to 256 threads (f32)
+    // or, up to 128 rows of either side, to 1024, of 256 x 256 to 512; and 64 activation rows to one of 65535 along y where K is too long for tiles.
+    if (N == 0 || N > (1u << 28) - 16 || M > (1u << 28) || (uint64_t)M * N > 1ull << 37) return fail(ERR_SHAPE, "M must be at most 2^28, N at most 2^28 - 16 and not 0, M N at most 2^37");
+    if (K > kFp8TilesLongest && M > 65535u * 64) return fail(ERR_SHAPE, "too many activation rows of this length");
     if (K == 0 || K % 16 || K > kFp8Longest) return fail(ERR_SHAPE, "K must be a non-zero multiple of 16 up to 2^30");
     if (!w || !ws || !x || !out) return fail(ERR_BAD_ARG, "null buffer");
     if (!on_16(w) || !on_16(x)) return fail(ERR_BAD_ARG, "w and x must be on 16 bytes");

@@ -9,6 +9,7 @@ namespace mtq {
 
 constexpr uint32_t kFp8Block = 128;
 constexpr float kFp8Most = 448.f;
+constexpr uint32_t kFp8TilesLongest = 1u << 22;   // K up to which a tile's rows have 31-bit offsets
 
 typedef int fp8_i32x8 __attribute__((ext_vector_type(8)));
 typedef float fp8_f32x4 __attribute__((ext_vector_type(4)));

@@ -60,7 +60,7 @@ int launch_fp8_quantize(int dtype, const void* x, void* codes, float* scales, ui
     Fp8QuantArgs a{x, (uint8_t*)codes, scales, rows, cols, (cols + kFp8Block - 1) / kFp8Block};
     const bool tiles = block_rows > 1;
     const uint64_t units = tiles ? (uint64_t)((rows + kFp8Block - 1) / kFp8Block) * a.blocks : ((uint64_t)rows * a.blocks + 15) / 16;
-    if (units > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more blocks than a launch can have workgroups");
+    if (units > max_workgroups(256)) return fail(ERR_SHAPE, "more blocks than a launch can have workgroups");
     const void* rows_fn[] = {(const void*)fp8_quantize_rows_kernel<DT_F32>, (const void*)fp8_quantize_rows_kernel<DT_F16>, (const void*)fp8_quantize_rows_kernel<DT_BF16>};
     const void* tiles_fn[] = {(const void*)fp8_quantize_tiles_kernel<DT_F32>, (const void*)fp8_quantize_tiles_kernel<DT_F16>, (const void*)fp8_quantize_tiles_kernel<DT_BF16>};
     void* args[] = {&a};

@@ -157,7 +157,7 @@ int fp8_rows_tiles(int dtype, const Fp8Args& a) {
     auto groups = [&](uint32_t mt, uint32_t nt) { return (uint64_t)((a.M + 16 * mt - 1) / (16 * mt)) * ((a.N + 16 * nt - 1) / (16 * nt)); };
     if (a.M <= 16 || groups(1, 1) <= cus) return 1;
     if (a.M <= 32 || groups(2, 2) <= cus) return 2;
-    return groups(4, 2) <= (dtype == DT_F32 ? 2 : 1) * cus || a.K > (1u << 22) ? 4 : 0;
+    return groups(4, 2) <= (dtype == DT_F32 ? 2 : 1) * cus || a.K > kFp8TilesLongest ? 4 : 0;
 }
 
 // Every workgroup quantises the rows anew, which costs less than a launch of its own (3 us) for one row, or for a few where the workgroups are
@@ -179,7 +179,6 @@ int launch_fp8_rows(int dtype, const Fp8Args& p, int mt, const LaunchCtx& lc) {
     Fp8Args a = p;
     const int nt = mt == 1 ? 1 : 2, nw = mt == 1 ? waves_of(a) : mt == 2 ? 8 : 4;
     const uint32_t ny = (a.M + 16 * mt - 1) / (16 * mt);
-    if (ny > 65535u) return fail(ERR_SHAPE, "too many activation rows");
     const void* fn = dtype == DT_F32 ? rows_fn<DT_F32>(mt, nw) : dtype == DT_F16 ? rows_fn<DT_F16>(mt, nw) : rows_fn<DT_BF16>(mt, nw);
     const size_t lds = (size_t)nw * nt * mt * 1024;
     void* args[] = {&a};

@@ -184,9 +184,7 @@ uint64_t tiles_of(const Fp8Args& a, uint32_t bm, uint32_t bn) { return (uint64_t
 
 template <int BM, int BN, int WM, int WN, int STAGES, bool HALVES, int... DTS> int launch(int dtype, const Fp8Args& p, uint32_t halved, const LaunchCtx& lc) {
     Fp8Args a = p;
-    const uint64_t total = tiles_of(a, BM, BN);
-    if (total + halved > 0x7FFFFFFFull) return fail(ERR_SHAPE, "more tiles than a launch can have workgroups");
-    uint32_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN, whole = (uint32_t)total - halved;
+    uint32_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN, whole = (uint32_t)tiles_of(a, BM, BN) - halved;
     const void* fn = nullptr;
     ((dtype == DTS ? (void)(fn = (const void*)fp8_tiles_kernel<DTS, BM, BN, WM, WN, STAGES, HALVES>) : (void)0), ...);
     constexpr size_t lds = STAGES * (BM + BN) * 128 + 2 * BM * kWindow * sizeof(float);

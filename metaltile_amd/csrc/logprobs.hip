@@ -349,8 +349,6 @@ template <int DT> __global__ __launch_bounds__(64 * kWaves) void logprobs_join_k
     if (wave == 0) finish<DT>(a, row, t, lds.comb, given);
 }
 
-constexpr uint32_t kGridMost = 0x7FFFFFFF;
-
 }  // namespace
 
 static uint32_t logprob_slices(uint32_t rows, uint32_t vocab) {
@@ -373,7 +371,7 @@ int launch_logprobs(int dtype, const void* logits, size_t stride, const uint32_t
     a.slices = scratch ? logprob_slices(rows, vocab) : 1;
     a.part = (float*)scratch;
     a.part_keys = scratch ? (uint64_t*)((char*)scratch + (size_t)rows * a.slices * 16) : nullptr;
-    if ((uint64_t)rows * a.slices > kGridMost) return fail(ERR_SHAPE, "more rows than a launch can have workgroups");
+    if ((uint64_t)rows * a.slices > max_workgroups(64 * kWaves)) return fail(ERR_SHAPE, "more rows than a launch can have workgroups");
     const void* fn = dtype == DT_F32 ? (const void*)logprobs_kernel<DT_F32> : dtype == DT_F16 ? (const void*)logprobs_kernel<DT_F16> : (const void*)logprobs_kernel<DT_BF16>;
     void* args[] = {&a};
     LaunchCtx first = lc;

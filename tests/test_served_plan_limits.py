@@ -32,3 +32,40 @@ def test_gated_delta_rule(dt):
     assert plan((1 << 19) - 1, 1 << 19)[0] == OK and plan(1 << 19, 1 << 19)[0] == SHAPE
     for seqs in (1 << 24, (1 << 30) + 1, (1 << 31) - 1, 0xFFFFFFFF):
         assert plan(seqs, 0xFFFFFFFF, hk=1, hv=1, dk=1, dv=1)[0] == SHAPE
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
+@pytest.mark.parametrize("op", ["fp8_qmm", "fp8_qmv"])
+def test_fp8_products(dt, op):
+    plan = lambda m, n, k: ops.plan(op, dt, 8, 128, m, n, k)
+    rng = np.random.default_rng(5)
+    for _ in range(2000):
+        m, n = (int(2 ** rng.uniform(0, hi)) for hi in ((8, 30), (30, 8), (30, 30))[int(rng.integers(3))])
+        _fits(*plan(m, n, 16 * int(2 ** rng.uniform(0, 26)))[:2])
+    most = (1 << 28) - 16
+    for m, n in ((1, most), (2, most), (33, most), (128, most), (129, most), (512, most), (1 << 20, 1 << 17), (1 << 28, 16), (1 << 28, 128), (1 << 28, 129), (1 << 28, 512)):
+        rc, launches, _, _ = plan(m, n, 16)
+        _fits(rc, launches)
+        assert rc == (SHAPE if op == "fp8_qmv" and m == 1 << 28 else OK)   # (as many blocks of x are more than the quantiser can have)
+    for m, n, k in ((1, most + 1, 16), ((1 << 28) + 1, 16, 16), (1 << 19, 1 << 19, 16), (1 << 22, 16, (1 << 22) + 16)):
+        rc, launches, _, _ = plan(m, n, k)
+        assert rc == SHAPE and not launches
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
+def test_fp8_quantize(dt):
+    plan = lambda rows, cols, block: ops.plan("fp8_quantize", dt, 8, block, rows, 0, cols)
+    rng = np.random.default_rng(6)
+    for _ in range(500):
+        _fits(*plan(int(2 ** rng.uniform(0, 30)), 16 * int(2 ** rng.uniform(0, 26)), int(rng.choice([1, 128])))[:2])
+    assert plan((1 << 28) - 16, 128, 1)[0] == OK and plan(1 << 28, 128, 1)[0] == SHAPE
+    assert plan(1 << 30, 128, 128)[0] == OK and plan(1 << 30, 256, 128)[0] == SHAPE
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
+def test_token_logprobs(dt):
+    plan = lambda rows, vocab: ops.plan("token_logprobs", dt, 0, 0, rows, vocab, 1)
+    rng = np.random.default_rng(7)
+    for _ in range(500):
+        _fits(*plan(int(2 ** rng.uniform(0, 32)), int(2 ** rng.uniform(0, 30)))[:2])
+    assert plan((1 << 24) - 1, 100)[0] == OK and plan(1 << 24, 100)[0] == SHAPE
