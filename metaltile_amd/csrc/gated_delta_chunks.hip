@@ -38,7 +38,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 struct ChunkArgs {
     DeltaArgs d;
     uint8_t* scratch;
-    uint32_t lo, hi;        // this launch's slots for chunks: sequence i's chunk c has slot from_i / 64 + i + c
+    uint32_t lo, hi;        // this launch's slots for chunks: sequence i's chunk c has slot first_slot(i) + c
+    uint32_t by_tokens;     // how slots are numbered
     uint32_t whole;         // rows of q and k on 16 bytes
     uint32_t parts;         // workgroups of the first launch for a chunk and key head
 };
@@ -106,15 +107,28 @@ template <int DT> __device__ __forceinline__ void load8(const void* p, size_t i,
     }
 }
 
+// A sequence's first slot, in one of two numberings of which a call takes the one with fewer slots: from / 64 + seq, which gives every sequence a
+// slot, or by tokens alone, from / 17: a sequence that takes chunks has 17 tokens or more, and floor(n / 17) >= ceil(n / 64) for those, so the next one
+// begins behind its last slot (256 sequences of two tokens: 31 slots instead of 264, which are 2 MB each with 16 and 32 heads of 128 bf16).
+constexpr uint32_t kFewestChunked = kFewTokens + 1;
+__device__ __host__ __forceinline__ uint32_t first_slot(uint32_t from, uint32_t seq, uint32_t by_tokens) {
+    return by_tokens ? from / kFewestChunked : from / kChunk + seq;
+}
+// Slots of a call; `by_tokens`: in which numbering.
+inline uint64_t slots_of(const DeltaArgs& d, uint32_t& by_tokens) {
+    const uint64_t with = (uint64_t)d.n_tokens / kChunk + d.n_seqs, tokens = (uint64_t)d.n_tokens / kFewestChunked + 1;
+    by_tokens = tokens < with;
+    return by_tokens ? tokens : with;
+}
 // The sequence that a slot belongs to: the last whose first slot is not behind it.
-__device__ __forceinline__ uint32_t first_slot(const DeltaSeq& s, uint32_t seq) { return s.from / kChunk + seq; }
-__device__ __forceinline__ uint32_t seq_of(const DeltaArgs& a, uint32_t slot) {
+__device__ __forceinline__ uint32_t seq_of(const ChunkArgs& c, uint32_t slot) {
+    const DeltaArgs& a = c.d;
     if (!a.offsets) {   // (equal lengths: no memory to be read)
         uint32_t lo = 0, hi = a.n_seqs;
         const uint32_t each = a.n_tokens / a.n_seqs;
         while (hi - lo > 1) {
             const uint32_t mid = lo + (hi - lo) / 2;
-            if (mid * each / kChunk + mid <= slot) lo = mid;
+            if (first_slot(mid * each, mid, c.by_tokens) <= slot) lo = mid;
             else hi = mid;
         }
         return lo;
@@ -124,7 +138,7 @@ __device__ __forceinline__ uint32_t seq_of(const DeltaArgs& a, uint32_t slot) {
     while (step * 64 < a.n_seqs) step *= 64;   // (sequences are less than 2^24)
     for (;; step /= 64) {
         const uint32_t i = lo + (threadIdx.x & 63u) * step;
-        const bool before = i < a.n_seqs && min(a.offsets[i < a.n_seqs ? i : 0], a.n_tokens) / kChunk + i <= slot;
+        const bool before = i < a.n_seqs && first_slot(min(a.offsets[i < a.n_seqs ? i : 0], a.n_tokens), i, c.by_tokens) <= slot;
         const uint32_t n = (uint32_t)__popcll(__ballot(before));
         if (n) lo += (n - 1) * step;
         if (step == 1) return lo;
@@ -170,9 +184,9 @@ template <int DT, int DKP, int NT> __global__ __launch_bounds__(256, DKP * NT <=
     const DeltaArgs& d = a.d;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15u, g = lane >> 4;
     const uint32_t units = d.hk * a.parts, slot = a.lo + blockIdx.x / units, kh = blockIdx.x % units / a.parts, part = blockIdx.x % a.parts;
-    const uint32_t seq = seq_of(d, slot);
+    const uint32_t seq = seq_of(a, slot);
     const DeltaSeq s = delta_seq(d, seq);
-    const uint32_t first = first_slot(s, seq);
+    const uint32_t first = first_slot(s.from, seq, a.by_tokens);
     if (!s.any || slot < first || s.to - s.from <= kFewTokens || (uint64_t)(slot - first) * kChunk >= s.to - s.from) return;
     const uint32_t t0 = s.from + (slot - first) * kChunk, n = s.to - t0 < kChunk ? s.to - t0 : kChunk;
     uint8_t* out = a.scratch + (size_t)(slot - a.lo) * L::slot_bytes(d.hk, d.hv);
@@ -689,7 +703,7 @@ template <int DT, int DKP, int NT, bool TOUCH, int PER_SIMD> __global__ __launch
     const uint32_t seq = pair / d.hv, h = pair % d.hv;
     const DeltaSeq s = delta_seq(d, seq);
     if (!s.any) return;
-    const uint32_t len = s.to - s.from, first = first_slot(s, seq);
+    const uint32_t len = s.to - s.from, first = first_slot(s.from, seq, a.by_tokens);
     DeltaSeq one = s;                      // what goes token by token, and from which states
     const float* from = d.state_in;
     if (len <= kFewTokens) {
@@ -746,7 +760,7 @@ template <int DT, int DKP, int NT> int launch_chunks(const DeltaArgs& d, void* s
     a.d = d;
     a.scratch = (uint8_t*)scratch;
     a.whole = delta_rows_whole(d);
-    const uint32_t total = d.n_tokens / kChunk + d.n_seqs, at_once = (uint32_t)(bytes / L::slot_bytes(d.hk, d.hv));
+    const uint32_t total = (uint32_t)slots_of(d, a.by_tokens), at_once = (uint32_t)(bytes / L::slot_bytes(d.hk, d.hv));
     uint32_t pairs = d.n_seqs * d.hv, columns = (d.dv + 15) / 16, beside = heads_beside(d);
     const uint64_t grid = walk_grid(d);   // (the first launch has less than 2^16 workgroups, as a slot of the scratch has more than 16 KB a head)
     // A wave more makes three on one of the four SIMDs, 168 registers each: rows of 384 terms and more need up to 256, and go without. Two
@@ -803,7 +817,8 @@ bool delta_chunks_serve(const DeltaArgs& d) {
 // window before left. 0: not even one chunk fits.
 size_t delta_chunks_scratch_bytes(const DeltaArgs& d, size_t most) {
     if (most > ((size_t)1 << 30)) most = (size_t)1 << 30;
-    const size_t one = slot_bytes_of(d), all = one * ((size_t)d.n_tokens / kChunk + d.n_seqs);
+    uint32_t by_tokens;
+    const size_t one = slot_bytes_of(d), all = one * slots_of(d, by_tokens);
     return all <= most ? all : most / one * one;
 }
 

@@ -69,3 +69,17 @@ def test_token_logprobs(dt):
     for _ in range(500):
         _fits(*plan(int(2 ** rng.uniform(0, 32)), int(2 ** rng.uniform(0, 30)))[:2])
     assert plan((1 << 24) - 1, 100)[0] == OK and plan(1 << 24, 100)[0] == SHAPE
+
+
+@pytest.mark.parametrize("dt,slot", [(DType.BF16, 2.0), (DType.F16, 2.8), (DType.F32, 3.6)], ids=lambda v: getattr(v, "name", None))
+def test_short_sequences_reserve_scratch_by_their_tokens(dt, slot):
+    """A chunk's slot has (16 heads x 3 operands x 64 x 128 terms of 16 bits, 32 heads x 37 KB) about 2 MB in bf16. Only a sequence of 17 tokens or more
+    takes any, so a call has at most one for each 17 of its tokens, however many sequences it has, and makes its two launches once."""
+    for seqs, tokens in ((256, 512), (64, 128), (1000, 1040), (4096, 8192)):
+        rc, launches, scratch, count = ops.plan("gated_delta_rule", dt, 0, 128, 16, 32, 128, seqs, tokens)
+        slots = tokens // 17 + 1
+        assert rc == OK and scratch <= min(slots * slot * (1 << 20), 1 << 30)
+        assert count == 2 * -(-slots // int((1 << 30) / (slot * (1 << 20))))
+    # Prompts: a slot for each 64 tokens, and one for each sequence.
+    _, _, scratch, _ = ops.plan("gated_delta_rule", dt, 0, 128, 16, 32, 128, 2, 4096)
+    assert scratch <= (4096 // 64 + 2) * slot * (1 << 20)
