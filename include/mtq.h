@@ -359,7 +359,9 @@ MTQ_API int mtq_fp8_qmm(int dtype, const void *w, const float *w_scales, const v
                         uint32_t M, uint32_t N, uint32_t K);
 
 /* The same from activations T[M, K], quantised as mtq_fp8_quantize does with block_rows 1: the decode step's call. Codes
- * and scales of more than a row go through a library-owned buffer (allocated on first use, grown on demand). */
+ * and scales of more than a row (or of one that is long) go through a library-owned buffer (allocated on first use, grown on
+ * demand). Without that memory up to 16 rows are quantised in LDS while they fit (K of about 9 K, of one row 150 K), and a call
+ * with more fails. */
 MTQ_API int mtq_fp8_qmv(int dtype, const void *w, const float *w_scales, const void *x, void *out, uint32_t M, uint32_t N,
                         uint32_t K);
 

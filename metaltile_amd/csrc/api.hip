@@ -1419,7 +1419,7 @@ static int op_fp8_qmv(int dtype, const void* w, const float* ws, const void* x, 
     if (fp8_fused_takes(direct)) return launch_fp8_fused(dtype, direct, lc);
     const size_t codes = ((size_t)M * K + 255) / 256 * 256, scales = (size_t)M * fp8_blocks(K) * 4;
     rc = ensure_scratch(codes + scales);
-    if (rc) return rc;
+    if (rc) return fp8_fused_fits(direct) ? launch_fp8_fused(dtype, direct, lc) : rc;   // (no memory: quantised in LDS)
     float* xs = (float*)((char*)g.scratch_buf + codes);
     LaunchCtx first = lc, last = lc;
     first.stop = nullptr;

@@ -160,6 +160,8 @@ int fp8_rows_tiles(int dtype, const Fp8Args& a) {
     return groups(4, 2) <= (dtype == DT_F32 ? 2 : 1) * cus || a.K > kFp8TilesLongest ? 4 : 0;
 }
 
+// A workgroup's rows of x are sixteen at most, and all of K has to be in LDS.
+bool fp8_fused_fits(const Fp8Args& p) { return p.M <= 16 && fused_lds(p, 16) <= 160 * 1024; }
 // Every workgroup quantises the rows anew, which costs less than a launch of its own (3 us) for one row, or for a few where the workgroups are
 // few too (us, fused and not, K = 4096: 1 x 14336 16.9 / 18.2; 4 x 1024 6.8 / 9.0; 2 x 14336 19.4 / 18.6; 4 x 14336 24.5 / 19.7).
 bool fp8_fused_takes(const Fp8Args& p) { return (p.M == 1 || (p.M <= 4 && (uint64_t)p.M * ((p.N + 15) / 16) <= 256)) && fused_lds(p, 16) <= 40 * 1024; }

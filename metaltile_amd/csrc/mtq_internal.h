@@ -304,7 +304,8 @@ int launch_fp8_quantize(int dtype, const void* x, void* codes, float* scales, ui
 // (mt: sixteens of activation rows that a workgroup has; fp8_rows_tiles: how many it should have, or 0 where launch_fp8_tiles is the faster)
 int fp8_rows_tiles(int dtype, const Fp8Args& p);
 int launch_fp8_rows(int dtype, const Fp8Args& p, int mt, const LaunchCtx& lc);
-// (x: T, quantised on the way)
+// (x: T, quantised on the way; fits: whether it can be, takes: where that is the faster)
+bool fp8_fused_fits(const Fp8Args& p);
 bool fp8_fused_takes(const Fp8Args& p);
 int launch_fp8_fused(int dtype, const Fp8Args& p, const LaunchCtx& lc);
 int launch_fp8_tiles(int dtype, const Fp8Args& p, const LaunchCtx& lc);
