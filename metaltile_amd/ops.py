@@ -7,6 +7,7 @@ launches are asynchronous on the library stream; `GpuBuffer.read_*` waits.
 from __future__ import annotations
 
 import ctypes as C
+from collections.abc import Iterable
 
 from . import _lib
 from .dtypes import DType
@@ -165,12 +166,12 @@ def gated_delta_rule(dtype, q, k, v, g, beta, state_in, state_out, y, n_seqs, n_
     """The recurrence of a linear-attention layer over n_seqs sequences of n_tokens tokens in all: y f32[n_tokens, hv, dv] and the states
     f32[n_slots, hv, dv, dk] behind it. q, k: T[n_tokens, hk, dk], v: T[n_tokens, hv, dv], tokens row_stride elements apart (one number, or
     three for q, k and v; None: packed); g, beta f32[n_tokens, hv]. offsets u32[n_seqs + 1] (None: equal lengths), slots u32[n_seqs] (None:
-    0, 1, ..). state_in None: zeros. norm_eps >= 0: q and k over their 2-norms."""
+    0, 1, ..). state_in None: zeros. Without tokens q, k, v, g, beta and y may be None. norm_eps >= 0: q and k over their 2-norms."""
     lib = _ensure_init()
-    strides = (hk * dk, hk * dk, hv * dv) if row_stride is None else (row_stride,) * 3 if isinstance(row_stride, int) else tuple(row_stride)
+    strides = (hk * dk, hk * dk, hv * dv) if row_stride is None else tuple(row_stride) if isinstance(row_stride, Iterable) else (row_stride,) * 3
     at = lambda b: None if b is None else _p(b)
-    _lib.check(lib.mtq_gated_delta_rule(int(dtype), _p(q), strides[0], _p(k), strides[1], _p(v), strides[2], _p(g), _p(beta), at(offsets), at(slots),
-                                        at(state_in), _p(state_out), _p(y), n_seqs, n_tokens, n_seqs if n_slots is None else n_slots, hk, hv, dk, dv,
+    _lib.check(lib.mtq_gated_delta_rule(int(dtype), at(q), strides[0], at(k), strides[1], at(v), strides[2], at(g), at(beta), at(offsets), at(slots),
+                                        at(state_in), _p(state_out), at(y), n_seqs, n_tokens, n_seqs if n_slots is None else n_slots, hk, hv, dk, dv,
                                         scale, norm_eps))
 
 
