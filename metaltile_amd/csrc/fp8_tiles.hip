@@ -25,11 +25,12 @@ namespace mtq {
 
 namespace {
 
-// 16 bytes a lane from rsrc + voff (past the end: zeros) to LDS: lane l's at lds + 16 l. No register is written; counts in vmcnt.
+// 16 bytes a lane from rsrc + voff (past the end: zeros) to LDS: lane l's at lds + 16 l. No register is written; counts in vmcnt. M0 is read one wait
+// state behind its write at the earliest, which no one but this block sees to.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"   // M0 is a reserved register: naming it as clobbered is the point
 __device__ __forceinline__ void lds_load16(uint32_t lds, uint32_t voff, __attribute__((ext_vector_type(4))) uint32_t rsrc) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 __device__ __forceinline__ __attribute__((ext_vector_type(4))) uint32_t tile_rsrc(const uint8_t* base, uint32_t bytes) {

@@ -651,12 +651,12 @@ template <int DT, int DKP, int NT, bool AHEAD> __device__ __forceinline__ uint32
 
 // The walk's last wave: brings what the others read kAheadChunks chunks later from memory into the XCD's L2, a word of every 128-byte line (a
 // chunk takes less time than a line's way from memory, and registers hold one chunk ahead). The words go to LDS, so that nothing waits for
-// them. The workgroups of a head's columns share its lines.
+// them. The workgroups of a head's columns share its lines. (M0 is read one wait state behind its write at the earliest.)
 constexpr uint32_t kAheadChunks = 4;
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"   // M0 is a reserved register: naming it as clobbered is the point
 __device__ __forceinline__ void touch(const void* line, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(line) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(line) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 template <int DT, int DKP, int NT> __device__ __forceinline__ void walk_touch(const DeltaArgs& d, const WalkPlace& w, WalkLds<DKP>& lds, uint32_t columns) {

@@ -21,15 +21,15 @@ template <int B, int E, class F> __device__ __forceinline__ void qm_static_for(F
 
 // One 16-byte-per-lane load from global memory straight into LDS: lane l's bytes land at
 // lds_base + 16 * l (lds_base is wave-uniform and goes through M0); the global address is
-// sbase + voff per lane. Counts in vmcnt like any vector memory load.
+// sbase + voff per lane. Counts in vmcnt like any vector memory load. M0 is read one wait state behind its write at the earliest.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"   // M0 is a reserved register: naming it as clobbered is the point
 __device__ __forceinline__ void qm_load_to_lds(uint32_t lds_base, uint32_t voff, const void* sbase) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_base), "v"(voff), "s"(sbase) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_base), "v"(voff), "s"(sbase) : "memory", "m0");
 }
 // The same with 4 bytes per lane: lane l's dword lands at lds_base + 4 * l.
 __device__ __forceinline__ void qm_load_to_lds_b32(uint32_t lds_base, uint32_t voff, const void* sbase) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_base), "v"(voff), "s"(sbase) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_base), "v"(voff), "s"(sbase) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 // 16 bytes per lane from sbase + voff into registers. The result is valid only after a qm_wait_vm
