@@ -382,7 +382,7 @@ MTQ_API int mtq_fp8_qmv(int dtype, const void *w, const float *w_scales, const v
  * sequences are left alone, and offsets behind n_tokens read as n_tokens. hk divides hv; dk <= 256, dv <= 65536, n_seqs hv < 2^24.
  * A NaN or an infinity among the inputs reaches what comes behind it in its sequence and head (from v and the state: in its column).
  * So does one that the recurrence itself comes to (keys too long for their beta). Sums of squares are f32 as well: a q or k whose sum passes
- * its range counts as zeros where it is normalised.
+ * its range counts as zeros where it is normalised. In chunks what is under about 2^-109 keeps fewer than 24 bits.
  * Sequences that may be long go in chunks of 64 tokens through a library-owned buffer (allocated on first use, grown on demand up
  * to a gigabyte, or what the option scratch.most_kb allows; more chunks than fit go in turns). */
 MTQ_API int mtq_gated_delta_rule(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v,

@@ -15,8 +15,8 @@
 // Everything is held in f32 and multiplied as bf16 on the matrix cores without losing it: an f32 value is the sum of three bf16 terms (8
 // bits each, by rounding and taking the rest), a bf16 q or k is one, an f16 one two. Of the products of terms those of 2^-24 and less of the
 // whole are left out: 3 products for bf16 q and k against f32, 5 for f16, 6 for f32 against f32. That is f32 arithmetic at the rate of the
-// matrix cores over 3 to 6, two to five times what their own f32 instructions do. Sums of decays are f64 (differences of far ones would
-// lose an f32's last digits).
+// matrix cores over 3 to 6, two to five times what their own f32 instructions do. (Terms end at 2^-133, bf16's smallest: of values under about
+// 2^-109 the last bits are lost.) Sums of decays are f64 (differences of far ones would lose an f32's last digits).
 //
 // What the first launch leaves for the second lies in the order in which lanes hand it to the matrix cores, 16 bytes a lane, so that the
 // walk reads whole lines into registers and waits for no transposition.
