@@ -342,8 +342,8 @@ MTQ_API int mtq_dequant_gather(int dtype, int bits, uint32_t group_size, const v
  * row has one f32 scale; value = code * scale. Activations have blocks of 1 x 128 (scales f32[rows, ceil(cols / 128)]),
  * weights of 128 x 128 (scales f32[ceil(rows / 128), ceil(cols / 128)]); blocks at the right and lower edge may be cut.
  * All three calls: cols (K) a multiple of 16; x, codes and w on 16 bytes, rows packed. What is more than a launch
- * can have is MTQ_ERR_SHAPE: 2^28 blocks of 1 x 128 (2^24 of 128 x 128) and more in quantising, more than 2^28 rows of x,
- * 2^28 - 16 of w or 2^37 results in a product.
+ * can have (2^32 threads) is MTQ_ERR_SHAPE: 2^28 blocks of 1 x 128 (2^24 of 128 x 128) and more in quantising; no product of
+ * up to 2^28 rows of x, 2^28 - 16 of w and 2^37 results.
  *
  * fp8_quantize: block_rows 1 or 128. scale = max |x| / 448 over the block, not less than 2^-126 (1 where all are zero);
  * code = the e4m3 value nearest to the f32 quotient x / scale, ties to even. A NaN's code is NaN and does not count for

@@ -1389,15 +1389,18 @@ static int op_fp8_quantize(int dtype, const void* x, void* codes, float* scales,
 static int check_fp8(int dtype, const void* w, const float* ws, const void* x, const void* out, uint32_t M, uint32_t N, uint32_t K) {
     int rc = check_dtype(dtype);
     if (rc) return rc;
-    // What a launch can have (max_workgroups), whichever kernel takes the call: 16 weight rows to 256 threads; tiles of 128 x 128 results to 256 threads (f32)
-    // or, up to 128 rows of either side, to 1024, of 256 x 256 to 512; and 64 activation rows to one of 65535 along y where K is too long for tiles.
-    if (N == 0 || N > (1u << 28) - 16 || M > (1u << 28) || (uint64_t)M * N > 1ull << 37) return fail(ERR_SHAPE, "M must be at most 2^28, N at most 2^28 - 16 and not 0, M N at most 2^37");
-    if (K > kFp8TilesLongest && M > 65535u * 64) return fail(ERR_SHAPE, "too many activation rows of this length");
+    if (M > kFp8Longest || N == 0 || N > kFp8Longest) return fail(ERR_SHAPE, "M and N must be at most 2^30, N not 0");
     if (K == 0 || K % 16 || K > kFp8Longest) return fail(ERR_SHAPE, "K must be a non-zero multiple of 16 up to 2^30");
     if (!w || !ws || !x || !out) return fail(ERR_BAD_ARG, "null buffer");
     if (!on_16(w) || !on_16(x)) return fail(ERR_BAD_ARG, "w and x must be on 16 bytes");
     if (!on(4, ws) || !on(esize(dtype), out)) return fail(ERR_BAD_ARG, "scales and results must be aligned to their types");
     return ERR_OK;
+}
+
+// The launch that a product takes has to be one that there can be: asked before the quantiser's, too.
+static int check_fp8_launch(int dtype, const Fp8Args& a) {
+    const int mt = fp8_rows_tiles(dtype, a);
+    return (mt ? fp8_rows_fit(a, mt) : fp8_tiles_fit(dtype, a)) ? ERR_OK : fail(ERR_SHAPE, "more rows or results than a launch can have workgroups");
 }
 
 static int op_fp8_qmm(int dtype, const void* w, const float* ws, const void* x, const float* xs, void* out, uint32_t M, uint32_t N, uint32_t K, const LaunchCtx& lc) {
@@ -1407,6 +1410,7 @@ static int op_fp8_qmm(int dtype, const void* w, const float* ws, const void* x, 
     if (!xs) return fail(ERR_BAD_ARG, "null buffer");
     if (!on(4, xs)) return fail(ERR_BAD_ARG, "scales must be on 4 bytes");
     Fp8Args a{(const uint8_t*)w, ws, x, xs, out, M, N, K};
+    if ((rc = check_fp8_launch(dtype, a))) return rc;
     const int mt = fp8_rows_tiles(dtype, a);
     return mt ? launch_fp8_rows(dtype, a, mt, lc) : launch_fp8_tiles(dtype, a, lc);
 }
@@ -1416,6 +1420,7 @@ static int op_fp8_qmv(int dtype, const void* w, const float* ws, const void* x, 
     int rc = check_fp8(dtype, w, ws, x, out, M, N, K);
     if (rc) return rc;
     const Fp8Args direct{(const uint8_t*)w, ws, x, nullptr, out, M, N, K};
+    if ((rc = check_fp8_launch(dtype, direct))) return rc;   // (the fused form's is that of 16 rows)
     if (fp8_fused_takes(direct)) return launch_fp8_fused(dtype, direct, lc);
     const size_t codes = ((size_t)M * K + 255) / 256 * 256, scales = (size_t)M * fp8_blocks(K) * 4;
     rc = ensure_scratch(codes + scales);

@@ -177,15 +177,26 @@ int launch_fp8_fused(int dtype, const Fp8Args& p, const LaunchCtx& lc) {
     return ERR_OK;
 }
 
+static dim3 rows_grid(const Fp8Args& a, int mt, int& nt, int& nw) {
+    nt = mt == 1 ? 1 : 2;
+    nw = mt == 1 ? waves_of(a) : mt == 2 ? 8 : 4;
+    return dim3((a.N + 16 * nt - 1) / (16 * nt), (a.M + 16 * mt - 1) / (16 * mt));
+}
+bool fp8_rows_fit(const Fp8Args& a, int mt) {
+    int nt, nw;
+    const dim3 grid = rows_grid(a, mt, nt, nw);
+    return grid.x <= max_workgroups(64 * nw) && grid.y <= 65535u;
+}
+
 int launch_fp8_rows(int dtype, const Fp8Args& p, int mt, const LaunchCtx& lc) {
     Fp8Args a = p;
-    const int nt = mt == 1 ? 1 : 2, nw = mt == 1 ? waves_of(a) : mt == 2 ? 8 : 4;
-    const uint32_t ny = (a.M + 16 * mt - 1) / (16 * mt);
+    int nt, nw;
+    const dim3 grid = rows_grid(a, mt, nt, nw);
     const void* fn = dtype == DT_F32 ? rows_fn<DT_F32>(mt, nw) : dtype == DT_F16 ? rows_fn<DT_F16>(mt, nw) : rows_fn<DT_BF16>(mt, nw);
     const size_t lds = (size_t)nw * nt * mt * 1024;
     void* args[] = {&a};
     MTQ_HIP(set_max_dynamic_lds(fn, lds));
-    MTQ_HIP(launch_kernel(fn, dim3((a.N + 16 * nt - 1) / (16 * nt), ny), dim3(64 * nw), args, lds, lc));
+    MTQ_HIP(launch_kernel(fn, grid, dim3(64 * nw), args, lds, lc));
     return ERR_OK;
 }
 

@@ -198,17 +198,39 @@ template <int BM, int BN, int WM, int WN, int STAGES, bool HALVES, int... DTS> i
 
 }  // namespace
 
-int launch_fp8_tiles(int dtype, const Fp8Args& p, const LaunchCtx& lc) {
-    if (dtype == DT_F32) return launch<128, 128, 2, 2, 2, false, DT_F32>(dtype, p, 0, lc);
+// Which tiles a call takes: their number (those cut in two count twice), and threads for each.
+enum TileForm { TILES_F32, TILES_64, TILES_128, TILES_256 };
+struct TilePick {
+    TileForm form;
+    uint64_t groups;
+    uint32_t threads, halved;
+};
+static TilePick pick_tiles(int dtype, const Fp8Args& p) {
+    if (dtype == DT_F32) return {TILES_F32, tiles_of(p, 128, 128), 256, 0};
     const uint64_t cus = (uint64_t)fp8_num_cus();
-    if (tiles_of(p, 128, 64) <= cus) return launch<128, 64, 4, 2, 4, false, DT_F16, DT_BF16>(dtype, p, 0, lc);
+    if (tiles_of(p, 128, 64) <= cus) return {TILES_64, tiles_of(p, 128, 64), 512, 0};
     const uint64_t large = tiles_of(p, 256, 256), small = tiles_of(p, 128, 128), over = large % cus;
     // What is over after whole rounds of the CUs is cut in two where that gives each CU one half at most.
     const uint32_t halved = over && 2 * over <= cus ? (uint32_t)over : 0;
     // (the rounds' times as measured, in units of a tenth of a round of small tiles)
     const uint64_t large_time = large / cus * 24 + (halved ? 15 : over ? 24 : 0), small_time = (small + cus - 1) / cus * 10;
-    if (large_time < small_time) return launch<256, 256, 2, 4, 2, true, DT_F16, DT_BF16>(dtype, p, halved, lc);
-    return launch<128, 128, 4, 4, 4, false, DT_F16, DT_BF16>(dtype, p, 0, lc);
+    if (large_time < small_time) return {TILES_256, large + halved, 512, halved};
+    return {TILES_128, small, 1024, 0};
+}
+
+bool fp8_tiles_fit(int dtype, const Fp8Args& p) {
+    const TilePick t = pick_tiles(dtype, p);
+    return t.groups <= max_workgroups(t.threads);
+}
+
+int launch_fp8_tiles(int dtype, const Fp8Args& p, const LaunchCtx& lc) {
+    const TilePick t = pick_tiles(dtype, p);
+    switch (t.form) {
+        case TILES_F32: return launch<128, 128, 2, 2, 2, false, DT_F32>(dtype, p, 0, lc);
+        case TILES_64: return launch<128, 64, 4, 2, 4, false, DT_F16, DT_BF16>(dtype, p, 0, lc);
+        case TILES_256: return launch<256, 256, 2, 4, 2, true, DT_F16, DT_BF16>(dtype, p, t.halved, lc);
+        default: return launch<128, 128, 4, 4, 4, false, DT_F16, DT_BF16>(dtype, p, 0, lc);
+    }
 }
 
 }  // namespace mtq

@@ -304,6 +304,9 @@ int launch_fp8_quantize(int dtype, const void* x, void* codes, float* scales, ui
 // (mt: sixteens of activation rows that a workgroup has; fp8_rows_tiles: how many it should have, or 0 where launch_fp8_tiles is the faster)
 int fp8_rows_tiles(int dtype, const Fp8Args& p);
 int launch_fp8_rows(int dtype, const Fp8Args& p, int mt, const LaunchCtx& lc);
+// (fit: whether the launch has no more threads than there can be)
+bool fp8_rows_fit(const Fp8Args& p, int mt);
+bool fp8_tiles_fit(int dtype, const Fp8Args& p);
 // (x: T, quantised on the way; fits: whether it can be, takes: where that is the faster)
 bool fp8_fused_fits(const Fp8Args& p);
 bool fp8_fused_takes(const Fp8Args& p);

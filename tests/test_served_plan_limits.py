@@ -47,9 +47,11 @@ def test_fp8_products(dt, op):
         rc, launches, _, _ = plan(m, n, 16)
         _fits(rc, launches)
         assert rc == (SHAPE if op == "fp8_qmv" and m == 1 << 28 else OK)   # (as many blocks of x are more than the quantiser can have)
-    for m, n, k in ((1, most + 1, 16), ((1 << 28) + 1, 16, 16), (1 << 19, 1 << 19, 16), (1 << 22, 16, (1 << 22) + 16)):
+    for m, n, k in ((1, most + 1, 16), ((1 << 30) + 1, 16, 16), (1 << 22, 16, (1 << 22) + 16), (1 << 27, 1 << 27, 16)):
         rc, launches, _, _ = plan(m, n, k)
         assert rc == SHAPE and not launches
+    if op == "fp8_qmm":   # more rows of w where tiles take them
+        assert plan(100, 1 << 29, 16)[0] == (OK if dt == DType.F32 else SHAPE) and plan(200, 1 << 30, 16)[0] == (SHAPE if dt == DType.F32 else OK)
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
