@@ -365,6 +365,63 @@ MTQ_API int mtq_fp8_qmm(int dtype, const void *w, const float *w_scales, const v
 MTQ_API int mtq_fp8_qmv(int dtype, const void *w, const float *w_scales, const void *x, void *out, uint32_t M, uint32_t N,
                         uint32_t K);
 
+/* A layer's entrance in front of such products: h = x + residual, y = h * norm_weight / sqrt(mean(h^2) + eps), and y's codes and scales as
+ * mtq_fp8_quantize with block_rows 1 gives them, of the f32 y. x, residual, sum T[rows, cols], norm_weight T[cols]; residual NULL: h = x;
+ * sum (NULL: not wanted) receives h rounded to T, for the next residual; it may be x or residual itself. The norm is that of the f32 h. Sums
+ * are f32: a row whose squares pass f32's range comes out as zeros, and a NaN or an infinity makes its row's codes NaN or zeros.
+ * cols a multiple of 16; all buffers on 16 bytes, scales on 4, rows packed; rows < 2^28 and rows * cols / 128 < 2^31. */
+MTQ_API int mtq_add_rms_norm_fp8(int dtype, const void *x, const void *residual, const void *norm_weight, float eps, void *sum,
+                                 void *codes, float *scales, uint32_t rows, uint32_t cols);
+
+/* ---- attention over a paged cache in 4 bits ------------------------------ */
+
+/* A cache of keys and values in pages of page_size tokens (a power of two, 16 .. 65536). Codes, scales and biases are those of
+ * mtq_affine_quantize with 4 bits: of each token and key head head_dim / 8 words and head_dim / group_size scales and biases, group_size 32, 64
+ * or 128. Each array is contiguous and on 16 bytes, so that a page is also what mtq_affine_dequantize reads. head_dim 64, 128, 256. */
+typedef struct mtq_kv_cache {
+    void *k_codes, *k_scales, *k_biases; /* u32[n_pages, n_heads, page_size, head_dim / 8], T[n_pages, n_heads, page_size, head_dim / group_size] */
+    void *v_codes, *v_scales, *v_biases;
+    uint32_t n_pages, page_size, n_heads, head_dim, group_size;
+} mtq_kv_cache;
+
+/* The tokens of a call. Sequence i has lens[i] tokens in all, of which the last n are the call's own: rows offsets[i] .. offsets[i + 1] - 1
+ * of its arrays (u32[n_seqs + 1] on the device, ascending), or with offsets NULL n_tokens / n_seqs each. Token p of a sequence lies on
+ * page pages[i * pages_stride + p / page_size]; an id >= n_pages names no page. No sequence is longer than max_len (larger lens read as
+ * max_len), which is at most pages_stride * page_size and decides how the work is cut up. Where a sequence has more rows than
+ * tokens, the first rows have no place. Rows outside all sequences are left alone, and offsets behind n_tokens read as n_tokens.
+ * pages, offsets and lens are device memory, read when the kernel runs: a captured call follows them. */
+typedef struct mtq_kv_batch {
+    const uint32_t *pages, *offsets, *lens;
+    uint32_t pages_stride, n_seqs, n_tokens, max_len;
+} mtq_kv_batch;
+
+/* New keys and values into their pages, with the position rotation of queries and keys on the way. q: T, a token's hq heads of head_dim side
+ * by side, k and v: n_heads of them, tokens q_stride / k_stride / v_stride elements apart (so that the three may be parts of one row); q_out
+ * receives the rotated queries, tokens q_out_stride apart (it may be q itself). hq 0: no queries. A head's first `rot` values
+ * (even, 0 .. head_dim) are turned by the token's place p in its sequence: of pair j (values j and j + rot / 2, or with `neighbours`
+ * 2 j and 2 j + 1) (a, b) -> (a c - b s, b c + a s), c = cos_sin[p][j], s = cos_sin[p][rot / 2 + j], cos_sin f32[n_positions, rot],
+ * n_positions >= max_len; each product and sum rounded to f32, queries to T at the end. Keys (as f32) and values are quantised as
+ * mtq_affine_quantize does; a group with a NaN or an infinity reads as NaN. A row without a place is not rotated, and one on no page is not stored.
+ * No place twice. q, k, v, q_out on 16 bytes with strides of whole 16 bytes. n_tokens < 2^24. */
+MTQ_API int mtq_kv_append(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch *batch, const void *q, size_t q_stride, void *q_out,
+                          size_t q_out_stride, uint32_t hq, const void *k, size_t k_stride, const void *v, size_t v_stride,
+                          const float *cos_sin, uint32_t n_positions, uint32_t rot, uint32_t neighbours);
+
+/* The reader: the cached keys and values of the batch's rows (of a whole sequence where it has as many rows as tokens), value = scale * code +
+ * bias, product and sum rounded to f32, then to T: k_out, v_out T[n_tokens, n_heads, head_dim] (either may be NULL: not wanted). Rows without a place or
+ * on no page keep their bytes. */
+MTQ_API int mtq_kv_read(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch *batch, void *k_out, void *v_out);
+
+/* Softmax attention of the batch's rows over their sequences' tokens: out = sum_j p_j v_j, p = softmax_j(scale * q . k_j), over the tokens j
+ * up to the row's own place, with window > 0 the last `window` of them; tokens on no page do not count. q and out: T, hq heads
+ * of head_dim side by side, q_stride / out_stride elements apart (on 16 bytes, strides of whole 16 bytes); hq a multiple of n_heads,
+ * query head h goes with key head h / (hq / n_heads). A row that sees no token is zeros. Scores, softmax and sums are f32. For bf16
+ * p times a value's scale is rounded to bf16 once, for f16 it keeps 16 bits and for f32 24. Codes are operands as they are. What a row does not see does not
+ * reach it, NaN or not. Sequences of few rows are cut along their tokens and joined through a library-owned buffer (allocated
+ * on first use); without that memory they are not cut. n_tokens < 2^24, hq <= 65536. */
+MTQ_API int mtq_kv_attention(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch *batch, const void *q, size_t q_stride, void *out,
+                             size_t out_stride, uint32_t hq, float scale, uint32_t window);
+
 /* ---- either side of a model's layers ------------------------------------- */
 
 /* The gated delta rule: the recurrence of a linear-attention layer, between its input projections and
@@ -477,7 +534,11 @@ enum mtq_op {
     MTQ_OP_FP8_QMM = 9,         /* M, N, K */
     MTQ_OP_FP8_QMV = 10,
     MTQ_OP_GATED_DELTA_RULE = 11, /* E sequences of T tokens in all (by offsets), M = hk, N = hv, K = dk, group_size = dv */
-    MTQ_OP_TOKEN_LOGPROBS = 12  /* M rows, N = vocab, K = n_top */
+    MTQ_OP_TOKEN_LOGPROBS = 12, /* M rows, N = vocab, K = n_top */
+    MTQ_OP_ADD_RMS_NORM_FP8 = 13, /* M rows, K columns */
+    MTQ_OP_KV_APPEND = 14,      /* E sequences of T rows in all (by offsets), M = hq, N = n_heads, K = head_dim, bits = max_len; pages of 16 */
+    MTQ_OP_KV_READ = 15,
+    MTQ_OP_KV_ATTENTION = 16
 };
 #define MTQ_PLAN_MAX_LAUNCHES 8
 typedef struct mtq_plan_launch {

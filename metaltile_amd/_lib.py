@@ -48,8 +48,18 @@ class MtqPlanInfo(C.Structure):
     _fields_ = [("n_launches", C.c_int), ("launch", MtqPlanLaunch * PLAN_MAX_LAUNCHES), ("scratch_bytes", C.c_size_t)]
 
 
+class MtqKvCache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k_codes", "k_scales", "k_biases", "v_codes", "v_scales", "v_biases")] + \
+               [(n, C.c_uint32) for n in ("n_pages", "page_size", "n_heads", "head_dim", "group_size")]
+
+
+class MtqKvBatch(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("pages", "offsets", "lens")] + [(n, C.c_uint32) for n in ("pages_stride", "n_seqs", "n_tokens", "max_len")]
+
+
 _u32 = C.c_uint32
 _vp = C.c_void_p
+_cachep, _batchp = C.POINTER(MtqKvCache), C.POINTER(MtqKvBatch)
 _u32p = C.POINTER(C.c_uint32)
 _dblp = C.POINTER(C.c_double)
 _bufp = C.POINTER(MtqBuf)
@@ -96,6 +106,10 @@ SIGNATURES = {
     "mtq_gated_delta_rule": (C.c_int, [C.c_int, _vp, C.c_size_t, _vp, C.c_size_t, _vp, C.c_size_t, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                        _u32, _u32, _u32, _u32, _u32, _u32, _u32, C.c_float, C.c_float]),
     "mtq_token_logprobs": (C.c_int, [C.c_int, _vp, C.c_size_t, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _u32, _u32]),
+    "mtq_add_rms_norm_fp8": (C.c_int, [C.c_int, _vp, _vp, _vp, C.c_float, _vp, _vp, _vp, _u32, _u32]),
+    "mtq_kv_append": (C.c_int, [C.c_int, _cachep, _batchp, _vp, C.c_size_t, _vp, C.c_size_t, _u32, _vp, C.c_size_t, _vp, C.c_size_t, _vp, _u32, _u32, _u32]),
+    "mtq_kv_read": (C.c_int, [C.c_int, _cachep, _batchp, _vp, _vp]),
+    "mtq_kv_attention": (C.c_int, [C.c_int, _cachep, _batchp, _vp, C.c_size_t, _vp, C.c_size_t, _u32, C.c_float, _u32]),
     "mtq_dispatch": (C.c_int, [C.c_char_p, C.c_int, _bufp, C.c_int, _u32p, C.c_int, _u32p, _u32p, _dblp]),
     "mtq_measure": (C.c_int, [C.c_char_p, C.c_int, _bufp, C.c_int, _u32p, C.c_int, _u32p, _u32p, C.c_int, C.c_int, _dblp]),
     "mtq_dispatch_chain": (C.c_int, [C.POINTER(MtqDispatchSpec), C.c_int, C.c_int, _dblp, _dblp, _dblp]),

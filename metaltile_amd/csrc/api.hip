@@ -1477,6 +1477,87 @@ static int op_token_logprobs(int dtype, const void* logits, size_t stride, const
     return launch_logprobs(dtype, logits, stride, tokens, n_given, token_logprobs, entropy, top_ids, top_logprobs, n_top, rows, vocab, scratch, lc);
 }
 
+static int op_add_rms_norm_fp8(int dtype, const NormFp8Args& a, const LaunchCtx& lc) {
+    int rc = check_dtype(dtype);
+    if (rc) return rc;
+    if (a.cols == 0 || a.cols % 16 || a.cols > kFp8Longest) return fail(ERR_SHAPE, "cols must be a non-zero multiple of 16 up to 2^30");
+    if (!(a.eps >= 0.f)) return fail(ERR_BAD_ARG, "eps must not be negative");
+    if (a.rows >= 1u << 28 || (uint64_t)a.rows * fp8_blocks(a.cols) >= 1ull << 31) return fail(ERR_SHAPE, "rows must be less than 2^28, and 2^31 blocks");
+    if (a.rows == 0) return ERR_OK;
+    if (!a.x || !a.weight || !a.codes || !a.scales) return fail(ERR_BAD_ARG, "null buffer");
+    if (!on(16, a.x, a.residual, a.weight, a.sum, a.codes)) return fail(ERR_BAD_ARG, "buffers must be on 16 bytes");
+    if (!on(4, a.scales)) return fail(ERR_BAD_ARG, "scales must be on 4 bytes");
+    return launch_norm_fp8(dtype, a, lc);
+}
+
+// The cache and the batch of a call as the kernels take them.
+static int check_kv(int dtype, const mtq_kv_cache* c, const mtq_kv_batch* b, KvArgs& a) {
+    int rc = check_dtype(dtype);
+    if (rc) return rc;
+    if (!c || !b) return fail(ERR_BAD_ARG, "null cache or batch");
+    if (c->page_size < 16 || c->page_size > 65536 || (c->page_size & (c->page_size - 1))) return fail(ERR_SHAPE, "page_size must be a power of two in 16..65536");
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return fail(ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
+    if ((c->group_size != 32 && c->group_size != 64 && c->group_size != 128) || c->group_size > c->head_dim) return fail(ERR_SHAPE, "group_size must be 32, 64 or 128 and divide head_dim");
+    if (c->n_heads == 0 || c->n_heads > 65536) return fail(ERR_SHAPE, "n_heads must be in 1..65536");
+    if (b->n_tokens >= 1u << 24 || b->n_seqs >= 1u << 24) return fail(ERR_SHAPE, "n_tokens and n_seqs must be less than 2^24");
+    if (b->max_len > 1u << 30 || b->max_len > (uint64_t)b->pages_stride * c->page_size) return fail(ERR_SHAPE, "max_len must be at most pages_stride * page_size, and 2^30");
+    if (!b->offsets && b->n_seqs && b->n_tokens % b->n_seqs) return fail(ERR_SHAPE, "without offsets n_seqs must divide n_tokens");
+    a.k = {(uint32_t*)c->k_codes, c->k_scales, c->k_biases};
+    a.v = {(uint32_t*)c->v_codes, c->v_scales, c->v_biases};
+    a.pages = b->pages; a.offsets = b->offsets; a.lens = b->lens;
+    a.pages_stride = b->pages_stride; a.n_pages = c->n_pages; a.page_log2 = (uint32_t)__builtin_ctz(c->page_size);
+    a.hkv = c->n_heads; a.dim = c->head_dim; a.group = c->group_size;
+    a.n_seqs = b->n_seqs; a.n_tokens = b->n_tokens; a.max_len = b->max_len;
+    if (a.n_seqs == 0 || a.n_tokens == 0) return ERR_OK;   // (no row: nothing else is looked at)
+    if (!a.lens || (a.max_len && !a.pages)) return fail(ERR_BAD_ARG, "null buffer");
+    if (a.n_pages)
+        for (const KvPart* p : {&a.k, &a.v})
+            if (!p->codes || !p->scales || !p->biases) return fail(ERR_BAD_ARG, "null buffer");
+    if (!on(16, a.k.codes, a.k.scales, a.k.biases, a.v.codes, a.v.scales, a.v.biases)) return fail(ERR_BAD_ARG, "the cache's arrays must be on 16 bytes");
+    if (!on(4, a.pages, a.offsets, a.lens)) return fail(ERR_BAD_ARG, "pages, offsets and lens must be on 4 bytes");
+    return ERR_OK;
+}
+// Rows of heads T[rows, heads, dim], `stride` elements apart.
+static int check_heads(int dtype, const void* p, uint64_t stride, uint64_t heads, uint32_t dim) {
+    if (!p) return fail(ERR_BAD_ARG, "null buffer");
+    if (stride < heads * dim) return fail(ERR_SHAPE, "a token's heads do not fit its stride");
+    if (stride > SIZE_MAX / 8 >> 24) return fail(ERR_SHAPE, "the stride is too large");
+    if (!on(16, p) || stride * esize(dtype) % 16) return fail(ERR_BAD_ARG, "rows must be on 16 bytes, their strides whole 16 bytes");
+    return ERR_OK;
+}
+
+static int op_kv_append(int dtype, const mtq_kv_cache* c, const mtq_kv_batch* b, KvAppendArgs& a, uint32_t n_positions, const LaunchCtx& lc) {
+    int rc = check_kv(dtype, c, b, a.kv);
+    if (rc) return rc;
+    if (a.hq > 65536) return fail(ERR_SHAPE, "hq must be at most 65536");
+    if (a.rot % 2 || a.rot > a.kv.dim) return fail(ERR_SHAPE, "rot must be even and at most head_dim");
+    if (a.rot && n_positions < a.kv.max_len) return fail(ERR_SHAPE, "the table must have a row for each of max_len positions");
+    if (a.kv.n_seqs == 0 || a.kv.n_tokens == 0) return ERR_OK;
+    if ((rc = check_heads(dtype, a.k, a.k_stride, a.kv.hkv, a.kv.dim)) || (rc = check_heads(dtype, a.v, a.v_stride, a.kv.hkv, a.kv.dim))) return rc;
+    if (a.hq && ((rc = check_heads(dtype, a.q, a.q_stride, a.hq, a.kv.dim)) || (rc = check_heads(dtype, a.q_out, a.q_out_stride, a.hq, a.kv.dim)))) return rc;
+    if (a.q && a.q == a.q_out && a.q_stride != a.q_out_stride) return fail(ERR_BAD_ARG, "queries that are turned in place must keep their stride");
+    if (a.rot && !a.cos_sin) return fail(ERR_BAD_ARG, "null buffer");
+    if (!on(16, a.cos_sin)) return fail(ERR_BAD_ARG, "cos_sin must be on 16 bytes");
+    return launch_kv_append(dtype, a, lc);
+}
+
+static int op_kv_read(int dtype, const mtq_kv_cache* c, const mtq_kv_batch* b, KvReadArgs& a, const LaunchCtx& lc) {
+    int rc = check_kv(dtype, c, b, a.kv);
+    if (rc) return rc;
+    if (a.kv.n_seqs == 0 || a.kv.n_tokens == 0 || (!a.k && !a.v)) return ERR_OK;
+    if (!on(16, a.k, a.v)) return fail(ERR_BAD_ARG, "rows must be on 16 bytes");
+    return launch_kv_read(dtype, a, lc);
+}
+
+static int op_kv_attention(int dtype, const mtq_kv_cache* c, const mtq_kv_batch* b, KvAttentionArgs& a, const LaunchCtx& lc) {
+    int rc = check_kv(dtype, c, b, a.kv);
+    if (rc) return rc;
+    if (a.hq == 0 || a.hq > 65536 || a.hq % a.kv.hkv) return fail(ERR_SHAPE, "hq must be a multiple of n_heads up to 65536");
+    if (a.kv.n_seqs == 0 || a.kv.n_tokens == 0) return ERR_OK;
+    if ((rc = check_heads(dtype, a.q, a.q_stride, a.hq, a.kv.dim)) || (rc = check_heads(dtype, a.out, a.out_stride, a.hq, a.kv.dim))) return rc;
+    return launch_kv_attention(dtype, a, lc);
+}
+
 // ---------------------------------------------------------------------------
 // extern "C"
 // ---------------------------------------------------------------------------
@@ -1828,6 +1909,36 @@ int mtq_token_logprobs(int dtype, const void* logits, size_t row_stride, const u
     return op_token_logprobs(dtype, logits, row_stride, tokens, n_given, token_logprobs, entropy, top_ids, top_logprobs, n_top, n_rows, vocab, make_ctx());
 }
 
+int mtq_add_rms_norm_fp8(int dtype, const void* x, const void* residual, const void* norm_weight, float eps, void* sum, void* codes, float* scales, uint32_t rows,
+                         uint32_t cols) {
+    int rc = need_ready();
+    if (rc) return rc;
+    return op_add_rms_norm_fp8(dtype, {x, residual, norm_weight, sum, (uint8_t*)codes, scales, rows, cols, eps}, make_ctx());
+}
+
+int mtq_kv_append(int dtype, const mtq_kv_cache* cache, const mtq_kv_batch* batch, const void* q, size_t q_stride, void* q_out, size_t q_out_stride, uint32_t hq,
+                  const void* k, size_t k_stride, const void* v, size_t v_stride, const float* cos_sin, uint32_t n_positions, uint32_t rot, uint32_t neighbours) {
+    int rc = need_ready();
+    if (rc) return rc;
+    KvAppendArgs a{{}, q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, cos_sin, hq, rot, neighbours};
+    return op_kv_append(dtype, cache, batch, a, n_positions, make_ctx());
+}
+
+int mtq_kv_read(int dtype, const mtq_kv_cache* cache, const mtq_kv_batch* batch, void* k_out, void* v_out) {
+    int rc = need_ready();
+    if (rc) return rc;
+    KvReadArgs a{{}, k_out, v_out};
+    return op_kv_read(dtype, cache, batch, a, make_ctx());
+}
+
+int mtq_kv_attention(int dtype, const mtq_kv_cache* cache, const mtq_kv_batch* batch, const void* q, size_t q_stride, void* out, size_t out_stride, uint32_t hq,
+                     float scale, uint32_t window) {
+    int rc = need_ready();
+    if (rc) return rc;
+    KvAttentionArgs a{{}, q, out, q_stride, out_stride, hq, window, scale};
+    return op_kv_attention(dtype, cache, batch, a, make_ctx());
+}
+
 int mtq_kernel_supported(const char* kernel_name) { return find_kernel(kernel_name) ? 1 : 0; }
 int mtq_kernel_count(void) { return kTableLen; }
 const char* mtq_kernel_name(int i) { return i >= 0 && i < kTableLen ? kTable[i].name : nullptr; }
@@ -2036,7 +2147,7 @@ int mtq_plan(int op, int dtype, int bits, uint32_t group_size, uint32_t M, uint3
              mtq_plan_info* info) {
     if (!info) return fail(ERR_BAD_ARG, "plan: info must not be null");
     memset(info, 0, sizeof(*info));
-    if (op < MTQ_OP_QMV || op > MTQ_OP_TOKEN_LOGPROBS) return fail(ERR_BAD_ARG, "plan: unknown op");
+    if (op < MTQ_OP_QMV || op > MTQ_OP_KV_ATTENTION) return fail(ERR_BAD_ARG, "plan: unknown op");
     // Stand-in operand addresses: distinct, 256-byte aligned, never dereferenced (no launch happens).
     auto at = [](int i) { return (void*)(uintptr_t)(0x100000000ull + ((uint64_t)i << 36)); };
     void *w = at(1), *s = at(2), *b = at(3), *x = at(4), *aux = at(6), *aux2 = at(7);
@@ -2073,6 +2184,26 @@ int mtq_plan(int op, int dtype, int bits, uint32_t group_size, uint32_t M, uint3
         case MTQ_OP_TOKEN_LOGPROBS:
             rc = op_token_logprobs(dtype, x, N, (const uint32_t*)aux, 1, (float*)out, (float*)s, (uint32_t*)b, (float*)w, K, M, N, lc);
             break;
+        case MTQ_OP_ADD_RMS_NORM_FP8: rc = op_add_rms_norm_fp8(dtype, {x, b, w, out, (uint8_t*)aux, (float*)s, M, K, 0.f}, lc); break;
+        case MTQ_OP_KV_APPEND:
+        case MTQ_OP_KV_READ:
+        case MTQ_OP_KV_ATTENTION: {
+            const uint32_t pages = ((uint32_t)bits + 15u) / 16u;
+            const mtq_kv_cache cache{w, s, b, at(9), at(10), at(11), E * pages, 16, N, K, group_size};
+            const mtq_kv_batch batch{(const uint32_t*)aux, (const uint32_t*)aux2, (const uint32_t*)at(12), pages, E, T, (uint32_t)bits};
+            const uint64_t wide = (uint64_t)M * K, narrow = (uint64_t)N * K;
+            if (op == MTQ_OP_KV_APPEND) {
+                KvAppendArgs p{{}, x, at(13), at(14), out, wide, narrow, narrow, wide, (const float*)at(15), M, K, 0};
+                rc = op_kv_append(dtype, &cache, &batch, p, (uint32_t)bits, lc);
+            } else if (op == MTQ_OP_KV_READ) {
+                KvReadArgs p{{}, x, out};
+                rc = op_kv_read(dtype, &cache, &batch, p, lc);
+            } else {
+                KvAttentionArgs p{{}, x, out, wide, wide, M, 0, 1.f};
+                rc = op_kv_attention(dtype, &cache, &batch, p, lc);
+            }
+            break;
+        }
         default: rc = op_rms_norm_qmv(dtype, bits, group_size, x, aux, w, s, b, out, (const float*)aux2, N, K, lc); break;
     }
     info->n_launches = g_plan.n;

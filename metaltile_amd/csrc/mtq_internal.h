@@ -332,4 +332,50 @@ bool delta_chunks_serve(const DeltaArgs& d);
 size_t delta_chunks_scratch_bytes(const DeltaArgs& d, size_t most);
 int launch_delta_chunks(const DeltaArgs& d, void* scratch, size_t bytes, const LaunchCtx& lc);
 
+// A paged cache in 4 bits (kv_cache.h), and the tokens of a call. Page sizes are powers of two, 16 and more.
+struct KvPart {
+    uint32_t* codes = nullptr;
+    void *scales = nullptr, *biases = nullptr;
+};
+struct KvArgs {
+    KvPart k, v;
+    const uint32_t *pages = nullptr, *offsets = nullptr, *lens = nullptr;   // [n_seqs, pages_stride], [n_seqs + 1] (null: equal numbers), [n_seqs]
+    uint32_t pages_stride = 0, n_pages = 0, page_log2 = 4, hkv = 0, dim = 0, group = 0;
+    uint32_t n_seqs = 0, n_tokens = 0, max_len = 0;
+};
+struct KvAppendArgs {
+    KvArgs kv;
+    const void *q = nullptr, *k = nullptr, *v = nullptr;   // T, a token's heads side by side; strides in elements
+    void* q_out = nullptr;
+    uint64_t q_stride = 0, k_stride = 0, v_stride = 0, q_out_stride = 0;
+    const float* cos_sin = nullptr;   // [positions, rot]: cosines of rot / 2 angles, then their sines
+    uint32_t hq = 0, rot = 0, neighbours = 0;
+};
+struct KvReadArgs {
+    KvArgs kv;
+    void *k = nullptr, *v = nullptr;  // T [n_tokens, hkv, dim]; either may be null
+};
+struct KvAttentionArgs {
+    KvArgs kv;
+    const void* q = nullptr;
+    void* out = nullptr;
+    uint64_t q_stride = 0, out_stride = 0;
+    uint32_t hq = 0, window = 0;      // window 0: all tokens before
+    float scale = 1.f;
+};
+int launch_kv_append(int dtype, const KvAppendArgs& p, const LaunchCtx& lc);
+int launch_kv_read(int dtype, const KvReadArgs& p, const LaunchCtx& lc);
+int launch_kv_attention(int dtype, const KvAttentionArgs& p, const LaunchCtx& lc);
+
+// Residual addition, RMS norm and 8-bit output (norm_fp8.hip).
+struct NormFp8Args {
+    const void *x = nullptr, *residual = nullptr, *weight = nullptr;   // residual null: none
+    void* sum = nullptr;                                               // null: not wanted
+    uint8_t* codes = nullptr;
+    float* scales = nullptr;
+    uint32_t rows = 0, cols = 0;
+    float eps = 0.f;
+};
+int launch_norm_fp8(int dtype, const NormFp8Args& p, const LaunchCtx& lc);
+
 }  // namespace mtq

@@ -18,6 +18,10 @@ def _p(b):
     return b.ptr if isinstance(b, GpuBuffer) else int(b)
 
 
+def _at(b):
+    return None if b is None else _p(b)
+
+
 def qmv(dtype: DType, bits: int, group_size: int, w, scales, biases, x, out, M: int, N: int, K: int):
     lib = _ensure_init()
     _lib.check(lib.mtq_qmv(int(dtype), bits, group_size, _p(w), _p(scales), _p(biases), _p(x), _p(out), M, N, K))
@@ -161,6 +165,57 @@ def fp8_qmv(dtype, w, w_scales, x, out, M, N, K):
     _lib.check(lib.mtq_fp8_qmv(int(dtype), _p(w), _p(w_scales), _p(x), _p(out), M, N, K))
 
 
+def add_rms_norm_fp8(dtype, x, residual, norm_weight, eps, sum_out, codes, scales, rows, cols):
+    """h = x + residual (None: x alone), rounded to T in sum_out (None: not wanted; may be x or residual), and its RMS norm times norm_weight as e4m3
+    codes u8[rows, cols] with a f32 scale for each 1 x 128 block: the activations of fp8_qmm."""
+    lib = _ensure_init()
+    _lib.check(lib.mtq_add_rms_norm_fp8(int(dtype), _p(x), _at(residual), _p(norm_weight), eps, _at(sum_out), _p(codes), _p(scales), rows, cols))
+
+
+class KvCache(_lib.MtqKvCache):
+    """A paged cache of keys and values in 4 bits: codes u32[n_pages, n_heads, page_size, head_dim / 8], scales and biases
+    T[n_pages, n_heads, page_size, head_dim / group_size] of each. Holds on to the buffers it is given."""
+
+    def __init__(self, k_codes, k_scales, k_biases, v_codes, v_scales, v_biases, n_pages, page_size, n_heads, head_dim, group_size):
+        self.buffers = (k_codes, k_scales, k_biases, v_codes, v_scales, v_biases)
+        super().__init__(*map(_p, self.buffers), n_pages, page_size, n_heads, head_dim, group_size)
+
+
+class KvBatch(_lib.MtqKvBatch):
+    """n_seqs sequences of lens (u32[n_seqs] on the device, at most max_len) tokens, the n_tokens rows of a call among them as their last: by offsets
+    (u32[n_seqs + 1] on the device) or, with None, equally many each. pages u32[n_seqs, pages_stride] on the device."""
+
+    def __init__(self, pages, pages_stride, lens, n_seqs, n_tokens, max_len, offsets=None):
+        self.buffers = (pages, offsets, lens)
+        super().__init__(_p(pages), _at(offsets), _p(lens), pages_stride, n_seqs, n_tokens, max_len)
+
+
+def kv_append(dtype, cache, batch, k, v, *, row_stride=None, q=None, q_out=None, hq=0, q_out_stride=None, cos_sin=None, n_positions=0, rot=0, neighbours=False):
+    """Keys and values T[n_tokens, n_heads, head_dim] of the batch's rows into their pages, keys and queries T[n_tokens, hq, head_dim] turned by their positions
+    first: the first `rot` values of a head by cos_sin f32[n_positions, rot] (cosines, then sines), paired as halves or as neighbours. Turned queries to
+    q_out. Tokens row_stride elements apart (one number, or three for q, k and v; None: packed)."""
+    lib = _ensure_init()
+    wide, narrow = hq * cache.head_dim, cache.n_heads * cache.head_dim
+    strides = (wide, narrow, narrow) if row_stride is None else tuple(row_stride) if isinstance(row_stride, Iterable) else (row_stride,) * 3
+    _lib.check(lib.mtq_kv_append(int(dtype), cache, batch, _at(q), strides[0], _at(q_out), wide if q_out_stride is None else q_out_stride, hq, _at(k), strides[1], _at(v),
+                                 strides[2], _at(cos_sin), n_positions, rot, int(neighbours)))
+
+
+def kv_read(dtype, cache, batch, k_out, v_out):
+    """Cached keys and values of the batch's rows as T[n_tokens, n_heads, head_dim] (None: not wanted)."""
+    lib = _ensure_init()
+    _lib.check(lib.mtq_kv_read(int(dtype), cache, batch, _at(k_out), _at(v_out)))
+
+
+def kv_attention(dtype, cache, batch, q, out, hq, scale, *, window=0, q_stride=None, out_stride=None):
+    """Softmax attention of the batch's rows q T[n_tokens, hq, head_dim] over their sequences' cached tokens, up to each row's own place and, with
+    window > 0, the last `window` of them. Strides in elements between tokens (None: packed)."""
+    lib = _ensure_init()
+    wide = hq * cache.head_dim
+    _lib.check(lib.mtq_kv_attention(int(dtype), cache, batch, _at(q), wide if q_stride is None else q_stride, _at(out), wide if out_stride is None else out_stride, hq, scale,
+                                    window))
+
+
 def gated_delta_rule(dtype, q, k, v, g, beta, state_in, state_out, y, n_seqs, n_tokens, hk, hv, dk, dv, *, row_stride=None, offsets=None, slots=None,
                      n_slots=None, scale=1.0, norm_eps=-1.0):
     """The recurrence of a linear-attention layer over n_seqs sequences of n_tokens tokens in all: y f32[n_tokens, hv, dv] and the states
@@ -199,7 +254,8 @@ def sync():
 
 
 PLAN_OPS = {"qmv": 0, "qmm": 1, "qmm_mma": 2, "qvm": 3, "gather_csr": 4, "gather_indices": 5, "gather_single": 6, "rms_norm_qmv": 7,
-            "fp8_quantize": 8, "fp8_qmm": 9, "fp8_qmv": 10, "gated_delta_rule": 11, "token_logprobs": 12}
+            "fp8_quantize": 8, "fp8_qmm": 9, "fp8_qmv": 10, "gated_delta_rule": 11, "token_logprobs": 12,
+            "add_rms_norm_fp8": 13, "kv_append": 14, "kv_read": 15, "kv_attention": 16}
 
 
 def plan(op: str, dtype, bits: int, group_size: int, M: int = 1, N: int = 0, K: int = 0, E: int = 1, T: int = 0):
