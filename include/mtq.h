@@ -418,7 +418,7 @@ MTQ_API int mtq_kv_read(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch
  * query head h goes with key head h / (hq / n_heads). A row that sees no token is zeros. Scores, softmax and sums are f32. For bf16
  * p times a value's scale is rounded to bf16 once, for f16 it keeps 16 bits and for f32 24. Codes are operands as they are. What a row does not see does not
  * reach it, NaN or not. Sequences of few rows are cut along their tokens and joined through a library-owned buffer (allocated
- * on first use); without that memory they are not cut. n_tokens < 2^24, hq <= 65536. */
+ * on first use); without that memory they are not cut. n_tokens < 2^24, hq <= 65536, n_tokens * hq < 2^31. */
 MTQ_API int mtq_kv_attention(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch *batch, const void *q, size_t q_stride, void *out,
                              size_t out_stride, uint32_t hq, float scale, uint32_t window);
 
@@ -634,6 +634,8 @@ MTQ_API int mtq_flush_cache(void);
  *   "gather.names_exact"   the exact-dequant gather names of mtq_dispatch (mt_moe_gather_qmm_int4, _m8, _m16, _m32, _b3 ..
  *                          _b8): 0 = always on the GEMV kernels (exact s*q + b, as those reference kernels compute), 1 = grouped
  *                          on the tile kernel above 8 rows per expert like the typed entry points (w_hat rounded to T first)
+ *   "kv.waves"             mtq_kv_attention: workgroups of 4 waves (1) or of as many as fit (2), 0 = choose
+ *   "kv.slices"            and slices of a sequence's tokens that are joined behind, 0 = choose, or 1..1024
  *   "scratch.most_kb"      largest library-owned scratch buffer in KB, 0 = no limit: a call that wants more goes the way it goes
  *                          where that memory cannot be allocated
  *   "qvm.wgs"              qvm: workgroups to aim for when K is sliced, 0 = choose

@@ -1555,7 +1555,11 @@ static int op_kv_attention(int dtype, const mtq_kv_cache* c, const mtq_kv_batch*
     if (a.hq == 0 || a.hq > 65536 || a.hq % a.kv.hkv) return fail(ERR_SHAPE, "hq must be a multiple of n_heads up to 65536");
     if (a.kv.n_seqs == 0 || a.kv.n_tokens == 0) return ERR_OK;
     if ((rc = check_heads(dtype, a.q, a.q_stride, a.hq, a.kv.dim)) || (rc = check_heads(dtype, a.out, a.out_stride, a.hq, a.kv.dim))) return rc;
-    return launch_kv_attention(dtype, a, lc);
+    if ((uint64_t)a.kv.n_tokens * a.hq >= 1ull << 31) return fail(ERR_SHAPE, "n_tokens * hq must be less than 2^31");
+    const KvPlan plan = kv_attention_plan(dtype, a);
+    // (no memory for the slices' sums: sequences are not cut)
+    void* scratch = plan.scratch && ensure_scratch(plan.scratch) == ERR_OK ? g.scratch_buf : nullptr;
+    return launch_kv_attention(dtype, a, plan, scratch, lc);
 }
 
 // ---------------------------------------------------------------------------
@@ -2391,6 +2395,16 @@ int mtq_set_option(const char* name, int value) {
     if (!strcmp(name, "qmv.norm_mfma")) {
         if (value < 0 || value > 2) return fail(ERR_BAD_ARG, "qmv.norm_mfma must be 0 (choose), 1 (never) or 2 (wherever the shape allows)");
         options().qmv_norm_mfma = value;
+        return MTQ_OK;
+    }
+    if (!strcmp(name, "kv.waves")) {
+        if (value < 0 || value > 2) return fail(ERR_BAD_ARG, "kv.waves must be 0 (choose), 1 (workgroups of 4 waves) or 2 (of as many as fit)");
+        options().kv_waves = value;
+        return MTQ_OK;
+    }
+    if (!strcmp(name, "kv.slices")) {
+        if (value < 0 || value > 1024) return fail(ERR_BAD_ARG, "kv.slices must be 0 (choose) or 1..1024");
+        options().kv_slices = value;
         return MTQ_OK;
     }
     if (!strcmp(name, "scratch.most_kb")) {
