@@ -33,7 +33,7 @@ template <int DT, int D, int G> struct RowsLds {
     static constexpr int JOIN = 16 * (D + 4) * 4;                // rows' values, and behind each its maximum and sum
     static constexpr int WAVE = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
     // Waves of a SIMD at a time, by the registers that the sums, queries and a block's numbers take; and of a large workgroup.
-    static constexpr int AT_ONCE = DT != DT_F32 && D <= 128 && G >= 64 ? 4 : 2;
+    static constexpr int AT_ONCE = DT != DT_F32 && D <= 128 && G >= 64 ? 3 : 2;
     static constexpr int MOST = 4 * AT_ONCE * WAVE <= 160 * 1024 ? 4 * AT_ONCE : 4;
     static_assert(MOST * WAVE <= 160 * 1024, "");
 };
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(64 * NW, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows
     uint8_t* mine = lds + wave * L::WAVE;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)mine;
     const uint32_t rows = s.rows * shared;   // (fewer than 2^24 2^16: checked against the launch on the host)
-    const float c = fabsf(a.scale) * kLog2e;
+    const float c = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);   // (not 0: what is hidden scores -inf)
     const uint32_t k16 = kv_sixteen<T::QK>(), v16 = kv_sixteen<DT_BF16>();
 
     for (uint32_t row0 = 0; row0 < rows; row0 += 16) {
@@ -136,33 +136,42 @@ __global__ __launch_bounds__(64 * NW, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows
             }
         };
 
-        kr_f32x4 o[NG][NT] = {}, ones[NG] = {};   // values by group and tile, and -24 sum p s
-        float bias[NG] = {}, sum = 0.f, bar = -INFINITY;
-        auto block = [&](uint32_t b, auto masked) {
+        kr_f32x4 o[NG][NT] = {};   // values by group and tile
+        float ones[NG] = {}, bias[NG] = {}, sum = 0.f, bar = -INFINITY;   // (ones: -24 sum p s)
+        auto block = [&](uint32_t b, bool whole) {   // whole: every row sees all of the block
             const uint8_t* at = mine + (b & 1u) * L::STAGE;
             const uint32_t t0 = lo + 32u * b, h = lo / 16u + 2u * b;
-            // Scales and biases of this lane's tokens 4 g .. 4 g + 3 of a half.
-            auto numbers = [&](const uint8_t* p, int array, int half, float (&v)[4][NG]) {
-                constexpr int WORDS = NG * ES;
-                uint32_t w[WORDS];
-                const uint8_t* from8 = p + (array * 2 + half) * L::HALF + g * (4 * WORDS);
-#pragma unroll
-                for (int i = 0; i < WORDS; i += 2) {
-                    const uint2 two = *(const uint2*)(from8 + 4 * i);
-                    w[i] = two.x;
-                    w[i + 1] = two.y;
+            // Scales or biases of this lane's tokens 4 g .. 4 g + 3 of a half, as they are stored, and one of them.
+            struct Numbers {
+                uint32_t w[NG * ES];
+                __device__ __forceinline__ float operator()(int i, int n) const {
+                    const int e = i * NG + n;
+                    if constexpr (DT == DT_F32) return __uint_as_float(w[e]);
+                    else return kr_elem<DT>(w[e / 2], e & 1);
                 }
+                __device__ __forceinline__ void keep(int i, uint32_t yes) {   // or 0 in the place of token i's
+                    const uint32_t all = 0u - yes;
+                    if constexpr (NG * ES == 2) {
+                        w[i / 2] &= i & 1 ? all | 0xFFFFu : all | 0xFFFF0000u;
+                    } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int n = 0; n < NG; n++) {
-                        const int e = i * NG + n;
-                        if constexpr (DT == DT_F32) v[i][n] = __uint_as_float(w[e]);
-                        else v[i][n] = kr_elem<DT>(w[e / 2], e & 1);
+                        for (int j = 0; j < NG * ES / 4; j++) w[i * (NG * ES / 4) + j] &= all;
                     }
+                }
             };
-            float x[2][4];
-            bool seen[2][4];
+            auto numbers = [&](const uint8_t* p, int array, int half) {
+                Numbers v;
+                const uint8_t* from8 = p + (array * 2 + half) * L::HALF + g * (4 * NG * ES);
+#pragma unroll
+                for (int i = 0; i < NG * ES; i += 2) {
+                    const uint2 two = *(const uint2*)(from8 + 4 * i);
+                    v.w[i] = two.x;
+                    v.w[i + 1] = two.y;
+                }
+                return v;
+            };
+            float x[2][4];   // scores, then weights
+            uint32_t seen = 0xFFu;   // (a bit for each score: what is not whole is a small part of the blocks)
             float top = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 2; t++) {
@@ -181,106 +190,110 @@ __global__ __launch_bounds__(64 * NW, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows
 #pragma unroll
                     for (int e = T::Q - 1; e >= 0; e--) acc[i * 32 / G] = kr_mfma<T::QK>(k, q[e][i], acc[i * 32 / G]);
                 }
-                float ks[4][NG], kb[4][NG];
-                numbers(at + L::CODES, 0, t, ks);
-                numbers(at + L::CODES, 1, t, kb);
-                const bool there = !masked || half_of(h + t) < kv.n_pages;
+                const Numbers ks = numbers(at + L::CODES, 0, t), kb = numbers(at + L::CODES, 1, t);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float v = ks[i][0] * acc[0][i];
-                    v = fmaf(kb[i][0], qsum[0], v);
+                    float v = ks(i, 0) * acc[0][i];
+                    v = fmaf(kb(i, 0), qsum[0], v);
 #pragma unroll
-                    for (int n = 1; n < NG; n++) v = fmaf(kb[i][n], qsum[n], fmaf(ks[i][n], acc[n][i], v));
-                    if constexpr (masked) {
-                        const uint32_t tok = t0 + 16 * t + 4 * g + i;
-                        seen[t][i] = there && tok >= from && tok < end;
-                        v = seen[t][i] ? v : -INFINITY;
-                    }
+                    for (int n = 1; n < NG; n++) v = fmaf(kb(i, n), qsum[n], fmaf(ks(i, n), acc[n][i], v));
                     x[t][i] = v;
-                    top = fmaxf(top, v);
                 }
+                if (!whole) {
+                    const bool there = half_of(h + t) < kv.n_pages;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t tok = t0 + 16 * t + 4 * g + i;
+                        if (!(there && tok >= from && tok < end)) {
+                            x[t][i] = -INFINITY;
+                            seen &= ~(1u << (4 * t + i));
+                        }
+                    }
+                }
+                top = fmaxf(top, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
+                __builtin_amdgcn_sched_barrier(0);   // (one tile's operands at a time: what is asked for early has to be held)
             }
             if (__any(top * c > bar + kSlack)) {   // (base 2; of nothing seen: not so)
                 const float to = fmaxf(bar, kv_column_max(top) * c);
-                const float keep = bar == -INFINITY ? 0.f : exp2f(bar - to);
-                if (to > bar) {
-                    sum *= keep;
+                const float keep = to > bar ? __builtin_amdgcn_exp2f(bar - to) : 1.f;
+                sum *= keep;
 #pragma unroll
-                    for (int n = 0; n < NG; n++) {
-                        bias[n] *= keep;
+                for (int n = 0; n < NG; n++) {
+                    bias[n] *= keep;
+                    ones[n] *= keep;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) ones[n][i] *= keep;
+                    for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int t = 0; t < NT; t++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) o[n][t][i] *= keep;
-                    }
-                    bar = to;
+                        for (int i = 0; i < 4; i++) o[n][t][i] *= keep;
                 }
+                bar = to;
             }
             const float from_bar = bar == -INFINITY ? 0.f : bar;
-            float ps[NG][2][4];
+            const uint8_t* values = at + L::CODES + L::LOADS * 256;
+            Numbers vs[2];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                float vs[4][NG], vb[4][NG];
-                const uint8_t* values = at + L::CODES + L::LOADS * 256 + L::CODES;
-                numbers(values, 0, t, vs);
-                numbers(values, 1, t, vb);
+                vs[t] = numbers(values + L::CODES, 0, t);
+                Numbers vb = numbers(values + L::CODES, 1, t);
+                if (!whole) {   // (a weight of 0 does not keep a NaN out)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float p = __builtin_amdgcn_exp2f(fmaf(x[t][i], c, -from_bar));
-                    if constexpr (masked) p = seen[t][i] ? p : 0.f;
-                    sum += p;
-#pragma unroll
-                    for (int n = 0; n < NG; n++) {
-                        const float sc = !masked || seen[t][i] ? vs[i][n] : 0.f, bi = !masked || seen[t][i] ? vb[i][n] : 0.f;
-                        ps[n][t][i] = p * sc;
-                        bias[n] = fmaf(p, fmaf(8.f, sc, bi), bias[n]);
+                    for (int i = 0; i < 4; i++) {
+                        vs[t].keep(i, seen >> (4 * t + i) & 1u);
+                        vb.keep(i, seen >> (4 * t + i) & 1u);
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(x[t][i], c, -from_bar));
+                    x[t][i] = p;
+                    sum += p;
+#pragma unroll
+                    for (int n = 0; n < NG; n++) bias[n] = fmaf(p, fmaf(8.f, vs[t](i, n), vb(i, n)), bias[n]);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
             const kr_u32x4 less24 = {0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u};   // -24 in bf16
-            const uint8_t* vt = at + L::CODES + L::LOADS * 256;
 #pragma unroll
             for (int n = 0; n < NG; n++) {
                 kr_u32x4 pt[T::P];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {   // tokens 4 g + 2 j, + 1 of the first half, then of the second
-                    float y0[T::P], y1[T::P];
-                    kv_split(ps[n][j / 2][2 * j % 4], y0);
-                    kv_split(ps[n][j / 2][2 * j % 4 + 1], y1);
+                    float y[2][T::P];
 #pragma unroll
-                    for (int e = 0; e < T::P; e++) pt[e][j] = kv_pack_bf16(y0[e], y1[e]);
+                    for (int e = 0; e < 2; e++) {
+                        const int i = 2 * j % 4 + e;
+                        kv_split(x[j / 2][i] * vs[j / 2](i, n), y[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < T::P; e++) pt[e][j] = kv_pack_bf16(y[0][e], y[1][e]);
                 }
+                kr_f32x4 less = {0.f, 0.f, 0.f, 0.f};   // (every row of it is the same)
+#pragma unroll
+                for (int e = T::P - 1; e >= 0; e--) less = kr_mfma<DT_BF16>(less24, pt[e], less);
                 const uint32_t word = n * W + r % W, sub = r / W;   // this lane's word of a token, and which of its nibbles
                 uint32_t w[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) w[j] = *(const uint32_t*)(vt + j / 4 * (L::CODES / 2) + ((word / 4) * 16 + 4 * g + j % 4) * 16 + (word % 4) * 4);
+                for (int j = 0; j < 8; j++) w[j] = *(const uint32_t*)(values + j / 4 * (L::CODES / 2) + ((word / 4) * 16 + 4 * g + j % 4) * 16 + (word % 4) * 4);
                 // W 16 (G 128): nibble t; W 8: nibble 2 t + sub, turned to bits 3..6 of byte t; W 4: nibble 4 t + sub, to bits 3..6 of half t.
-                uint32_t even[8], odd[8];
+                if constexpr (W != 16) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if constexpr (W == 16) {
-                        even[j] = w[j] << 3;
-                        odd[j] = w[j] >> 1;
-                    } else {
-                        even[j] = __builtin_amdgcn_alignbit(w[j], w[j], (4 * sub + 29) & 31);
-                    }
+                    for (int j = 0; j < 8; j++) w[j] = __builtin_amdgcn_alignbit(w[j], w[j], (4 * sub + 29) & 31);
                 }
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     kr_u32x4 v;
+                    const int byte = W == 16 ? t / 2 : W == 8 ? t : 2 * t;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const uint32_t first = W == 16 && t & 1 ? odd[2 * j] : even[2 * j], second = W == 16 && t & 1 ? odd[2 * j + 1] : even[2 * j + 1];
-                        const int byte = W == 16 ? t / 2 : W == 8 ? t : 2 * t;
-                        v[j] = (__builtin_amdgcn_perm(second, first, 0x0C000C00u | (uint32_t)(4 + byte) << 16 | (uint32_t)byte) & 0x00780078u) | v16;
+                        uint32_t two = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x0C000C00u | (uint32_t)(4 + byte) << 16 | (uint32_t)byte);
+                        if constexpr (W == 16) two = t & 1 ? two >> 1 : two << 3;
+                        v[j] = (two & 0x00780078u) | v16;
                     }
 #pragma unroll
                     for (int e = T::P - 1; e >= 0; e--) o[n][t] = kr_mfma<DT_BF16>(v, pt[e], o[n][t]);
                 }
-#pragma unroll
-                for (int e = T::P - 1; e >= 0; e--) ones[n] = kr_mfma<DT_BF16>(less24, pt[e], ones[n]);
+                ones[n] += less[0];
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
 
@@ -298,8 +311,7 @@ __global__ __launch_bounds__(64 * NW, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows
                 else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 const uint32_t t0 = lo + 32u * b, h = lo / 16u + 2u * b;
                 const bool whole = t0 >= last_from && t0 + 32u <= first_end && half_of(h) < kv.n_pages && half_of(h + 1u) < kv.n_pages;
-                if (whole) block(b, std::false_type{});
-                else block(b, std::true_type{});
+                block(b, whole);
                 if (b + 2u < b1) {
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the stage is read)
                     if (lo / 16u + 2u * (b + 2u) + 1u - page_from > 63u) pages_at(lo / 16u + 2u * (b + 1u));   // (the next block's are still asked for)
@@ -313,11 +325,11 @@ __global__ __launch_bounds__(64 * NW, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows
         float* join = (float*)mine + r * (D + 4);
 #pragma unroll
         for (int n = 0; n < NG; n++) {
-            const float more = kv_column_sum(bias[n]);
+            const float more = kv_column_sum(bias[n]) + ones[n];
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) join[n * G + kv_number<G>(t, 4 * g + i)] = o[n][t][i] + ones[n][i] + more;
+                for (int i = 0; i < 4; i++) join[n * G + kv_number<G>(t, 4 * g + i)] = o[n][t][i] + more;
         }
         if (g == 0) {
             join[D] = bar;
