@@ -2397,6 +2397,11 @@ int mtq_set_option(const char* name, int value) {
         options().qmv_norm_mfma = value;
         return MTQ_OK;
     }
+    if (!strcmp(name, "kv.kernel")) {
+        if (value < 0 || value > 2) return fail(ERR_BAD_ARG, "kv.kernel must be 0 (choose), 1 (few rows a sequence) or 2 (many)");
+        options().kv_kernel = value;
+        return MTQ_OK;
+    }
     if (!strcmp(name, "kv.waves")) {
         if (value < 0 || value > 2) return fail(ERR_BAD_ARG, "kv.waves must be 0 (choose), 1 (workgroups of 4 waves) or 2 (of as many as fit)");
         options().kv_waves = value;

@@ -65,5 +65,9 @@ struct KvParts {
     float* sums = nullptr;     // [rows, query heads, slices, 2]
     uint32_t slices = 1;
 };
+int launch_kv_rows(int dtype, const KvAttentionArgs& p, const KvParts& parts, bool large, const LaunchCtx& lc);
+int launch_kv_tiles(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc);
+int launch_kv_join(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc);
+uint32_t kv_tile_rows(int dtype, uint32_t dim);
 
 }  // namespace mtq

@@ -367,28 +367,6 @@ __global__ __launch_bounds__(64 * NW, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows
     }
 }
 
-// A wave for each row and query head: its slices joined.
-template <int DT, int D> __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a, KvParts parts) {
-    const uint32_t lane = threadIdx.x & 63u, at = blockIdx.x * 4 + (threadIdx.x >> 6), row = at / a.hq, h = at - row * a.hq;
-    if (row >= a.kv.n_tokens) return;
-    KvSeq s;
-    if (!kv_seq_of(a.kv, row, s)) return;
-    const float* sums = parts.sums + (uint64_t)at * parts.slices * 2;
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < parts.slices; i += 64) top = fmaxf(top, sums[2 * i]);
-    for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i, 64));
-    float total = 0.f, v[D / 64] = {};
-    for (uint32_t i = 0; i < parts.slices; i++) {
-        const float bar = sums[2 * i], part = sums[2 * i + 1], f = bar == -INFINITY ? (part == 0.f ? 0.f : 1.f) : exp2f(bar - top);
-        if (f == 0.f && part == 0.f) continue;
-        total = fmaf(part, f, total);
-#pragma unroll
-        for (int j = 0; j < D / 64; j++) v[j] = fmaf(parts.values[((uint64_t)at * parts.slices + i) * D + lane + 64 * j], f, v[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < D / 64; j++) store_elem<DT>(a.out, (uint64_t)row * a.out_stride + (uint64_t)h * D + lane + 64 * j, total == 0.f ? 0.f : v[j] / total);
-}
-
 template <int DT, int D, int G> int launch(const KvAttentionArgs& p, KvParts parts, bool large, const LaunchCtx& lc) {
     using L = RowsLds<DT, D, G>;
     KvAttentionArgs a = p;
@@ -403,9 +381,7 @@ template <int DT, int D, int G> int launch(const KvAttentionArgs& p, KvParts par
     MTQ_HIP(set_max_dynamic_lds(fn, bytes));
     void* args[] = {&a, &parts};
     MTQ_HIP(launch_kernel(fn, dim3(a.kv.n_seqs * a.kv.hkv * parts.slices), dim3(64 * waves), args, bytes, first));
-    if (parts.slices > 1)
-        MTQ_HIP(launch_kernel((const void*)kv_join_kernel<DT, D>, dim3((a.kv.n_tokens * a.hq + 3) / 4), dim3(256), args, 0, last));
-    return ERR_OK;
+    return parts.slices > 1 ? launch_kv_join(DT, a, parts, last) : ERR_OK;
 }
 
 template <int DT> int launch_of(const KvAttentionArgs& p, const KvParts& parts, bool large, const LaunchCtx& lc) {

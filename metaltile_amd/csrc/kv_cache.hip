@@ -133,12 +133,11 @@ template <int DT> __global__ __launch_bounds__(256) void kv_append_kernel(KvAppe
     }
     const int64_t to = kv_slot(kv, s.seq, head, place);
     if (to < 0) return;
-    const KvPart& part = value ? kv.v : kv.k;
-    part.codes[(uint64_t)to * words + e0 / 8] = word;
+    (value ? kv.v.codes : kv.k.codes)[(uint64_t)to * words + e0 / 8] = word;
     if (e0 % kv.group == 0) {
         const uint64_t g = (uint64_t)to * (kv.dim / kv.group) + e0 / kv.group;
-        store_elem<DT>(part.scales, g, scale);
-        store_elem<DT>(part.biases, g, mn);
+        store_elem<DT>(value ? kv.v.scales : kv.k.scales, g, scale);
+        store_elem<DT>(value ? kv.v.biases : kv.k.biases, g, mn);
     }
 }
 
@@ -155,12 +154,13 @@ template <int DT> __global__ __launch_bounds__(256) void kv_read_kernel(KvReadAr
     if (head >= kv.hkv) return;
     const int64_t from = kv_slot(kv, s.seq, head, place);
     if (from < 0) return;
-    const KvPart& part = blockIdx.y ? kv.v : kv.k;
+    const uint32_t* codes = blockIdx.y ? kv.v.codes : kv.k.codes;
+    const void *scales = blockIdx.y ? kv.v.scales : kv.k.scales, *biases = blockIdx.y ? kv.v.biases : kv.k.biases;
     void* out = blockIdx.y ? a.v : a.k;
     if (!out) return;
     const uint64_t g = (uint64_t)from * (kv.dim / kv.group) + e0 / kv.group;
-    const uint32_t word = part.codes[(uint64_t)from * words + e0 / 8];
-    const float scale = load_elem<DT>(part.scales, g), bias = load_elem<DT>(part.biases, g);
+    const uint32_t word = codes[(uint64_t)from * words + e0 / 8];
+    const float scale = load_elem<DT>(scales, g), bias = load_elem<DT>(biases, g);
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {

@@ -129,6 +129,7 @@ struct Options {
     int qmv_codes_nw = 0;         // its waves along N (0 = choose; 2..8),
     int qmv_codes_stage = 0;      // its steps of activations between barriers (0 = choose; 1, 2, 4),
     int qmv_codes_slices = 0;     // its slices of K (0 = choose; 1..16)
+    int kv_kernel = 0;            // attention over the 4-bit cache: 0 = choose, 1 = the kernel for few rows a sequence, 2 = the one for many
     int kv_waves = 0;             // attention over the 4-bit cache: workgroups of 4 waves (1) or of as many as fit (2), 0 = choose
     int kv_slices = 0;            // and slices of a sequence's tokens, 0 = choose
     int scratch_most_kb = 0;      // largest library-owned scratch buffer (0 = no limit): a call that needs more finds no memory
@@ -367,16 +368,15 @@ struct KvAttentionArgs {
 };
 int launch_kv_append(int dtype, const KvAppendArgs& p, const LaunchCtx& lc);
 int launch_kv_read(int dtype, const KvReadArgs& p, const LaunchCtx& lc);
-// slices: parts of a sequence's tokens whose sums are joined through scratch (null: one). large: workgroups of as many waves as fit.
+// slices: parts of a sequence's tokens whose sums are joined through scratch (null: one). tiles: the kernel for many rows; else large: its
+// workgroups have as many waves as fit.
 struct KvPlan {
-    bool large = false;
+    bool tiles = false, large = false;
     uint32_t slices = 1;
     size_t scratch = 0;
 };
 KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& p);
 int launch_kv_attention(int dtype, const KvAttentionArgs& p, const KvPlan& plan, void* scratch, const LaunchCtx& lc);
-struct KvParts;
-int launch_kv_rows(int dtype, const KvAttentionArgs& p, const KvParts& parts, bool large, const LaunchCtx& lc);
 
 // Residual addition, RMS norm and 8-bit output (norm_fp8.hip).
 struct NormFp8Args {

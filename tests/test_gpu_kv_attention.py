@@ -72,6 +72,42 @@ def test_attention(dt, lens, rows, more):
     c.hold()
 
 
+@pytest.fixture
+def option():
+    lib, used = _ensure_init(), set()
+
+    def put(name, value):
+        used.add(name)
+        _lib.check(lib.mtq_set_option(name.encode(), value))
+
+    yield put
+    for name in used:
+        _lib.check(lib.mtq_set_option(name.encode(), 0))
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
+@pytest.mark.parametrize("lens,rows,more", CASES, ids=lambda v: str(v).replace(" ", "")[:40])
+def test_either_kernel(dt, lens, rows, more, option):
+    """Whatever the sizes: the kernel for few rows with small and large workgroups, the one for many, in one slice and in several."""
+    print(f"[case] kv_attention {dt.name} {str(lens)[:40]} {str(rows)[:40]} {more}, both kernels", flush=True)
+    c = Attention(dt, lens, rows, **more)
+    for kernel, waves, slices in ((1, 1, 1), (1, 2, 1), (1, 1, 3), (2, 0, 1), (2, 0, 5)):
+        for name, value in (("kv.kernel", kernel), ("kv.waves", waves), ("kv.slices", slices)):
+            option(name, value)
+        c.out.upload(b"\xa5" * c.out.nbytes)
+        c.call()
+        c.hold()
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
+@pytest.mark.parametrize("dim,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 32), (256, 64), (256, 128)])
+def test_every_head(dt, dim, group):
+    for lens, rows in (([330, 70], [1, 2]), ([330, 70], [100, 70])):
+        c = Attention(dt, lens, rows, dim=dim, group=group, hq=6, hkv=2)
+        c.call()
+        c.hold()
+
+
 @pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
 @pytest.mark.parametrize("rows", [[1, 1], [200, 40]], ids=str)
 def test_pages_that_are_none(dt, rows):
