@@ -4,7 +4,7 @@
 //
 // Codes are operands of the matrix instructions as they are: a nibble in the mantissa of 16 is the number 16 + c, in bf16 (bits 3..6) and in f16 (bits
 // 6..9), one mask and one OR for two of them. What that adds is taken out in f32:
-//   scores  sum_d q (16 + c) with -16 sum_d q as the sum's start; times s, plus b sum_d q, for each group
+//   scores  s sum_d q (16 + c) + (b - 16 s) sum_d q, for each group
 //   values  sum_j (p s) (16 + c) - 24 sum_j (p s) + sum_j p (b + 8 s), where the first two sums have the same rounded p s, so that its rounding
 //           meets c - 8, a code's distance from the middle, and the last is f32
 // p s is rounded to bf16 for bf16 (half a step, as the result is), and is two or three bf16 terms for f16 and f32; an f32 query is three terms.
@@ -45,8 +45,9 @@ template <int N> __device__ __forceinline__ void kv_split(float v, float (&t)[N]
         v -= t[i];
     }
 }
-__device__ __forceinline__ uint32_t kv_pack_bf16(float a, float b) {
-    return (uint32_t)f32_to_elem_bits<DT_BF16>(a) | (uint32_t)f32_to_elem_bits<DT_BF16>(b) << 16;
+__device__ __forceinline__ uint32_t kv_pack_bf16(float a, float b) {   // (one instruction as a vector of two, four as two numbers)
+    typedef __attribute__((ext_vector_type(2))) float f32x2;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2_t));
 }
 
 // Sum and maximum over the lanes of a column (lane & 15).

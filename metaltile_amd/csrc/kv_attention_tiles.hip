@@ -15,7 +15,7 @@ constexpr uint32_t kBlock = 64;   // tokens
 
 template <int DT, int D, int G, int NW> struct TilesShape {
     static constexpr int Q = KvTerms<DT>::Q, NG = D / G, STEPS = D / 32, NT = G / 16, TH = 64 * NW;
-    static constexpr int MT = D * Q <= 128 ? 4 : D * Q <= 384 ? 2 : 1;   // sixteens of rows of a wave: sums and queries fill its registers
+    static constexpr int MT = D * Q <= 192 ? 2 : 1;   // sixteens of rows of a wave: sums and queries fill its registers
     static constexpr int ROWS = 16 * MT * NW;
     static constexpr int VT = 1024 + 16;                          // a tile of values, and what keeps the tiles' writes in different banks
     static constexpr int K = kBlock * D * 2, V = kBlock / 32 * (D / 16) * VT, S = 4 * NG * kBlock * 4;
@@ -24,7 +24,7 @@ template <int DT, int D, int G, int NW> struct TilesShape {
 };
 
 template <int DT, int D, int G, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void kv_tiles_kernel(KvAttentionArgs a, KvParts parts, uint32_t tiles) {
+__global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a, KvParts parts, uint32_t tiles) {
     using L = TilesShape<DT, D, G, NW>;
     using T = KvTerms<DT>;
     constexpr int MT = L::MT, NG = L::NG, NT = L::NT, STEPS = L::STEPS, TH = L::TH;
@@ -193,13 +193,13 @@ __global__ __launch_bounds__(64 * NW, 1) void kv_tiles_kernel(KvAttentionArgs a,
                 }
             }
         }
-        float* sc = (float*)(st + L::K + L::V);   // [K scales, K biases, V scales, V biases + 8 scales][group][token]
+        float* sc = (float*)(st + L::K + L::V);   // [K scales, K biases - 16 scales, V scales, V biases + 8 scales][group][token]
         bool fine = true;
 #pragma unroll
         for (int u = 0; u < SI; u++) {
             const uint32_t i = u * TH + th, n = i % NG, t = i / NG % kBlock, value = i / (NG * kBlock);
             if (SITEMS % TH == 0 || i < SITEMS) {
-                const float second = value ? fmaf(8.f, sraw[u], braw[u]) : braw[u];
+                const float second = fmaf(value ? 8.f : -16.f, sraw[u], braw[u]);
                 sc[((2 * value) * NG + n) * kBlock + t] = sraw[u];
                 sc[((2 * value + 1) * NG + n) * kBlock + t] = second;
                 fine = fine && (!value || (fabsf(sraw[u]) < INFINITY && fabsf(second) < INFINITY));
@@ -223,10 +223,7 @@ __global__ __launch_bounds__(64 * NW, 1) void kv_tiles_kernel(KvAttentionArgs a,
             for (int n = 0; n < NG; n++) {
                 kr_f32x4 acc[MT];
 #pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    const float start = -16.f * qsum[m][n];
-                    acc[m] = kr_f32x4{start, start, start, start};
-                }
+                for (int m = 0; m < MT; m++) acc[m] = kr_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = n * (G / 32); i < (n + 1) * (G / 32); i++) {
                     const kr_u32x4 k = *(const kr_u32x4*)(kt + i * 1024);
@@ -458,7 +455,7 @@ int launch_kv_tiles(int dtype, const KvAttentionArgs& p, const KvParts& parts, c
 // Rows of a tile, by which the slices are chosen.
 uint32_t kv_tile_rows(int dtype, uint32_t dim) {
     const uint32_t work = dim * (dtype == DT_F32 ? 3 : 1);
-    return 16 * kWaves * (work <= 128 ? 4 : work <= 384 ? 2 : 1);
+    return 16 * kWaves * (work <= 192 ? 2 : 1);
 }
 
 }  // namespace mtq
