@@ -1499,6 +1499,8 @@ static int check_kv(int dtype, const mtq_kv_cache* c, const mtq_kv_batch* b, KvA
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return fail(ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
     if ((c->group_size != 32 && c->group_size != 64 && c->group_size != 128) || c->group_size > c->head_dim) return fail(ERR_SHAPE, "group_size must be 32, 64 or 128 and divide head_dim");
     if (c->n_heads == 0 || c->n_heads > 65536) return fail(ERR_SHAPE, "n_heads must be in 1..65536");
+    // (kernels count a pool's tokens and heads in 32 bits; as many would be 256 GiB of codes with the shortest heads)
+    if ((uint64_t)c->n_heads * c->page_size > UINT32_MAX || (uint64_t)c->n_pages * c->n_heads * c->page_size > UINT32_MAX) return fail(ERR_SHAPE, "n_pages * n_heads * page_size must be less than 2^32");
     if (b->n_tokens >= 1u << 24 || b->n_seqs >= 1u << 24) return fail(ERR_SHAPE, "n_tokens and n_seqs must be less than 2^24");
     if (b->max_len > 1u << 30 || b->max_len > (uint64_t)b->pages_stride * c->page_size) return fail(ERR_SHAPE, "max_len must be at most pages_stride * page_size, and 2^30");
     if (!b->offsets && b->n_seqs && b->n_tokens % b->n_seqs) return fail(ERR_SHAPE, "without offsets n_seqs must divide n_tokens");

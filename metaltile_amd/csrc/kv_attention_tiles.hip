@@ -11,16 +11,16 @@ namespace mtq {
 
 namespace {
 
-constexpr uint32_t kBlock = 64;   // tokens
+constexpr uint32_t kBlock = 32;   // tokens
 
 template <int DT, int D, int G, int NW> struct TilesShape {
     static constexpr int Q = KvTerms<DT>::Q, NG = D / G, STEPS = D / 32, NT = G / 16, TH = 64 * NW;
     static constexpr int MT = D * Q <= 192 ? 2 : 1;   // sixteens of rows of a wave: sums and queries fill its registers
     static constexpr int ROWS = 16 * MT * NW;
     static constexpr int VT = 1024 + 16;                          // a tile of values, and what keeps the tiles' writes in different banks
-    static constexpr int K = kBlock * D * 2, V = kBlock / 32 * (D / 16) * VT, S = 4 * NG * kBlock * 4;
-    static constexpr int STAGE = K + V + S;
-    static constexpr int LDS = 2 * STAGE + 2 * 16 * 4;
+    static constexpr int K = kBlock * D * 2, V = D / 16 * VT, S = 2 * NG * kBlock * 4;
+    static constexpr int KSTAGE = K + S, VSTAGE = V + S;
+    static constexpr int LDS = 2 * (KSTAGE + VSTAGE) + 8 * 4;
 };
 
 template <int DT, int D, int G, int NW>
@@ -28,8 +28,8 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
     using L = TilesShape<DT, D, G, NW>;
     using T = KvTerms<DT>;
     constexpr int MT = L::MT, NG = L::NG, NT = L::NT, STEPS = L::STEPS, TH = L::TH;
-    constexpr int KITEMS = (int)kBlock * (D / 32), VITEMS = (int)kBlock / 4 * (D / 8), SITEMS = 2 * (int)kBlock * NG;
-    constexpr int KI = (KITEMS + TH - 1) / TH, VI = (VITEMS + TH - 1) / TH, SI = (SITEMS + TH - 1) / TH;
+    constexpr int ITEMS = D / 2, RI = (ITEMS + 63) / 64, SI = (16 * NG + 63) / 64;   // pieces of 16 bytes of 16 tokens' codes, and a lane's of them and of the scales
+    static_assert(NW == 4 || NW == 8, "");
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const KvArgs& kv = a.kv;
     const uint32_t th = threadIdx.x, lane = th & 63u, wave = __builtin_amdgcn_readfirstlane(th >> 6), r = lane & 15u, g = lane >> 4;
@@ -62,14 +62,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
     auto end_of = [&](uint32_t i) { const int32_t e = (int32_t)(s.len + i / shared + 1u) - (int32_t)s.rows; return e > 0 ? (uint32_t)e : 0u; };
     auto from_of = [&](uint32_t e) { return a.window && e > a.window ? e - a.window : 0u; };
     const uint32_t last = row0 + L::ROWS - 1u < rows ? row0 + L::ROWS - 1u : rows - 1u;
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(end_of(last)), lo = __builtin_amdgcn_readfirstlane(from_of(end_of(row0))) & ~31u;
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(end_of(last)), first_of_all = __builtin_amdgcn_readfirstlane(end_of(row0)), lo = __builtin_amdgcn_readfirstlane(from_of(end_of(row0))) & ~31u;
     const uint32_t blocks = kv.n_pages && hi > lo ? (hi - lo + kBlock - 1u) / kBlock : 0u, per = (blocks + parts.slices - 1u) / parts.slices;
     const uint32_t b0 = slice * per < blocks ? slice * per : blocks, b1 = b0 + per < blocks ? b0 + per : blocks;
     // This wave's rows, and a lane's.
     const uint32_t wave0 = row0 + wave * 16 * MT, wave_last = wave0 + 16 * MT - 1u < rows ? wave0 + 16 * MT - 1u : rows - 1u;
     const bool any = wave0 < rows;
     const uint32_t first_end = __builtin_amdgcn_readfirstlane(any ? end_of(wave0) : 0u), last_end = __builtin_amdgcn_readfirstlane(any ? end_of(wave_last) : 0u);
-    const uint32_t first_from = from_of(first_end), last_from = from_of(last_end);
+    const uint32_t last_from = from_of(last_end);
     uint32_t end[MT], from[MT];
     uint64_t row_at[MT];   // its row of the call
     uint32_t qh[MT];
@@ -112,113 +112,107 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
         for (int n = 0; n < NG; n++) qsum[m][n] = kv_column_sum(qsum[m][n]);
     }
 
-    // A block's codes from memory into registers, and from there as operands into its stage.
+    // A block's codes from memory into registers, and from there as operands into its stage. A wave brings the keys or the values of one of a block's two
+    // sixteens of tokens, which lie on one page; of eight waves the first four have the even blocks.
     const uint32_t k16 = kv_sixteen<T::QK>(), v16 = kv_sixteen<DT_BF16>();
-    uint4 kraw[KI];
-    uint32_t vraw[VI][4];
+    const uint32_t half = wave & 1u, turn = wave / 4u;
+    const bool values = wave & 2u;
+    const uint8_t* const codes = (const uint8_t*)(values ? kv.v.codes : kv.k.codes);
+    const void *const scales = values ? kv.v.scales : kv.k.scales, *const biases = values ? kv.v.biases : kv.k.biases;
+    uint4 raw[RI];
     float sraw[SI], braw[SI];
-    uint32_t there = 0;   // of a block that is fetched: a bit for each of its sixteens of tokens that is on a page
+    uint32_t raw_there = 0;   // whether what is in them is on a page
+    // The pages of 64 of this wave's sixteens at a time, one to a lane: a scalar load would be waited for by whoever reads the LDS next.
+    constexpr uint32_t STEP = NW / 4;
+    uint32_t pages = 0, pages_from = 0;
+    auto pages_at = [&](uint32_t b) {
+        const uint32_t mine = b + lane * STEP, at = lo + mine * kBlock + 16 * half;
+        pages_from = b;
+        pages = mine < b1 && at < hi ? kv.pages[(uint64_t)s.seq * kv.pages_stride + (at >> kv.page_log2)] : 0xFFFFFFFFu;
+    };
     auto fetch = [&](uint32_t b) {
-        const uint32_t t0 = lo + b * kBlock;
-        uint64_t slot[4];
-        there = 0;
+        if ((b - pages_from) / STEP > 63u) pages_at(b);
+        const uint32_t page = __builtin_amdgcn_readlane(pages, (b - pages_from) / STEP), at = lo + b * kBlock + 16 * half;
+        raw_there = page < kv.n_pages;
+        // (of no page: one that is there. The pool has fewer than 2^32 tokens and heads: host)
+        const uint32_t slot = (((raw_there ? page : 0u) * kv.hkv + head) << kv.page_log2) + (at & ((1u << kv.page_log2) - 1u));
+        const uint8_t* from_codes = codes + (uint64_t)slot * (D / 2);
 #pragma unroll
-        for (int h = 0; h < 4; h++) {
-            const uint32_t at = t0 + 16 * h;
-            const uint32_t page = at < hi ? kv.pages[(uint64_t)s.seq * kv.pages_stride + (at >> kv.page_log2)] : 0xFFFFFFFFu;
-            const bool ok = page < kv.n_pages;
-            there |= (uint32_t)ok << h;
-            slot[h] = (((uint64_t)(ok ? page : 0u) * kv.hkv + head) << kv.page_log2) + (at & ((1u << kv.page_log2) - 1u));   // (of no page: one that is there)
-        }
-        auto slot_of = [&](uint32_t h) { return h & 2u ? (h & 1u ? slot[3] : slot[2]) : (h & 1u ? slot[1] : slot[0]); };
-#pragma unroll
-        for (int u = 0; u < KI; u++) {
-            const uint32_t i = u * TH + th;
-            if (KITEMS % TH == 0 || i < KITEMS)
-                kraw[u] = *(const uint4*)((const uint8_t*)kv.k.codes + (slot_of(i / (16 * (D / 32))) + i % 16) * (D / 2) + i / 16 % (D / 32) * 16);
-        }
-#pragma unroll
-        for (int u = 0; u < VI; u++) {
-            const uint32_t i = u * TH + th, quad = i / (D / 8), w = i % (D / 8);
-            if (VITEMS % TH == 0 || i < VITEMS) {
-                const uint32_t* p = kv.v.codes + (slot_of(quad / 4) + quad % 4 * 4) * (D / 8) + w;
-#pragma unroll
-                for (int j = 0; j < 4; j++) vraw[u][j] = p[j * (D / 8)];
+        for (int u = 0; u < RI; u++) {
+            const uint32_t i = u * 64 + lane;
+            if (ITEMS % 64 == 0 || i < ITEMS) {
+                if (values) {   // a word of each of four tokens
+                    const uint32_t* p = (const uint32_t*)(from_codes + (i / (D / 8)) * (4 * (D / 2)) + i % (D / 8) * 4);
+                    raw[u] = make_uint4(p[0], p[D / 8], p[2 * (D / 8)], p[3 * (D / 8)]);
+                } else {        // four words of a token
+                    raw[u] = *(const uint4*)(from_codes + i % 16 * (D / 2) + i / 16 * 16);
+                }
             }
         }
 #pragma unroll
         for (int u = 0; u < SI; u++) {
-            const uint32_t i = u * TH + th, n = i % NG, t = i / NG % kBlock;
-            if (SITEMS % TH == 0 || i < SITEMS) {
-                const bool value = i / (NG * kBlock);
-                const void *scales = value ? kv.v.scales : kv.k.scales, *biases = value ? kv.v.biases : kv.k.biases;
-                const uint64_t at = (slot_of(t / 16) + t % 16) * NG + n;
-                const bool in = (there >> (t / 16) & 1u) && t0 + t < hi;   // (where no token is: zeros)
-                sraw[u] = in ? load_elem<DT>(scales, at) : 0.f;
-                braw[u] = in ? load_elem<DT>(biases, at) : 0.f;
-            }
+            const uint32_t i = (u * 64 + lane) % (16 * NG);   // token and group
+            sraw[u] = load_elem<DT>(scales, (uint64_t)slot * NG + i);
+            braw[u] = load_elem<DT>(biases, (uint64_t)slot * NG + i);
         }
     };
-    uint32_t* const odd = (uint32_t*)(lds + 2 * L::STAGE);   // [stage][wave]: whether the values' scales or biases that the wave brought hold a NaN or an infinity
+    // [stage][sixteen]: bit 0: on a page (with the keys); bit 1: scales or biases that are no numbers (with the values)
+    uint32_t* const flags = (uint32_t*)(lds + 2 * (L::KSTAGE + L::VSTAGE));
     auto store = [&](uint32_t b) {
-        uint8_t* st = lds + (b & 1u) * L::STAGE;
+        uint8_t* st = lds + (values ? 2 * L::KSTAGE + (b & 1u) * L::VSTAGE : (b & 1u) * L::KSTAGE);
 #pragma unroll
-        for (int u = 0; u < KI; u++) {
-            const uint32_t i = u * TH + th;
-            if (KITEMS % TH == 0 || i < KITEMS) {
-                const uint32_t w[4] = {kraw[u].x, kraw[u].y, kraw[u].z, kraw[u].w};
+        for (int u = 0; u < RI; u++) {
+            const uint32_t i = u * 64 + lane, w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+            if (ITEMS % 64 == 0 || i < ITEMS) {
+                if (values) {
+                    const uint32_t quad = i / (D / 8), word = i % (D / 8);
+                    uint8_t* to = st + (word / 2) * L::VT + (quad * 16 + word % 2 * 8) * 16 + half * 8;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    kr_u32x4 k;
+                    for (int e = 0; e < 8; e++) {
+                        kr_u32x2 v;
 #pragma unroll
-                    for (int p = 0; p < 4; p++) k[p] = kv_pair<T::QK>(w[j], p, k16);
-                    *(kr_u32x4*)(st + ((i / 16) * 64 + j * 16 + i % 16) * 16) = k;   // (i / 16: sixteen of tokens and step)
-                }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < VI; u++) {
-            const uint32_t i = u * TH + th, quad = i / (D / 8), w = i % (D / 8);
-            if (VITEMS % TH == 0 || i < VITEMS) {
-                uint8_t* to = st + L::K + (quad / 8 * (D / 16) + w / 2) * L::VT + (quad % 4 * 16 + w % 2 * 8) * 16 + quad / 4 % 2 * 8;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    kr_u32x2 v;
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const uint32_t two = __builtin_amdgcn_perm(vraw[u][2 * j + 1], vraw[u][2 * j], 0x0C000C00u | (uint32_t)(4 + e / 2) << 16 | (uint32_t)(e / 2));
-                        v[j] = ((e & 1 ? two >> 1 : two << 3) & 0x00780078u) | v16;
+                        for (int j = 0; j < 2; j++) {
+                            const uint32_t two = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x0C000C00u | (uint32_t)(4 + e / 2) << 16 | (uint32_t)(e / 2));
+                            v[j] = ((e & 1 ? two >> 1 : two << 3) & 0x00780078u) | v16;
+                        }
+                        *(kr_u32x2*)(to + e * 16) = v;
                     }
-                    *(kr_u32x2*)(to + e * 16) = v;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        kr_u32x4 k;
+#pragma unroll
+                        for (int p = 0; p < 4; p++) k[p] = kv_pair<T::QK>(w[j], p, k16);
+                        *(kr_u32x4*)(st + (half * STEPS * 64 + (i / 16) * 64 + j * 16 + i % 16) * 16) = k;   // (i / 16: step)
+                    }
                 }
             }
         }
-        float* sc = (float*)(st + L::K + L::V);   // [K scales, K biases - 16 scales, V scales, V biases + 8 scales][group][token]
+        float* to = (float*)(st + (values ? L::V : L::K)) + 16 * half;   // [scales, biases - 16 scales of keys, + 8 scales of values][group][token]
         bool fine = true;
 #pragma unroll
         for (int u = 0; u < SI; u++) {
-            const uint32_t i = u * TH + th, n = i % NG, t = i / NG % kBlock, value = i / (NG * kBlock);
-            if (SITEMS % TH == 0 || i < SITEMS) {
-                const float second = fmaf(value ? 8.f : -16.f, sraw[u], braw[u]);
-                sc[((2 * value) * NG + n) * kBlock + t] = sraw[u];
-                sc[((2 * value + 1) * NG + n) * kBlock + t] = second;
-                fine = fine && (!value || (fabsf(sraw[u]) < INFINITY && fabsf(second) < INFINITY));
-            }
+            const uint32_t i = (u * 64 + lane) % (16 * NG);
+            const bool in = raw_there && lo + b * kBlock + 16 * half + i / NG < hi;   // (where no token is: zeros)
+            const float first = in ? sraw[u] : 0.f, second = in ? fmaf(values ? 8.f : -16.f, sraw[u], braw[u]) : 0.f;
+            to[i % NG * kBlock + i / NG] = first;   // (by several lanes the same)
+            to[(NG + i % NG) * kBlock + i / NG] = second;
+            fine = fine && fabsf(first) < INFINITY && fabsf(second) < INFINITY;
         }
         const bool all_fine = __all(fine);
-        if (lane == 0) odd[(b & 1u) * 16 + wave] = !all_fine;
+        if (lane == 0) flags[(values ? 4u : 0u) + (b & 1u) * 2u + half] = values ? !all_fine : raw_there;
     };
 
     kr_f32x4 o[MT][NG][NT] = {};
     float ones[MT][NG] = {}, bias[MT][NG] = {}, sum[MT] = {}, bar[MT];
 #pragma unroll
     for (int m = 0; m < MT; m++) bar[m] = -INFINITY;
-    auto part = [&](const uint8_t* st, uint32_t sb, uint32_t t0, uint32_t on_page, uint32_t stage) {   // 32 tokens from t0 on
-        const float* sc = (const float*)(st + L::K + L::V) + sb * 32 + 4 * g;
-        float x[MT][2][4];
+    auto scores = [&](uint32_t b, float (&x)[MT][2][4]) {
+        const uint8_t* st = lds + (b & 1u) * L::KSTAGE;
+        const float* sc = (const float*)(st + L::K) + 4 * g;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const uint8_t* kt = st + (sb * 2 + t) * (STEPS * 1024) + lane * 16;
+            const uint8_t* kt = st + t * (STEPS * 1024) + lane * 16;
 #pragma unroll
             for (int n = 0; n < NG; n++) {
                 kr_f32x4 acc[MT];
@@ -239,8 +233,15 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
                     for (int i = 0; i < 4; i++) x[m][t][i] = fmaf(kb[i], qsum[m][n], n ? fmaf(ks[i], acc[m][i], x[m][t][i]) : ks[i] * acc[m][i]);
             }
         }
-        const bool whole = t0 >= last_from && t0 + 32u <= first_end && (on_page >> (2 * sb) & 3u) == 3u;
-        uint32_t seen = 0xFFFFFFFFu;   // (8 bits for each m)
+    };
+    // What a row does not see scores -inf; the bars are raised where scores pass them.
+    uint32_t seen = 0xFFFFFFFFu;   // (8 bits for each m)
+    bool whole = true, whole_of_all = true;   // (every row of the wave, and of the workgroup, sees all of the block)
+    auto look = [&](uint32_t b, uint32_t there, float (&x)[MT][2][4]) {
+        const uint32_t t0 = lo + b * kBlock;
+        whole = t0 >= last_from && t0 + kBlock <= first_end && there == 3u;
+        whole_of_all = t0 >= from_of(hi) && t0 + kBlock <= first_of_all && there == 3u;
+        seen = 0xFFFFFFFFu;
         if (!whole) {
 #pragma unroll
             for (int m = 0; m < MT; m++)
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const uint32_t tok = t0 + 16 * t + 4 * g + i;
-                        if (!((on_page >> (2 * sb + t) & 1u) && tok >= from[m] && tok < end[m])) {
+                        if (!((there >> t & 1u) && tok >= from[m] && tok < end[m])) {
                             x[m][t][i] = -INFINITY;
                             seen &= ~(1u << (8 * m + 4 * t + i));
                         }
@@ -279,6 +280,32 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
                 bar[m] = to;
             }
         }
+    };
+    // A weight of 0 does not keep a NaN out: where some rows of the workgroup do not see all of a block, values' scales and biases that are no numbers
+    // become zeros, and the rows that see them have a NaN in that group's sum.
+    auto take_out = [&](uint32_t b) {
+        float* sc = (float*)(lds + 2 * L::KSTAGE + (b & 1u) * L::VSTAGE + L::V);
+#pragma unroll
+        for (int n = 0; n < NG; n++)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float vs = sc[n * kBlock + 16 * t + 4 * g + i], vb = sc[(NG + n) * kBlock + 16 * t + 4 * g + i];
+                    if (!(fabsf(vs) < INFINITY && fabsf(vb) < INFINITY)) {
+#pragma unroll
+                        for (int m = 0; m < MT; m++)
+                            if (seen >> (8 * m + 4 * t + i) & 1u) bias[m][n] = __builtin_nanf("");
+                    }
+                }
+        __syncthreads();
+        for (uint32_t i = th; i < NG * kBlock; i += TH)
+            if (!(fabsf(sc[i]) < INFINITY && fabsf(sc[NG * kBlock + i]) < INFINITY)) sc[i] = sc[NG * kBlock + i] = 0.f;
+        __syncthreads();
+    };
+    auto add_values = [&](uint32_t b, float (&x)[MT][2][4]) {
+        const uint8_t* st = lds + 2 * L::KSTAGE + (b & 1u) * L::VSTAGE;
+        const float* sc = (const float*)(st + L::V) + 4 * g;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
             const float from_bar = bar[m] == -INFINITY ? 0.f : bar[m];
@@ -290,32 +317,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
                     sum[m] += x[m][t][i];
                 }
         }
-        bool clean = true;   // (a weight of 0 does not keep a NaN out: where some rows do not see all, they are taken out, and put to the rows that see them)
-        if (!whole) {
-            uint32_t some = 0;
-            for (int w = 0; w < NW; w++) some |= odd[stage * 16 + w];
-            clean = __builtin_amdgcn_readfirstlane(some) == 0;
-        }
         const kr_u32x4 less24 = {0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u};   // -24 in bf16
 #pragma unroll
         for (int n = 0; n < NG; n++) {
             kr_f32x4 vs[2], vb[2];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                vs[t] = *(const kr_f32x4*)(sc + (2 * NG + n) * kBlock + 16 * t);
-                vb[t] = *(const kr_f32x4*)(sc + (3 * NG + n) * kBlock + 16 * t);
-            }
-            if (!clean) {
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (!(fabsf(vs[t][i]) < INFINITY && fabsf(vb[t][i]) < INFINITY)) {
-                            vs[t][i] = vb[t][i] = 0.f;
-#pragma unroll
-                            for (int m = 0; m < MT; m++)
-                                if (seen >> (8 * m + 4 * t + i) & 1u) bias[m][n] = __builtin_nanf("");
-                        }
+                vs[t] = *(const kr_f32x4*)(sc + n * kBlock + 16 * t);
+                vb[t] = *(const kr_f32x4*)(sc + (NG + n) * kBlock + 16 * t);
             }
             kr_u32x4 pt[MT][T::P];
 #pragma unroll
@@ -339,7 +348,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
             }
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                const kr_u32x4 v = *(const kr_u32x4*)(st + L::K + (sb * (D / 16) + n * NT + t) * L::VT + lane * 16);
+                const kr_u32x4 v = *(const kr_u32x4*)(st + (n * NT + t) * L::VT + lane * 16);
 #pragma unroll
                 for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -348,27 +357,44 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
         }
     };
 
+    // The scores of a block are computed beside the values of the one before, so that the matrix cores have the one while the vector units have the
+    // other. In turn b the keys of block b + 2 and the values of b + 1 go into the stages that turn b - 1 has read, and a wave's next codes are asked for.
     if (b0 < b1) {
-        fetch(b0);
-        uint32_t now = there, next = 0;   // (the fetched blocks' `there`)
-        store(b0);
-        if (b0 + 1u < b1) {
-            fetch(b0 + 1u);
-            next = there;
-        }
+        float x[MT][2][4];
+        const uint32_t ahead = values ? 1u : 2u;
+        uint32_t mine = b0 + (NW == 8 ? (b0 ^ turn) & 1u : 0u);   // this wave's next block
+        pages_at(mine);
+        fetch(mine);
+        auto bring = [&](uint32_t upto) {   // this wave's blocks up to that one
+            if (mine > upto || mine >= b1) return;
+            store(mine);
+            mine += STEP;
+            if (mine < b1) fetch(mine);
+        };
+        bring(b0);
+        if (!values) bring(b0 + 1u);
+        __syncthreads();
+        scores(b0, x);
+        look(b0, __builtin_amdgcn_readfirstlane(flags[(b0 & 1u) * 2u] | flags[(b0 & 1u) * 2u + 1u] << 1), x);
         __syncthreads();
         for (uint32_t b = b0; b < b1; b++) {
-            const uint32_t on_page = now;
-            if (b + 1u < b1) store(b + 1u);
-            now = next;
-            if (b + 2u < b1) {
-                fetch(b + 2u);
-                next = there;
+            if (!whole_of_all) {
+                const uint32_t* f = flags + 4u + (b & 1u) * 2u;
+                if (__builtin_amdgcn_readfirstlane(f[0] | f[1])) take_out(b);
             }
-            const uint32_t t0 = lo + b * kBlock;
-#pragma unroll 1
-            for (uint32_t sb = 0; sb < 2; sb++)
-                if (t0 + 32 * sb < last_end && t0 + 32 * sb + 32u > first_from) part(lds + (b & 1u) * L::STAGE, sb, t0 + 32 * sb, on_page, b & 1u);
+            const uint32_t* f = flags + ((b + 1u) & 1u) * 2u;
+            const uint32_t f0 = f[0], f1 = f[1];
+            bring(b + ahead);
+            float next[MT][2][4];
+            scores(b + 1u, next);   // (behind the last block: of what is there, and not used)
+            add_values(b, x);
+            if (b + 1u < b1) look(b + 1u, __builtin_amdgcn_readfirstlane(f0 | f1 << 1), next);
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[m][t][i] = next[m][t][i];
             __syncthreads();
         }
     }
@@ -408,7 +434,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
     }
 }
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
 
 template <int DT, int D, int G> int launch(const KvAttentionArgs& p, KvParts parts, const LaunchCtx& lc) {
     using L = TilesShape<DT, D, G, kWaves>;
