@@ -207,31 +207,38 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
     float ones[MT][NG] = {}, bias[MT][NG] = {}, sum[MT] = {}, bar[MT];
 #pragma unroll
     for (int m = 0; m < MT; m++) bar[m] = -INFINITY;
-    auto scores = [&](uint32_t b, float (&x)[MT][2][4]) {
+    // A sixteen of a block's keys and their numbers, out of the LDS; and its scores.
+    struct Keys {
+        kr_u32x4 k[STEPS];
+        kr_f32x4 s[NG], b[NG];
+    };
+    auto read_keys = [&](uint32_t b, int t, Keys& to) {
         const uint8_t* st = lds + (b & 1u) * L::KSTAGE;
         const float* sc = (const float*)(st + L::K) + 4 * g;
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const uint8_t* kt = st + t * (STEPS * 1024) + lane * 16;
+        for (int i = 0; i < STEPS; i++) to.k[i] = *(const kr_u32x4*)(st + (t * STEPS + i) * 1024 + lane * 16);
 #pragma unroll
-            for (int n = 0; n < NG; n++) {
-                kr_f32x4 acc[MT];
+        for (int n = 0; n < NG; n++) {
+            to.s[n] = *(const kr_f32x4*)(sc + n * kBlock + 16 * t);
+            to.b[n] = *(const kr_f32x4*)(sc + (NG + n) * kBlock + 16 * t);
+        }
+    };
+    auto scores = [&](const Keys& from, int t, float (&x)[MT][2][4]) {
 #pragma unroll
-                for (int m = 0; m < MT; m++) acc[m] = kr_f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NG; n++) {
+            kr_f32x4 acc[MT];
 #pragma unroll
-                for (int i = n * (G / 32); i < (n + 1) * (G / 32); i++) {
-                    const kr_u32x4 k = *(const kr_u32x4*)(kt + i * 1024);
+            for (int m = 0; m < MT; m++) acc[m] = kr_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int m = 0; m < MT; m++)
-#pragma unroll
-                        for (int e = T::Q - 1; e >= 0; e--) acc[m] = kr_mfma<T::QK>(k, q[m][e][i], acc[m]);
-                }
-                const kr_f32x4 ks = *(const kr_f32x4*)(sc + n * kBlock + 16 * t), kb = *(const kr_f32x4*)(sc + (NG + n) * kBlock + 16 * t);
+            for (int i = n * (G / 32); i < (n + 1) * (G / 32); i++)
 #pragma unroll
                 for (int m = 0; m < MT; m++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x[m][t][i] = fmaf(kb[i], qsum[m][n], n ? fmaf(ks[i], acc[m][i], x[m][t][i]) : ks[i] * acc[m][i]);
-            }
+                    for (int e = T::Q - 1; e >= 0; e--) acc[m] = kr_mfma<T::QK>(from.k[i], q[m][e][i], acc[m]);
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[m][t][i] = fmaf(from.b[n][i], qsum[m][n], n ? fmaf(from.s[n][i], acc[m][i], x[m][t][i]) : from.s[n][i] * acc[m][i]);
         }
     };
     // What a row does not see scores -inf; the bars are raised where scores pass them.
@@ -303,58 +310,67 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
             if (!(fabsf(sc[i]) < INFINITY && fabsf(sc[NG * kBlock + i]) < INFINITY)) sc[i] = sc[NG * kBlock + i] = 0.f;
         __syncthreads();
     };
-    auto add_values = [&](uint32_t b, float (&x)[MT][2][4]) {
-        const uint8_t* st = lds + 2 * L::KSTAGE + (b & 1u) * L::VSTAGE;
-        const float* sc = (const float*)(st + L::V) + 4 * g;
+    // A block's weights out of its scores, one sixteen of them; a group's values and their numbers out of the LDS; p s as operands; and the values' sums.
+    auto weigh = [&](int t, float (&x)[MT][2][4]) {
 #pragma unroll
         for (int m = 0; m < MT; m++) {
             const float from_bar = bar[m] == -INFINITY ? 0.f : bar[m];
 #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x[m][t][i] = __builtin_amdgcn_exp2f(fmaf(x[m][t][i], c, -from_bar));
+                sum[m] += x[m][t][i];
+            }
+        }
+    };
+    struct Values {
+        kr_u32x4 v[NT];
+        kr_f32x4 s[2], b[2];
+    };
+    auto read_values = [&](uint32_t b, int n, Values& to) {
+        const uint8_t* st = lds + 2 * L::KSTAGE + (b & 1u) * L::VSTAGE;
+        const float* sc = (const float*)(st + L::V) + 4 * g;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            to.s[t] = *(const kr_f32x4*)(sc + n * kBlock + 16 * t);
+            to.b[t] = *(const kr_f32x4*)(sc + (NG + n) * kBlock + 16 * t);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) to.v[t] = *(const kr_u32x4*)(st + (n * NT + t) * L::VT + lane * 16);
+    };
+    auto operands = [&](const Values& from, int n, const float (&x)[MT][2][4], kr_u32x4 (&pt)[MT][T::P]) {
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+#pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[m][t][i] = __builtin_amdgcn_exp2f(fmaf(x[m][t][i], c, -from_bar));
-                    sum[m] += x[m][t][i];
-                }
+                for (int i = 0; i < 4; i++) bias[m][n] = fmaf(x[m][t][i], from.b[t][i], bias[m][n]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float y[2][T::P];
+#pragma unroll
+                for (int e = 0; e < 2; e++) kv_split(x[m][j / 2][2 * j % 4 + e] * from.s[j / 2][2 * j % 4 + e], y[e]);
+#pragma unroll
+                for (int e = 0; e < T::P; e++) pt[m][e][j] = kv_pack_bf16(y[0][e], y[1][e]);
+            }
         }
+    };
+    auto add_values = [&](const Values& from, int n, const kr_u32x4 (&pt)[MT][T::P]) {
         const kr_u32x4 less24 = {0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u};   // -24 in bf16
+        kr_f32x4 less[MT];
 #pragma unroll
-        for (int n = 0; n < NG; n++) {
-            kr_f32x4 vs[2], vb[2];
+        for (int m = 0; m < MT; m++) {
+            less[m] = kr_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                vs[t] = *(const kr_f32x4*)(sc + n * kBlock + 16 * t);
-                vb[t] = *(const kr_f32x4*)(sc + (NG + n) * kBlock + 16 * t);
-            }
-            kr_u32x4 pt[MT][T::P];
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) bias[m][n] = fmaf(x[m][t][i], vb[t][i], bias[m][n]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    float y[2][T::P];
-#pragma unroll
-                    for (int e = 0; e < 2; e++) kv_split(x[m][j / 2][2 * j % 4 + e] * vs[j / 2][2 * j % 4 + e], y[e]);
-#pragma unroll
-                    for (int e = 0; e < T::P; e++) pt[m][e][j] = kv_pack_bf16(y[0][e], y[1][e]);
-                }
-                kr_f32x4 less = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int e = T::P - 1; e >= 0; e--) less = kr_mfma<DT_BF16>(less24, pt[m][e], less);
-                ones[m][n] += less[0];
-            }
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const kr_u32x4 v = *(const kr_u32x4*)(st + (n * NT + t) * L::VT + lane * 16);
-#pragma unroll
-                for (int m = 0; m < MT; m++)
-#pragma unroll
-                    for (int e = T::P - 1; e >= 0; e--) o[m][n][t] = kr_mfma<DT_BF16>(v, pt[m][e], o[m][n][t]);
-            }
+            for (int e = T::P - 1; e >= 0; e--) less[m] = kr_mfma<DT_BF16>(less24, pt[m][e], less[m]);
         }
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int e = T::P - 1; e >= 0; e--) o[m][n][t] = kr_mfma<DT_BF16>(from.v[t], pt[m][e], o[m][n][t]);
+#pragma unroll
+        for (int m = 0; m < MT; m++) ones[m][n] += less[m][0];
     };
 
     // The scores of a block are computed beside the values of the one before, so that the matrix cores have the one while the vector units have the
@@ -374,7 +390,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
         bring(b0);
         if (!values) bring(b0 + 1u);
         __syncthreads();
-        scores(b0, x);
+        {
+            Keys keys;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                read_keys(b0, t, keys);
+                scores(keys, t, x);
+            }
+        }
         look(b0, __builtin_amdgcn_readfirstlane(flags[(b0 & 1u) * 2u] | flags[(b0 & 1u) * 2u + 1u] << 1), x);
         __syncthreads();
         for (uint32_t b = b0; b < b1; b++) {
@@ -385,9 +408,29 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
             const uint32_t* f = flags + ((b + 1u) & 1u) * 2u;
             const uint32_t f0 = f[0], f1 = f[1];
             bring(b + ahead);
+            // What the LDS is asked for in one part is used in the next (behind the last block the keys are those that are there, and not used).
             float next[MT][2][4];
-            scores(b + 1u, next);   // (behind the last block: of what is there, and not used)
-            add_values(b, x);
+            Keys first, second;
+            Values group[2];
+            kr_u32x4 pt[MT][T::P];
+            read_keys(b + 1u, 0, first);
+            weigh(0, x);
+            __builtin_amdgcn_sched_barrier(0);
+            read_keys(b + 1u, 1, second);
+            scores(first, 0, next);
+            weigh(1, x);
+            __builtin_amdgcn_sched_barrier(0);
+            read_values(b, 0, group[0]);
+            scores(second, 1, next);
+            __builtin_amdgcn_sched_barrier(0);
+            operands(group[0], 0, x, pt);
+#pragma unroll
+            for (int n = 0; n < NG; n++) {
+                if (n + 1 < NG) read_values(b, n + 1, group[(n + 1) & 1]);
+                add_values(group[n & 1], n, pt);
+                __builtin_amdgcn_sched_barrier(0);
+                if (n + 1 < NG) operands(group[(n + 1) & 1], n + 1, x, pt);
+            }
             if (b + 1u < b1) look(b + 1u, __builtin_amdgcn_readfirstlane(f0 | f1 << 1), next);
 #pragma unroll
             for (int m = 0; m < MT; m++)
