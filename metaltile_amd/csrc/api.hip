@@ -2195,7 +2195,7 @@ int mtq_plan(int op, int dtype, int bits, uint32_t group_size, uint32_t M, uint3
         case MTQ_OP_KV_READ:
         case MTQ_OP_KV_ATTENTION: {
             const uint32_t pages = ((uint32_t)bits + 15u) / 16u;
-            const mtq_kv_cache cache{w, s, b, at(9), at(10), at(11), E * pages, 16, N, K, group_size};
+            const mtq_kv_cache cache{w, s, b, at(9), at(10), at(11), 1, 16, N, K, group_size};
             const mtq_kv_batch batch{(const uint32_t*)aux, (const uint32_t*)aux2, (const uint32_t*)at(12), pages, E, T, (uint32_t)bits};
             const uint64_t wide = (uint64_t)M * K, narrow = (uint64_t)N * K;
             if (op == MTQ_OP_KV_APPEND) {
