@@ -312,7 +312,7 @@ template <int U> const void* append_kernel(int dtype, int pairs) {
     return dtype == DT_F32 ? append_kernel_of<U, DT_F32>(pairs) : dtype == DT_F16 ? append_kernel_of<U, DT_F16>(pairs) : append_kernel_of<U, DT_BF16>(pairs);
 }
 // Several units a thread where that leaves the chip full: their loads are under way together.
-uint32_t units_each(uint32_t n_tokens, uint64_t units, uint32_t most) { return (uint64_t)n_tokens * units >= 256ull * most * 2048 ? most : 1u; }
+uint32_t units_each(uint32_t n_tokens, uint64_t units, uint32_t most) { return (uint64_t)n_tokens * units >= 256ull * most * 512 ? most : 1u; }
 
 }  // namespace
 
