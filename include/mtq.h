@@ -634,9 +634,9 @@ MTQ_API int mtq_flush_cache(void);
  *   "gather.names_exact"   the exact-dequant gather names of mtq_dispatch (mt_moe_gather_qmm_int4, _m8, _m16, _m32, _b3 ..
  *                          _b8): 0 = always on the GEMV kernels (exact s*q + b, as those reference kernels compute), 1 = grouped
  *                          on the tile kernel above 8 rows per expert like the typed entry points (w_hat rounded to T first)
- *   "kv.kernel"            mtq_kv_attention: 0 = choose, 1 = the kernel for few rows a sequence, 2 = the one for many
- *   "kv.waves"             that for few: workgroups of 4 waves (1) or of as many as fit (2), 0 = choose
- *   "kv.slices"            either: slices of a sequence's tokens that are joined behind, 0 = choose, or 1..1024
+ *   "kv.kernel"            mtq_kv_attention: 0 = choose, 1 = the kernel for few rows a sequence, 2 = the one for many, 3 = the one for up to
+ *                          four, 4 = the one for prompts (f16 and bf16; others as 2)
+ *   "kv.slices"            slices that a sequence's tokens are cut into at most, whose sums are joined behind, 0 = choose, or 1..1024
  *   "scratch.most_kb"      largest library-owned scratch buffer in KB, 0 = no limit: a call that wants more goes the way it goes
  *                          where that memory cannot be allocated
  *   "qvm.wgs"              qvm: workgroups to aim for when K is sliced, 0 = choose

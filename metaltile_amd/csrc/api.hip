@@ -1559,7 +1559,7 @@ static int op_kv_attention(int dtype, const mtq_kv_cache* c, const mtq_kv_batch*
     if ((rc = check_heads(dtype, a.q, a.q_stride, a.hq, a.kv.dim)) || (rc = check_heads(dtype, a.out, a.out_stride, a.hq, a.kv.dim))) return rc;
     if ((uint64_t)a.kv.n_tokens * a.hq >= 1ull << 31) return fail(ERR_SHAPE, "n_tokens * hq must be less than 2^31");
     const KvPlan plan = kv_attention_plan(dtype, a);
-    // (no memory for the slices' sums: sequences are not cut)
+    // (no memory: sequences are not cut, and keys and values not laid out)
     void* scratch = plan.scratch && ensure_scratch(plan.scratch) == ERR_OK ? g.scratch_buf : nullptr;
     return launch_kv_attention(dtype, a, plan, scratch, lc);
 }
@@ -2400,13 +2400,8 @@ int mtq_set_option(const char* name, int value) {
         return MTQ_OK;
     }
     if (!strcmp(name, "kv.kernel")) {
-        if (value < 0 || value > 2) return fail(ERR_BAD_ARG, "kv.kernel must be 0 (choose), 1 (few rows a sequence) or 2 (many)");
+        if (value < 0 || value > 4) return fail(ERR_BAD_ARG, "kv.kernel must be 0 (choose), 1 (few rows a sequence), 2 (many), 3 (up to four at a time) or 4 (prompts, in f16 and bf16)");
         options().kv_kernel = value;
-        return MTQ_OK;
-    }
-    if (!strcmp(name, "kv.waves")) {
-        if (value < 0 || value > 2) return fail(ERR_BAD_ARG, "kv.waves must be 0 (choose), 1 (workgroups of 4 waves) or 2 (of as many as fit)");
-        options().kv_waves = value;
         return MTQ_OK;
     }
     if (!strcmp(name, "kv.slices")) {

@@ -52,22 +52,191 @@ __device__ __forceinline__ uint32_t kv_pack_bf16(float a, float b) {   // (one i
 
 // Sum and maximum over the lanes of a column (lane & 15).
 __device__ __forceinline__ float kv_column_sum(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 __device__ __forceinline__ float kv_column_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+
+// SIZE bytes a lane from `from` to LDS: lane l's at lds + SIZE l. No register is written; counts in vmcnt. M0 is read one wait state behind its write at
+// the earliest, which no one but this block sees to.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // M0 is a reserved register: naming it as clobbered is the point
+__device__ __forceinline__ void kv_load16(uint32_t lds, const void* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void kv_load4(uint32_t lds, const void* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
+}
+#pragma clang diagnostic pop
 
 // What joins the parts of a row: the maximum in base 2, the sum of the weights, and the weighted values, rows of dim.
 struct KvParts {
     float* values = nullptr;   // [rows, query heads, slices, dim]
-    float* sums = nullptr;     // [rows, query heads, slices, 2]
-    uint32_t slices = 1;
+    float* sums = nullptr;     // [rows, query heads, slices, 2]; a sum of -1 (kNoMore): no slice from here on
+    uint32_t slices = 1;       // that a sequence has at most
+    uint32_t pieces = 1;       // of the kernels for few rows: what all sequences' tokens are cut into, about (kv_piece)
+    uint32_t least = 1;        // blocks of 64 tokens that a piece has
 };
-int launch_kv_rows(int dtype, const KvAttentionArgs& p, const KvParts& parts, bool large, const LaunchCtx& lc);
+constexpr float kNoMore = -1.f;
+constexpr uint32_t kCutSeqs = 512;   // sequences that are cut into pieces at most: each workgroup looks at all of them
+
+// Workgroup `index` of a key head's: a sequence, and one of the equal slices that its tokens are cut into. Lengths are known here only, and sequences of
+// 1 to 8192 tokens, each cut into as many, left the card with the longest one's slices: so a piece is a share of all tokens, and a sequence has as many as its
+// tokens need. False: no piece. All lanes of a wave call.
+struct KvPiece {
+    KvSeq s;
+    uint32_t slice = 0, slices = 1;
+};
+__device__ __forceinline__ bool kv_piece(const KvAttentionArgs& a, const KvParts& parts, uint32_t index, KvPiece& p) {
+    const KvArgs& kv = a.kv;
+    if (parts.slices == 1) {
+        p.s = kv_seq(kv, index);
+        return p.s.rows != 0;
+    }
+    constexpr uint32_t MOST = kCutSeqs / 64;
+    const uint32_t lane = threadIdx.x & 63u, each = (kv.n_seqs + 63u) / 64u;   // sequences of a lane
+    uint32_t n[MOST], all = 0;                                                 // their blocks of 64 tokens
+#pragma unroll
+    for (uint32_t j = 0; j < MOST; j++) {
+        n[j] = 0xFFFFFFFFu;   // no rows
+        const uint32_t i = lane * each + j;
+        if (j < each && i < kv.n_seqs) {
+            const KvSeq s = kv_seq(kv, i);
+            if (s.rows) {
+                const int32_t end = (int32_t)(s.len + 1u) - (int32_t)s.rows;   // of the first row
+                const uint32_t from = a.window && end > (int32_t)a.window ? (uint32_t)end - a.window : 0u;
+                n[j] = (s.len - from + 63u) / 64u;
+                all += n[j];
+            }
+        }
+    }
+    for (int i = 1; i < 64; i <<= 1) all += (uint32_t)__shfl_xor((int)all, i, 64);
+    uint32_t share = (all + parts.pieces - 1u) / parts.pieces;
+    if (share < parts.least) share = parts.least;
+    uint32_t mine = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < MOST; j++)
+        if (j < each) {
+            n[j] = n[j] == 0xFFFFFFFFu ? 0u : n[j] <= share ? 1u : (n[j] + share - 1u) / share;
+            if (n[j] > parts.slices) n[j] = parts.slices;
+            mine += n[j];
+        }
+    uint32_t upto = mine;
+    for (int i = 1; i < 64; i <<= 1) {
+        const uint32_t other = (uint32_t)__shfl_up((int)upto, i, 64);
+        if (lane >= (uint32_t)i) upto += other;
+    }
+    const uint64_t above = __ballot(upto > index);
+    if (!above) return false;
+    const uint32_t who = (uint32_t)__builtin_ctzll(above);
+    uint32_t rest = index - (upto - mine), at = 0, slices = 1;   // (this lane's answer; `who` has the one that counts)
+    bool found = false;
+#pragma unroll
+    for (uint32_t j = 0; j < MOST; j++)
+        if (j < each && !found) {
+            if (rest < n[j]) {
+                found = true;
+                at = lane * each + j;
+                slices = n[j];
+            } else {
+                rest -= n[j];
+            }
+        }
+    p.slice = (uint32_t)__builtin_amdgcn_readlane((int)rest, (int)who);
+    p.slices = (uint32_t)__builtin_amdgcn_readlane((int)slices, (int)who);
+    p.s = kv_seq(kv, (uint32_t)__builtin_amdgcn_readlane((int)at, (int)who));
+    return true;
+}
+
+constexpr uint32_t kBlock = 32;   // tokens of a step of the kernels for many rows
+// A workgroup of those: ROWS rows of a key head (new tokens times the query heads that share it), and blocks b0 .. b1 - 1 of the tokens that they see.
+struct KvTile {
+    KvSeq s;
+    uint32_t head, shared, rows, row0, slice, slices;   // row0 .. row0 + ROWS - 1 of the sequence's `rows`
+    uint32_t lo, hi, first_end, b0, b1;                 // they see tokens lo (of block 0) .. hi - 1; its first row those below first_end
+};
+template <uint32_t ROWS> __device__ __forceinline__ bool kv_tile(const KvAttentionArgs& a, const KvParts& parts, uint32_t tiles, KvTile& to) {
+    const KvArgs& kv = a.kv;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t shared = a.hq / kv.hkv, head = blockIdx.x % kv.hkv, at_tile = blockIdx.x / kv.hkv, slice = at_tile / tiles;
+    // Sequence i's tiles begin at (its first row) * shared / ROWS + i, which leaves room for as many as it has. The last ones see the most and come first.
+    const uint32_t tile = tiles - 1u - at_tile % tiles;
+    uint32_t seq;
+    if (kv.offsets) {
+        uint32_t lo = 0, n = kv.n_seqs;   // of the sequences lo .. lo + n - 1 the last that begins at `tile` or before
+        while (n > 1) {
+            const uint32_t step = (n + 63u) / 64u, i = lo + lane * step;
+            const bool before = lane * step < n && (uint32_t)((uint64_t)(kv.offsets[i] < kv.n_tokens ? kv.offsets[i] : kv.n_tokens) * shared / ROWS) + i <= tile;
+            const uint32_t count = (uint32_t)__popcll(__ballot(before));
+            const uint32_t skip = count ? (count - 1u) * step : 0u;
+            lo += skip;
+            n = n - skip < step ? n - skip : step;
+        }
+        seq = __builtin_amdgcn_readfirstlane(lo);
+    } else {
+        const uint64_t per = (uint64_t)(kv.n_tokens / kv.n_seqs) * shared;   // (the beginnings of equal sequences: the last i with i per / ROWS + i <= tile)
+        uint32_t i = (uint32_t)((uint64_t)tile * ROWS / (per + ROWS));
+        while (i + 1u < kv.n_seqs && (i + 1u) * per / ROWS + i + 1u <= tile) i++;
+        seq = i;
+    }
+    const KvSeq s = kv_seq(kv, seq);
+    const uint32_t rows = s.rows * shared, first_tile = (uint32_t)((uint64_t)s.first_row * shared / ROWS) + seq;
+    if (tile < first_tile || (uint64_t)(tile - first_tile) * ROWS >= rows) return false;
+    const uint32_t row0 = (tile - first_tile) * ROWS;
+
+    auto end_of = [&](uint32_t i) { const int32_t e = (int32_t)(s.len + i / shared + 1u) - (int32_t)s.rows; return e > 0 ? (uint32_t)e : 0u; };
+    auto from_of = [&](uint32_t e) { return a.window && e > a.window ? e - a.window : 0u; };
+    const uint32_t last = row0 + ROWS - 1u < rows ? row0 + ROWS - 1u : rows - 1u;
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(end_of(last)), first_of_all = __builtin_amdgcn_readfirstlane(end_of(row0)), lo = __builtin_amdgcn_readfirstlane(from_of(end_of(row0))) & ~31u;
+    const uint32_t blocks = kv.n_pages && hi > lo ? (hi - lo + kBlock - 1u) / kBlock : 0u;
+    // A tile is cut into slices by what it sees, against what all see: of a prompt its last tiles, of several the longest one's.
+    uint32_t slices = 1;
+    if (parts.slices > 1) {
+        uint32_t all = 0;   // blocks that tiles see, as many or a few more
+        for (uint32_t i = lane; i < kv.n_seqs; i += 64) {
+            const KvSeq o = kv_seq(kv, i);
+            const uint32_t n = (o.rows * shared + ROWS - 1u) / ROWS, before = o.len > o.rows ? o.len - o.rows : 0u;
+            uint32_t mean = (before + o.len + ROWS / shared + 1u) / 2u;
+            if (a.window && mean > a.window + ROWS / shared) mean = a.window + ROWS / shared;
+            all += n * (mean / kBlock + 1u);
+        }
+        for (int i = 1; i < 64; i <<= 1) all += (uint32_t)__shfl_xor((int)all, i, 64);
+        uint32_t share = (all + parts.pieces - 1u) / parts.pieces;
+        if (share < parts.least) share = parts.least;
+        slices = __builtin_amdgcn_readfirstlane((blocks + share - 1u) / share);
+        if (slices > parts.slices) slices = parts.slices;
+        if (slices < 1u) slices = 1u;
+        if (slice >= slices) return false;
+    }
+    const uint32_t per = (blocks + slices - 1u) / slices;
+    const uint32_t b0 = slice * per < blocks ? slice * per : blocks, b1 = b0 + per < blocks ? b0 + per : blocks;
+    to = KvTile{s, head, shared, rows, row0, slice, slices, lo, hi, first_of_all, b0, b1};
+    return true;
+}
+__device__ __forceinline__ uint32_t kv_end(const KvTile& t, uint32_t i) {   // row i sees the tokens before this one
+    const int32_t e = (int32_t)(t.s.len + i / t.shared + 1u) - (int32_t)t.s.rows;
+    return e > 0 ? (uint32_t)e : 0u;
+}
+// Workgroups of a key head: pieces there can be.
+inline uint32_t kv_pieces(const KvAttentionArgs& a, const KvParts& parts) { return parts.slices == 1 ? a.kv.n_seqs : a.kv.n_seqs + parts.pieces; }
+int launch_kv_rows(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc);
+int launch_kv_quads(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc);
 int launch_kv_tiles(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc);
+// Keys and values of 32 tokens in T, as the matrix instructions take them (kv_attention_prompts.hip).
+struct KvImages {
+    uint8_t* data = nullptr;     // [sequences, key heads, blocks], 128 head_dim bytes each
+    uint32_t* flags = nullptr;   // [sequences, key heads, blocks]
+    uint32_t blocks = 0;         // of a sequence
+};
+int launch_kv_prompts(int dtype, const KvAttentionArgs& p, const KvParts& parts, const KvImages& images, const LaunchCtx& lc);
+uint32_t kv_prompt_rows(uint32_t dim);
 int launch_kv_join(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc);
 uint32_t kv_tile_rows(int dtype, uint32_t dim);
 

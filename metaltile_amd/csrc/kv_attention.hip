@@ -6,25 +6,60 @@ namespace mtq {
 namespace {
 
 // A wave for each row and query head: its slices joined.
-template <int DT, int D> __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a, KvParts parts) {
-    const uint32_t lane = threadIdx.x & 63u, at = blockIdx.x * 4 + (threadIdx.x >> 6), row = at / a.hq, h = at - row * a.hq;
-    if (row >= a.kv.n_tokens) return;
+// W waves to a row of a head, D / 4 lanes to a slice's numbers. The slices' loads go out together: with a branch on a slice's sum between them, 32 slices took 15 us.
+template <int DT, int D, int W> __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a, KvParts parts) {
+    constexpr uint32_t LANES = D / 4, TURNS = 64 * W / LANES;
+    __shared__ kr_f32x4 others[4 / W][W > 1 ? TURNS : 1][LANES + 1];   // (values; sum)
+    const uint32_t lane = threadIdx.x & 63u, in_block = threadIdx.x / (64 * W), at = blockIdx.x * (4 / W) + in_block, row = at / a.hq, h = at - row * a.hq;
     KvSeq s;
-    if (!kv_seq_of(a.kv, row, s)) return;
+    bool yes = row < a.kv.n_tokens;
+    if (yes) yes = kv_seq_of(a.kv, row, s);
+    const uint32_t unit = threadIdx.x % (64 * W), turn = unit / LANES, d = unit % LANES * 4;
     const float* sums = parts.sums + (uint64_t)at * parts.slices * 2;
+    const float* values = parts.values + (uint64_t)at * parts.slices * D + d;
+    uint32_t n = yes ? parts.slices : 0u;
     float top = -INFINITY;
-    for (uint32_t i = lane; i < parts.slices; i += 64) top = fmaxf(top, sums[2 * i]);
+    for (uint32_t i = lane; i - lane < n; i += 64) {
+        const float bar = i < n ? sums[2 * i] : -INFINITY, part = i < n ? sums[2 * i + 1] : 0.f;
+        const uint64_t no_more = __ballot(part == kNoMore);
+        if (no_more) n = i - lane + (uint32_t)__builtin_ctzll(no_more);
+        if (i < n) top = fmaxf(top, bar);
+    }
+    if (n == 0) yes = false;   // (of one slice: written already)
+    if (W == 1 && !yes) return;
     for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i, 64));
-    float total = 0.f, v[D / 64] = {};
-    for (uint32_t i = 0; i < parts.slices; i++) {
+    float total = 0.f;
+    kr_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t i = turn; i < n; i += TURNS) {
         const float bar = sums[2 * i], part = sums[2 * i + 1], f = bar == -INFINITY ? (part == 0.f ? 0.f : 1.f) : exp2f(bar - top);
-        if (f == 0.f && part == 0.f) continue;
+        const kr_f32x4 x = *(const kr_f32x4*)(values + (uint64_t)i * D);
+        const bool none = f == 0.f && part == 0.f;   // (values that no one wrote)
         total = fmaf(part, f, total);
 #pragma unroll
-        for (int j = 0; j < D / 64; j++) v[j] = fmaf(parts.values[((uint64_t)at * parts.slices + i) * D + lane + 64 * j], f, v[j]);
+        for (int j = 0; j < 4; j++) v[j] = none ? v[j] : fmaf(x[j], f, v[j]);
+    }
+    if (W == 1) {
+#pragma unroll
+        for (uint32_t i = LANES; i < 64; i <<= 1) {
+            total += __shfl_xor(total, i, 64);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] += __shfl_xor(v[j], i, 64);
+        }
+        if (turn) return;
+    } else {
+        others[0][turn][d / 4] = v;
+        if (d == 0) others[0][turn][LANES][0] = total;
+        __syncthreads();
+        if (turn || !yes) return;
+#pragma unroll
+        for (uint32_t i = 1; i < TURNS; i++) {
+            total += others[0][i][LANES][0];
+            v += others[0][i][d / 4];
+        }
     }
 #pragma unroll
-    for (int j = 0; j < D / 64; j++) store_elem<DT>(a.out, (uint64_t)row * a.out_stride + (uint64_t)h * D + lane + 64 * j, total == 0.f ? 0.f : v[j] / total);
+    for (int j = 0; j < 4; j++) store_elem<DT>(a.out, (uint64_t)row * a.out_stride + (uint64_t)h * D + d + j, total == 0.f ? 0.f : v[j] / total);
 }
 
 }  // namespace
@@ -32,13 +67,17 @@ template <int DT, int D> __global__ __launch_bounds__(256) void kv_join_kernel(K
 int launch_kv_join(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc) {
     KvAttentionArgs a = p;
     KvParts q = parts;
-    const void* fn[3][3] = {{(const void*)kv_join_kernel<DT_F32, 64>, (const void*)kv_join_kernel<DT_F32, 128>, (const void*)kv_join_kernel<DT_F32, 256>},
-                            {(const void*)kv_join_kernel<DT_F16, 64>, (const void*)kv_join_kernel<DT_F16, 128>, (const void*)kv_join_kernel<DT_F16, 256>},
-                            {(const void*)kv_join_kernel<DT_BF16, 64>, (const void*)kv_join_kernel<DT_BF16, 128>, (const void*)kv_join_kernel<DT_BF16, 256>}};
-    const uint64_t groups = ((uint64_t)a.kv.n_tokens * a.hq + 3) / 4;
+#define MTQ_KV_JOIN(DT) \
+    {{(const void*)kv_join_kernel<DT, 64, 1>, (const void*)kv_join_kernel<DT, 64, 4>}, \
+     {(const void*)kv_join_kernel<DT, 128, 1>, (const void*)kv_join_kernel<DT, 128, 4>}, \
+     {(const void*)kv_join_kernel<DT, 256, 1>, (const void*)kv_join_kernel<DT, 256, 4>}}
+    const void* fn[3][3][2] = {MTQ_KV_JOIN(DT_F32), MTQ_KV_JOIN(DT_F16), MTQ_KV_JOIN(DT_BF16)};
+#undef MTQ_KV_JOIN
+    const bool wide = parts.slices > 8;
+    const uint64_t groups = wide ? (uint64_t)a.kv.n_tokens * a.hq : ((uint64_t)a.kv.n_tokens * a.hq + 3) / 4;
     if (groups > max_workgroups(256)) return fail(ERR_SHAPE, "more rows and heads than a launch can have workgroups");
     void* args[] = {&a, &q};
-    MTQ_HIP(launch_kernel(fn[dtype][a.kv.dim == 64 ? 0 : a.kv.dim == 128 ? 1 : 2], dim3((uint32_t)groups), dim3(256), args, 0, lc));
+    MTQ_HIP(launch_kernel(fn[dtype][a.kv.dim == 64 ? 0 : a.kv.dim == 128 ? 1 : 2][wide], dim3((uint32_t)groups), dim3(256), args, 0, lc));
     return ERR_OK;
 }
 
@@ -51,38 +90,84 @@ static uint32_t num_cus() {
     return (uint32_t)n;
 }
 
+// Rows are new tokens times the query heads that share a key head, for each sequence on average:
+//   to 4     the kernel with a token to a lane (64 sequences of 4096 tokens, 4 rows, bf16: 63 us against 69 of the one below; 256 of them 220 / 240)
+//   to 128   the one with 16 rows to a wave (32 sequences of 4096 tokens, 128 rows: 264 us against 360 of the one below, 4 of 2048 tokens 62 / 41; 64 rows 147 / 366 and
+//            35 / 34); f32 to 32
+//   above    f16 and bf16: keys and values laid out in T first (256 rows: 494 / 372 and 115 / 45; a prompt of 8192 tokens 559 us against 942 of the next). It has to have
+//            scratch for as many tokens as max_len allows, up to 1 GiB; f32, and calls without: the codes as they are
 KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
     KvPlan p;
-    const uint64_t units = (uint64_t)a.kv.n_seqs * a.kv.hkv, cus = num_cus(), rows = (uint64_t)a.kv.n_tokens * (a.hq / a.kv.hkv);
+    const uint64_t cus = num_cus(), rows = (uint64_t)a.kv.n_tokens * (a.hq / a.kv.hkv), n_seqs = a.kv.n_seqs;
+    const uint64_t row_bytes = (uint64_t)a.kv.n_tokens * a.hq * (a.kv.dim + 2) * sizeof(float), most_bytes = (uint64_t)64 << 20;   // of a slice; of all
     const uint32_t span = a.window && a.window < a.kv.max_len ? a.window : a.kv.max_len;   // tokens that a row sees at most
-    p.tiles = rows > 32ull * a.kv.n_seqs;
-    if (options().kv_kernel) p.tiles = options().kv_kernel == 2;
-    uint64_t groups;   // of one slice
-    if (p.tiles) {
-        groups = (rows / kv_tile_rows(dtype, a.kv.dim) + a.kv.n_seqs) * a.kv.hkv;
-        const uint64_t want = (cus + groups - 1) / groups, most = span / 512;
-        p.slices = (uint32_t)(want < most ? want : most);
+    const uint64_t images = ((uint64_t)a.kv.max_len + kBlock - 1) / kBlock * n_seqs * a.kv.hkv * (128ull * a.kv.dim + 4);
+    const bool prompts = dtype != DT_F32 && images && images <= (1ull << 30);
+    p.kernel = options().kv_kernel ? options().kv_kernel : rows <= 4 * n_seqs ? 3 : rows > 128 * n_seqs && prompts ? 4 : rows > (dtype == DT_F32 ? 32 : 128) * n_seqs ? 2 : 1;
+    if (p.kernel == 4 && !prompts) p.kernel = 2;
+    if (p.kernel == 4) p.images = (size_t)((images + 255) / 256 * 256);
+    uint64_t slices, pieces;
+    if (p.kernel == 2 || p.kernel == 4) {
+        // Two tiles' worth of workgroups to a compute unit; the grid has room for twice that, since tiles that see little are not cut. Less than 256 tokens to a
+        // slice do not pay for what goes through memory (a prompt of 512 tokens in slices of 256: 26 us, whole 23).
+        const uint64_t groups = (rows / (p.kernel == 4 ? kv_prompt_rows(a.kv.dim) : kv_tile_rows(dtype, a.kv.dim)) + n_seqs) * a.kv.hkv, want = (4 * cus + groups - 1) / groups;
+        slices = span < 1024 ? 1 : want < span / 256 ? want : span / 256;
+        pieces = 2 * cus / a.kv.hkv;
+        p.least = 8;
+        if (options().kv_slices) {
+            slices = (uint64_t)options().kv_slices;
+            pieces = 0xFFFFFFFFu;
+            p.least = 1;
+        }
+        while (slices > 1 && groups * slices > max_workgroups(512)) slices--;
     } else {
-        groups = units;
-        p.large = units < 2 * cus;
-        const uint64_t want = ((p.large ? 1 : 4) * cus + units - 1) / units, most = span / (p.large ? 1024 : 512);
-        p.slices = (uint32_t)(want < most ? want : most);
+        // The same, and no piece longer than a sequence is on average; from eight workgroups to a compute unit on they fill it as they come (256 sequences of 1 to 8192
+        // tokens: 255 us, cut by the average 257).
+        const uint64_t seen = (uint64_t)span + a.kv.n_tokens < a.kv.max_len ? (uint64_t)span + a.kv.n_tokens : a.kv.max_len, blocks = (seen + 63) / 64;   // by all rows of a sequence
+        pieces = 2 * cus / a.kv.hkv > n_seqs ? 2 * cus / a.kv.hkv : n_seqs;
+        slices = blocks / 4 < pieces ? blocks / 4 : pieces;
+        if (n_seqs * a.kv.hkv >= 8 * cus) slices = 1;
+        if (options().kv_slices) {
+            slices = (uint64_t)options().kv_slices;
+            pieces = slices * n_seqs;
+        }
+        if (n_seqs > kCutSeqs) slices = 1;
+        while (slices > 1 && (n_seqs + pieces) * a.kv.hkv > max_workgroups(256)) {
+            pieces /= 2;
+            slices = slices < pieces ? slices : pieces;
+        }
+        if (slices > most_bytes / row_bytes) slices = most_bytes / row_bytes;
+        if (slices < 1) slices = 1;
+        p.least = (uint32_t)((blocks + slices - 1) / slices);   // (no sequence has more slices than there is room for)
     }
-    if (options().kv_waves) p.large = options().kv_waves == 2;
-    if (options().kv_slices) p.slices = (uint32_t)options().kv_slices;
-    if (p.slices < 1) p.slices = 1;
-    while (p.slices > 1 && groups * p.slices > max_workgroups(1024)) p.slices--;
-    p.scratch = p.slices > 1 ? (size_t)a.kv.n_tokens * a.hq * p.slices * (a.kv.dim + 2) * sizeof(float) : 0;
+    if (slices > most_bytes / row_bytes) slices = most_bytes / row_bytes;
+    p.slices = slices < 1 ? 1 : (uint32_t)slices;
+    p.pieces = pieces ? (uint32_t)pieces : 1;
+    p.scratch = p.images + (p.slices > 1 ? (size_t)(row_bytes * p.slices) : 0);
     return p;
 }
 
 int launch_kv_attention(int dtype, const KvAttentionArgs& a, const KvPlan& plan, void* scratch, const LaunchCtx& lc) {
+    if ((uint64_t)a.kv.n_seqs * a.kv.hkv > max_workgroups(256)) return fail(ERR_SHAPE, "more sequences and heads than a launch can have workgroups");
     KvParts parts;
-    parts.slices = scratch ? plan.slices : 1;
-    parts.values = (float*)scratch;
-    parts.sums = scratch ? parts.values + (size_t)a.kv.n_tokens * a.hq * parts.slices * a.kv.dim : nullptr;
-    if ((uint64_t)a.kv.n_seqs * a.kv.hkv * parts.slices > max_workgroups(1024)) return fail(ERR_SHAPE, "more sequences and heads than a launch can have workgroups");
-    return plan.tiles ? launch_kv_tiles(dtype, a, parts, lc) : launch_kv_rows(dtype, a, parts, plan.large, lc);
+    KvImages images;
+    if (scratch) {
+        images.blocks = (a.kv.max_len + kBlock - 1) / kBlock;
+        images.data = (uint8_t*)scratch;
+        images.flags = (uint32_t*)(images.data + (size_t)images.blocks * a.kv.n_seqs * a.kv.hkv * (128 * a.kv.dim));
+        parts.slices = plan.slices;
+        parts.pieces = plan.pieces;
+        parts.least = plan.least;
+        parts.values = (float*)((char*)scratch + plan.images);
+        parts.sums = parts.values + (size_t)a.kv.n_tokens * a.hq * parts.slices * a.kv.dim;
+    }
+    switch (plan.kernel) {
+        case 1: return launch_kv_rows(dtype, a, parts, lc);
+        case 3: return launch_kv_quads(dtype, a, parts, lc);
+        case 4:
+            if (scratch) return launch_kv_prompts(dtype, a, parts, images, lc);
+    }
+    return launch_kv_tiles(dtype, a, parts, lc);
 }
 
 }  // namespace mtq

@@ -11,18 +11,6 @@ namespace mtq {
 
 namespace {
 
-// SIZE bytes a lane from `from` to LDS: lane l's at lds + SIZE l. No register is written; counts in vmcnt. M0 is read one wait state behind its write at
-// the earliest, which no one but this block sees to.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"   // M0 is a reserved register: naming it as clobbered is the point
-__device__ __forceinline__ void kv_load16(uint32_t lds, const void* from) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
-}
-__device__ __forceinline__ void kv_load4(uint32_t lds, const void* from) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 // Sizes of a wave's part of the LDS, in bytes.
 template <int DT, int D, int G> struct RowsLds {
     static constexpr int ES = DT == DT_F32 ? 4 : 2, NG = D / G;
@@ -32,10 +20,8 @@ template <int DT, int D, int G> struct RowsLds {
     static constexpr int STAGE = 2 * CODES + 2 * LOADS * 256;
     static constexpr int JOIN = 16 * (D + 4) * 4;                // rows' values, and behind each its maximum and sum
     static constexpr int WAVE = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
-    // Waves of a SIMD at a time, by the registers that the sums, queries and a block's numbers take; and of a large workgroup.
-    static constexpr int AT_ONCE = DT != DT_F32 && D <= 128 && G >= 64 ? 3 : 2;
-    static constexpr int MOST = 4 * AT_ONCE * WAVE <= 160 * 1024 ? 4 * AT_ONCE : 4;
-    static_assert(MOST * WAVE <= 160 * 1024, "");
+    static constexpr int NW = 4, AT_ONCE = DT != DT_F32 && D <= 128 && G >= 64 ? 3 : 2;   // waves; of a SIMD at a time, by the registers
+    static_assert(NW * WAVE <= 160 * 1024, "");
 };
 
 // The values' number (row of the matrix instruction) `m` of tile t of a group, as its place in the group.
@@ -44,16 +30,19 @@ template <int G> __device__ __forceinline__ uint32_t kv_number(uint32_t t, uint3
     return 8 * (m % W) + (16 / W) * t + m / W;
 }
 
-template <int DT, int D, int G, int NW>
-__global__ __launch_bounds__(64 * NW, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows_kernel(KvAttentionArgs a, KvParts parts) {
+template <int DT, int D, int G>
+__global__ __launch_bounds__(256, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows_kernel(KvAttentionArgs a, KvParts parts) {
     using L = RowsLds<DT, D, G>;
     using T = KvTerms<DT>;
-    constexpr int STEPS = D / 32, NG = D / G, NT = G / 16, ES = L::ES, W = G / 8;
+    constexpr int NW = L::NW, STEPS = D / 32, NG = D / G, NT = G / 16, ES = L::ES, W = G / 8;
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const KvArgs& kv = a.kv;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15u, g = lane >> 4;
-    const uint32_t slice = blockIdx.x % parts.slices, at_head = blockIdx.x / parts.slices, head = at_head % kv.hkv, shared = a.hq / kv.hkv;
-    const KvSeq s = kv_seq(kv, at_head / kv.hkv);
+    const uint32_t head = blockIdx.x % kv.hkv, shared = a.hq / kv.hkv;
+    KvPiece piece;
+    if (!kv_piece(a, parts, blockIdx.x / kv.hkv, piece)) return;   // (all of the workgroup's waves find the same)
+    const KvSeq& s = piece.s;
+    const uint32_t slice = piece.slice, slices = piece.slices;
     uint8_t* mine = lds + wave * L::WAVE;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)mine;
     const uint32_t rows = s.rows * shared;   // (fewer than 2^24 2^16: checked against the launch on the host)
@@ -70,7 +59,7 @@ __global__ __launch_bounds__(64 * NW, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows
         const uint32_t first_end = __builtin_amdgcn_readfirstlane(end_of(row0)), last_end = __builtin_amdgcn_readfirstlane(end_of(last));
         const uint32_t lo = from_of(first_end) & ~31u, last_from = from_of(last_end);
         const uint32_t blocks = kv.n_pages && last_end > lo ? (last_end - lo + 31u) / 32u : 0u;
-        const uint32_t workers = parts.slices * NW, per = (blocks + workers - 1u) / workers;
+        const uint32_t workers = slices * NW, per = (blocks + workers - 1u) / workers;
         const uint32_t b0 = (slice * NW + wave) * per < blocks ? (slice * NW + wave) * per : blocks, b1 = b0 + per < blocks ? b0 + per : blocks;
 
         // Queries: words 4 i + g of the codes' rows meet values 32 i + 8 g .. + 7, in the order in which a word's nibbles come out.
@@ -350,7 +339,7 @@ __global__ __launch_bounds__(64 * NW, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows
 #pragma unroll
                 for (int j = 0; j < 4; j++) v[j] = f == 0.f && part == 0.f ? v[j] : fmaf(one[d + j], f, v[j]);
             }
-            if (parts.slices == 1) {
+            if (slices == 1) {
                 const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
                 for (int j = 0; j < 4; j++) store_elem<DT>(a.out, (uint64_t)tok * a.out_stride + (uint64_t)h * D + d + j, total == 0.f ? 0.f : v[j] * inv);
@@ -362,17 +351,20 @@ __global__ __launch_bounds__(64 * NW, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows
                     parts.sums[at * 2 + 1] = total;
                 }
             }
+            if (d == 0 && slice + 1u == slices && parts.slices > 1) {   // (of one slice: nothing to join)
+                const uint32_t n = slices == 1 ? 0u : slices;
+                if (n < parts.slices) parts.sums[(((uint64_t)tok * a.hq + h) * parts.slices + n) * 2 + 1] = kNoMore;
+            }
         }
         __syncthreads();   // (the next rows' loads go where these sums are)
     }
 }
 
-template <int DT, int D, int G> int launch(const KvAttentionArgs& p, KvParts parts, bool large, const LaunchCtx& lc) {
+template <int DT, int D, int G> int launch(const KvAttentionArgs& p, KvParts parts, const LaunchCtx& lc) {
     using L = RowsLds<DT, D, G>;
     KvAttentionArgs a = p;
-    const uint32_t waves = large ? L::MOST : 4;
-    const void* fn = large ? (const void*)kv_rows_kernel<DT, D, G, L::MOST> : (const void*)kv_rows_kernel<DT, D, G, 4>;
-    const size_t bytes = (size_t)waves * L::WAVE;
+    const void* fn = (const void*)kv_rows_kernel<DT, D, G>;
+    const size_t bytes = L::NW * L::WAVE;
     LaunchCtx first = lc, last = lc;
     if (parts.slices > 1) {
         first.stop = nullptr;
@@ -380,31 +372,31 @@ template <int DT, int D, int G> int launch(const KvAttentionArgs& p, KvParts par
     }
     MTQ_HIP(set_max_dynamic_lds(fn, bytes));
     void* args[] = {&a, &parts};
-    MTQ_HIP(launch_kernel(fn, dim3(a.kv.n_seqs * a.kv.hkv * parts.slices), dim3(64 * waves), args, bytes, first));
+    MTQ_HIP(launch_kernel(fn, dim3(kv_pieces(a, parts) * a.kv.hkv), dim3(64 * L::NW), args, bytes, first));
     return parts.slices > 1 ? launch_kv_join(DT, a, parts, last) : ERR_OK;
 }
 
-template <int DT> int launch_of(const KvAttentionArgs& p, const KvParts& parts, bool large, const LaunchCtx& lc) {
+template <int DT> int launch_of(const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc) {
     switch (p.kv.dim * 1000 + p.kv.group) {
-        case 64032: return launch<DT, 64, 32>(p, parts, large, lc);
-        case 64064: return launch<DT, 64, 64>(p, parts, large, lc);
-        case 128032: return launch<DT, 128, 32>(p, parts, large, lc);
-        case 128064: return launch<DT, 128, 64>(p, parts, large, lc);
-        case 128128: return launch<DT, 128, 128>(p, parts, large, lc);
-        case 256032: return launch<DT, 256, 32>(p, parts, large, lc);
-        case 256064: return launch<DT, 256, 64>(p, parts, large, lc);
-        case 256128: return launch<DT, 256, 128>(p, parts, large, lc);
+        case 64032: return launch<DT, 64, 32>(p, parts, lc);
+        case 64064: return launch<DT, 64, 64>(p, parts, lc);
+        case 128032: return launch<DT, 128, 32>(p, parts, lc);
+        case 128064: return launch<DT, 128, 64>(p, parts, lc);
+        case 128128: return launch<DT, 128, 128>(p, parts, lc);
+        case 256032: return launch<DT, 256, 32>(p, parts, lc);
+        case 256064: return launch<DT, 256, 64>(p, parts, lc);
+        case 256128: return launch<DT, 256, 128>(p, parts, lc);
     }
     return fail(ERR_UNSUPPORTED, "kv_attention: no kernel for this head_dim and group_size");
 }
 
 }  // namespace
 
-int launch_kv_rows(int dtype, const KvAttentionArgs& p, const KvParts& parts, bool large, const LaunchCtx& lc) {
+int launch_kv_rows(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc) {
     switch (dtype) {
-        case DT_F32: return launch_of<DT_F32>(p, parts, large, lc);
-        case DT_F16: return launch_of<DT_F16>(p, parts, large, lc);
-        default: return launch_of<DT_BF16>(p, parts, large, lc);
+        case DT_F32: return launch_of<DT_F32>(p, parts, lc);
+        case DT_F16: return launch_of<DT_F16>(p, parts, lc);
+        default: return launch_of<DT_BF16>(p, parts, lc);
     }
 }
 

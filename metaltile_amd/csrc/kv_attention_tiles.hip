@@ -11,8 +11,6 @@ namespace mtq {
 
 namespace {
 
-constexpr uint32_t kBlock = 32;   // tokens
-
 template <int DT, int D, int G, int NW> struct TilesShape {
     static constexpr int Q = KvTerms<DT>::Q, NG = D / G, STEPS = D / 32, NT = G / 16, TH = 64 * NW;
     static constexpr int MT = D * Q <= 192 ? 2 : 1;   // sixteens of rows of a wave: sums and queries fill its registers
@@ -33,38 +31,13 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const KvArgs& kv = a.kv;
     const uint32_t th = threadIdx.x, lane = th & 63u, wave = __builtin_amdgcn_readfirstlane(th >> 6), r = lane & 15u, g = lane >> 4;
-    const uint32_t shared = a.hq / kv.hkv, head = blockIdx.x % kv.hkv, at_slice = blockIdx.x / kv.hkv, slice = at_slice % parts.slices;
-    // Sequence i's tiles begin at (its first row) * shared / ROWS + i, which leaves room for as many as it has. The last ones see the most and come first.
-    const uint32_t tile = tiles - 1u - at_slice / parts.slices;
-    uint32_t seq;
-    if (kv.offsets) {
-        uint32_t lo = 0, n = kv.n_seqs;   // of the sequences lo .. lo + n - 1 the last that begins at `tile` or before
-        while (n > 1) {
-            const uint32_t step = (n + 63u) / 64u, i = lo + lane * step;
-            const bool before = lane * step < n && (uint32_t)((uint64_t)(kv.offsets[i] < kv.n_tokens ? kv.offsets[i] : kv.n_tokens) * shared / L::ROWS) + i <= tile;
-            const uint32_t count = (uint32_t)__popcll(__ballot(before));
-            const uint32_t skip = count ? (count - 1u) * step : 0u;
-            lo += skip;
-            n = n - skip < step ? n - skip : step;
-        }
-        seq = __builtin_amdgcn_readfirstlane(lo);
-    } else {
-        const uint64_t per = (uint64_t)(kv.n_tokens / kv.n_seqs) * shared;   // (the beginnings of equal sequences: the last i with i per / ROWS + i <= tile)
-        uint32_t i = (uint32_t)((uint64_t)tile * L::ROWS / (per + L::ROWS));
-        while (i + 1u < kv.n_seqs && (i + 1u) * per / L::ROWS + i + 1u <= tile) i++;
-        seq = i;
-    }
-    const KvSeq s = kv_seq(kv, seq);
-    const uint32_t rows = s.rows * shared, first_tile = (uint32_t)((uint64_t)s.first_row * shared / L::ROWS) + seq;
-    if (tile < first_tile || (uint64_t)(tile - first_tile) * L::ROWS >= rows) return;
-    const uint32_t row0 = (tile - first_tile) * L::ROWS;
-
-    auto end_of = [&](uint32_t i) { const int32_t e = (int32_t)(s.len + i / shared + 1u) - (int32_t)s.rows; return e > 0 ? (uint32_t)e : 0u; };
+    KvTile at_tile;
+    if (!kv_tile<L::ROWS>(a, parts, tiles, at_tile)) return;
+    const KvSeq& s = at_tile.s;
+    const uint32_t shared = at_tile.shared, head = at_tile.head, rows = at_tile.rows, row0 = at_tile.row0, slice = at_tile.slice, slices = at_tile.slices;
+    const uint32_t lo = at_tile.lo, hi = at_tile.hi, first_of_all = at_tile.first_end, b0 = at_tile.b0, b1 = at_tile.b1;
+    auto end_of = [&](uint32_t i) { return kv_end(at_tile, i); };
     auto from_of = [&](uint32_t e) { return a.window && e > a.window ? e - a.window : 0u; };
-    const uint32_t last = row0 + L::ROWS - 1u < rows ? row0 + L::ROWS - 1u : rows - 1u;
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(end_of(last)), first_of_all = __builtin_amdgcn_readfirstlane(end_of(row0)), lo = __builtin_amdgcn_readfirstlane(from_of(end_of(row0))) & ~31u;
-    const uint32_t blocks = kv.n_pages && hi > lo ? (hi - lo + kBlock - 1u) / kBlock : 0u, per = (blocks + parts.slices - 1u) / parts.slices;
-    const uint32_t b0 = slice * per < blocks ? slice * per : blocks, b1 = b0 + per < blocks ? b0 + per : blocks;
     // This wave's rows, and a lane's.
     const uint32_t wave0 = row0 + wave * 16 * MT, wave_last = wave0 + 16 * MT - 1u < rows ? wave0 + 16 * MT - 1u : rows - 1u;
     const bool any = wave0 < rows;
@@ -448,10 +421,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
         const uint32_t i = wave0 + 16 * m + r;
         const uint64_t at = (row_at[m] * a.hq + qh[m]) * parts.slices + slice;
         if (parts.slices > 1 && i < rows && g == 0) {
-            parts.sums[at * 2] = bar[m];
-            parts.sums[at * 2 + 1] = total;
+            if (slices > 1) {
+                parts.sums[at * 2] = bar[m];
+                parts.sums[at * 2 + 1] = total;
+            }
+            const uint32_t n = slices == 1 ? 0u : slices;   // (of one slice: nothing to join)
+            if (slice + 1u == slices && n < parts.slices) parts.sums[(at - slice + n) * 2 + 1] = kNoMore;
         }
-        const float by = parts.slices > 1 ? 1.f : total == 0.f ? 0.f : 1.f / total;
+        const float by = slices > 1 ? 1.f : total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
         for (int n = 0; n < NG; n++) {
             const float more = kv_column_sum(bias[m][n]) + ones[m][n];
@@ -461,8 +438,8 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
                 const uint32_t d = n * G + 16 * t + 4 * g;
                 kr_f32x4 v;
 #pragma unroll
-                for (int j = 0; j < 4; j++) v[j] = parts.slices == 1 && total == 0.f ? 0.f : (o[m][n][t][j] + more) * by;
-                if (parts.slices > 1) {
+                for (int j = 0; j < 4; j++) v[j] = slices == 1 && total == 0.f ? 0.f : (o[m][n][t][j] + more) * by;
+                if (slices > 1) {
                     *(kr_f32x4*)(parts.values + at * D + d) = v;
                 } else {
                     const uint64_t to = row_at[m] * a.out_stride + (uint64_t)qh[m] * D + d;

@@ -129,9 +129,8 @@ struct Options {
     int qmv_codes_nw = 0;         // its waves along N (0 = choose; 2..8),
     int qmv_codes_stage = 0;      // its steps of activations between barriers (0 = choose; 1, 2, 4),
     int qmv_codes_slices = 0;     // its slices of K (0 = choose; 1..16)
-    int kv_kernel = 0;            // attention over the 4-bit cache: 0 = choose, 1 = the kernel for few rows a sequence, 2 = the one for many
-    int kv_waves = 0;             // attention over the 4-bit cache: workgroups of 4 waves (1) or of as many as fit (2), 0 = choose
-    int kv_slices = 0;            // and slices of a sequence's tokens, 0 = choose
+    int kv_kernel = 0;            // attention over the 4-bit cache: 0 = choose, 1 = few rows a sequence, 2 = many, 3 = up to four, 4 = prompts
+    int kv_slices = 0;            // and slices that a sequence's tokens are cut into at most, 0 = choose
     int scratch_most_kb = 0;      // largest library-owned scratch buffer (0 = no limit): a call that needs more finds no memory
     int qmv_wide = 0;             // 16-row matrix-core GEMV for batches of 5..16 rows: 0 = choose per shape, 1 = never, 2 = wherever the shape allows
 };
@@ -368,12 +367,13 @@ struct KvAttentionArgs {
 };
 int launch_kv_append(int dtype, const KvAppendArgs& p, const LaunchCtx& lc);
 int launch_kv_read(int dtype, const KvReadArgs& p, const LaunchCtx& lc);
-// slices: parts of a sequence's tokens whose sums are joined through scratch (null: one). tiles: the kernel for many rows; else large: its
-// workgroups have as many waves as fit.
+// The kernel (1 few rows a sequence, 2 many, 3 up to four, 4 prompts); and how tokens are cut into slices whose sums are joined through scratch: `slices` of a sequence
+// or tile at most, `pieces` of all for a key head, of `least` blocks. `images` bytes of the scratch hold keys and values as kernel 4 takes them. Without scratch nothing is
+// cut, and kernel 2 is in 4's place.
 struct KvPlan {
-    bool tiles = false, large = false;
-    uint32_t slices = 1;
-    size_t scratch = 0;
+    int kernel = 1;
+    uint32_t slices = 1, pieces = 1, least = 1;
+    size_t images = 0, scratch = 0;
 };
 KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& p);
 int launch_kv_attention(int dtype, const KvAttentionArgs& p, const KvPlan& plan, void* scratch, const LaunchCtx& lc);

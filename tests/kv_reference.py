@@ -131,7 +131,7 @@ def spans(lens, offsets, max_len):
             yield i, offsets[i] + j, n - rows + j
 
 
-def attention(pool, q, offsets, hq, scale, window, dt):
+def attention(pool, q, offsets, hq, scale, window, dt, rounded=False):
     """(out, tolerance) f64[rows, hq, dim] of q[rows, hq, dim].
 
     Tolerance. A score is a sum of dim products of q and 16 + code, f32, scaled by group and joined with the bias' share: at most (dim + 24) roundings of 2^-24 of
@@ -139,6 +139,10 @@ def attention(pool, q, offsets, hq, scale, window, dt):
     argument of up to 2^4 in base 2 and its own error. p s is rounded by half a step of what it is held in (bf16 2^-8, 16 bits 2^-16, 24 bits 2^-23) and multiplies
     code - 8. Sums over n tokens are f32, one after the other within a lane of a matrix instruction's row and then over waves and slices: (n / 8 + 128) 2^-24 of the sum of
     magnitudes p (64 s + |v|). At the end half a step of T, and for f16 2^-25 below 2^-14.
+
+    `rounded`: keys, values and weights are in T (sequences of many rows, f16 and bf16). With u half a step of T a key is off by u |k|, a score by u scale sum |q| |k| and
+    a probability by e^(2 of the largest of these) - 1; p and v are off by u each, together less than 2.02 u of p |v|; and in f16 a key and a weight (of at least one that is 1)
+    below 2^-14 by 2^-25.
     """
     held = {DType.F32: 2.0 ** -23, DType.F16: 2.0 ** -16, DType.BF16: 2.0 ** -8}[dt]
     shared = hq // pool.hkv
@@ -164,9 +168,12 @@ def attention(pool, q, offsets, hq, scale, window, dt):
                 step_k, step_v = (_steps(pool, part, seq, h // shared, at) for part in (0, 1))
                 size = abs(scale) * ((48 * step_k + np.abs(kk)) @ np.abs(x))
                 rel = 2 * (pool.dim + 24) * 2.0 ** -24 * size.max() + 2.0 ** -19
+                if rounded:
+                    u, least = HALF_STEP[dt], 2.0 ** -25 if dt == DType.F16 else 0.0
+                    rel = np.expm1(rel + 2 * (abs(scale) * ((u * np.abs(kk) + least) @ np.abs(x))).max())
                 terms = p @ (64 * step_v + np.abs(vv))
                 out[row, h] = o
-                tol[row, h] = rel * (p @ np.abs(vv) + np.abs(o)) + held * (p @ np.abs(vc[h // shared][at])) + (at.size / 8 + 128) * 2.0 ** -24 * terms \
+                tol[row, h] = rel * (p @ np.abs(vv) + np.abs(o)) + (2.02 * u * (p @ np.abs(vv)) + at.size * least * (1 + np.abs(vv).max(0)) if rounded else held * (p @ np.abs(vc[h // shared][at]))) + (at.size / 8 + 128) * 2.0 ** -24 * terms \
                     + HALF_STEP[dt] * np.abs(o) + (2.0 ** -25 if dt == DType.F16 else 0)
     return out, tol
 

@@ -42,9 +42,13 @@ class Attention:
         assert np.all(rest == 0xA5)   # between rows and outside all sequences
         return unpack_f32(raw[:, :wide].tobytes(), self.dt).reshape(self.tokens, self.hq, self.dim)
 
-    def hold(self):
+    def rounded(self, kernel=0):
+        """Whether keys and values are rounded to T: in the kernel for prompts, of 16-bit types."""
+        return self.dt != DType.F32 and (kernel == 4 or kernel == 0 and self.tokens * (self.hq // self.pool.hkv) > 128 * len(self.pool.lens))
+
+    def hold(self, kernel=0):
         got = self.result()[self.offsets[0]:self.offsets[-1]]
-        want, tol = (x[self.offsets[0]:self.offsets[-1]] for x in ref.attention(self.pool, self.q, self.offsets, self.hq, self.scale, self.window, self.dt))
+        want, tol = (x[self.offsets[0]:self.offsets[-1]] for x in ref.attention(self.pool, self.q, self.offsets, self.hq, self.scale, self.window, self.dt, self.rounded(kernel)))
         assert np.array_equal(np.isnan(got), np.isnan(want))
         fine = ~np.isnan(want)
         far = np.abs(got - want)[fine] / np.maximum(tol[fine], 1e-30)
@@ -88,15 +92,15 @@ def option():
 @pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
 @pytest.mark.parametrize("lens,rows,more", CASES, ids=lambda v: str(v).replace(" ", "")[:40])
 def test_either_kernel(dt, lens, rows, more, option):
-    """Whatever the sizes: the kernel for few rows with small and large workgroups, the one for many, in one slice and in several."""
-    print(f"[case] kv_attention {dt.name} {str(lens)[:40]} {str(rows)[:40]} {more}, both kernels", flush=True)
+    """Whatever the sizes: the kernel for few rows, the ones for many, the one for up to four, in one slice and in several."""
+    print(f"[case] kv_attention {dt.name} {str(lens)[:40]} {str(rows)[:40]} {more}, all kernels", flush=True)
     c = Attention(dt, lens, rows, **more)
-    for kernel, waves, slices in ((1, 1, 1), (1, 2, 1), (1, 1, 3), (2, 0, 1), (2, 0, 5)):
-        for name, value in (("kv.kernel", kernel), ("kv.waves", waves), ("kv.slices", slices)):
-            option(name, value)
+    for kernel, slices in ((1, 1), (1, 3), (2, 1), (2, 5), (3, 1), (3, 4), (4, 1), (4, 3)):
+        option("kv.kernel", kernel)
+        option("kv.slices", slices)
         c.out.upload(b"\xa5" * c.out.nbytes)
         c.call()
-        c.hold()
+        c.hold(kernel)
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
@@ -109,22 +113,23 @@ def test_every_head(dt, dim, group):
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
-@pytest.mark.parametrize("rows", [[1, 1], [200, 40]], ids=str)
-def test_pages_that_are_none(dt, rows):
+@pytest.mark.parametrize("rows,kernel", [([1, 1], 0), ([200, 40], 0), ([200, 40], 4)], ids=str)
+def test_pages_that_are_none(dt, rows, kernel, option):
     """Tokens on no page do not count; a sequence that is on none is zeros."""
     c = Attention(dt, [220, 40], rows)
     c.pool.pages[0, [0, 3, 4, 9]], c.pool.pages[1] = c.pool.n_pages, ref.NO_PAGE
     c.pool.pb.upload(c.pool.pages.astype("<u4").tobytes())
+    option("kv.kernel", kernel)
     c.call()
-    c.hold()
+    c.hold(kernel)
     assert np.all(c.result()[c.offsets[1]:] == 0)
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
-@pytest.mark.parametrize("rows", [[3, 1], [130, 40]], ids=str)
+@pytest.mark.parametrize("rows,kernel", [([3, 1], 0), ([3, 1], 1), ([130, 40], 0), ([130, 40], 4)], ids=str)
 @pytest.mark.parametrize("what", ["q", "k_scale", "k_bias", "v_scale", "v_bias"])
 @pytest.mark.parametrize("window", [0, 20])
-def test_no_numbers(dt, rows, what, window):
+def test_no_numbers(dt, rows, kernel, what, window, option):
     """A NaN reaches the rows that see it, and of a value's only its group; none of the others."""
     c = Attention(dt, [140, 40], rows, window=window, dim=128, group=64)
     pool = c.pool
@@ -138,16 +143,18 @@ def test_no_numbers(dt, rows, what, window):
         for i, (codes, scales, biases) in enumerate(pool.parts):
             pool.bufs[3 * i + 1].upload(pack_f32(scales, dt))
             pool.bufs[3 * i + 2].upload(pack_f32(biases, dt))
+    option("kv.kernel", kernel)
     c.call()
-    c.hold()
+    c.hold(kernel)
     got = c.result()
     assert np.isnan(got).any() and not np.isnan(got).all()
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=lambda d: d.name)
-@pytest.mark.parametrize("rows", [[1], [100]], ids=str)
-def test_scores_far_apart(dt, rows):
+@pytest.mark.parametrize("rows,kernel", [([1], 0), ([1], 1), ([100], 0), ([100], 4)], ids=str)
+def test_scores_far_apart(dt, rows, kernel, option):
     """Scores of thousands: one token takes it all, wherever it is, and nothing passes the exponent."""
+    option("kv.kernel", kernel)
     for place in (0, 31, 32, 170):
         c = Attention(dt, [200], rows, hq=2, hkv=1, scale=1.0, seed=place + 2)
         codes, scales, biases = c.pool.parts[0]
@@ -196,9 +203,10 @@ def test_the_same_bits_again():
             assert c.out.read_bytes() == first
 
 
-@pytest.mark.parametrize("rows", [[1, 1, 1], [40, 1, 60]], ids=str)
-def test_captured(rows):
+@pytest.mark.parametrize("rows,kernel", [([1, 1, 1], 0), ([40, 1, 60], 0), ([40, 1, 60], 4)], ids=str)
+def test_captured(rows, kernel, option):
     """A captured call follows lens, pages and queries as they are when it is replayed, other calls with the same scratch between."""
+    option("kv.kernel", kernel)
     c = Attention(DType.BF16, [200, 90, 300], rows, hq=8, hkv=2, width=32)
     other = Attention(DType.F16, [1200], [1], hq=16, hkv=2, seed=9)
     other.call()
@@ -213,11 +221,11 @@ def test_captured(rows):
             c.qb.upload(pack_f32(c.q, c.dt))
             c.out.upload(b"\xa5" * c.out.nbytes)
             g.replay()
-            c.hold()
+            c.hold(kernel)
             got = c.out.read_bytes()
             other.out.upload(b"\xa5" * other.out.nbytes)
             other.call()
-            other.hold()
+            other.hold(kernel)
             c.call()
             ops.sync()
             assert c.out.read_bytes() == got
