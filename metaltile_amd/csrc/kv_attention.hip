@@ -6,18 +6,67 @@ namespace mtq {
 namespace {
 
 // A wave for each row and query head: its slices joined.
-// W waves to a row of a head, D / 4 lanes to a slice's numbers. The slices' loads go out together: with a branch on a slice's sum between them, 32 slices took 15 us.
-template <int DT, int D, int W> __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a, KvParts parts) {
-    constexpr uint32_t LANES = D / 4, TURNS = 64 * W / LANES;
-    __shared__ kr_f32x4 others[4 / W][W > 1 ? TURNS : 1][LANES + 1];   // (values; sum)
-    const uint32_t lane = threadIdx.x & 63u, in_block = threadIdx.x / (64 * W), at = blockIdx.x * (4 / W) + in_block, row = at / a.hq, h = at - row * a.hq;
-    KvSeq s;
-    bool yes = row < a.kv.n_tokens;
-    if (yes) yes = kv_seq_of(a.kv, row, s);
-    const uint32_t unit = threadIdx.x % (64 * W), turn = unit / LANES, d = unit % LANES * 4;
+// Rows outside all sequences are left alone.
+__device__ __forceinline__ bool kv_of_some_sequence(const KvArgs& kv, uint32_t row) {
+    return row < kv.n_tokens && (!kv.offsets || (row >= kv.offsets[0] && row < kv.offsets[kv.n_seqs]));
+}
+
+// Up to eight slices: sixteen lanes to a row of a head, so four of them to a wave (60000 rows of 64 values in up to three slices: 21 us with a wave each, most of it
+// latency). All loads of a row's values go out together.
+constexpr uint32_t kJoinMost = 8;
+template <int DT, int D> __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a, KvParts parts) {
+    const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, at = blockIdx.x * 16u + threadIdx.x / 16u, row = at / a.hq, h = at - row * a.hq;
+    const bool in = row < a.kv.n_tokens;
+    const float* sums = parts.sums + (uint64_t)(in ? at : 0u) * parts.slices * 2;
+    const float bar = l < parts.slices ? sums[2 * l] : -INFINITY, part = l < parts.slices ? sums[2 * l + 1] : 0.f;
+    const uint32_t end = (uint32_t)(__ballot(part == kNoMore) >> (lane & 48u)) & 0xFFFFu, n = end ? (uint32_t)__builtin_ctz(end) : parts.slices;
+    float top = l < n ? bar : -INFINITY;
+#pragma unroll
+    for (int i = 1; i < 16; i <<= 1) top = fmaxf(top, __shfl_xor(top, i, 64));
+    const float f = l >= n ? 0.f : bar == -INFINITY ? (part == 0.f ? 0.f : 1.f) : exp2f(bar - top);
+    const bool none = l >= n || (f == 0.f && part == 0.f);   // (its values are nothing, or not there)
+    float total = none ? 0.f : part * f;
+#pragma unroll
+    for (int i = 1; i < 16; i <<= 1) total += __shfl_xor(total, i, 64);
+    const uint32_t there = (uint32_t)(__ballot(!none) >> (lane & 48u)) & 0xFFFFu;
+    if (n == 0 || !kv_of_some_sequence(a.kv, row)) return;   // (of one slice: written already)
+    const float* values = parts.values + (uint64_t)at * parts.slices * D + 4 * l;
+    kr_f32x4 v[D / 64] = {};
+#pragma unroll
+    for (uint32_t i0 = 0; i0 < kJoinMost; i0 += 4) {
+        if (i0 >= n) break;
+        kr_f32x4 x[4][D / 64];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < D / 64; j++) x[i][j] = *(const kr_f32x4*)(values + (uint64_t)(i0 + i < n ? i0 + i : n - 1u) * D + 64 * j);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const float by = __shfl(f, (int)((lane & 48u) + i0 + i), 64);
+            if (there >> (i0 + i) & 1u) {
+#pragma unroll
+                for (int j = 0; j < D / 64; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[j][e] = fmaf(x[i][j][e], by, v[j][e]);
+            }
+        }
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int j = 0; j < D / 64; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) store_elem<DT>(a.out, (uint64_t)row * a.out_stride + (uint64_t)h * D + 64 * j + 4 * l + e, total == 0.f ? 0.f : v[j][e] * inv);
+}
+
+// More of them: a workgroup to a row of a head, D / 4 lanes to a slice's numbers. The slices' loads go out together: with a branch on a slice's sum between them,
+// 32 slices took 15 us.
+template <int DT, int D> __global__ __launch_bounds__(256) void kv_join_many_kernel(KvAttentionArgs a, KvParts parts) {
+    constexpr uint32_t LANES = D / 4, TURNS = 256 / LANES;
+    __shared__ kr_f32x4 others[TURNS][LANES + 1];   // (values; sum)
+    const uint32_t lane = threadIdx.x & 63u, at = blockIdx.x, row = at / a.hq, h = at - row * a.hq, turn = threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
     const float* sums = parts.sums + (uint64_t)at * parts.slices * 2;
     const float* values = parts.values + (uint64_t)at * parts.slices * D + d;
-    uint32_t n = yes ? parts.slices : 0u;
+    uint32_t n = parts.slices;
     float top = -INFINITY;
     for (uint32_t i = lane; i - lane < n; i += 64) {
         const float bar = i < n ? sums[2 * i] : -INFINITY, part = i < n ? sums[2 * i + 1] : 0.f;
@@ -25,8 +74,7 @@ template <int DT, int D, int W> __global__ __launch_bounds__(256) void kv_join_k
         if (no_more) n = i - lane + (uint32_t)__builtin_ctzll(no_more);
         if (i < n) top = fmaxf(top, bar);
     }
-    if (n == 0) yes = false;   // (of one slice: written already)
-    if (W == 1 && !yes) return;
+    if (n == 0 || !kv_of_some_sequence(a.kv, row)) return;   // (of one slice: written already)
     for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i, 64));
     float total = 0.f;
     kr_f32x4 v = {0.f, 0.f, 0.f, 0.f};
@@ -34,29 +82,19 @@ template <int DT, int D, int W> __global__ __launch_bounds__(256) void kv_join_k
     for (uint32_t i = turn; i < n; i += TURNS) {
         const float bar = sums[2 * i], part = sums[2 * i + 1], f = bar == -INFINITY ? (part == 0.f ? 0.f : 1.f) : exp2f(bar - top);
         const kr_f32x4 x = *(const kr_f32x4*)(values + (uint64_t)i * D);
-        const bool none = f == 0.f && part == 0.f;   // (values that no one wrote)
+        const bool none = f == 0.f && part == 0.f;   // (its values are nothing, or not there)
         total = fmaf(part, f, total);
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = none ? v[j] : fmaf(x[j], f, v[j]);
     }
-    if (W == 1) {
+    others[turn][d / 4] = v;
+    if (d == 0) others[turn][LANES][0] = total;
+    __syncthreads();
+    if (turn) return;
 #pragma unroll
-        for (uint32_t i = LANES; i < 64; i <<= 1) {
-            total += __shfl_xor(total, i, 64);
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] += __shfl_xor(v[j], i, 64);
-        }
-        if (turn) return;
-    } else {
-        others[0][turn][d / 4] = v;
-        if (d == 0) others[0][turn][LANES][0] = total;
-        __syncthreads();
-        if (turn || !yes) return;
-#pragma unroll
-        for (uint32_t i = 1; i < TURNS; i++) {
-            total += others[0][i][LANES][0];
-            v += others[0][i][d / 4];
-        }
+    for (uint32_t i = 1; i < TURNS; i++) {
+        total += others[i][LANES][0];
+        v += others[i][d / 4];
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) store_elem<DT>(a.out, (uint64_t)row * a.out_stride + (uint64_t)h * D + d + j, total == 0.f ? 0.f : v[j] / total);
@@ -67,17 +105,16 @@ template <int DT, int D, int W> __global__ __launch_bounds__(256) void kv_join_k
 int launch_kv_join(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc) {
     KvAttentionArgs a = p;
     KvParts q = parts;
-#define MTQ_KV_JOIN(DT) \
-    {{(const void*)kv_join_kernel<DT, 64, 1>, (const void*)kv_join_kernel<DT, 64, 4>}, \
-     {(const void*)kv_join_kernel<DT, 128, 1>, (const void*)kv_join_kernel<DT, 128, 4>}, \
-     {(const void*)kv_join_kernel<DT, 256, 1>, (const void*)kv_join_kernel<DT, 256, 4>}}
-    const void* fn[3][3][2] = {MTQ_KV_JOIN(DT_F32), MTQ_KV_JOIN(DT_F16), MTQ_KV_JOIN(DT_BF16)};
+#define MTQ_KV_JOIN(DT, D) {(const void*)kv_join_kernel<DT, D>, (const void*)kv_join_many_kernel<DT, D>}
+#define MTQ_KV_JOINS(DT) {MTQ_KV_JOIN(DT, 64), MTQ_KV_JOIN(DT, 128), MTQ_KV_JOIN(DT, 256)}
+    const void* fn[3][3][2] = {MTQ_KV_JOINS(DT_F32), MTQ_KV_JOINS(DT_F16), MTQ_KV_JOINS(DT_BF16)};
 #undef MTQ_KV_JOIN
-    const bool wide = parts.slices > 8;
-    const uint64_t groups = wide ? (uint64_t)a.kv.n_tokens * a.hq : ((uint64_t)a.kv.n_tokens * a.hq + 3) / 4;
+#undef MTQ_KV_JOINS
+    const bool many = parts.slices > kJoinMost;
+    const uint64_t rows = (uint64_t)a.kv.n_tokens * a.hq, groups = many ? rows : (rows + 15) / 16;
     if (groups > max_workgroups(256)) return fail(ERR_SHAPE, "more rows and heads than a launch can have workgroups");
     void* args[] = {&a, &q};
-    MTQ_HIP(launch_kernel(fn[dtype][a.kv.dim == 64 ? 0 : a.kv.dim == 128 ? 1 : 2][wide], dim3((uint32_t)groups), dim3(256), args, 0, lc));
+    MTQ_HIP(launch_kernel(fn[dtype][a.kv.dim == 64 ? 0 : a.kv.dim == 128 ? 1 : 2][many], dim3((uint32_t)groups), dim3(256), args, 0, lc));
     return ERR_OK;
 }
 
@@ -91,7 +128,8 @@ static uint32_t num_cus() {
 }
 
 // Rows are new tokens times the query heads that share a key head, for each sequence on average:
-//   to 4     the kernel with a token to a lane (64 sequences of 4096 tokens, 4 rows, bf16: 63 us against 69 of the one below; 256 of them 220 / 240)
+//   to 4     the kernel with a token to a lane, where heads have 128 values or more and there is work for the card (64 sequences of 4096 tokens, 4 rows, bf16: 70 us
+//            against 74 of the one below, f16 70 / 85, in groups of 32 80 / 108, 256 values 123 / 132; 64 values 67 / 50, one sequence of 1000 tokens 13.4 / 12.1)
 //   to 128   the one with 16 rows to a wave (32 sequences of 4096 tokens, 128 rows: 264 us against 360 of the one below, 4 of 2048 tokens 62 / 41; 64 rows 147 / 366 and
 //            35 / 34); f32 to 32
 //   above    f16 and bf16: keys and values laid out in T first (256 rows: 494 / 372 and 115 / 45; a prompt of 8192 tokens 559 us against 942 of the next). It has to have
@@ -103,8 +141,10 @@ KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
     const uint32_t span = a.window && a.window < a.kv.max_len ? a.window : a.kv.max_len;   // tokens that a row sees at most
     const uint64_t images = ((uint64_t)a.kv.max_len + kBlock - 1) / kBlock * n_seqs * a.kv.hkv * (128ull * a.kv.dim + 4);
     const bool prompts = dtype != DT_F32 && images && images <= (1ull << 30);
-    p.kernel = options().kv_kernel ? options().kv_kernel : rows <= 4 * n_seqs ? 3 : rows > 128 * n_seqs && prompts ? 4 : rows > (dtype == DT_F32 ? 32 : 128) * n_seqs ? 2 : 1;
+    const bool few = a.kv.dim >= 128 && n_seqs * a.kv.hkv * span >= 2048 * cus;
+    p.kernel = options().kv_kernel ? options().kv_kernel : few && rows <= 4 * n_seqs ? 3 : rows > 128 * n_seqs && prompts ? 4 : rows > (dtype == DT_F32 ? 32 : 128) * n_seqs ? 2 : 1;
     if (p.kernel == 4 && !prompts) p.kernel = 2;
+    if (p.kernel == 3 && a.kv.dim < 128) p.kernel = 1;
     if (p.kernel == 4) p.images = (size_t)((images + 255) / 256 * 256);
     uint64_t slices, pieces;
     if (p.kernel == 2 || p.kernel == 4) {

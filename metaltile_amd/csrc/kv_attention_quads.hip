@@ -42,7 +42,6 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
     using T = KvTerms<DT>;
     constexpr int QS = 1, NW = 4, NG = L::NG, ES = L::ES, WORDS = D / 8, ROWS = L::ROWS;
     constexpr int PASSES = D == 256 ? 2 : 1;             // of 128 numbers' words over sixteen lanes
-    constexpr int EACH = D == 64 ? 4 : 8;                // numbers of a lane's word in a pass (of 64 numbers two lanes share a word)
     constexpr int GROUPS = NG / PASSES;                  // of a pass
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const KvArgs& kv = a.kv;
@@ -95,7 +94,7 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
 #pragma unroll
             for (int u = 0; u < D / 32; u++) {    // 64 pieces in turn: by token (those of a quad turned by their sixteen), then piece
                 const uint32_t p = u * 64 + lane, row = p / PIECES, x = row / 16, piece = part ? p % PIECES : p % PIECES ^ (row * PIECES / 16) % PIECES;
-                const uint32_t at = D == 64 ? (x & 1u ? slot[2 * u + 1] : slot[2 * u]) : slot[u * 64 / (16 * PIECES)];
+                const uint32_t at = slot[u * 64 / (16 * PIECES)];
                 kv_load16(__builtin_amdgcn_readfirstlane(to + u * 1024), codes + (uint64_t)(at + (row % 16 ^ x)) * (D / 2) + piece * 16);
             }
 #pragma unroll
@@ -165,7 +164,7 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
             }
         }
 
-        kr_f32x4 o[QS][PASSES][EACH] = {}, ones[QS][PASSES] = {};   // values of a lane's word, rows r; -24 sum p s of its group
+        kr_f32x4 o[QS][PASSES][8] = {}, ones[QS][PASSES] = {};   // values of a lane's word, rows r; -24 sum p s of its group
         float bias[ROWS][NG] = {}, sum[ROWS] = {}, bar[ROWS];       // (a lane's tokens')
 #pragma unroll
         for (int i = 0; i < ROWS; i++) bar[i] = -INFINITY;
@@ -256,7 +255,7 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
                     for (int p = 0; p < PASSES; p++) {
                         ones[i / 4][p][i % 4] *= keep;
 #pragma unroll
-                        for (int e = 0; e < EACH; e++) o[i / 4][p][e][i % 4] *= keep;
+                        for (int e = 0; e < 8; e++) o[i / 4][p][e][i % 4] *= keep;
                     }
                     bar[i] = to;
                 }
@@ -278,7 +277,7 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
                 for (int k = 0; k < 4; k++)
 #pragma unroll
                     for (int t = 0; t < 4; t++)
-                        w[p][k][t] = *(const uint32_t*)(vt + (16 * sixteen + 4 * ((block4 - k) & 3u) + (t ^ sixteen)) * (D / 2) + (p * 16 + lane % (D == 64 ? 8 : 16)) * 4);
+                        w[p][k][t] = *(const uint32_t*)(vt + (16 * sixteen + 4 * ((block4 - k) & 3u) + (t ^ sixteen)) * (D / 2) + (p * 16 + lane % 16) * 4);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (b + 1u < b1) issue(b + 1u, 1);
             float ps[ROWS][NG];
@@ -306,9 +305,7 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
                     kr_u32x2 at[4][T::P];
                     kr_for<0, GROUPS>([&](auto group) {
                         constexpr int n = decltype(group)::value;
-                        constexpr int BLOCKS = D == 64 ? 2 : 4;   // of different words among four
-                        constexpr int MASK = (0 % BLOCKS * GROUPS / BLOCKS == n ? 1 : 0) | (1 % BLOCKS * GROUPS / BLOCKS == n ? 2 : 0) | (2 % BLOCKS * GROUPS / BLOCKS == n ? 4 : 0) |
-                                             (3 % BLOCKS * GROUPS / BLOCKS == n ? 8 : 0);   // those of this group's words
+                        constexpr int MASK = (0 == n ? 1 : 0) | (GROUPS / 4 == n ? 2 : 0) | (2 * GROUPS / 4 == n ? 4 : 0) | (3 * GROUPS / 4 == n ? 8 : 0);   // blocks of this group's words
                         float t[4][T::P];
 #pragma unroll
                         for (int r = 0; r < 4; r++) kv_split(ps[4 * m + r][p * GROUPS + n], t[r]);
@@ -337,13 +334,10 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
                     for (int k = 0; k < 4; k++) {
 #pragma unroll
                         for (int e = T::P - 1; e >= 0; e--) ones[m][p] = kq_mfma<DT_BF16, 0, 0>(at[k][e], less24, ones[m][p]);
-                        uint32_t wk[4];
 #pragma unroll
-                        for (int t = 0; t < 4; t++) wk[t] = D == 64 && block4 >= 2 ? w[p][k][t] >> 16 : w[p][k][t];
-#pragma unroll
-                        for (int i = 0; i < EACH; i += 2) {
+                        for (int i = 0; i < 8; i += 2) {
                             const uint32_t sel = 0x0C000C00u | (uint32_t)(4 + i / 2) << 16 | (uint32_t)(i / 2);
-                            const uint32_t y0 = __builtin_amdgcn_perm(wk[1], wk[0], sel), y1 = __builtin_amdgcn_perm(wk[3], wk[2], sel);
+                            const uint32_t y0 = __builtin_amdgcn_perm(w[p][k][1], w[p][k][0], sel), y1 = __builtin_amdgcn_perm(w[p][k][3], w[p][k][2], sel);
                             const kr_u32x2 even = {((y0 << 3) & 0x00780078u) | v16, ((y1 << 3) & 0x00780078u) | v16};
                             const kr_u32x2 odd = {((y0 >> 1) & 0x00780078u) | v16, ((y1 >> 1) & 0x00780078u) | v16};
 #pragma unroll
@@ -369,11 +363,11 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
                 const float less = kv_column_sum(ones[i / 4][p][i % 4]);
                 float mine_more = more[p * GROUPS];
 #pragma unroll
-                for (int n = 1; n < GROUPS; n++) mine_more = block4 % (D == 64 ? 2 : 4) * GROUPS / (D == 64 ? 2 : 4) == (uint32_t)n ? more[p * GROUPS + n] : mine_more;
+                for (int n = 1; n < GROUPS; n++) mine_more = block4 * GROUPS / 4 == (uint32_t)n ? more[p * GROUPS + n] : mine_more;
 #pragma unroll
-                for (int e = 0; e < EACH; e++) {
+                for (int e = 0; e < 8; e++) {
                     const float v = kv_column_sum(o[i / 4][p][e][i % 4]) + less + mine_more;
-                    if (sixteen == 0) join[i * (D + 4) + (p * 16 + lane % (D == 64 ? 8 : 16)) * 8 + (D == 64 ? block4 / 2 * 4 : 0) + e] = v;
+                    if (sixteen == 0) join[i * (D + 4) + (p * 16 + lane % 16) * 8 + e] = v;
                 }
             }
             if (lane == 0) {
@@ -435,8 +429,6 @@ template <int DT, int D, int G> int launch(const KvAttentionArgs& p, KvParts par
 
 template <int DT> int launch_of(const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc) {
     switch (p.kv.dim * 1000 + p.kv.group) {
-        case 64032: return launch<DT, 64, 32>(p, parts, lc);
-        case 64064: return launch<DT, 64, 64>(p, parts, lc);
         case 128032: return launch<DT, 128, 32>(p, parts, lc);
         case 128064: return launch<DT, 128, 64>(p, parts, lc);
         case 128128: return launch<DT, 128, 128>(p, parts, lc);

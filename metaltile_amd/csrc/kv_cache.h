@@ -47,24 +47,5 @@ __device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, uint32_t i) {
     s.len = len < a.max_len ? len : a.max_len;
     return s;
 }
-// The sequence that row t of the call belongs to; false: none. All lanes of a wave call, with the same t.
-__device__ __forceinline__ bool kv_seq_of(const KvArgs& a, uint32_t t, KvSeq& s) {
-    uint32_t i;
-    if (a.offsets) {
-        const uint32_t c = __builtin_amdgcn_readfirstlane(kv_count_upto(a.offsets, a.n_seqs + 1u, t));
-        if (c == 0 || c > a.n_seqs) return false;
-        i = c - 1u;
-    } else {
-        i = t / (a.n_tokens / a.n_seqs);
-    }
-    s = kv_seq(a, i);
-    return t >= s.first_row && t - s.first_row < s.rows;
-}
-// The index [page, head, place] of a token of a sequence, or -1: on no page.
-__device__ __forceinline__ int64_t kv_slot(const KvArgs& a, uint32_t seq, uint32_t head, uint32_t place) {
-    const uint32_t page = a.pages[(uint64_t)seq * a.pages_stride + (place >> a.page_log2)];
-    if (page >= a.n_pages) return -1;
-    return (int64_t)((((uint64_t)page * a.hkv + head) << a.page_log2) + (place & ((1u << a.page_log2) - 1u)));
-}
 
 }  // namespace mtq
