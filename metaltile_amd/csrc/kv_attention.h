@@ -87,6 +87,17 @@ struct KvParts {
 constexpr float kNoMore = -1.f;
 constexpr uint32_t kCutSeqs = 512;   // sequences that are cut into pieces at most: each workgroup looks at all of them
 
+// The sum of this lane's value and those of the lanes below.
+__device__ __forceinline__ uint32_t kv_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);   // (1, 2, 4 and 8 lanes below in the sixteen; nothing where there are none)
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);   // (the last of the sixteen below, then of the half)
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
 // Workgroup `index` of a key head's: a sequence, and one of the equal slices that its tokens are cut into. Lengths are known here only, and sequences of
 // 1 to 8192 tokens, each cut into as many, left the card with the longest one's slices: so a piece is a share of all tokens, and a sequence has as many as its
 // tokens need. False: no piece. All lanes of a wave call.
@@ -94,65 +105,58 @@ struct KvPiece {
     KvSeq s;
     uint32_t slice = 0, slices = 1;
 };
-__device__ __forceinline__ bool kv_piece(const KvAttentionArgs& a, const KvParts& parts, uint32_t index, KvPiece& p) {
+template <uint32_t EACH> __device__ __forceinline__ bool kv_piece_of(const KvAttentionArgs& a, const KvParts& parts, uint32_t index, KvPiece& p) {   // EACH sequences to a lane
     const KvArgs& kv = a.kv;
-    if (parts.slices == 1) {
-        p.s = kv_seq(kv, index);
-        return p.s.rows != 0;
-    }
-    constexpr uint32_t MOST = kCutSeqs / 64;
-    const uint32_t lane = threadIdx.x & 63u, each = (kv.n_seqs + 63u) / 64u;   // sequences of a lane
-    uint32_t n[MOST], all = 0;                                                 // their blocks of 64 tokens
+    const uint32_t lane = threadIdx.x & 63u, each = EACH == 1 ? 1u : (kv.n_seqs + 63u) / 64u;
+    KvSeq s[EACH];
+    uint32_t n[EACH], all = 0;   // their blocks of 64 tokens
 #pragma unroll
-    for (uint32_t j = 0; j < MOST; j++) {
-        n[j] = 0xFFFFFFFFu;   // no rows
+    for (uint32_t j = 0; j < EACH; j++) {
         const uint32_t i = lane * each + j;
-        if (j < each && i < kv.n_seqs) {
-            const KvSeq s = kv_seq(kv, i);
-            if (s.rows) {
-                const int32_t end = (int32_t)(s.len + 1u) - (int32_t)s.rows;   // of the first row
-                const uint32_t from = a.window && end > (int32_t)a.window ? (uint32_t)end - a.window : 0u;
-                n[j] = (s.len - from + 63u) / 64u;
-                all += n[j];
-            }
-        }
+        s[j] = KvSeq{0, 0, 0, 0};
+        if (j < each && i < kv.n_seqs) s[j] = kv_seq(kv, i);
+        const int32_t end = (int32_t)(s[j].len + 1u) - (int32_t)s[j].rows;   // of the first row
+        const uint32_t from = a.window && end > (int32_t)a.window ? (uint32_t)end - a.window : 0u;
+        n[j] = s[j].rows ? (s[j].len - from + 63u) / 64u : 0u;
+        all += n[j];
     }
-    for (int i = 1; i < 64; i <<= 1) all += (uint32_t)__shfl_xor((int)all, i, 64);
-    uint32_t share = (all + parts.pieces - 1u) / parts.pieces;
+    uint32_t share = ((uint32_t)__builtin_amdgcn_readlane((int)kv_scan(all), 63) + parts.pieces - 1u) / parts.pieces;
     if (share < parts.least) share = parts.least;
     uint32_t mine = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < MOST; j++)
-        if (j < each) {
-            n[j] = n[j] == 0xFFFFFFFFu ? 0u : n[j] <= share ? 1u : (n[j] + share - 1u) / share;
-            if (n[j] > parts.slices) n[j] = parts.slices;
-            mine += n[j];
-        }
-    uint32_t upto = mine;
-    for (int i = 1; i < 64; i <<= 1) {
-        const uint32_t other = (uint32_t)__shfl_up((int)upto, i, 64);
-        if (lane >= (uint32_t)i) upto += other;
+    for (uint32_t j = 0; j < EACH; j++) {
+        n[j] = s[j].rows == 0 ? 0u : n[j] <= share ? 1u : (n[j] + share - 1u) / share;
+        if (n[j] > parts.slices) n[j] = parts.slices;
+        mine += n[j];
     }
+    const uint32_t upto = kv_scan(mine);
     const uint64_t above = __ballot(upto > index);
     if (!above) return false;
-    const uint32_t who = (uint32_t)__builtin_ctzll(above);
-    uint32_t rest = index - (upto - mine), at = 0, slices = 1;   // (this lane's answer; `who` has the one that counts)
-    bool found = false;
+    const int who = __builtin_ctzll(above);
+    uint32_t rest = index - (upto - mine), slices = 1;   // (this lane's answer; `who` has the one that counts)
+    KvSeq found = s[0];
+    bool yes = false;
 #pragma unroll
-    for (uint32_t j = 0; j < MOST; j++)
-        if (j < each && !found) {
+    for (uint32_t j = 0; j < EACH; j++)
+        if (!yes) {
             if (rest < n[j]) {
-                found = true;
-                at = lane * each + j;
+                yes = true;
+                found = s[j];
                 slices = n[j];
             } else {
                 rest -= n[j];
             }
         }
-    p.slice = (uint32_t)__builtin_amdgcn_readlane((int)rest, (int)who);
-    p.slices = (uint32_t)__builtin_amdgcn_readlane((int)slices, (int)who);
-    p.s = kv_seq(kv, (uint32_t)__builtin_amdgcn_readlane((int)at, (int)who));
+    auto his = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, who); };
+    p.s = KvSeq{his(found.seq), his(found.first_row), his(found.rows), his(found.len)};
+    p.slice = his(rest);
+    p.slices = his(slices);
     return true;
+}
+__device__ __forceinline__ bool kv_piece(const KvAttentionArgs& a, const KvParts& parts, uint32_t index, KvPiece& p) {
+    if (parts.slices > 1) return a.kv.n_seqs <= 64 ? kv_piece_of<1>(a, parts, index, p) : kv_piece_of<kCutSeqs / 64>(a, parts, index, p);
+    p.s = kv_seq(a.kv, index);
+    return p.s.rows != 0;
 }
 
 constexpr uint32_t kBlock = 32;   // tokens of a step of the kernels for many rows
