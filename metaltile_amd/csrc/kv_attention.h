@@ -24,6 +24,7 @@ template <int DT> struct KvTerms {
     static constexpr int Q = DT == DT_F32 ? 3 : 1;                          // terms of a query
     static constexpr int P = DT == DT_F32 ? 3 : DT == DT_F16 ? 2 : 1;       // bf16 terms of p s
     static constexpr int QK = DT == DT_F16 ? DT_F16 : DT_BF16;              // the scores' operands
+    static constexpr bool CENTRED = DT == DT_F32;                           // operands are c - 8, not 16 + c
 };
 
 // Nibbles `p` and p + 4 of a word as 16 + c, in the lower and the upper half. `base` is 16 twice, in a vector register (one mask and OR then).
@@ -35,6 +36,13 @@ template <int QK> __device__ __forceinline__ uint32_t kv_sixteen() {
 template <int QK> __device__ __forceinline__ uint32_t kv_pair(uint32_t w, int p, uint32_t base) {
     const int up = (QK == DT_BF16 ? 3 : 6) - 4 * p;
     return ((up >= 0 ? w << up : w >> -up) & (QK == DT_BF16 ? 0x00780078u : 0x03C003C0u)) | base;
+}
+
+// f32 takes c - 8: of 16 + c the sums are four times as large, and what they lose by it was most of its error (of 1000 tokens 2.6e-6 of the result).
+template <int DT> __device__ __forceinline__ uint32_t kv_operand(uint32_t pair) {
+    if constexpr (!KvTerms<DT>::CENTRED) return pair;
+    const float low = __uint_as_float(pair << 16) - 24.f, high = __uint_as_float(pair & 0xFFFF0000u) - 24.f;
+    return __builtin_amdgcn_perm(__float_as_uint(high), __float_as_uint(low), 0x07060302u);   // (exact in bf16)
 }
 
 // An f32 value in bf16 terms.

@@ -212,7 +212,8 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
                     constexpr int W = decltype(word)::value;
                     const uint4& four = kw[W / 4];
                     const uint32_t w = W % 4 == 0 ? four.x : W % 4 == 1 ? four.y : W % 4 == 2 ? four.z : four.w;
-                    const kr_u32x2 first = {kv_pair<T::QK>(w, 0, k16), kv_pair<T::QK>(w, 1, k16)}, second = {kv_pair<T::QK>(w, 2, k16), kv_pair<T::QK>(w, 3, k16)};
+                    auto pair = [&](int p) { return kv_operand<DT>(kv_pair<T::QK>(w, p, k16)); };
+                    const kr_u32x2 first = {pair(0), pair(1)}, second = {pair(2), pair(3)};
 #pragma unroll
                     for (int m = 0; m < QS; m++)
 #pragma unroll
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
                         }
                 };
                 kr_for<n * G / 8, (n + 1) * G / 8>(step);
-                const float sc = ks(n), rest = fmaf(-16.f, sc, kb(n));
+                const float sc = ks(n), rest = fmaf(T::CENTRED ? 8.f : -16.f, sc, kb(n));
 #pragma unroll
                 for (int i = 0; i < ROWS; i++) x[i] = fmaf(rest, qsum[i][n], n ? fmaf(sc, acc[i / 4][i % 4], x[i]) : sc * acc[i / 4][i % 4]);
             });
@@ -332,14 +333,16 @@ __global__ __launch_bounds__(256, (QuadsLds<DT, D, G>::AT_ONCE)) void kv_quads_k
                     const kr_u32x2 less24 = {0xC1C0C1C0u, 0xC1C0C1C0u};   // -24 in bf16
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
+                        if constexpr (!T::CENTRED) {
 #pragma unroll
-                        for (int e = T::P - 1; e >= 0; e--) ones[m][p] = kq_mfma<DT_BF16, 0, 0>(at[k][e], less24, ones[m][p]);
+                            for (int e = T::P - 1; e >= 0; e--) ones[m][p] = kq_mfma<DT_BF16, 0, 0>(at[k][e], less24, ones[m][p]);
+                        }
 #pragma unroll
                         for (int i = 0; i < 8; i += 2) {
                             const uint32_t sel = 0x0C000C00u | (uint32_t)(4 + i / 2) << 16 | (uint32_t)(i / 2);
                             const uint32_t y0 = __builtin_amdgcn_perm(w[p][k][1], w[p][k][0], sel), y1 = __builtin_amdgcn_perm(w[p][k][3], w[p][k][2], sel);
-                            const kr_u32x2 even = {((y0 << 3) & 0x00780078u) | v16, ((y1 << 3) & 0x00780078u) | v16};
-                            const kr_u32x2 odd = {((y0 >> 1) & 0x00780078u) | v16, ((y1 >> 1) & 0x00780078u) | v16};
+                            auto pair = [&](uint32_t y) { return kv_operand<DT>((y & 0x00780078u) | v16); };
+                            const kr_u32x2 even = {pair(y0 << 3), pair(y1 << 3)}, odd = {pair(y0 >> 1), pair(y1 >> 1)};
 #pragma unroll
                             for (int e = T::P - 1; e >= 0; e--) {
                                 o[m][p][i] = kq_mfma<DT_BF16, 0, 0>(at[k][e], even, o[m][p][i]);

@@ -167,7 +167,7 @@ __global__ __launch_bounds__(256, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows_ker
                 kr_f32x4 acc[NG];
 #pragma unroll
                 for (int n = 0; n < NG; n++) {
-                    const float start = -16.f * qsum[n];
+                    const float start = T::CENTRED ? 0.f : -16.f * qsum[n];
                     acc[n] = kr_f32x4{start, start, start, start};
                 }
 #pragma unroll
@@ -175,17 +175,18 @@ __global__ __launch_bounds__(256, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows_ker
                     const uint32_t w = *(const uint32_t*)(at + t * (L::CODES / 2) + i * 256 + (r * 4 + g) * 4);
                     kr_u32x4 k;
 #pragma unroll
-                    for (int p = 0; p < 4; p++) k[p] = kv_pair<T::QK>(w, p, k16);
+                    for (int p = 0; p < 4; p++) k[p] = kv_operand<DT>(kv_pair<T::QK>(w, p, k16));
 #pragma unroll
                     for (int e = T::Q - 1; e >= 0; e--) acc[i * 32 / G] = kr_mfma<T::QK>(k, q[e][i], acc[i * 32 / G]);
                 }
                 const Numbers ks = numbers(at + L::CODES, 0, t), kb = numbers(at + L::CODES, 1, t);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
+                    auto rest = [&](int n) { return T::CENTRED ? fmaf(8.f, ks(i, n), kb(i, n)) : kb(i, n); };
                     float v = ks(i, 0) * acc[0][i];
-                    v = fmaf(kb(i, 0), qsum[0], v);
+                    v = fmaf(rest(0), qsum[0], v);
 #pragma unroll
-                    for (int n = 1; n < NG; n++) v = fmaf(kb(i, n), qsum[n], fmaf(ks(i, n), acc[n][i], v));
+                    for (int n = 1; n < NG; n++) v = fmaf(rest(n), qsum[n], fmaf(ks(i, n), acc[n][i], v));
                     x[t][i] = v;
                 }
                 if (!whole) {
@@ -257,8 +258,10 @@ __global__ __launch_bounds__(256, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows_ker
                     for (int e = 0; e < T::P; e++) pt[e][j] = kv_pack_bf16(y[0][e], y[1][e]);
                 }
                 kr_f32x4 less = {0.f, 0.f, 0.f, 0.f};   // (every row of it is the same)
+                if constexpr (!T::CENTRED) {
 #pragma unroll
-                for (int e = T::P - 1; e >= 0; e--) less = kr_mfma<DT_BF16>(less24, pt[e], less);
+                    for (int e = T::P - 1; e >= 0; e--) less = kr_mfma<DT_BF16>(less24, pt[e], less);
+                }
                 const uint32_t word = n * W + r % W, sub = r / W;   // this lane's word of a token, and which of its nibbles
                 uint32_t w[8];
 #pragma unroll
@@ -276,7 +279,7 @@ __global__ __launch_bounds__(256, (RowsLds<DT, D, G>::AT_ONCE)) void kv_rows_ker
                     for (int j = 0; j < 4; j++) {
                         uint32_t two = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x0C000C00u | (uint32_t)(4 + byte) << 16 | (uint32_t)byte);
                         if constexpr (W == 16) two = t & 1 ? two >> 1 : two << 3;
-                        v[j] = (two & 0x00780078u) | v16;
+                        v[j] = kv_operand<DT>((two & 0x00780078u) | v16);
                     }
 #pragma unroll
                     for (int e = T::P - 1; e >= 0; e--) o[n][t] = kr_mfma<DT_BF16>(v, pt[e], o[n][t]);

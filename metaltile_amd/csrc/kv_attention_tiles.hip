@@ -146,7 +146,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
 #pragma unroll
                         for (int j = 0; j < 2; j++) {
                             const uint32_t two = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x0C000C00u | (uint32_t)(4 + e / 2) << 16 | (uint32_t)(e / 2));
-                            v[j] = ((e & 1 ? two >> 1 : two << 3) & 0x00780078u) | v16;
+                            v[j] = kv_operand<DT>(((e & 1 ? two >> 1 : two << 3) & 0x00780078u) | v16);
                         }
                         *(kr_u32x2*)(to + e * 16) = v;
                     }
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
                     for (int j = 0; j < 4; j++) {
                         kr_u32x4 k;
 #pragma unroll
-                        for (int p = 0; p < 4; p++) k[p] = kv_pair<T::QK>(w[j], p, k16);
+                        for (int p = 0; p < 4; p++) k[p] = kv_operand<DT>(kv_pair<T::QK>(w[j], p, k16));
                         *(kr_u32x4*)(st + (half * STEPS * 64 + (i / 16) * 64 + j * 16 + i % 16) * 16) = k;   // (i / 16: step)
                     }
                 }
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
         for (int u = 0; u < SI; u++) {
             const uint32_t i = (u * 64 + lane) % (16 * NG);
             const bool in = raw_there && lo + b * kBlock + 16 * half + i / NG < hi;   // (where no token is: zeros)
-            const float first = in ? sraw[u] : 0.f, second = in ? fmaf(values ? 8.f : -16.f, sraw[u], braw[u]) : 0.f;
+            const float first = in ? sraw[u] : 0.f, second = in ? fmaf(values || T::CENTRED ? 8.f : -16.f, sraw[u], braw[u]) : 0.f;
             to[i % NG * kBlock + i / NG] = first;   // (by several lanes the same)
             to[(NG + i % NG) * kBlock + i / NG] = second;
             fine = fine && fabsf(first) < INFINITY && fabsf(second) < INFINITY;
@@ -333,8 +333,10 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_tiles_kernel(KvAttentionArgs a,
 #pragma unroll
         for (int m = 0; m < MT; m++) {
             less[m] = kr_f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (!T::CENTRED) {
 #pragma unroll
-            for (int e = T::P - 1; e >= 0; e--) less[m] = kr_mfma<DT_BF16>(less24, pt[m][e], less[m]);
+                for (int e = T::P - 1; e >= 0; e--) less[m] = kr_mfma<DT_BF16>(less24, pt[m][e], less[m]);
+            }
         }
 #pragma unroll
         for (int t = 0; t < NT; t++)
