@@ -130,8 +130,9 @@ static uint32_t num_cus() {
 // Rows are new tokens times the query heads that share a key head, for each sequence on average:
 //   to 4     the kernel with a token to a lane, where heads have 128 values or more and there is work for the card (64 sequences of 4096 tokens, 4 rows, bf16: 70 us
 //            against 74 of the one below, f16 70 / 85, in groups of 32 80 / 108, 256 values 123 / 132; 64 values 67 / 50, one sequence of 1000 tokens 13.4 / 12.1)
-//   to 128   the one with 16 rows to a wave (32 sequences of 4096 tokens, 128 rows: 264 us against 360 of the one below, 4 of 2048 tokens 62 / 41; 64 rows 147 / 366 and
-//            35 / 34); f32 to 32
+//   to 128   the one with 16 rows to a wave, where sequences and heads fill the card (32 sequences of 4096 tokens, 128 rows: 264 us against 360 of the one below, 64 rows
+//            147 / 366), else to 64 (4 of 2048 tokens, 128 rows 62 / 41, 64 rows 35 / 34); f32 to half of
+//            that (64 rows 244 / 417, 128 rows 466 / 412; 32 rows 27 / 32, 64 rows 45 / 33)
 //   above    f16 and bf16: keys and values laid out in T first (256 rows: 494 / 372 and 115 / 45; a prompt of 8192 tokens 559 us against 942 of the next). It has to have
 //            scratch for as many tokens as max_len allows, up to 1 GiB; f32, and calls without: the codes as they are
 KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
@@ -141,8 +142,8 @@ KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
     const uint32_t span = a.window && a.window < a.kv.max_len ? a.window : a.kv.max_len;   // tokens that a row sees at most
     const uint64_t images = ((uint64_t)a.kv.max_len + kBlock - 1) / kBlock * n_seqs * a.kv.hkv * (128ull * a.kv.dim + 4);
     const bool prompts = dtype != DT_F32 && images && images <= (1ull << 30);
-    const bool few = a.kv.dim >= 128 && n_seqs * a.kv.hkv * span >= 2048 * cus;
-    p.kernel = options().kv_kernel ? options().kv_kernel : few && rows <= 4 * n_seqs ? 3 : rows > 128 * n_seqs && prompts ? 4 : rows > (dtype == DT_F32 ? 32 : 128) * n_seqs ? 2 : 1;
+    const bool filled = n_seqs * a.kv.hkv * span >= 2048 * cus, few = a.kv.dim >= 128 && filled;
+    p.kernel = options().kv_kernel ? options().kv_kernel : few && rows <= 4 * n_seqs ? 3 : rows <= (filled ? 128 : 64) / (dtype == DT_F32 ? 2 : 1) * n_seqs ? 1 : prompts ? 4 : 2;
     if (p.kernel == 4 && !prompts) p.kernel = 2;
     if (p.kernel == 3 && a.kv.dim < 128) p.kernel = 1;
     if (p.kernel == 4) p.images = (size_t)((images + 255) / 256 * 256);

@@ -44,7 +44,7 @@ class Attention:
 
     def rounded(self, kernel=0):
         """Whether keys and values are rounded to T: in the kernel for prompts, of 16-bit types."""
-        return self.dt != DType.F32 and (kernel == 4 or kernel == 0 and self.tokens * (self.hq // self.pool.hkv) > 128 * len(self.pool.lens))
+        return self.dt != DType.F32 and (kernel == 4 or kernel == 0 and self.tokens * (self.hq // self.pool.hkv) > 64 * len(self.pool.lens))   # (of calls that do not fill the card)
 
     def hold(self, kernel=0):
         got = self.result()[self.offsets[0]:self.offsets[-1]]
