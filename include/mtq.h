@@ -377,7 +377,8 @@ MTQ_API int mtq_add_rms_norm_fp8(int dtype, const void *x, const void *residual,
 
 /* A cache of keys and values in pages of page_size tokens (a power of two, 16 .. 65536). Codes, scales and biases are those of
  * mtq_affine_quantize with 4 bits: of each token and key head head_dim / 8 words and head_dim / group_size scales and biases, group_size 32, 64
- * or 128. Each array is contiguous and on 16 bytes, so that a page is also what mtq_affine_dequantize reads. head_dim 64, 128, 256. */
+ * or 128. Each array is contiguous and on 16 bytes, so that a page is also what mtq_affine_dequantize reads. head_dim 64, 128, 256;
+ * n_pages * n_heads * page_size < 2^32. */
 typedef struct mtq_kv_cache {
     void *k_codes, *k_scales, *k_biases; /* u32[n_pages, n_heads, page_size, head_dim / 8], T[n_pages, n_heads, page_size, head_dim / group_size] */
     void *v_codes, *v_scales, *v_biases;
@@ -415,10 +416,14 @@ MTQ_API int mtq_kv_read(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch
 /* Softmax attention of the batch's rows over their sequences' tokens: out = sum_j p_j v_j, p = softmax_j(scale * q . k_j), over the tokens j
  * up to the row's own place, with window > 0 the last `window` of them; tokens on no page do not count. q and out: T, hq heads
  * of head_dim side by side, q_stride / out_stride elements apart (on 16 bytes, strides of whole 16 bytes); hq a multiple of n_heads,
- * query head h goes with key head h / (hq / n_heads). A row that sees no token is zeros. Scores, softmax and sums are f32. For bf16
- * p times a value's scale is rounded to bf16 once, for f16 it keeps 16 bits and for f32 24. Codes are operands as they are. What a row does not see does not
- * reach it, NaN or not. Sequences of few rows are cut along their tokens and joined through a library-owned buffer (allocated
- * on first use); without that memory they are not cut. n_tokens < 2^24, hq <= 65536, n_tokens * hq < 2^31. */
+ * query head h goes with key head h / (hq / n_heads). A row that sees no token is zeros, and what a row does not see does not reach it, NaN or
+ * not. Scores, softmax and sums are f32. Where sequences have few rows (new tokens times the query heads of a key head), and always for f32, codes are
+ * operands as they are: p times a value's scale is rounded to bf16 once for bf16, for f16 it keeps 16 bits and for f32 24. From 64 to 128 rows a
+ * sequence on (on average, by how much there is) f16 and bf16 take keys and values as they are rounded to T, and weights too.
+ * Tokens are cut into slices, which are joined through a library-owned buffer (allocated on first use), by what all sequences have: the same call gives
+ * the same bits, another batch around a sequence may change its last ones. Keys and values in T go through that buffer too, with room
+ * for n_seqs * max_len tokens (4 * n_heads * head_dim bytes each, up to a gigabyte; more: codes as they are). Without that memory nothing is cut, and codes are operands
+ * as they are. n_tokens < 2^24, hq <= 65536, n_tokens * hq < 2^31. */
 MTQ_API int mtq_kv_attention(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch *batch, const void *q, size_t q_stride, void *out,
                              size_t out_stride, uint32_t hq, float scale, uint32_t window);
 

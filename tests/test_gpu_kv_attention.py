@@ -1,4 +1,6 @@
 """Attention over the paged 4-bit cache against 64 bits; the tolerance is derived in kv_reference.attention. Memory where no token is holds NaN and infinities."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -244,7 +246,6 @@ def test_pages_past_32_bits():
     far = np.array(near.pool.pages)
     take = rng.permutation(np.arange(n_pages - 8, n_pages))
     lib = _ensure_init()
-    import ctypes as C
     for old, new in zip(np.unique(near.pool.pages[near.pool.pages < near.pool.n_pages]), take):
         far[near.pool.pages == old] = new
         for i, (codes, scales, biases) in enumerate(near.pool.parts):
@@ -261,6 +262,65 @@ def test_pages_past_32_bits():
     assert near.out.read_bytes() == want
     for b in bufs:
         b.free()
+
+
+@pytest.mark.parametrize("kernel", [1, 2, 3, 4])
+@pytest.mark.parametrize("seqs,longest,window", [(130, 400, 0), (130, 400, 90), (512, 60, 0), (600, 60, 0)])
+def test_many_sequences(seqs, longest, window, kernel, option):
+    """More sequences than a wave has lanes, than are cut, some without rows and some without tokens: pieces of every length."""
+    print(f"[case] kv_attention {seqs} sequences, kernel {kernel}", flush=True)
+    rng = np.random.default_rng(seqs)
+    lens = [int(n) for n in rng.integers(0, longest, seqs)]
+    c = Attention(DType.BF16, lens, [int(n) for n in rng.integers(0, 3, seqs)], hq=2, hkv=1, window=window)
+    option("kv.kernel", kernel)
+    for slices in (0, 1, 4, 30):
+        option("kv.slices", slices)
+        c.out.upload(b"\xa5" * c.out.nbytes)
+        c.call()
+        c.hold(kernel)
+
+
+@pytest.mark.parametrize("kernel", [1, 2, 3, 4])
+def test_shared_pages(kernel, option):
+    """Sequences whose first pages are the same ones."""
+    c = Attention(DType.F16, [200, 180, 90], [3, 40, 20])
+    c.pool.pages[1, :8] = c.pool.pages[0, :8]
+    c.pool.pages[2, :4] = c.pool.pages[0, :4]
+    c.pool.pb.upload(c.pool.pages.astype("<u4").tobytes())
+    option("kv.kernel", kernel)
+    c.call()
+    c.hold(kernel)
+
+
+@pytest.mark.parametrize("kernel", [1, 2, 3, 4])
+def test_a_callers_stream(kernel, option):
+    """Queries copied on the caller's stream, the call behind them, and the result back: no wait in between."""
+    hip = C.CDLL("libamdhip64.so")
+    stream, lib = C.c_void_p(), _ensure_init()
+    c = Attention(DType.BF16, [900, 300], [70, 30], hq=4, hkv=2)
+    option("kv.kernel", kernel)
+    option("kv.slices", 3)
+    q, got = c.qb.read_bytes(), np.zeros(c.out.nbytes, np.uint8)
+    c.qb.upload(b"\0" * c.qb.nbytes)
+    assert hip.hipStreamCreate(C.byref(stream)) == 0
+    try:
+        _lib.check(lib.mtq_set_stream(stream))
+        assert hip.hipMemcpyAsync(C.c_void_p(c.qb.ptr), q, C.c_size_t(len(q)), 1, stream) == 0
+        c.call()
+        assert hip.hipMemcpyAsync(got.ctypes.data_as(C.c_void_p), C.c_void_p(c.out.ptr), C.c_size_t(got.nbytes), 2, stream) == 0
+        assert hip.hipStreamSynchronize(stream) == 0
+    finally:
+        _lib.check(lib.mtq_set_stream(None))
+        hip.hipStreamDestroy(stream)
+    c.hold(kernel)
+    assert got.tobytes() == c.out.read_bytes()
+
+
+def test_a_pool_past_32_bits_of_tokens():
+    c = Attention(DType.BF16, [20], [4])
+    with pytest.raises(MtqError) as e:
+        ops.kv_attention(c.dt, ops.KvCache(*c.pool.bufs, 1 << 27, 16, 2, 128, 64), c.batch, c.qb, c.out, 4, 1.0)
+    assert e.value.code == -3 and c.out.read_bytes() == b"\xa5" * c.out.nbytes
 
 
 def test_refusals():
