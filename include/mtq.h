@@ -423,7 +423,7 @@ MTQ_API int mtq_kv_read(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch
  * Tokens are cut into slices, which are joined through a library-owned buffer (allocated on first use), by what all sequences have: the same call gives
  * the same bits, another batch around a sequence may change its last ones. Keys and values in T go through that buffer too, with room
  * for n_seqs * max_len tokens (4 * n_heads * head_dim bytes each, up to a gigabyte; more: codes as they are). Without that memory nothing is cut, and codes are operands
- * as they are. n_tokens < 2^24, hq <= 65536, n_tokens * hq < 2^31. */
+ * as they are. scale is finite; n_tokens < 2^24, hq <= 65536, n_tokens * hq < 2^31. */
 MTQ_API int mtq_kv_attention(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch *batch, const void *q, size_t q_stride, void *out,
                              size_t out_stride, uint32_t hq, float scale, uint32_t window);
 

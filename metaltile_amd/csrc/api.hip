@@ -1555,6 +1555,7 @@ static int op_kv_attention(int dtype, const mtq_kv_cache* c, const mtq_kv_batch*
     int rc = check_kv(dtype, c, b, a.kv);
     if (rc) return rc;
     if (a.hq == 0 || a.hq > 65536 || a.hq % a.kv.hkv) return fail(ERR_SHAPE, "hq must be a multiple of n_heads up to 65536");
+    if (!(fabsf(a.scale) < INFINITY)) return fail(ERR_BAD_ARG, "scale must be a finite number");
     if (a.kv.n_seqs == 0 || a.kv.n_tokens == 0) return ERR_OK;
     if ((rc = check_heads(dtype, a.q, a.q_stride, a.hq, a.kv.dim)) || (rc = check_heads(dtype, a.out, a.out_stride, a.hq, a.kv.dim))) return rc;
     if ((uint64_t)a.kv.n_tokens * a.hq >= 1ull << 31) return fail(ERR_SHAPE, "n_tokens * hq must be less than 2^31");

@@ -106,18 +106,58 @@ __device__ __forceinline__ uint32_t kv_scan(uint32_t v) {
     return v;
 }
 
-// Workgroup `index` of a key head's: a sequence, and one of the equal slices that its tokens are cut into. Lengths are known here only, and sequences of
+// Rows of a sequence and key head (new tokens times the query heads that share it) go to workgroups in sets of ROWS. Sequence i's sets begin at
+// (its first row * shared + i * loose) / ROWS, loose = ROWS - the largest power of two in `shared` up to ROWS: a sequence's rows are whole multiples of that, so there is room for
+// as many sets as it has, and often for no more.
+template <uint32_t ROWS> __host__ __device__ inline uint32_t kv_loose(uint32_t shared) {
+    const uint32_t g = shared & (0u - shared);
+    return g < ROWS ? ROWS - g : 0u;
+}
+template <uint32_t ROWS> inline uint64_t kv_sets(const KvAttentionArgs& a) {   // that there is room for
+    const uint32_t shared = a.hq / a.kv.hkv;
+    return ((uint64_t)a.kv.n_tokens * shared + (uint64_t)a.kv.n_seqs * kv_loose<ROWS>(shared)) / ROWS;
+}
+// The sequence that set `index` lies in, and which of its sets it is. False: none. All lanes of a wave call.
+template <uint32_t ROWS> __device__ __forceinline__ bool kv_find(const KvAttentionArgs& a, uint32_t index, KvSeq& s, uint32_t& set) {
+    const KvArgs& kv = a.kv;
+    const uint32_t lane = threadIdx.x & 63u, shared = a.hq / kv.hkv, loose = kv_loose<ROWS>(shared);
+    auto begin = [&](uint32_t first_row, uint32_t i) { return (uint32_t)(((uint64_t)first_row * shared + (uint64_t)i * loose) / ROWS); };
+    uint32_t seq;
+    if (kv.offsets) {
+        uint32_t lo = 0, n = kv.n_seqs;   // of the sequences lo .. lo + n - 1 the last that begins at `index` or before
+        while (n > 1) {
+            const uint32_t step = (n + 63u) / 64u, i = lo + lane * step;
+            const bool before = lane * step < n && begin(kv.offsets[i] < kv.n_tokens ? kv.offsets[i] : kv.n_tokens, i) <= index;
+            const uint32_t count = (uint32_t)__popcll(__ballot(before));
+            const uint32_t skip = count ? (count - 1u) * step : 0u;
+            lo += skip;
+            n = n - skip < step ? n - skip : step;
+        }
+        seq = __builtin_amdgcn_readfirstlane(lo);
+    } else {
+        const uint32_t rows = kv.n_tokens / kv.n_seqs;   // (the last i with begin(i rows, i) <= index)
+        const uint64_t per = (uint64_t)rows * shared + loose, i = per ? (uint64_t)index * ROWS / per : 0u;
+        seq = (uint32_t)(i < kv.n_seqs ? i : kv.n_seqs - 1u);
+        while (seq + 1u < kv.n_seqs && begin((seq + 1u) * rows, seq + 1u) <= index) seq++;
+    }
+    s = kv_seq(kv, seq);
+    const uint32_t first = begin(s.first_row, seq);
+    set = index - first;
+    return index >= first && (uint64_t)set * ROWS < (uint64_t)s.rows * shared;
+}
+
+// Workgroup `index` of a key head's: a sequence's set of rows, and one of the equal slices that its tokens are cut into. Lengths are known here only, and sequences of
 // 1 to 8192 tokens, each cut into as many, left the card with the longest one's slices: so a piece is a share of all tokens, and a sequence has as many as its
 // tokens need. False: no piece. All lanes of a wave call.
 struct KvPiece {
     KvSeq s;
-    uint32_t slice = 0, slices = 1;
+    uint32_t set = 0, slice = 0, slices = 1;
 };
-template <uint32_t EACH> __device__ __forceinline__ bool kv_piece_of(const KvAttentionArgs& a, const KvParts& parts, uint32_t index, KvPiece& p) {   // EACH sequences to a lane
+template <uint32_t ROWS, uint32_t EACH> __device__ __forceinline__ bool kv_piece_of(const KvAttentionArgs& a, const KvParts& parts, uint32_t index, KvPiece& p) {   // EACH sequences to a lane
     const KvArgs& kv = a.kv;
-    const uint32_t lane = threadIdx.x & 63u, each = EACH == 1 ? 1u : (kv.n_seqs + 63u) / 64u;
+    const uint32_t lane = threadIdx.x & 63u, each = EACH == 1 ? 1u : (kv.n_seqs + 63u) / 64u, shared = a.hq / kv.hkv;
     KvSeq s[EACH];
-    uint32_t n[EACH], all = 0;   // their blocks of 64 tokens
+    uint32_t n[EACH], sets[EACH], all = 0;   // their blocks of 64 tokens
 #pragma unroll
     for (uint32_t j = 0; j < EACH; j++) {
         const uint32_t i = lane * each + j;
@@ -125,46 +165,50 @@ template <uint32_t EACH> __device__ __forceinline__ bool kv_piece_of(const KvAtt
         if (j < each && i < kv.n_seqs) s[j] = kv_seq(kv, i);
         const int32_t end = (int32_t)(s[j].len + 1u) - (int32_t)s[j].rows;   // of the first row
         const uint32_t from = a.window && end > (int32_t)a.window ? (uint32_t)end - a.window : 0u;
-        n[j] = s[j].rows ? (s[j].len - from + 63u) / 64u : 0u;
-        all += n[j];
+        sets[j] = (s[j].rows * shared + ROWS - 1u) / ROWS;
+        n[j] = (s[j].len - from + 63u) / 64u;
+        all += n[j] * sets[j];
     }
     uint32_t share = ((uint32_t)__builtin_amdgcn_readlane((int)kv_scan(all), 63) + parts.pieces - 1u) / parts.pieces;
     if (share < parts.least) share = parts.least;
     uint32_t mine = 0;
 #pragma unroll
     for (uint32_t j = 0; j < EACH; j++) {
-        n[j] = s[j].rows == 0 ? 0u : n[j] <= share ? 1u : (n[j] + share - 1u) / share;
+        n[j] = n[j] <= share ? 1u : (n[j] + share - 1u) / share;
         if (n[j] > parts.slices) n[j] = parts.slices;
-        mine += n[j];
+        mine += n[j] * sets[j];
     }
     const uint32_t upto = kv_scan(mine);
     const uint64_t above = __ballot(upto > index);
     if (!above) return false;
     const int who = __builtin_ctzll(above);
-    uint32_t rest = index - (upto - mine), slices = 1;   // (this lane's answer; `who` has the one that counts)
+    uint32_t rest = index - (upto - mine), slices = 1, of = 1;   // (this lane's answer; `who` has the one that counts)
     KvSeq found = s[0];
     bool yes = false;
 #pragma unroll
     for (uint32_t j = 0; j < EACH; j++)
         if (!yes) {
-            if (rest < n[j]) {
+            if (rest < n[j] * sets[j]) {
                 yes = true;
                 found = s[j];
                 slices = n[j];
+                of = sets[j];
             } else {
-                rest -= n[j];
+                rest -= n[j] * sets[j];
             }
         }
     auto his = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, who); };
     p.s = KvSeq{his(found.seq), his(found.first_row), his(found.rows), his(found.len)};
-    p.slice = his(rest);
+    rest = his(rest);
+    of = his(of);
+    p.slice = rest / of;
+    p.set = rest - p.slice * of;
     p.slices = his(slices);
     return true;
 }
-__device__ __forceinline__ bool kv_piece(const KvAttentionArgs& a, const KvParts& parts, uint32_t index, KvPiece& p) {
-    if (parts.slices > 1) return a.kv.n_seqs <= 64 ? kv_piece_of<1>(a, parts, index, p) : kv_piece_of<kCutSeqs / 64>(a, parts, index, p);
-    p.s = kv_seq(a.kv, index);
-    return p.s.rows != 0;
+template <uint32_t ROWS> __device__ __forceinline__ bool kv_piece(const KvAttentionArgs& a, const KvParts& parts, uint32_t index, KvPiece& p) {
+    if (parts.slices > 1) return a.kv.n_seqs <= 64 ? kv_piece_of<ROWS, 1>(a, parts, index, p) : kv_piece_of<ROWS, kCutSeqs / 64>(a, parts, index, p);
+    return kv_find<ROWS>(a, index, p.s, p.set);
 }
 
 constexpr uint32_t kBlock = 32;   // tokens of a step of the kernels for many rows
@@ -178,30 +222,10 @@ template <uint32_t ROWS> __device__ __forceinline__ bool kv_tile(const KvAttenti
     const KvArgs& kv = a.kv;
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t shared = a.hq / kv.hkv, head = blockIdx.x % kv.hkv, at_tile = blockIdx.x / kv.hkv, slice = at_tile / tiles;
-    // Sequence i's tiles begin at (its first row) * shared / ROWS + i, which leaves room for as many as it has. The last ones see the most and come first.
-    const uint32_t tile = tiles - 1u - at_tile % tiles;
-    uint32_t seq;
-    if (kv.offsets) {
-        uint32_t lo = 0, n = kv.n_seqs;   // of the sequences lo .. lo + n - 1 the last that begins at `tile` or before
-        while (n > 1) {
-            const uint32_t step = (n + 63u) / 64u, i = lo + lane * step;
-            const bool before = lane * step < n && (uint32_t)((uint64_t)(kv.offsets[i] < kv.n_tokens ? kv.offsets[i] : kv.n_tokens) * shared / ROWS) + i <= tile;
-            const uint32_t count = (uint32_t)__popcll(__ballot(before));
-            const uint32_t skip = count ? (count - 1u) * step : 0u;
-            lo += skip;
-            n = n - skip < step ? n - skip : step;
-        }
-        seq = __builtin_amdgcn_readfirstlane(lo);
-    } else {
-        const uint64_t per = (uint64_t)(kv.n_tokens / kv.n_seqs) * shared;   // (the beginnings of equal sequences: the last i with i per / ROWS + i <= tile)
-        uint32_t i = (uint32_t)((uint64_t)tile * ROWS / (per + ROWS));
-        while (i + 1u < kv.n_seqs && (i + 1u) * per / ROWS + i + 1u <= tile) i++;
-        seq = i;
-    }
-    const KvSeq s = kv_seq(kv, seq);
-    const uint32_t rows = s.rows * shared, first_tile = (uint32_t)((uint64_t)s.first_row * shared / ROWS) + seq;
-    if (tile < first_tile || (uint64_t)(tile - first_tile) * ROWS >= rows) return false;
-    const uint32_t row0 = (tile - first_tile) * ROWS;
+    KvSeq s;
+    uint32_t set;
+    if (!kv_find<ROWS>(a, tiles - 1u - at_tile % tiles, s, set)) return false;   // (the last ones see the most and come first)
+    const uint32_t rows = s.rows * shared, row0 = set * ROWS;
 
     auto end_of = [&](uint32_t i) { const int32_t e = (int32_t)(s.len + i / shared + 1u) - (int32_t)s.rows; return e > 0 ? (uint32_t)e : 0u; };
     auto from_of = [&](uint32_t e) { return a.window && e > a.window ? e - a.window : 0u; };
@@ -237,7 +261,7 @@ __device__ __forceinline__ uint32_t kv_end(const KvTile& t, uint32_t i) {   // r
     return e > 0 ? (uint32_t)e : 0u;
 }
 // Workgroups of a key head: pieces there can be.
-inline uint32_t kv_pieces(const KvAttentionArgs& a, const KvParts& parts) { return parts.slices == 1 ? a.kv.n_seqs : a.kv.n_seqs + parts.pieces; }
+template <uint32_t ROWS> inline uint64_t kv_pieces(const KvAttentionArgs& a, const KvParts& parts) { return kv_sets<ROWS>(a) + (parts.slices == 1 ? 0u : parts.pieces); }
 int launch_kv_rows(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc);
 int launch_kv_quads(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc);
 int launch_kv_tiles(int dtype, const KvAttentionArgs& p, const KvParts& parts, const LaunchCtx& lc);

@@ -172,8 +172,9 @@ KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
             slices = (uint64_t)options().kv_slices;
             pieces = slices * n_seqs;
         }
-        if (n_seqs > kCutSeqs) slices = 1;
-        while (slices > 1 && (n_seqs + pieces) * a.kv.hkv > max_workgroups(256)) {
+        const uint64_t sets = kv_sets<4>(a);   // (or fewer)
+        if (n_seqs > kCutSeqs || sets * blocks >= 1ull << 32) slices = 1;
+        while (slices > 1 && (sets + pieces) * a.kv.hkv > max_workgroups(256)) {
             pieces /= 2;
             slices = slices < pieces ? slices : pieces;
         }

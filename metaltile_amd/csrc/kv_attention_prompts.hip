@@ -73,7 +73,7 @@ template <int DT, int D, int G> __global__ __launch_bounds__(256) void kv_lay_ke
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t head = blockIdx.x % kv.hkv, rest = blockIdx.x / kv.hkv, per = (to.blocks + 3u) / 4u, block = rest % per * 4u + wave;
     const KvSeq s = kv_seq(kv, rest / per);
-    if (s.rows == 0 || block * kBlock >= s.len) return;
+    if (s.rows == 0 || kv.n_pages == 0 || block * kBlock >= s.len) return;
     const int32_t first = (int32_t)(s.len + 1u) - (int32_t)s.rows;   // what the first row sees: tokens up to here
     if (a.window && first > (int32_t)a.window && (block + 1u) * kBlock <= (uint32_t)first - a.window) return;
     uint32_t slot[2], there = 0;
@@ -449,7 +449,7 @@ template <int DT, int D, int G> int launch(const KvAttentionArgs& p, KvParts par
     static_assert(LDS <= 160 * 1024, "");
     KvAttentionArgs a = p;
     const void *lay = (const void*)kv_lay_kernel<DT, D, G>, *fn = (const void*)kv_prompts_kernel<DT, D, G>;
-    const uint64_t tiles64 = (uint64_t)a.kv.n_tokens * (a.hq / a.kv.hkv) / L::ROWS + a.kv.n_seqs;
+    const uint64_t tiles64 = kv_sets<L::ROWS>(a);
     if (tiles64 * a.kv.hkv * parts.slices > max_workgroups(512)) return fail(ERR_SHAPE, "more rows and heads than a launch can have workgroups");
     uint32_t tiles = (uint32_t)tiles64;
     LaunchCtx first = lc, second = lc, last = lc;

@@ -465,7 +465,7 @@ template <int DT, int D, int G> int launch(const KvAttentionArgs& p, KvParts par
     KvAttentionArgs a = p;
     static_assert(L::LDS <= 160 * 1024, "");
     const void* fn = (const void*)kv_tiles_kernel<DT, D, G, kWaves<D>>;
-    const uint64_t tiles64 = (uint64_t)a.kv.n_tokens * (a.hq / a.kv.hkv) / L::ROWS + a.kv.n_seqs;
+    const uint64_t tiles64 = kv_sets<L::ROWS>(a);
     if (tiles64 * a.kv.hkv * parts.slices > max_workgroups(64 * kWaves<D>)) return fail(ERR_SHAPE, "more rows and heads than a launch can have workgroups");
     uint32_t tiles = (uint32_t)tiles64;
     LaunchCtx first = lc;

@@ -280,6 +280,23 @@ def test_many_sequences(seqs, longest, window, kernel, option):
         c.hold(kernel)
 
 
+@pytest.mark.parametrize("kernel", [0, 1, 3])
+@pytest.mark.parametrize("hq", [1, 3, 4, 24])
+def test_prompts_among_tokens(kernel, hq, option):
+    """Single tokens with a prompt or two among them, in the kernels for few rows: as many sets of rows as a sequence needs, whatever the number of query heads."""
+    rng = np.random.default_rng(hq)
+    lens = [int(n) for n in rng.integers(1, 200, 70)]
+    rows = [1] * 70
+    rows[13], rows[69], rows[0], rows[40] = min(lens[13], 90), min(lens[69], 40), 0, 3
+    c = Attention(DType.BF16, lens, rows, hq=hq, hkv=1)
+    option("kv.kernel", kernel)
+    for slices in (0, 1, 3):
+        option("kv.slices", slices)
+        c.out.upload(b"\xa5" * c.out.nbytes)
+        c.call()
+        c.hold(kernel)
+
+
 @pytest.mark.parametrize("kernel", [1, 2, 3, 4])
 def test_shared_pages(kernel, option):
     """Sequences whose first pages are the same ones."""
@@ -337,6 +354,10 @@ def test_refusals():
     refused(-2, dt=4)
     refused(-2, q=c.qb.ptr + 4)
     refused(-2, out=c.out.ptr + 8)
+    for scale in (np.nan, np.inf, -np.inf):
+        with pytest.raises(MtqError) as e:
+            ops.kv_attention(dt, cache, batch, c.qb, c.out, 4, scale)
+        assert e.value.code == -2
     refused(-3, hq=0)
     refused(-3, hq=3)
     refused(-3, q_stride=128)
