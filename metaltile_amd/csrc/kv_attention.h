@@ -1,10 +1,10 @@
-// What both attention kernels over the 4-bit cache have in common.
+// What the attention kernels over the 4-bit cache have in common.
 //
 //   out = sum_j p_j v_j,  p = softmax_j(scale q . k_j),  k_j = s c + b and v_j = s c + b with codes c in 0..15 and s, b of a token and group
 //
 // Codes are operands of the matrix instructions as they are: a nibble in the mantissa of 16 is the number 16 + c, in bf16 (bits 3..6) and in f16 (bits
 // 6..9), one mask and one OR for two of them. What that adds is taken out in f32:
-//   scores  s sum_d q (16 + c) + (b - 16 s) sum_d q, for each group
+//   scores  s sum_d q (16 + c) + (b - 16 s) sum_d q, for each group (or s (sum_d q (16 + c) - 16 sum_d q) + b sum_d q)
 //   values  sum_j (p s) (16 + c) - 24 sum_j (p s) + sum_j p (b + 8 s), where the first two sums have the same rounded p s, so that its rounding
 //           meets c - 8, a code's distance from the middle, and the last is f32
 // p s is rounded to bf16 for bf16 (half a step, as the result is), and is two or three bf16 terms for f16 and f32; an f32 query is three terms.

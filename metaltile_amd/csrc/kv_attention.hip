@@ -1,4 +1,4 @@
-// Which kernel a call of the attention over the 4-bit cache takes, and into how many slices its tokens are cut.
+// Which kernel a call of the attention over the 4-bit cache takes, how its tokens are cut, and the slices' sums joined.
 #include "kv_attention.h"
 
 namespace mtq {

@@ -1,9 +1,14 @@
-// Attention over the 4-bit cache for sequences of many rows (prompts), f16 and bf16.
+// Attention over the 4-bit cache for sequences of many rows (prompts), f16 and bf16: bound by the matrix cores.
 //
-// A workgroup has 64 NW.. rows of one key head (new tokens times the query heads that share it), each wave 16 MT of them as columns of its
-// matrix instructions, and goes through the tokens that they see 32 at a time. Keys and values are made s c + b in T once for all waves, on their way into the LDS,
-// in the order in which the instructions take them: with the codes themselves as operands (kv_attention_tiles.hip) every score and weight is scaled by its group
-// in f32, which was more work of the vector units than all of the softmax. The price is a rounding of keys and values to T, as the reader has it.
+// Keys and values are made s c + b in T first, once for all query heads and tiles, by a launch of its own (14 us for 8192 tokens of 8 heads of 128 values), in
+// the order in which the instructions take them. With the codes themselves as operands (kv_attention_tiles.hip) every score and weight is scaled by its group in f32, and every
+// tile makes the same codes operands again: a prompt of 8192 tokens 942 us; s c + b made in each tile 881, here 524 - 551 (1050 - 1000 TFLOP/s; a large matrix product
+// has 1180 on the same card). The price is a rounding of keys, values and weights to T: half a step each, as the reader's output and the result have it.
+//
+// A workgroup has 16 MT rows for each of its waves, of one key head (new tokens times the query heads that share it), as columns of their matrix instructions, and goes through
+// the tokens that they see 32 at a time. A block's keys and values come by load-to-LDS instructions, three stages of each, asked for two turns ahead; one barrier a turn.
+// Workgroups of four waves, two to a compute unit, which go their own ways: one of eight has 614 us for that prompt. Rows of 48 to a wave (531), no scores ahead and
+// three waves to a SIMD (521) and other orders of a turn's parts (524 - 535) are level.
 #include "kv_attention.h"
 
 namespace mtq {

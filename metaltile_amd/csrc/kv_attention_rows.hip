@@ -1,10 +1,12 @@
-// Attention over the 4-bit cache for sequences of few rows (single tokens, drafts): bound by the cache's way from memory.
+// Attention over the 4-bit cache for sequences of few rows (single tokens, drafts).
 //
-// A wave has 16 rows (a sequence's new tokens times the query heads that share a key head) and a run of its tokens, 32 at a time, which come into its own part of
-// the LDS by load-to-LDS instructions a block ahead: no register holds what is on its way, and no wave waits for another until all have
-// their sums. 16 tokens lie on one page. Pieces of 16 bytes go into the LDS by piece and token, so that the words that a matrix instruction takes at once
+// A workgroup has 16 rows (of a sequence's new tokens times the query heads that share a key head) and a piece of its tokens, each of its four waves a run of that, 32 tokens
+// at a time, which come into its own part of the LDS by load-to-LDS instructions a block ahead: no register holds what is on its way, and no wave waits for another until
+// all have their sums. 16 tokens lie on one page. Pieces of 16 bytes go into the LDS by piece and token, so that the words that a matrix instruction takes at once
 // lie in different banks. The values' words have eight numbers of one token, while the instruction wants numbers of eight tokens: byte by byte two tokens'
 // words are put together, each lane with its number's nibble turned to the place first (kv_attention.h has the arithmetic).
+// Bound by the vector units from 16 rows on, which have 419 instructions for 32 tokens, and by latency in small calls: 32 sequences of 4096 tokens, 16 rows, bf16: 48 us
+// (3.2 TB/s); one of 1000 tokens 11 us, of which the join is 4; 12 sequences of up to 1024 visible tokens, 10 rows, f32: 16 us.
 #include "kv_attention.h"
 
 namespace mtq {

@@ -1,10 +1,11 @@
-// Attention over the 4-bit cache for sequences of many rows (prompts): bound by the vector units beside the matrix cores.
+// Attention over the 4-bit cache for sequences of many rows, codes as operands: f32, and what has no room for keys and values in T (kv_attention_prompts.hip).
 //
-// A workgroup has 64 NW.. rows of one key head (new tokens times the query heads that share it), each wave 16 MT of them as columns of its
-// matrix instructions, and goes through the tokens that they see 64 at a time. Codes are made operands once for all waves: a thread turns 32 codes of keys and
-// 32 of values into numbers of 16 bits on their way into the LDS, in the order in which the instructions take them, scales and biases into f32; two stages, so that
+// A workgroup has 16 MT rows for each of its waves, of one key head (new tokens times the query heads that share it), as columns of their
+// matrix instructions, and goes through the tokens that they see 32 at a time. Codes are made operands once for all waves: a wave turns the codes of keys or of values of
+// 16 tokens into numbers of 16 bits on their way into the LDS, in the order in which the instructions take them, scales and biases into f32; two stages, so that
 // a block's codes come from memory while the one before is computed. Four tokens of one query to a lane (kv_attention.h), so that a scale is read
-// once for MT of them.
+// once for MT of them. Bound by the vector units beside the matrix cores, a third of whose work is what goes into the LDS: four f32 prompts of 1000 tokens, 16 heads of 128
+// values 122 us; a bf16 prompt of 8192 tokens, 32 heads, 942 us (583 TFLOP/s).
 #include "kv_attention.h"
 
 namespace mtq {
