@@ -158,15 +158,17 @@ template <uint32_t ROWS, uint32_t EACH> __device__ __forceinline__ bool kv_piece
     const uint32_t lane = threadIdx.x & 63u, each = EACH == 1 ? 1u : (kv.n_seqs + 63u) / 64u, shared = a.hq / kv.hkv;
     KvSeq s[EACH];
     uint32_t n[EACH], sets[EACH], all = 0;   // their blocks of 64 tokens
+    auto from_of = [&](uint32_t j) {         // what the first row sees first
+        const int32_t end = (int32_t)(s[j].len + 1u) - (int32_t)s[j].rows;
+        return a.window && end > (int32_t)a.window ? (uint32_t)end - a.window : 0u;
+    };
 #pragma unroll
     for (uint32_t j = 0; j < EACH; j++) {
         const uint32_t i = lane * each + j;
         s[j] = KvSeq{0, 0, 0, 0};
         if (j < each && i < kv.n_seqs) s[j] = kv_seq(kv, i);
-        const int32_t end = (int32_t)(s[j].len + 1u) - (int32_t)s[j].rows;   // of the first row
-        const uint32_t from = a.window && end > (int32_t)a.window ? (uint32_t)end - a.window : 0u;
         sets[j] = (s[j].rows * shared + ROWS - 1u) / ROWS;
-        n[j] = (s[j].len - from + 63u) / 64u;
+        n[j] = (s[j].len - from_of(j) + 63u) / 64u;
         all += n[j] * sets[j];
     }
     uint32_t share = ((uint32_t)__builtin_amdgcn_readlane((int)kv_scan(all), 63) + parts.pieces - 1u) / parts.pieces;
@@ -178,11 +180,24 @@ template <uint32_t ROWS, uint32_t EACH> __device__ __forceinline__ bool kv_piece
         if (n[j] > parts.slices) n[j] = parts.slices;
         mine += n[j] * sets[j];
     }
-    const uint32_t upto = kv_scan(mine);
-    const uint64_t above = __ballot(upto > index);
-    if (!above) return false;
-    const int who = __builtin_ctzll(above);
-    uint32_t rest = index - (upto - mine), slices = 1, of = 1;   // (this lane's answer; `who` has the one that counts)
+    // Up to 64 sequences: those whose pieces are nearest to a share first, so that a compute unit gets long, middling and short ones alike.
+    uint32_t begin = 0;
+    if constexpr (EACH == 1) {
+        const uint32_t whole = (s[0].len - from_of(0) + 63u) / 64u, length = (whole + n[0] - 1u) / n[0], class_of = length * 8u > share * 7u ? 0u : length * 8u > share * 5u ? 1u : length * 8u > share * 3u ? 2u : 3u;
+        uint32_t before = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t mine_of = class_of == i ? mine : 0u, upto = kv_scan(mine_of);
+            begin = class_of == i ? before + upto - mine_of : begin;
+            before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        }
+    } else {
+        begin = kv_scan(mine) - mine;
+    }
+    const uint64_t his_is = __ballot(index - begin < mine);   // (of one lane at most)
+    if (!his_is) return false;
+    const int who = __builtin_ctzll(his_is);
+    uint32_t rest = index - begin, slices = 1, of = 1;   // (this lane's answer; `who` has the one that counts)
     KvSeq found = s[0];
     bool yes = false;
 #pragma unroll
