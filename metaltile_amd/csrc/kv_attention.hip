@@ -162,12 +162,12 @@ KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
         }
         while (slices > 1 && groups * slices > max_workgroups(512)) slices--;
     } else {
-        // The same, and no piece longer than a sequence is on average; from eight workgroups to a compute unit on they fill it as they come (256 sequences of 1 to 8192
-        // tokens: 255 us, cut by the average 257).
+        // The same, and no piece longer than two of a sequence's average. Where sequences and heads fill the card as they come they are not cut: from three to a compute unit on
+        // while a sequence has no more than 8192 tokens (500 sequences of 1000 tokens: 125 us, cut 156; 128 of 1 to 700: 26 / 29; a longer one would end alone), else from eight.
         const uint64_t seen = (uint64_t)span + a.kv.n_tokens < a.kv.max_len ? (uint64_t)span + a.kv.n_tokens : a.kv.max_len, blocks = (seen + 63) / 64;   // by all rows of a sequence
-        pieces = 2 * cus / a.kv.hkv > n_seqs ? 2 * cus / a.kv.hkv : n_seqs;
+        pieces = 2 * cus / a.kv.hkv > n_seqs / 2 ? 2 * cus / a.kv.hkv : n_seqs / 2;
         slices = blocks / 4 < pieces ? blocks / 4 : pieces;
-        if (n_seqs * a.kv.hkv >= 8 * cus) slices = 1;
+        if (n_seqs * a.kv.hkv >= (blocks <= 128 ? 3 : 8) * cus) slices = 1;
         if (options().kv_slices) {
             slices = (uint64_t)options().kv_slices;
             pieces = slices * n_seqs;

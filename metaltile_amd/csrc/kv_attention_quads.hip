@@ -10,8 +10,8 @@
 //           tokens a block multiplies goes round with k, so that each block of a group's words has p times that group's scale
 // Tokens lie in the LDS by rows. Of values those of a quad are in an order turned by their sixteen, of keys a row's pieces of 16 bytes in one turned by its place, which keeps
 // reads of both free of bank conflicts. A block's keys are asked for again as soon as they are in registers, and so are its values.
-// 64 sequences of 4096 tokens, 8 heads of 128 values, bf16: 63 us uncut (4.8 TB/s; 16 rows to a wave: 74), 256 of them 220 us (5.5 TB/s); of 1 to 8192 tokens 81 us, of which
-// the join is 5 and the rest above the even ones' time the card running empty; one of 131071 tokens, f16: 40 us (3.6 TB/s).
+// 64 sequences of 4096 tokens, 8 heads of 128 values, bf16: 63 us uncut (4.8 TB/s; 16 rows to a wave: 74), 256 of them 220 us (5.5 TB/s); of 1 to 8192 tokens 72 us, of which
+// the join is 5; one of 131071 tokens, f16: 40 us (3.6 TB/s).
 #include "kv_attention.h"
 
 namespace mtq {
