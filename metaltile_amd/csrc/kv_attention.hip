@@ -166,7 +166,8 @@ KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
         // while a sequence has no more than 8192 tokens (500 sequences of 1000 tokens: 125 us, cut 156; 128 of 1 to 700: 26 / 29; a longer one would end alone), else from eight.
         const uint64_t seen = (uint64_t)span + a.kv.n_tokens < a.kv.max_len ? (uint64_t)span + a.kv.n_tokens : a.kv.max_len, blocks = (seen + 63) / 64;   // by all rows of a sequence
         pieces = 2 * cus / a.kv.hkv > n_seqs / 2 ? 2 * cus / a.kv.hkv : n_seqs / 2;
-        slices = blocks / 4 < pieces ? blocks / 4 : pieces;
+        const uint64_t most = blocks < 10 ? 1 : blocks / (p.kernel == 3 ? 4 : 2);   // (a step of 64 or 32 tokens for each wave: 2000 tokens 10.7 us, of twice that 11.9; 640 tokens uncut 10.9)
+        slices = most < pieces ? most : pieces;
         if (n_seqs * a.kv.hkv >= (blocks <= 128 ? 3 : 8) * cus) slices = 1;
         if (options().kv_slices) {
             slices = (uint64_t)options().kv_slices;

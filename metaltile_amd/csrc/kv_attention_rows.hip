@@ -6,7 +6,7 @@
 // lie in different banks. The values' words have eight numbers of one token, while the instruction wants numbers of eight tokens: byte by byte two tokens'
 // words are put together, each lane with its number's nibble turned to the place first (kv_attention.h has the arithmetic).
 // Bound by the vector units from 16 rows on, which have 419 instructions for 32 tokens, and by latency in small calls: 32 sequences of 4096 tokens, 16 rows, bf16: 48 us
-// (3.2 TB/s); one of 1000 tokens 11 us, of which the join is 4; 12 sequences of up to 1024 visible tokens, 10 rows, f32: 16 us.
+// (3.2 TB/s); one of 1000 tokens 11 us, of which the join is 4; 12 sequences of up to 1024 visible tokens, 10 rows, f32: 15 us.
 #include "kv_attention.h"
 
 namespace mtq {
