@@ -34,7 +34,8 @@ template <int DT, int D, int G> struct QuadsLds {
     static constexpr int PART = CODES + 2 * LOADS * 256;
     static constexpr int JOIN = ROWS * (D + 4) * 4;
     static constexpr int WAVE = 2 * PART > JOIN ? 2 * PART : JOIN;
-    static constexpr int AT_ONCE = DT == DT_F32 && D == 256 && G == 32 ? 1 : DT == DT_F32 || D > 128 ? 2 : 3;   // waves of a SIMD, by the registers (f32, 256 values in groups of 32: 295 us with one wave, 663 with two that spill)
+    // Waves of a SIMD, by the registers: with more of them an instance spills (f32, 256 values in groups of 32: 295 us with one, 663 with two).
+    static constexpr int AT_ONCE = D == 256 && (G == 32 || (DT == DT_F32 && G == 64)) ? 1 : DT == DT_F32 || D > 128 ? 2 : 3;
     static_assert(4 * WAVE <= 160 * 1024, "");
 };
 

@@ -22,7 +22,9 @@ template <int DT, int D, int G> struct RowsLds {
     static constexpr int STAGE = 2 * CODES + 2 * LOADS * 256;
     static constexpr int JOIN = 16 * (D + 4) * 4;                // rows' values, and behind each its maximum and sum
     static constexpr int WAVE = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
-    static constexpr int NW = 4, AT_ONCE = DT != DT_F32 && D <= 128 && G >= 64 ? 3 : D == 256 && (DT == DT_F32 || G == 32) ? 1 : 2;   // waves; of a SIMD at a time, by the registers (256 values in groups of 32, f32: 370 us with one, 987 with two that spill; bf16 225 / 337)
+    static constexpr int NW = 4;   // waves
+    // Of a SIMD at a time, by the registers: with more of them an instance spills (256 values in groups of 32, f32: 370 us with one wave, 987 with two; bf16 225 / 337).
+    static constexpr int AT_ONCE = DT != DT_F32 && D <= 128 && G >= 64 ? 3 : D == 256 && (DT == DT_F32 || G == 32 || (DT == DT_F16 && G == 64)) ? 1 : 2;
     static_assert(NW * WAVE <= 160 * 1024, "");
 };
 
