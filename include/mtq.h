@@ -414,7 +414,7 @@ MTQ_API int mtq_kv_append(int dtype, const mtq_kv_cache *cache, const mtq_kv_bat
 MTQ_API int mtq_kv_read(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch *batch, void *k_out, void *v_out);
 
 /* Softmax attention of the batch's rows over their sequences' tokens: out = sum_j p_j v_j, p = softmax_j(scale * q . k_j), over the tokens j
- * up to the row's own place, with window > 0 the last `window` of them; tokens on no page do not count. q and out: T, hq heads
+ * up to the row's own place, with window > 0 the last `window` of them (max_len and more: all, as with 0); tokens on no page do not count. q and out: T, hq heads
  * of head_dim side by side, q_stride / out_stride elements apart (on 16 bytes, strides of whole 16 bytes); hq a multiple of n_heads,
  * query head h goes with key head h / (hq / n_heads). A row that sees no token is zeros, and what a row does not see does not reach it, NaN or
  * not. Scores, softmax and sums are f32. Where sequences have few rows (new tokens times the query heads of a key head), and always for f32, codes are

@@ -1557,6 +1557,7 @@ static int op_kv_attention(int dtype, const mtq_kv_cache* c, const mtq_kv_batch*
     if (a.hq == 0 || a.hq > 65536 || a.hq % a.kv.hkv) return fail(ERR_SHAPE, "hq must be a multiple of n_heads up to 65536");
     if (!(fabsf(a.scale) < INFINITY)) return fail(ERR_BAD_ARG, "scale must be a finite number");
     if (a.kv.n_seqs == 0 || a.kv.n_tokens == 0) return ERR_OK;
+    if (a.window >= a.kv.max_len) a.window = 0;   // (no row sees more tokens; below, windows are lengths that signed numbers hold)
     if ((rc = check_heads(dtype, a.q, a.q_stride, a.hq, a.kv.dim)) || (rc = check_heads(dtype, a.out, a.out_stride, a.hq, a.kv.dim))) return rc;
     if ((uint64_t)a.kv.n_tokens * a.hq >= 1ull << 31) return fail(ERR_SHAPE, "n_tokens * hq must be less than 2^31");
     const KvPlan plan = kv_attention_plan(dtype, a);

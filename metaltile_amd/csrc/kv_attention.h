@@ -160,7 +160,7 @@ template <uint32_t ROWS, uint32_t EACH> __device__ __forceinline__ bool kv_piece
     uint32_t n[EACH], sets[EACH], all = 0;   // their blocks of 64 tokens
     auto from_of = [&](uint32_t j) {         // what the first row sees first
         const int32_t end = (int32_t)(s[j].len + 1u) - (int32_t)s[j].rows;
-        return a.window && end > (int32_t)a.window ? (uint32_t)end - a.window : 0u;
+        return a.window && end > 0 && (uint32_t)end > a.window ? (uint32_t)end - a.window : 0u;
     };
 #pragma unroll
     for (uint32_t j = 0; j < EACH; j++) {

@@ -80,7 +80,7 @@ template <int DT, int D, int G> __global__ __launch_bounds__(256) void kv_lay_ke
     const KvSeq s = kv_seq(kv, rest / per);
     if (s.rows == 0 || kv.n_pages == 0 || block * kBlock >= s.len) return;
     const int32_t first = (int32_t)(s.len + 1u) - (int32_t)s.rows;   // what the first row sees: tokens up to here
-    if (a.window && first > (int32_t)a.window && (block + 1u) * kBlock <= (uint32_t)first - a.window) return;
+    if (a.window && first > 0 && (uint32_t)first > a.window && (block + 1u) * kBlock <= (uint32_t)first - a.window) return;
     uint32_t slot[2], there = 0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {

@@ -209,7 +209,7 @@ def kv_read(dtype, cache, batch, k_out, v_out):
 
 def kv_attention(dtype, cache, batch, q, out, hq, scale, *, window=0, q_stride=None, out_stride=None):
     """Softmax attention of the batch's rows q T[n_tokens, hq, head_dim] over their sequences' cached tokens, up to each row's own place and, with
-    window > 0, the last `window` of them. Strides in elements between tokens (None: packed)."""
+    window > 0, the last `window` of them (as many as max_len or more: all). Strides in elements between tokens (None: packed)."""
     lib = _ensure_init()
     wide = hq * cache.head_dim
     _lib.check(lib.mtq_kv_attention(int(dtype), cache, batch, _at(q), wide if q_stride is None else q_stride, _at(out), wide if out_stride is None else out_stride, hq, scale,
