@@ -419,7 +419,8 @@ MTQ_API int mtq_kv_read(int dtype, const mtq_kv_cache *cache, const mtq_kv_batch
  * query head h goes with key head h / (hq / n_heads). A row that sees no token is zeros, and what a row does not see does not reach it, NaN or
  * not. Scores, softmax and sums are f32. Where sequences have few rows (new tokens times the query heads of a key head), and always for f32, codes are
  * operands as they are: p times a value's scale is rounded to bf16 once for bf16, for f16 it keeps 16 bits and for f32 24. From 64 to 128 rows a
- * sequence on (on average, by how much there is) f16 and bf16 take keys and values as they are rounded to T, and weights too.
+ * sequence on (on average, by how much there is) f16 and bf16 take keys and values as they are rounded to T, and weights too
+ * (f16: with all its bits down to 2^-25 of a row's largest weight).
  * Tokens are cut into slices, which are joined through a library-owned buffer (allocated on first use), by what all sequences have: the same call gives
  * the same bits, another batch around a sequence may change its last ones. Keys and values in T go through that buffer too, with room
  * for n_seqs * max_len tokens (4 * n_heads * head_dim bytes each, up to a gigabyte; more: codes as they are). Without that memory nothing is cut, and codes are operands

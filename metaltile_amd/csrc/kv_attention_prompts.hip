@@ -3,7 +3,7 @@
 // Keys and values are made s c + b in T first, once for all query heads and tiles, by a launch of its own (14 us for 8192 tokens of 8 heads of 128 values), in
 // the order in which the instructions take them. With the codes themselves as operands (kv_attention_tiles.hip) every score and weight is scaled by its group in f32, and every
 // tile makes the same codes operands again: a prompt of 8192 tokens 942 us; s c + b made in each tile 881, here 524 - 551 (1050 - 1000 TFLOP/s; a large matrix product
-// has 1180 on the same card). The price is a rounding of keys, values and weights to T: half a step each, as the reader's output and the result have it.
+// has 1180 on the same card). The price is a rounding of keys, values and weights to T: half a step each, as the reader's output and the result have it (weights in f16 down to 2^-25 of a row's largest).
 //
 // A workgroup has 16 MT rows for each of its waves, of one key head (new tokens times the query heads that share it), as columns of their matrix instructions, and goes through
 // the tokens that they see 32 at a time. A block's keys and values come by load-to-LDS instructions, three stages of each, asked for two turns ahead; one barrier a turn.
@@ -59,6 +59,13 @@ template <int DT> struct Codes {   // a word of each of two tokens: of(e): both 
             return kv_pack_bf16(fmaf(s[0], (float)x, b[0]), fmaf(s[1], (float)y, b[1]));
         }
     }
+};
+
+// A score at the bar weighs 2^LIFT, and the bar is raised when one passes it by 2^SLACK. f16 has its bits down to 2^-14 only and numbers up to 2^16: with 2^11 at the bar, weights
+// down to 2^-25 of the largest are rounded by half a step of theirs (with 1 at the bar 12000 tokens of 2^-21.6 beside one whose value is 0 came out 3 % off, of 2^-24.5 44 %).
+// A prompt of 8192 tokens has 563 us as before; 2^13 and 2^2 would take 573. bf16 has f32's exponents.
+template <int DT> struct Weights {
+    static constexpr float SLACK = DT == DT_F16 ? 4.f : kSlack, LIFT = DT == DT_F16 ? 11.f : 0.f;
 };
 
 template <int D> struct PromptShape {
@@ -274,7 +281,7 @@ __global__ __launch_bounds__(64 * PromptShape<D>::NW, 2) void kv_prompts_kernel(
 #pragma unroll
         for (int m = 0; m < MT; m++) {
             top[m] = fmaxf(fmaxf(fmaxf(x[m][0][0], x[m][0][1]), fmaxf(x[m][0][2], x[m][0][3])), fmaxf(fmaxf(x[m][1][0], x[m][1][1]), fmaxf(x[m][1][2], x[m][1][3])));
-            over = over || top[m] * c > bar[m] + kSlack;
+            over = over || top[m] * c > bar[m] + Weights<DT>::SLACK;
         }
         if (__any(over)) {
 #pragma unroll
@@ -324,7 +331,7 @@ __global__ __launch_bounds__(64 * PromptShape<D>::NW, 2) void kv_prompts_kernel(
     auto weigh = [&](int t, float (&x)[MT][2][4]) {
 #pragma unroll
         for (int m = 0; m < MT; m++) {
-            const float from_bar = bar[m] == -INFINITY ? 0.f : bar[m];
+            const float from_bar = bar[m] == -INFINITY ? 0.f : bar[m] - Weights<DT>::LIFT;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 x[m][t][i] = __builtin_amdgcn_exp2f(fmaf(x[m][t][i], c, -from_bar));
