@@ -163,12 +163,13 @@ KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
         while (slices > 1 && groups * slices > max_workgroups(512)) slices--;
     } else {
         // The same, and no piece longer than two of a sequence's average. Where sequences and heads fill the card as they come they are not cut: from three to a compute unit on
-        // while a sequence has no more than 8192 tokens (500 sequences of 1000 tokens: 125 us, cut 156; 128 of 1 to 700: 26 / 29; a longer one would end alone), else from eight.
+        // while no sequence is long, else from eight, since one that is ends alone. Of 1 to 1000 tokens 128 sequences of 16 rows take 34.8 us, cut 36.4, f32 heads of 64 values
+        // 26.9 / 29.1; of 1 to 4096 103.7 / 93.5 and 81.6 / 76.4, and of 1 to 8192 with four rows in f32 266 / 210. Four rows of bf16: to 4096 84 / 87 (even ones 126 / 132), to 8192 149 / 132.
         const uint64_t seen = (uint64_t)span + a.kv.n_tokens < a.kv.max_len ? (uint64_t)span + a.kv.n_tokens : a.kv.max_len, blocks = (seen + 63) / 64;   // by all rows of a sequence
         pieces = 2 * cus / a.kv.hkv > n_seqs / 2 ? 2 * cus / a.kv.hkv : n_seqs / 2;
         const uint64_t most = blocks < 10 ? 1 : blocks / (p.kernel == 3 ? 4 : 2);   // (a step of 64 or 32 tokens for each wave: 2000 tokens 10.7 us, of twice that 11.9; 640 tokens uncut 10.9)
         slices = most < pieces ? most : pieces;
-        if (n_seqs * a.kv.hkv >= (blocks <= 128 ? 3 : 8) * cus) slices = 1;
+        if (n_seqs * a.kv.hkv >= (blocks <= (p.kernel == 3 && dtype != DT_F32 ? 64u : 32u) ? 3 : 8) * cus) slices = 1;
         if (options().kv_slices) {
             slices = (uint64_t)options().kv_slices;
             pieces = slices * n_seqs;
