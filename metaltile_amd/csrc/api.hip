@@ -1537,7 +1537,7 @@ static int op_kv_append(int dtype, const mtq_kv_cache* c, const mtq_kv_batch* b,
     if (a.kv.n_seqs == 0 || a.kv.n_tokens == 0) return ERR_OK;
     if ((rc = check_heads(dtype, a.k, a.k_stride, a.kv.hkv, a.kv.dim)) || (rc = check_heads(dtype, a.v, a.v_stride, a.kv.hkv, a.kv.dim))) return rc;
     if (a.hq && ((rc = check_heads(dtype, a.q, a.q_stride, a.hq, a.kv.dim)) || (rc = check_heads(dtype, a.q_out, a.q_out_stride, a.hq, a.kv.dim)))) return rc;
-    if (a.q && a.q == a.q_out && a.q_stride != a.q_out_stride) return fail(ERR_BAD_ARG, "queries that are turned in place must keep their stride");
+    if (a.hq && a.q == a.q_out && a.q_stride != a.q_out_stride) return fail(ERR_BAD_ARG, "queries that are turned in place must keep their stride");
     if (a.rot && !a.cos_sin) return fail(ERR_BAD_ARG, "null buffer");
     if (!on(16, a.cos_sin)) return fail(ERR_BAD_ARG, "cos_sin must be on 16 bytes");
     return launch_kv_append(dtype, a, lc);
