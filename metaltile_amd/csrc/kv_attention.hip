@@ -133,7 +133,7 @@ static uint32_t num_cus() {
 //   to 128   the one with 16 rows to a wave, where sequences and heads fill the card (32 sequences of 4096 tokens, 128 rows: 264 us against 360 of the one below, 64 rows
 //            147 / 366), else to 64 (4 of 2048 tokens, 128 rows 62 / 41, 64 rows 35 / 34); f32 to half of
 //            that (64 rows 244 / 417, 128 rows 466 / 412; 32 rows 27 / 32, 64 rows 45 / 33)
-//   above    f16 and bf16: keys and values laid out in T first (256 rows: 494 / 372 and 115 / 45; a prompt of 8192 tokens 559 us against 942 of the next). It has to have
+//   above    f16 and bf16: keys and values laid out in T first (256 rows: 494 / 372 and 115 / 45; a prompt of 8192 tokens 531 us against 942 of the next). It has to have
 //            scratch for as many tokens as max_len allows, up to 1 GiB; f32, and calls without: the codes as they are
 KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
     KvPlan p;
@@ -163,13 +163,14 @@ KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
         while (slices > 1 && groups * slices > max_workgroups(512)) slices--;
     } else {
         // The same, and no piece longer than two of a sequence's average. Where sequences and heads fill the card as they come they are not cut: from three to a compute unit on
-        // while no sequence is long, else from eight, since one that is ends alone. Of 1 to 1000 tokens 128 sequences of 16 rows take 34.8 us, cut 36.4, f32 heads of 64 values
-        // 26.9 / 29.1; of 1 to 4096 103.7 / 93.5 and 81.6 / 76.4, and of 1 to 8192 with four rows in f32 266 / 210. Four rows of bf16: to 4096 84 / 87 (even ones 126 / 132), to 8192 149 / 132.
+        // while no sequence is long, else from eight, since one that is ends alone. 128 sequences of 1 to 1000 tokens, 16 rows: 34.8 us, cut 36.4, f32 heads of 64 values 26.9 / 29.1;
+        // of 1 to 4096 103.7 / 93.5 and 81.6 / 76.4, of 1 to 8192 with four rows of f32 266 / 210. Four rows in 16 bits, to 4096: 84 / 87 and with 64 values 52.5 / 49.1, even
+        // ones 126 / 132 and 75.5 / 81; to 8192 149 / 132.
         const uint64_t seen = (uint64_t)span + a.kv.n_tokens < a.kv.max_len ? (uint64_t)span + a.kv.n_tokens : a.kv.max_len, blocks = (seen + 63) / 64;   // by all rows of a sequence
         pieces = 2 * cus / a.kv.hkv > n_seqs / 2 ? 2 * cus / a.kv.hkv : n_seqs / 2;
         const uint64_t most = blocks < 10 ? 1 : blocks / (p.kernel == 3 ? 4 : 2);   // (a step of 64 or 32 tokens for each wave: 2000 tokens 10.7 us, of twice that 11.9; 640 tokens uncut 10.9)
         slices = most < pieces ? most : pieces;
-        if (n_seqs * a.kv.hkv >= (blocks <= (p.kernel == 3 && dtype != DT_F32 ? 64u : 32u) ? 3 : 8) * cus) slices = 1;
+        if (n_seqs * a.kv.hkv >= (blocks <= (dtype != DT_F32 && rows <= 4 * n_seqs ? 64u : 32u) ? 3 : 8) * cus) slices = 1;
         if (options().kv_slices) {
             slices = (uint64_t)options().kv_slices;
             pieces = slices * n_seqs;
@@ -182,7 +183,7 @@ KvPlan kv_attention_plan(int dtype, const KvAttentionArgs& a) {
         }
         if (slices > most_bytes / row_bytes) slices = most_bytes / row_bytes;
         if (slices < 1) slices = 1;
-        p.least = (uint32_t)((blocks + slices - 1) / slices);   // (no sequence has more slices than there is room for)
+        p.least = (uint32_t)((blocks + slices - 1) / slices);   // (of what max_len allows, so a short sequence under a large max_len has few pieces: 1000 tokens under 131072 take 16.6 us, under 1000 10.7)
     }
     if (slices > most_bytes / row_bytes) slices = most_bytes / row_bytes;
     p.slices = slices < 1 ? 1 : (uint32_t)slices;

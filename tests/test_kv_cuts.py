@@ -11,7 +11,7 @@ def _cut(dt, seqs, longest, new=1, dim=128, hq=32, hkv=8):
     return len(launches) == 2
 
 
-@pytest.mark.parametrize("dt,new,dim", [(DType.F32, 1, 128), (DType.F16, 4, 128), (DType.BF16, 4, 128), (DType.BF16, 1, 64), (DType.F32, 1, 64)], ids=str)
+@pytest.mark.parametrize("dt,new,dim", [(DType.F32, 1, 128), (DType.F16, 4, 128), (DType.BF16, 4, 128), (DType.BF16, 4, 64), (DType.F32, 1, 64)], ids=str)
 def test_sequences_that_may_be_long_are_cut(dt, new, dim):
     """One that is long ends alone where none is cut, also when there are three workgroups to each compute unit."""
     for longest in (4096, 6000, 8192, 20000):
@@ -21,6 +21,8 @@ def test_sequences_that_may_be_long_are_cut(dt, new, dim):
 
 
 @pytest.mark.parametrize("dt", [DType.F16, DType.BF16], ids=str)
-def test_four_rows(dt):
-    assert _cut(dt, 128, 6000) and _cut(dt, 96, 8192)
-    assert not _cut(dt, 128, 4096) and not _cut(dt, 300, 1000) and not _cut(dt, 256, 8192)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_four_rows(dt, dim):
+    cut = lambda seqs, longest: _cut(dt, seqs, longest, dim=dim)  # noqa: E731
+    assert cut(128, 6000) and cut(96, 8192)
+    assert not cut(128, 4096) and not cut(300, 1000) and not cut(256, 8192)
