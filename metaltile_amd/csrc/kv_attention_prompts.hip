@@ -2,12 +2,13 @@
 //
 // Keys and values are made s c + b in T first, once for all query heads and tiles, by a launch of its own (14 us for 8192 tokens of 8 heads of 128 values), in
 // the order in which the instructions take them. With the codes themselves as operands (kv_attention_tiles.hip) every score and weight is scaled by its group in f32, and every
-// tile makes the same codes operands again: a prompt of 8192 tokens 942 us; s c + b made in each tile 881, here 524 - 551 (1050 - 1000 TFLOP/s; a large matrix product
-// has 1180 on the same card). The price is a rounding of keys, values and weights to T: half a step each, as the reader's output and the result have it (weights in f16 down to 2^-25 of a row's largest).
+// tile makes the same codes operands again: a prompt of 8192 tokens 942 us; s c + b made in each tile 881, here 531 on one card and 564 on another (1035 and 975 TFLOP/s; a
+// large matrix product has 1180). The price is a rounding of keys, values and weights to T: half a step each, as the reader's output and the result have it (weights in f16 down to
+// 2^-25 of a row's largest).
 //
 // A workgroup has 16 MT rows for each of its waves, of one key head (new tokens times the query heads that share it), as columns of their matrix instructions, and goes through
 // the tokens that they see 32 at a time. A block's keys and values come by load-to-LDS instructions, three stages of each, asked for two turns ahead; one barrier a turn.
-// Workgroups of four waves, two to a compute unit, which go their own ways: one of eight has 614 us for that prompt. Rows of 48 to a wave (531), no scores ahead and
+// Workgroups of four waves, two to a compute unit, which go their own ways: one of eight has 614 us for that prompt, where this has 524. Rows of 48 to a wave (531), no scores ahead and
 // three waves to a SIMD (521) and other orders of a turn's parts (524 - 535) are level.
 #include "kv_attention.h"
 
